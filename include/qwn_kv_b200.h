@@ -46,8 +46,17 @@ enum {
     QWN_CUDA_CAP_BATCHED_DEVICE = 1ull << 8,  /* device-pointer batched decode */
     QWN_CUDA_CAP_SPLIT_KV_MERGE = 1ull << 9,  /* partial (m,l,o) export + merge */
     QWN_CUDA_CAP_PAGE_EVICTION = 1ull << 10,  /* page scores, eviction, compaction */
-    QWN_CUDA_CAP_LINEAR_ATTENTION = 1ull << 11 /* qwn_linear_attention_* */
+    QWN_CUDA_CAP_LINEAR_ATTENTION = 1ull << 11, /* qwn_linear_attention_* */
+    QWN_CUDA_CAP_ROTARY_KV = 1ull << 12,      /* qwn_kv_append_rotary, qwn_kv_load_tokens */
+    QWN_CUDA_CAP_INT8_LINEAR = 1ull << 13     /* qwn_rmsnorm_q8, qwn_matmul_q8_* */
 };
+
+/* types of rows in device memory */
+typedef enum {
+    QWN_DTYPE_F32 = 1,
+    QWN_DTYPE_F16 = 2,
+    QWN_DTYPE_BF16 = 3
+} QwnDType;
 
 typedef enum {
     QWN_KV_CODEC_Q8_B64_F32 = 1,  /* reference Q8: fp32 scale per 64 channels */
@@ -387,6 +396,144 @@ QWN_CUDA_ABI_API int qwn_linear_attention_prefill(QwnLinearAttentionState *state
 QWN_CUDA_ABI_API int qwn_linear_attention_prefill_host(QwnLinearAttentionState *state, const float *q,
                                                        const float *k, const float *v, float decay,
                                                        int32_t seq_len, float *o);
+
+/* ---- rows into the cache with their rotation, and back ---------------------
+ * The reference's decoder rotates Q and K on the host before it stores them
+ * (c/qwanto_decode.c:1657-1927).  qwn_kv_append_rotary takes the projection's
+ * rows as they are: per row and head, the first rotary_dim dims turn by the
+ * row's angles,
+ *     x'[i] = x[i] c[p] - x[j] s[p],   x'[j] = x[j] c[p] + x[i] s[p],
+ * over the pairs p < rotary_dim/2 (QWN_ROTARY_HALVES: i = p, j = p +
+ * rotary_dim/2; QWN_ROTARY_NEIGHBOURS: i = 2p, j = 2p + 1), in fp32 with each
+ * product and sum rounded by itself; K and V are then quantised into the
+ * row's page by the pool's codec, as qwn_kv_store_tokens stores fp32 rows,
+ * and Q goes to query_out_dev.  One call serves one token of every sequence
+ * (row_begin_dev NULL) as well as ragged runs of prompt rows.  The tokens
+ * must have been reserved (qwn_kv_seq_append).  A sequence appears once in a
+ * call; other work on the same tokens must be ordered by the caller.
+ * A row outside its sequence, or whose angle is outside the table, latches
+ * BAD_LENGTH; a bad sequence id BAD_SEQUENCE: the row stores nothing and its
+ * query_out rows are zero.
+ * Rows start on four values: 16 bytes for fp32, 8 for the 16-bit types, row
+ * strides multiples of 4 (INVALID_ARGUMENT otherwise). */
+enum { QWN_ROTARY_HALVES = 0, QWN_ROTARY_NEIGHBOURS = 1 };
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t layer, num_seqs;
+    const int32_t *seq_ids_dev;     /* [num_seqs] or NULL = 0..num_seqs-1 */
+    const int32_t *row_begin_dev;   /* [num_seqs+1] ascending: rows [begin[i], begin[i+1]) are sequence i's;
+                                       NULL: row i is sequence i's (num_rows = num_seqs) */
+    const int32_t *first_pos_dev;   /* [num_seqs] cache position of each sequence's first row;
+                                       NULL: the rows are the sequence's newest tokens */
+    const int32_t *rotary_pos_dev;  /* [num_rows] table row of each row's angles, where it is not the
+                                       cache position (after an eviction); NULL: the cache position */
+    uint32_t num_rows;
+    uint32_t dtype;                 /* QwnDType of query, key and value */
+    uint32_t query_heads;           /* multiple of kv_heads; 0: no query rows */
+    uint32_t query_out_dtype;       /* QwnDType; qwn_kv_decode reads fp32 */
+    uint32_t rotary_dim;            /* multiple of 8 up to 128; 0: no rotation */
+    uint32_t rotary_style;          /* QWN_ROTARY_* */
+    uint32_t max_position;          /* rows of the table */
+    uint32_t reserved;
+    const float *rotations_dev;     /* [max_position][rotary_dim]: cosines of the rotary_dim/2 angles, then sines */
+    uint64_t query_stride, key_stride, value_stride; /* values between rows; 0: heads x 128 */
+    const void *query_dev;          /* [num_rows][query_heads][128] */
+    const void *key_dev;            /* [num_rows][kv_heads][128] */
+    const void *value_dev;
+    void *query_out_dev;            /* [num_rows][query_heads][128], contiguous; may be query_dev */
+    void *stream;
+} QwnKvAppendRotaryRequest;
+QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *pool, const QwnKvAppendRotaryRequest *request);
+
+/* Cached tokens back to rows, as the values their codes stand for (what the
+ * attention computes with): a prompt's next chunk attends over them, a
+ * sequence moves to another pool or codec.  Rows that cannot be read (bad
+ * sequence, position or page, latched) are zero.  Alignment as above. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t layer, num_seqs;
+    const int32_t *seq_ids_dev;
+    const int32_t *row_begin_dev;   /* as in QwnKvAppendRotaryRequest */
+    const int32_t *first_pos_dev;
+    uint32_t num_rows;
+    uint32_t dtype;                 /* QwnDType of the outputs */
+    uint64_t key_stride, value_stride; /* values between rows; 0: kv_heads x 128 */
+    void *key_out_dev;              /* [num_rows][kv_heads][128]; either may be NULL */
+    void *value_out_dev;
+    void *stream;
+} QwnKvLoadTokensRequest;
+QWN_CUDA_ABI_API int qwn_kv_load_tokens(QwnKvPoolHandle *pool, const QwnKvLoadTokensRequest *request);
+
+/* ---- int8 activations and products -----------------------------------------
+ * qwn_rmsnorm_q8 turns a layer's input rows into the int8 rows that
+ * qwn_matmul_q8 (and, through the host, ABI v1's HyperVSQ-2 products) take:
+ *     h = x + residual                              (fp32)
+ *     y = h / sqrt(mean(h^2) + eps) * weight        (QWN_NORM_RMS; QWN_NORM_NONE: y = h * weight)
+ *     scale = max|y| / 127 over the finite y, 1 if that is 0
+ *     code = y / scale rounded to nearest even, 0 where y is not finite
+ * the rules of the pool's Q8 codecs (c/qwanto_turboquant.c:555-586) over a
+ * whole row.  residual_out receives h in the rows' type; y comes from h before
+ * that rounding.  rows_out, where given, receives code x scale: what a product
+ * that stays in 16 bits must see to agree with the int8 ones. */
+enum { QWN_NORM_RMS = 0, QWN_NORM_NONE = 1 };
+#define QWN_RMSNORM_MAX_WIDTH 32768u
+typedef struct {
+    QwnCudaAbiHeader header;
+    int32_t device_id;
+    uint32_t rows, width;           /* width up to QWN_RMSNORM_MAX_WIDTH */
+    uint32_t dtype;                 /* QwnDType of x, residual, weight and residual_out */
+    uint32_t mode;                  /* QWN_NORM_* */
+    float eps;
+    uint32_t rows_dtype;            /* QwnDType of rows_out */
+    uint32_t reserved;
+    uint64_t x_stride, residual_stride, residual_out_stride, codes_stride, rows_stride; /* values; 0: width */
+    const void *x_dev;              /* [rows][width] */
+    const void *residual_dev;       /* optional */
+    const void *weight_dev;         /* optional [width] */
+    void *residual_out_dev;         /* optional; may be residual_dev or x_dev (with their stride) */
+    int8_t *codes_dev;              /* [rows][width] */
+    float *scales_dev;              /* [rows] */
+    void *rows_out_dev;             /* optional */
+    void *stream;
+} QwnRmsNormQ8Request;
+QWN_CUDA_ABI_API int qwn_rmsnorm_q8(const QwnRmsNormQ8Request *request);
+
+/* out[m][n] = (sum_k codes[m][k] weight[n][k]) * scales[m] * weight_scales[n] + bias[n]:
+ * int8 products summed exactly in int32, scaled in fp32, rounded once.
+ * create copies weight, scales and bias from device memory into the handle's
+ * own layout and returns when the copy is done.  A handle may be used from
+ * several streams at once: a call keeps nothing in it. */
+#define QWN_MATMUL_Q8_MAX_IN 131071u /* |sum| < 2^31 with codes of -128 */
+typedef struct {
+    QwnCudaAbiHeader header;
+    int32_t device_id;
+    uint32_t out_features, in_features;
+    uint32_t reserved;
+    uint64_t weight_stride;         /* bytes between the weight's rows; 0: in_features */
+    const int8_t *weight_dev;       /* [out_features][in_features] */
+    const float *scales_dev;        /* [out_features] */
+    const float *bias_dev;          /* optional [out_features] */
+    void *stream;                   /* the copies run here */
+} QwnMatmulQ8Options;
+typedef struct { QwnCudaAbiHeader header; void *opaque; } QwnMatmulQ8Handle;
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t rows;
+    uint32_t out_dtype;             /* QwnDType */
+    uint64_t codes_stride;          /* bytes between rows, a multiple of 16; 0: in_features */
+    uint64_t out_stride;            /* values between rows; 0: out_features */
+    const int8_t *codes_dev;        /* [rows][in_features], 16-byte aligned */
+    const float *scales_dev;        /* [rows] */
+    void *out_dev;                  /* [rows][out_features] */
+    void *stream;
+} QwnMatmulQ8Request;
+QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *options, QwnMatmulQ8Handle *handle);
+/* waits for the device's work, then frees the handle's memory */
+QWN_CUDA_ABI_API int qwn_matmul_q8_destroy(QwnMatmulQ8Handle *handle);
+QWN_CUDA_ABI_API int qwn_matmul_q8(QwnMatmulQ8Handle *handle, const QwnMatmulQ8Request *request);
+/* return and clear the latched status bits (WAIT_TIMEOUT: a product gave up on a wait and its output is not
+ * complete); synchronises the device */
+QWN_CUDA_ABI_API int qwn_matmul_q8_check(QwnMatmulQ8Handle *handle, uint32_t *status_bits);
 
 #ifdef __cplusplus
 }

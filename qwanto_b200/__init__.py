@@ -22,11 +22,12 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import (CODEC_F16, CODEC_Q4_G32, CODEC_Q8_B64_F32, CODEC_Q8_HEAD_F16, CODEC_TQ35_G64, QwnCudaError, check,
-                   init, lib)
+from ._lib import (CODEC_F16, CODEC_Q4_G32, CODEC_Q8_B64_F32, CODEC_Q8_HEAD_F16, CODEC_TQ35_G64, DTYPE_BF16,
+                   DTYPE_F16, DTYPE_F32, QwnCudaError, check, init, lib)
 
 __all__ = ["CudaContext", "KvPool", "lib", "QwnCudaError", "generate_rows", "merge_partials",
-           "CODEC_Q8_B64_F32", "CODEC_Q8_HEAD_F16", "CODEC_TQ35_G64", "CODEC_Q4_G32", "CODEC_F16", "launch_count", "merge_partials_packed"]
+           "CODEC_Q8_B64_F32", "CODEC_Q8_HEAD_F16", "CODEC_TQ35_G64", "CODEC_Q4_G32", "CODEC_F16", "launch_count", "merge_partials_packed",
+           "MatmulQ8", "rmsnorm_q8", "DTYPE_F32", "DTYPE_F16", "DTYPE_BF16"]
 
 TILE_BYTES = {CODEC_Q8_B64_F32: 4352, CODEC_Q8_HEAD_F16: 4160, CODEC_TQ35_G64: 2048, CODEC_Q4_G32: 2560,
               CODEC_F16: 8192}
@@ -191,6 +192,37 @@ class KvPool:
         check("qwn_kv_store_tokens", lib().qwn_kv_store_tokens(C.byref(self.h), seq, layer, first_pos, n_tokens,
                                                                 _ptr(key), _ptr(value), _stream(stream)))
 
+    def append_rotary(self, layer: int, num_seqs: int, num_rows: int, dtype: int, key, value, query=None,
+                      query_heads: int = 0, query_out=None, query_out_dtype: int = DTYPE_F32, rotations=None,
+                      rotary_dim: int = 0, max_position: int = 0, neighbours: bool = False, row_begin=None,
+                      first_pos=None, rotary_pos=None, seq_ids=None, query_stride: int = 0, key_stride: int = 0,
+                      value_stride: int = 0, stream=None) -> None:
+        """Rotate the projection's rows by their positions, store K and V in
+        their pages and Q in query_out (qwn_kv_append_rotary): one row per
+        sequence, or with row_begin [num_seqs + 1] ragged runs of rows.
+        Strides are in values between rows (0: contiguous)."""
+        r = init(_lib.AppendRotaryRequest())
+        r.layer, r.num_seqs, r.num_rows, r.dtype = layer, num_seqs, num_rows, dtype
+        r.seq_ids_dev, r.row_begin_dev = _ptr(seq_ids), _ptr(row_begin)
+        r.first_pos_dev, r.rotary_pos_dev = _ptr(first_pos), _ptr(rotary_pos)
+        r.query_heads, r.query_out_dtype, r.rotary_dim = query_heads, query_out_dtype, rotary_dim
+        r.rotary_style, r.max_position, r.rotations_dev = int(neighbours), max_position, _ptr(rotations)
+        r.query_stride, r.key_stride, r.value_stride = query_stride, key_stride, value_stride
+        r.query_dev, r.key_dev, r.value_dev, r.query_out_dev = _ptr(query), _ptr(key), _ptr(value), _ptr(query_out)
+        r.stream = _stream(stream)
+        check("qwn_kv_append_rotary", lib().qwn_kv_append_rotary(C.byref(self.h), C.byref(r)))
+
+    def load_tokens(self, layer: int, num_seqs: int, num_rows: int, dtype: int, key_out=None, value_out=None,
+                    row_begin=None, first_pos=None, seq_ids=None, key_stride: int = 0, value_stride: int = 0,
+                    stream=None) -> None:
+        """Cached tokens back to rows (qwn_kv_load_tokens), as the values their codes stand for."""
+        r = init(_lib.LoadTokensRequest())
+        r.layer, r.num_seqs, r.num_rows, r.dtype = layer, num_seqs, num_rows, dtype
+        r.seq_ids_dev, r.row_begin_dev, r.first_pos_dev = _ptr(seq_ids), _ptr(row_begin), _ptr(first_pos)
+        r.key_stride, r.value_stride = key_stride, value_stride
+        r.key_out_dev, r.value_out_dev, r.stream = _ptr(key_out), _ptr(value_out), _stream(stream)
+        check("qwn_kv_load_tokens", lib().qwn_kv_load_tokens(C.byref(self.h), C.byref(r)))
+
     def prefill_synthetic(self, seq_ids, lens, seed: int, outlier_mask: np.ndarray | None = None,
                           stream=None) -> None:
         ids = np.ascontiguousarray(seq_ids, dtype=np.int32)
@@ -214,6 +246,61 @@ class KvPool:
         r.host_output = _ptr(host_output)
         tel = telemetry if telemetry is not None else init(_lib.Telemetry())
         check("qwn_kv_decode_step_host", lib().qwn_kv_decode_step_host(C.byref(self.h), C.byref(r), C.byref(tel)))
+
+
+def rmsnorm_q8(x, rows: int, width: int, dtype: int, codes, scales, weight=None, eps: float = 1e-6, residual=None,
+               residual_out=None, norm: bool = True, x_stride: int = 0, residual_stride: int = 0,
+               residual_out_stride: int = 0, codes_stride: int = 0, rows_out=None, rows_dtype: int = DTYPE_BF16,
+               rows_stride: int = 0, device: int = 0, stream=None) -> None:
+    """Rows to int8 codes with one scale each, after the residual's addition
+    and the root-mean-square norm (qwn_rmsnorm_q8); norm=False only quantises.
+    Strides are in values between rows (0: width)."""
+    r = init(_lib.RmsNormQ8Request())
+    r.device_id, r.rows, r.width, r.dtype, r.mode, r.eps = device, rows, width, dtype, int(not norm), eps
+    r.rows_dtype = rows_dtype
+    r.x_stride, r.residual_stride, r.residual_out_stride = x_stride, residual_stride, residual_out_stride
+    r.codes_stride, r.rows_stride = codes_stride, rows_stride
+    r.x_dev, r.residual_dev, r.weight_dev, r.residual_out_dev = _ptr(x), _ptr(residual), _ptr(weight), _ptr(residual_out)
+    r.codes_dev, r.scales_dev, r.rows_out_dev, r.stream = _ptr(codes), _ptr(scales), _ptr(rows_out), _stream(stream)
+    check("qwn_rmsnorm_q8", lib().qwn_rmsnorm_q8(C.byref(r)))
+
+
+class MatmulQ8:
+    """An int8 weight [out_features][in_features] with a scale per output (and
+    optionally a bias), kept on the device: rows of int8 codes with a scale
+    each are multiplied by it (qwn_matmul_q8_*)."""
+
+    def __init__(self, weight, out_features: int, in_features: int, scales, bias=None, weight_stride: int = 0,
+                 device: int = 0, stream=None):
+        o = init(_lib.MatmulQ8Options())
+        o.device_id, o.out_features, o.in_features, o.weight_stride = device, out_features, in_features, weight_stride
+        o.weight_dev, o.scales_dev, o.bias_dev, o.stream = _ptr(weight), _ptr(scales), _ptr(bias), _stream(stream)
+        self.h = init(_lib.Handle())
+        check("qwn_matmul_q8_create", lib().qwn_matmul_q8_create(C.byref(o), C.byref(self.h)))
+        self.out_features, self.in_features, self.device = out_features, in_features, device
+
+    def __call__(self, codes, scales, rows: int, out, out_dtype: int, codes_stride: int = 0, out_stride: int = 0,
+                 stream=None) -> None:
+        r = init(_lib.MatmulQ8Request())
+        r.rows, r.out_dtype, r.codes_stride, r.out_stride = rows, out_dtype, codes_stride, out_stride
+        r.codes_dev, r.scales_dev, r.out_dev, r.stream = _ptr(codes), _ptr(scales), _ptr(out), _stream(stream)
+        check("qwn_matmul_q8", lib().qwn_matmul_q8(C.byref(self.h), C.byref(r)))
+
+    def check(self) -> int:
+        bits = C.c_uint32(0)
+        check("qwn_matmul_q8_check", lib().qwn_matmul_q8_check(C.byref(self.h), C.byref(bits)))
+        return int(bits.value)
+
+    def close(self) -> None:
+        if self.h is not None and self.h.opaque:
+            lib().qwn_matmul_q8_destroy(C.byref(self.h))
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class CudaContext:

@@ -29,6 +29,13 @@ CAP_TQ_KV = 1 << 7
 CAP_BATCHED_DEVICE = 1 << 8
 CAP_SPLIT_KV_MERGE = 1 << 9
 CAP_PAGE_EVICTION = 1 << 10
+CAP_LINEAR_ATTENTION = 1 << 11
+CAP_ROTARY_KV = 1 << 12
+CAP_INT8_LINEAR = 1 << 13
+
+DTYPE_F32 = 1
+DTYPE_F16 = 2
+DTYPE_BF16 = 3
 
 ST_POOL_EXHAUSTED = 1 << 0
 ST_TABLE_OVERFLOW = 1 << 1
@@ -189,6 +196,47 @@ class LinearAttentionState(C.Structure):
                 ("reserved", C.c_uint32), ("staging", C.c_void_p), ("staging_bytes", C.c_uint64)]
 
 
+class AppendRotaryRequest(C.Structure):
+    _fields_ = [("header", Header), ("layer", C.c_uint32), ("num_seqs", C.c_uint32), ("seq_ids_dev", C.c_void_p),
+                ("row_begin_dev", C.c_void_p), ("first_pos_dev", C.c_void_p), ("rotary_pos_dev", C.c_void_p),
+                ("num_rows", C.c_uint32), ("dtype", C.c_uint32), ("query_heads", C.c_uint32),
+                ("query_out_dtype", C.c_uint32), ("rotary_dim", C.c_uint32), ("rotary_style", C.c_uint32),
+                ("max_position", C.c_uint32), ("reserved", C.c_uint32), ("rotations_dev", C.c_void_p),
+                ("query_stride", C.c_uint64), ("key_stride", C.c_uint64), ("value_stride", C.c_uint64),
+                ("query_dev", C.c_void_p), ("key_dev", C.c_void_p), ("value_dev", C.c_void_p),
+                ("query_out_dev", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class LoadTokensRequest(C.Structure):
+    _fields_ = [("header", Header), ("layer", C.c_uint32), ("num_seqs", C.c_uint32), ("seq_ids_dev", C.c_void_p),
+                ("row_begin_dev", C.c_void_p), ("first_pos_dev", C.c_void_p), ("num_rows", C.c_uint32),
+                ("dtype", C.c_uint32), ("key_stride", C.c_uint64), ("value_stride", C.c_uint64),
+                ("key_out_dev", C.c_void_p), ("value_out_dev", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class RmsNormQ8Request(C.Structure):
+    _fields_ = [("header", Header), ("device_id", C.c_int32), ("rows", C.c_uint32), ("width", C.c_uint32),
+                ("dtype", C.c_uint32), ("mode", C.c_uint32), ("eps", C.c_float), ("rows_dtype", C.c_uint32),
+                ("reserved", C.c_uint32), ("x_stride", C.c_uint64), ("residual_stride", C.c_uint64),
+                ("residual_out_stride", C.c_uint64), ("codes_stride", C.c_uint64), ("rows_stride", C.c_uint64),
+                ("x_dev", C.c_void_p), ("residual_dev", C.c_void_p), ("weight_dev", C.c_void_p),
+                ("residual_out_dev", C.c_void_p), ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p),
+                ("rows_out_dev", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class MatmulQ8Options(C.Structure):
+    _fields_ = [("header", Header), ("device_id", C.c_int32), ("out_features", C.c_uint32),
+                ("in_features", C.c_uint32), ("reserved", C.c_uint32), ("weight_stride", C.c_uint64),
+                ("weight_dev", C.c_void_p), ("scales_dev", C.c_void_p), ("bias_dev", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class MatmulQ8Request(C.Structure):
+    _fields_ = [("header", Header), ("rows", C.c_uint32), ("out_dtype", C.c_uint32), ("codes_stride", C.c_uint64),
+                ("out_stride", C.c_uint64), ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("stream", C.c_void_p)]
+
+
 _P = C.POINTER
 _SIGS = {
     "qwn_cuda_abi_query": (C.c_int, [_P(AbiInfo)]),
@@ -229,6 +277,13 @@ _SIGS = {
     "qwn_kv_decode_split": (C.c_int, [_P(Handle), _P(SplitRequest)]),
     "qwn_kv_store_tokens": (C.c_int, [_P(Handle), C.c_int32, C.c_uint32, C.c_uint32, C.c_uint32,
                                       C.c_void_p, C.c_void_p, C.c_void_p]),
+    "qwn_kv_append_rotary": (C.c_int, [_P(Handle), _P(AppendRotaryRequest)]),
+    "qwn_kv_load_tokens": (C.c_int, [_P(Handle), _P(LoadTokensRequest)]),
+    "qwn_rmsnorm_q8": (C.c_int, [_P(RmsNormQ8Request)]),
+    "qwn_matmul_q8_create": (C.c_int, [_P(MatmulQ8Options), _P(Handle)]),
+    "qwn_matmul_q8_destroy": (C.c_int, [_P(Handle)]),
+    "qwn_matmul_q8": (C.c_int, [_P(Handle), _P(MatmulQ8Request)]),
+    "qwn_matmul_q8_check": (C.c_int, [_P(Handle), _P(C.c_uint32)]),
     "qwn_kv_generate_rows": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64,
                                        C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "qwn_kv_prefill_synthetic": (C.c_int, [_P(Handle), C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64,

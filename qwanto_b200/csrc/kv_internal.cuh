@@ -29,6 +29,25 @@ std::string last_error();
 extern std::atomic<uint64_t> g_launches;
 inline void count_launch(uint64_t n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
+// the calling thread's device for the length of a call
+struct DeviceScope {
+    int prev = -1;
+    bool ok = true;
+    explicit DeviceScope(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+    }
+    ~DeviceScope() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+    // the error of a device that cannot be selected
+    int fail(const char *what) const {
+        set_cuda_error(what, cudaGetLastError());
+        return QWN_CUDA_STATUS_UNAVAILABLE;
+    }
+};
+
 inline bool header_ok(const QwnCudaAbiHeader &h, size_t expected) {
     return h.abi_version == QWN_CUDA_ABI_VERSION && h.struct_size >= expected;
 }

@@ -35,26 +35,6 @@ const void *attention_kernel_ptr(uint32_t codec, int hg);
 
 namespace {
 
-struct StoreGeo {
-    uint8_t *pages;
-    uint64_t page_bytes;
-    uint32_t tile_bytes, tpp, page_tokens, kv_heads, mp, total_pages, max_seqs;
-    const int32_t *page_table;
-    const int32_t *seq_lens;
-    uint32_t *status;
-};
-
-__device__ __forceinline__ uint8_t *tile_for(const StoreGeo &g, int32_t seq, uint32_t layer,
-                                             uint32_t head, int32_t pos) {
-    const uint32_t lp = (uint32_t)pos / g.page_tokens;
-    if (lp >= g.mp) { latch(g.status, QWN_KV_STATUS_TABLE_OVERFLOW); return nullptr; }
-    const int32_t pg = g.page_table[(size_t)seq * g.mp + lp];
-    if (pg < 0 || (uint32_t)pg >= g.total_pages) { latch(g.status, QWN_KV_STATUS_BAD_PAGE); return nullptr; }
-    const uint32_t tin = ((uint32_t)pos % g.page_tokens) / 16u;
-    return g.pages + (size_t)pg * g.page_bytes +
-           ((size_t)(layer * g.kv_heads + head) * g.tpp + tin) * g.tile_bytes;
-}
-
 // append the newest token (position len-1) of each sequence in the batch
 template <int CODEC>
 __global__ void append_kernel(StoreGeo g, uint32_t layer, uint32_t n, const int32_t *seq_ids,
@@ -221,23 +201,6 @@ __global__ void __launch_bounds__(32) seq_append_kernel(uint32_t n, const int32_
 __global__ void iota_i32(int32_t *p, size_t n) {
     for (size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (size_t)gridDim.x * blockDim.x)
         p[e] = (int32_t)e;
-}
-
-StoreGeo store_geo(Pool *p) {
-    StoreGeo g;
-    g.pages = p->pages;
-    g.page_bytes = p->page_bytes;
-    g.tile_bytes = (uint32_t)p->tile_bytes;
-    g.tpp = p->tiles_per_page;
-    g.page_tokens = p->page_tokens;
-    g.kv_heads = p->kv_heads;
-    g.mp = p->max_pages_per_seq;
-    g.total_pages = p->total_pages;
-    g.max_seqs = p->max_seqs;
-    g.page_table = p->page_table;
-    g.seq_lens = p->seq_lens;
-    g.status = p->status;
-    return g;
 }
 
 template <template <int> class K, class... Args>

@@ -1,5 +1,5 @@
-// Quantize-on-append device code shared by the append, prefill and fused
-// attention kernels.  One warp stores one token-head; lane l holds dims
+// Quantize-on-append device code and the way back, shared by the append,
+// prefill, rotary and fused attention kernels.  One warp stores one token-head; lane l holds dims
 // 4l..4l+3 of K and of V.  The rules are the reference quantizers'
 // (c/qwanto_turboquant.c:555-586 for Q8, :162-213 for TurboQuant); the byte
 // positions are this library's tile layout (see qwn_oracle.c for the
@@ -10,6 +10,44 @@
 
 namespace qkv {
 namespace {
+
+// what a kernel needs of the pool to find a token's tile
+struct StoreGeo {
+    uint8_t *pages;
+    uint64_t page_bytes;
+    uint32_t tile_bytes, tpp, page_tokens, kv_heads, mp, total_pages, max_seqs;
+    const int32_t *page_table;
+    const int32_t *seq_lens;
+    uint32_t *status;
+};
+
+__device__ __forceinline__ uint8_t *tile_for(const StoreGeo &g, int32_t seq, uint32_t layer,
+                                             uint32_t head, int32_t pos) {
+    const uint32_t lp = (uint32_t)pos / g.page_tokens;
+    if (lp >= g.mp) { latch(g.status, QWN_KV_STATUS_TABLE_OVERFLOW); return nullptr; }
+    const int32_t pg = g.page_table[(size_t)seq * g.mp + lp];
+    if (pg < 0 || (uint32_t)pg >= g.total_pages) { latch(g.status, QWN_KV_STATUS_BAD_PAGE); return nullptr; }
+    const uint32_t tin = ((uint32_t)pos % g.page_tokens) / 16u;
+    return g.pages + (size_t)pg * g.page_bytes +
+           ((size_t)(layer * g.kv_heads + head) * g.tpp + tin) * g.tile_bytes;
+}
+
+inline StoreGeo store_geo(Pool *p) {
+    StoreGeo g;
+    g.pages = p->pages;
+    g.page_bytes = p->page_bytes;
+    g.tile_bytes = (uint32_t)p->tile_bytes;
+    g.tpp = p->tiles_per_page;
+    g.page_tokens = p->page_tokens;
+    g.kv_heads = p->kv_heads;
+    g.mp = p->max_pages_per_seq;
+    g.total_pages = p->total_pages;
+    g.max_seqs = p->max_seqs;
+    g.page_table = p->page_table;
+    g.seq_lens = p->seq_lens;
+    g.status = p->status;
+    return g;
+}
 
 // ---------------------------------------------------------------------------
 // quantize-on-append: one warp stores one token-head; lane holds dims
@@ -244,6 +282,107 @@ __device__ void store_token<QWN_KV_CODEC_TQ35_G64>(uint8_t *tile, int t, float4 
                 (uint32_t)tq_f32_to_f16(range) | ((uint32_t)tq_f32_to_f16(mn) << 16);
         }
     }
+}
+
+// ---------------------------------------------------------------------------
+// the way back: dims 4*lane .. 4*lane+3 of K (which 0) or V (which 1) of
+// token t of a tile, as the values their codes stand for
+// ---------------------------------------------------------------------------
+template <int CODEC>
+__device__ float4 load_token(const uint8_t *tile, int t, int which, int lane);
+
+// four biased int8 codes (code + 128) times their scale
+__device__ __forceinline__ float4 q8_values(uint32_t w, float s) {
+    return make_float4((float)((int)(w & 0xFF) - 128) * s, (float)((int)((w >> 8) & 0xFF) - 128) * s,
+                       (float)((int)((w >> 16) & 0xFF) - 128) * s, (float)((int)(w >> 24) - 128) * s);
+}
+__device__ __forceinline__ uint32_t q8_codes(const uint8_t *tile, int t, int which, int lane) {
+    if (!which) return *reinterpret_cast<const uint32_t *>(tile + k8_off(t, 4 * lane));
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w |= (uint32_t)tile[v8_off(t, 4 * lane + i)] << (8 * i);
+    return w;
+}
+template <>
+__device__ __forceinline__ float4 load_token<QWN_KV_CODEC_Q8_HEAD_F16>(const uint8_t *tile, int t, int which,
+                                                                       int lane) {
+    const float s = h2f(*reinterpret_cast<const uint16_t *>(tile + (which ? 4128 : 4096) + s16_off(t)));
+    return q8_values(q8_codes(tile, t, which, lane), s);
+}
+template <>
+__device__ __forceinline__ float4 load_token<QWN_KV_CODEC_Q8_B64_F32>(const uint8_t *tile, int t, int which,
+                                                                      int lane) {
+    const float s = *reinterpret_cast<const float *>(tile + (which ? 4224 : 4096) + s32_off(t, lane >> 4));
+    return q8_values(q8_codes(tile, t, which, lane), s);
+}
+template <>
+__device__ __forceinline__ float4 load_token<QWN_KV_CODEC_F16>(const uint8_t *tile, int t, int which, int lane) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(tile + f16_off(which, t, 4 * lane));
+    return make_float4(h2f((uint16_t)w.x), h2f((uint16_t)(w.x >> 16)), h2f((uint16_t)w.y), h2f((uint16_t)(w.y >> 16)));
+}
+// min + code * (range / levels), the parameters as stored (range in the low half word)
+__device__ __forceinline__ float tq_value(uint32_t code, float step, float mn) { return fmaf((float)code, step, mn); }
+
+template <>
+__device__ __forceinline__ float4 load_token<QWN_KV_CODEC_Q4_G32>(const uint8_t *tile, int t, int which, int lane) {
+    const int c = lane >> 3;
+    const uint32_t par = *reinterpret_cast<const uint32_t *>(tile + (which ? 2304 : 2048) + 32 * (t & 7) + 8 * c +
+                                                             4 * (t >> 3));
+    const float step = __fdiv_rn(h2f((uint16_t)par), 15.f), mn = h2f((uint16_t)(par >> 16));
+    uint32_t q[4];
+    if (!which) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + 64 * t + 16 * ((lane & 7) >> 1) + 4 * c) >>
+                           (4 * (lane & 1));
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = (w >> (8 * i)) & 15u;
+    } else {
+        const int mb = 2 * c + ((lane & 7) >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int lv = 4 * (4 * (lane & 1) + i) + ((t & 7) >> 1);
+            const int chunk = (mb >> 2) ^ ((lv >> 2) & 1);
+            const uint32_t b = tile[1024 + 32 * lv + 16 * chunk + 4 * (mb & 3) + (t >> 3) + 2 * (t & 1)];
+            q[i] = (b >> (2 * (lane & 2))) & 15u;
+        }
+    }
+    return make_float4(tq_value(q[0], step, mn), tq_value(q[1], step, mn), tq_value(q[2], step, mn),
+                       tq_value(q[3], step, mn));
+}
+
+// the code that tq35_put stored for dim d of token t
+__device__ __forceinline__ uint32_t tq35_get(const uint8_t *half, int which, int t, int d) {
+    const int x = d >> 6, m = (d & 63) >> 1;
+    uint32_t eb, ob, pb, n;
+    if (!which) {
+        const int tig = m >> 3;
+        n = (uint32_t)lb_k_nibble(m);
+        eb = 32 * t + 8 * tig + 4 * x;
+        ob = 512 + 16 * t + 4 * tig;
+        pb = 768 + 8 * t + 2 * tig;
+    } else {
+        const int c = 2 * x + (d & 1), r = m & 15, mb = 2 * c + (m >> 4);
+        const int lv = ((r & 7) << 2) | ((t & 7) >> 1);
+        n = (uint32_t)((r >> 3) + 2 * (t >> 3) + 4 * (t & 1));
+        eb = 16 * lv + 4 * (2 * x + (mb & 1));
+        ob = 512 + 8 * lv + 4 * (mb & 1);
+        pb = 768 + 4 * lv + 2 * (mb & 1);
+    }
+    if (!(d & 1)) return (half[eb + (n >> 1)] >> ((n & 1) * 4)) & 15u;
+    const uint32_t w = half[ob + (n >> 1)] >> ((n & 1) * 4);
+    if (x == 0) return w & 7u;
+    return ((w >> 3) & 1u) | (((half[pb + (n >> 2)] >> ((2 * n) & 7)) & 3u) << 1);
+}
+template <>
+__device__ __forceinline__ float4 load_token<QWN_KV_CODEC_TQ35_G64>(const uint8_t *tile, int t, int which, int lane) {
+    const uint8_t *half = tile + which * 1024;
+    const uint32_t par = *reinterpret_cast<const uint32_t *>(half + 896 + 16 * (t & 7) + 8 * (lane >> 4) +
+                                                             4 * (t >> 3));
+    const float range = h2f((uint16_t)par), mn = h2f((uint16_t)(par >> 16));
+    const float even = __fdiv_rn(range, 15.f), odd = __fdiv_rn(range, 7.f);
+    const int d = 4 * lane;
+    return make_float4(tq_value(tq35_get(half, which, t, d), even, mn), tq_value(tq35_get(half, which, t, d + 1), odd, mn),
+                       tq_value(tq35_get(half, which, t, d + 2), even, mn),
+                       tq_value(tq35_get(half, which, t, d + 3), odd, mn));
 }
 
 }  // namespace

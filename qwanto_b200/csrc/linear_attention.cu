@@ -42,18 +42,6 @@ constexpr int kLaWarps = 8;   // row stripes (decode producers, prefill stages)
 constexpr int kLaThreads = kLaCols * kLaWarps;
 constexpr int kLaMaxDim = 512;
 
-struct DeviceScope {
-    int prev = -1;
-    explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) cudaSetDevice(dev);
-    }
-    ~DeviceScope() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
-
 // ---------------------------------------------------------------------------
 // Decode.  A persistent CTA walks units (head, 32-column block) with a stride
 // of the grid.  Warps 0..7 produce: for their rows i = w, w+8, ... they load

@@ -1,0 +1,39 @@
+// Rows of fp32, fp16 and bf16 in device memory: loads and stores through fp32,
+// and the checks that the entry points taking such rows share.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "kv_internal.cuh"
+
+namespace qkv {
+namespace {
+
+// four consecutive values of a row, in fp32
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const __half *p) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(h2f((uint16_t)w.x), h2f((uint16_t)(w.x >> 16)), h2f((uint16_t)w.y), h2f((uint16_t)(w.y >> 16)));
+}
+__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+__device__ __forceinline__ void store4(__half *p, float4 v) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+}
+
+inline bool dtype_ok(uint32_t d) { return d == QWN_DTYPE_F32 || d == QWN_DTYPE_F16 || d == QWN_DTYPE_BF16; }
+inline int invalid(const char *msg) {
+    set_error(msg);
+    return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+}
+
+}  // namespace
+}  // namespace qkv
