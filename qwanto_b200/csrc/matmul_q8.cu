@@ -5,25 +5,41 @@
 // host activations and 2-bit weights (c/cuda/qwn_hypervsq2_cuda_abi.cu); this
 // one keeps both sides on the device.
 //
+// Both kernels give the tensor core the weights as its A operand (128 outputs
+// per CTA on TMEM's lanes) and the tokens as B (the columns), so that a few
+// tokens cost a narrow MMA and a warp's lanes write consecutive outputs.
+// Operand tiles are 128 codes deep, loaded by TMA with 128-byte swizzle.
 // Weights are copied once into rows of a multiple of 128 bytes, zero past
-// in_features, so a product never branches on in_features' remainder.
+// in_features, so a product never branches on in_features' remainder; TMA
+// fills what lies outside the codes with zeros.
+#include <algorithm>
 #include <cstring>
+#include <map>
 #include <new>
+#include <type_traits>
+#include <utility>
 
 #include "kv_internal.cuh"
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace qkv {
 namespace {
 
-constexpr uint32_t kMmK = 128;  // bytes of a weight row's granule
+constexpr uint32_t kMmK = 128;       // codes per operand tile row: one swizzled row
+constexpr uint32_t kMmRows = 128;    // outputs (weight rows) per CTA
+constexpr uint32_t kWBytes = kMmRows * kMmK;
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMmThreads = 192; // TMA warp, MMA warp, four warps that read TMEM
+constexpr uint32_t kMaxSplit = 8;    // CTAs of a cluster that share an output tile
 
 struct MatmulQ8 {
-    int device = 0;
+    int device = 0, sms = 148;
     uint32_t n = 0, k = 0, kpad = 0;
     int8_t *w = nullptr;
     float *scales = nullptr, *bias = nullptr;
     uint32_t *status = nullptr;
+    CUtensorMap wmap;
 };
 
 MatmulQ8 *matmul_from(const QwnMatmulQ8Handle *h) {
@@ -40,70 +56,382 @@ void matmul_release(MatmulQ8 *m) {
 }
 
 struct MmArgs {
-    const int8_t *x, *w;
     const float *sx, *sw, *bias;
     void *out;
-    uint64_t x_stride, out_stride;
-    uint32_t m, n, k, kpad, out_dtype;
+    uint64_t out_stride;
+    uint32_t m, n, kblocks;
+    uint32_t *status;
 };
 
-__device__ __forceinline__ void store_out(const MmArgs &a, uint32_t row, uint32_t col, float v) {
-    const size_t o = (size_t)row * a.out_stride + col;
-    if (a.out_dtype == QWN_DTYPE_F32) static_cast<float *>(a.out)[o] = v;
-    else if (a.out_dtype == QWN_DTYPE_F16) static_cast<__half *>(a.out)[o] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(a.out)[o] = __float2bfloat16_rn(v);
+template <typename T>
+__device__ __forceinline__ void store_out(T *p, float v) {
+    if constexpr (std::is_same_v<T, float>) *p = v;
+    else if constexpr (std::is_same_v<T, __half>) *p = __float2half_rn(v);
+    else *p = __float2bfloat16_rn(v);
+}
+// one rounding for the sum (beyond 2^24) and one for each factor, in fp32; then the output's
+__device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias) {
+    return fmaf((float)sum * sx, sw, bias);
 }
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, dot products of four codes at a time
-constexpr int kSimpleTile = 64, kSimpleK = 64;
-__global__ void __launch_bounds__(256) matmul_q8_simple_kernel(MmArgs a) {
-    __shared__ int xs[kSimpleTile][kSimpleK / 4 + 1], ws[kSimpleTile][kSimpleK / 4 + 1];
-    const uint32_t m0 = blockIdx.y * kSimpleTile, n0 = blockIdx.x * kSimpleTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < a.kpad; k0 += kSimpleK) {
-        for (int i = threadIdx.x; i < kSimpleTile * kSimpleK / 4; i += 256) {
-            const int r = i / (kSimpleK / 4), c = i % (kSimpleK / 4);
-            const uint32_t kk = k0 + 4 * c;
-            int xv = 0, wv = 0;
-            if (m0 + r < a.m && kk < a.k) {
-                const int8_t *p = a.x + (size_t)(m0 + r) * a.x_stride + kk;
-                if (kk + 4 <= a.k) xv = *reinterpret_cast<const int *>(p);
-                else
-                    for (uint32_t j = 0; kk + j < a.k; j++) xv |= (int)((uint32_t)(uint8_t)p[j] << (8 * j));
+// ---------------------------------------------------------------------------
+// Few tokens: bound by the weights' bytes.  One CTA per 128 outputs, tile of
+// `nt` tokens and share of k; the cluster's CTAs take a share of k each, so
+// that a few hundred outputs already load from every SM.  Their int32 sums
+// meet in shared memory: CTA r adds the partial sums of its share of the
+// tokens over the cluster (exact in any order) and writes them.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kMmThreads) matmul_q8_split_kernel(const __grid_constant__ CUtensorMap wmap,
+                                                                     const __grid_constant__ CUtensorMap xmap,
+                                                                     MmArgs a, uint32_t nt, uint32_t splits,
+                                                                     uint32_t stages, uint32_t columns) {
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ uint32_t tmem_at;
+    __shared__ int issued, gave_up;
+    __shared__ float sx[256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t rank = splits > 1 ? cluster_rank() : 0;
+    const uint32_t n0 = blockIdx.x / splits * kMmRows, m0 = blockIdx.y * nt;
+    const uint32_t kb0 = (uint32_t)((uint64_t)a.kblocks * rank / splits);
+    const uint32_t kb1 = (uint32_t)((uint64_t)a.kblocks * (rank + 1) / splits);
+    const uint32_t count = kb1 - kb0, stage_bytes = kWBytes + nt * kMmK;
+    const uint32_t valid = min(nt, a.m - m0);  // tokens of this tile that exist
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < stages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&done, 1);
+        issued = gave_up = 0;
+        fence_barrier_init();
+        tma_prefetch(&wmap);
+        tma_prefetch(&xmap);
+    }
+    if (warp == 1) tmem_alloc<1>(&tmem_at, columns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        uint32_t i = 0;
+        for (; i < count; i++) {
+            const uint32_t s = i % stages;
+            if (i >= stages && !mbar_wait_bounded(&empty[s], (i / stages - 1) & 1)) { ok = false; break; }
+            mbar_expect_tx(&full[s], stage_bytes);
+            const uint32_t dst = base + s * stage_bytes;
+            const int x = (int)((kb0 + i) * kMmK);
+            tma_load(dst, &wmap, x, (int)n0, smem_u32(&full[s]));
+            tma_load(dst + kWBytes, &xmap, x, (int)m0, smem_u32(&full[s]));
+        }
+        issued = (int)i;
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t desc = i8_desc(kMmRows, nt);
+        for (uint32_t i = 0; i < count; i++) {
+            const uint32_t s = i % stages;
+            if (!mbar_wait_bounded(&full[s], (i / stages) & 1)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t wd = smem_desc(base + s * stage_bytes), xd = smem_desc(base + s * stage_bytes + kWBytes);
+#pragma unroll
+            for (int j = 0; j < (int)kMmK / 32; j++)  // 32 codes further: 32 bytes of the swizzled row
+                mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, desc, i > 0 || j > 0);
+            mma_commit(&empty[s]);
+        }
+        mma_commit(&done);
+    }
+    if (warp >= 2) {
+        for (uint32_t c = threadIdx.x - 64; c < valid; c += 128) sx[c] = a.sx[m0 + c];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        ok = mbar_wait_bounded(&done, 0);
+        tc_fence_after();
+    }
+    if (!ok) {
+        gave_up = 1;
+        latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
+    }
+    __syncwarp();
+    const uint32_t quarter = warp & 3, feature = quarter * 32 + lane;  // TMEM lanes this warp may read
+    const uint32_t lanes = tmem + (quarter << 21);
+    const uint32_t n = n0 + feature;
+    const float sw = n < a.n ? a.sw[n] : 0.f, bias = a.bias && n < a.n ? a.bias[n] : 0.f;
+    T *out = static_cast<T *>(a.out) + n;
+    if (splits == 1) {
+        if (warp >= 2 && ok) {
+            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
+                uint32_t v[16];
+                tmem_load16(v, lanes + c0);
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++)
+                    if (c0 + i < valid && n < a.n)
+                        store_out(out + (uint64_t)(m0 + c0 + i) * a.out_stride, scaled((int)v[i], sx[c0 + i], sw, bias));
             }
-            if (n0 + r < a.n) wv = *reinterpret_cast<const int *>(a.w + (size_t)(n0 + r) * a.kpad + kk);
-            xs[r][c] = xv;
-            ws[r][c] = wv;
         }
-        __syncthreads();
+    } else {
+        // partial sums [token][128 outputs] over the operand tiles, which the MMAs have finished with
+        if (warp >= 2) {
+            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
+                uint32_t v[16];
+                tmem_load16(v, lanes + c0);
 #pragma unroll
-        for (int c = 0; c < kSimpleK / 4; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[ty + 16 * i][c], ws[tx + 16 * j][c], acc[i][j]);
-        __syncthreads();
+                for (uint32_t i = 0; i < 16; i++)
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + ((c0 + i) * kMmRows + feature) * 4), "r"(v[i])
+                                 : "memory");
+            }
+        }
+        cluster_sync();
+        if (warp >= 2 && n < a.n) {
+            const uint32_t c_end = valid * (rank + 1) / splits;
+            for (uint32_t c = valid * rank / splits; c < c_end; c++) {
+                const uint32_t at = base + (c * kMmRows + feature) * 4;
+                int sum = 0;
+                for (uint32_t p = 0; p < splits; p++) sum += ld_cluster(cluster_addr(at, p));
+                store_out(out + (uint64_t)(m0 + c) * a.out_stride, scaled(sum, sx[c], sw, bias));
+            }
+        }
+        cluster_sync();  // this CTA's partial sums stay until the others have read them
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t row = m0 + ty + 16 * i;
-        if (row >= a.m) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t col = n0 + tx + 16 * j;
-            if (col >= a.n) continue;
-            const float v = (float)acc[i][j] * a.sx[row] * a.sw[col];
-            store_out(a, row, col, a.bias ? v + a.bias[col] : v);
-        }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (gave_up && threadIdx.x == 0)  // copies in flight land before the memory goes
+        for (uint32_t i = issued > (int)stages ? (uint32_t)issued - stages : 0; i < (uint32_t)issued; i++)
+            mbar_wait_bounded(&full[i % stages], (i / stages) & 1);
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free<1>(tmem, columns);
     }
 }
 
-cudaError_t launch_matmul(const MmArgs &a, cudaStream_t s) {
-    const dim3 grid((a.n + kSimpleTile - 1) / kSimpleTile, (a.m + kSimpleTile - 1) / kSimpleTile);
-    matmul_q8_simple_kernel<<<grid, 256, 0, s>>>(a);
-    count_launch();
-    return cudaGetLastError();
+// ---------------------------------------------------------------------------
+// Many tokens: bound by the tensor core.  A pair of CTAs on two SMs shares
+// 256 outputs x `nt` tokens: each CTA brings its 128 weight rows and half of
+// the tokens, one tcgen05.mma of both SMs multiplies them, and each CTA's TMEM
+// receives its 128 outputs.  Pairs stay resident and walk over the tiles; two
+// accumulators let the TMEM warps write one tile while the next is multiplied.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kPairStages = 6;
+constexpr uint32_t kPairTokens = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __grid_constant__ CUtensorMap wmap,
+                                                                       const __grid_constant__ CUtensorMap xmap,
+                                                                       MmArgs a, uint32_t nt, uint32_t m_tiles,
+                                                                       uint32_t tiles) {
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_at;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1;
+    const uint32_t half = nt / 2, stage_bytes = kWBytes + half * kMmK;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kPairStages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 8);  // the TMEM warps of both CTAs
+        }
+        fence_barrier_init();
+        tma_prefetch(&wmap);
+        tma_prefetch(&xmap);
+    }
+    if (warp == 1) tmem_alloc<2>(&tmem_at, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers exist
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        uint32_t i = 0;
+        for (uint32_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
+            const int n0 = (int)(t / m_tiles * 2 * kMmRows + rank * kMmRows);
+            const int m0 = (int)(t % m_tiles * nt + rank * half);
+            for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
+                const uint32_t s = i % kPairStages;
+                if (i >= kPairStages && !mbar_wait_cluster(&empty[s], (i / kPairStages - 1) & 1)) { ok = false; break; }
+                if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);  // this CTA's bytes and the other's
+                const uint32_t bar = cluster_addr(smem_u32(&full[s]), 0);
+                const uint32_t dst = base + s * stage_bytes;
+                tma_load_pair(dst, &wmap, (int)(kb * kMmK), n0, bar);
+                tma_load_pair(dst + kWBytes, &xmap, (int)(kb * kMmK), m0, bar);
+            }
+        }
+        if (!ok && rank == 0)  // the copies in flight land before the memory goes
+            for (uint32_t j = i > kPairStages ? i - kPairStages : 0; j < i; j++)
+                mbar_wait_cluster(&full[j % kPairStages], (j / kPairStages) & 1);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        const uint32_t desc = i8_desc(2 * kMmRows, nt);
+        uint32_t i = 0, n = 0;
+        for (uint32_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs, n++) {
+            const uint32_t buf = n & 1, d = tmem + buf * kPairTokens;
+            if (n >= 2 && !mbar_wait_cluster(&acc_empty[buf], (n / 2 - 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+            for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
+                const uint32_t s = i % kPairStages;
+                if (!mbar_wait_cluster(&full[s], (i / kPairStages) & 1)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t wd = smem_desc(base + s * stage_bytes), xd = smem_desc(base + s * stage_bytes + kWBytes);
+#pragma unroll
+                for (int j = 0; j < (int)kMmK / 32; j++) mma_i8<2>(d, wd + 2 * j, xd + 2 * j, desc, kb > 0 || j > 0);
+                mma_commit_pair(&empty[s]);
+            }
+            mma_commit_pair(&acc_full[buf]);
+        }
+    } else if (warp >= 2) {
+        const uint32_t quarter = warp & 3;
+        uint32_t n = 0;
+        for (uint32_t t = blockIdx.x >> 1; t < tiles; t += pairs, n++) {
+            const uint32_t buf = n & 1, m0 = t % m_tiles * nt, valid = min(nt, a.m - m0);
+            const uint32_t col = t / m_tiles * 2 * kMmRows + rank * kMmRows + quarter * 32 + lane;
+            const bool in = col < a.n;
+            const float sw = in ? a.sw[col] : 0.f, bias = a.bias && in ? a.bias[col] : 0.f;
+            float sx[kPairTokens / 32];
+#pragma unroll
+            for (uint32_t j = 0; j < kPairTokens / 32; j++) sx[j] = j * 32 + lane < valid ? a.sx[m0 + j * 32 + lane] : 0.f;
+            if (!mbar_wait_cluster(&acc_full[buf], (n / 2) & 1)) { ok = false; break; }
+            tc_fence_after();
+            T *out = static_cast<T *>(a.out) + (uint64_t)m0 * a.out_stride + col;
+#pragma unroll
+            for (uint32_t j = 0; j < kPairTokens / 32; j++) {
+                if (j * 32 < valid) {
+                    uint32_t v[32];
+                    tmem_load32(v, tmem + (quarter << 21) + buf * kPairTokens + j * 32);
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i++) {
+                        const float s = __shfl_sync(0xffffffffu, sx[j], i);
+                        if (in && j * 32 + i < valid) store_out(out, scaled((int)v[i], s, sw, bias));
+                        out += a.out_stride;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acc_empty[buf]), 0));
+        }
+    }
+    if (!ok) latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    cluster_sync();  // neither CTA's memory or barriers go while the other may still use them
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free<2>(tmem, 512);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+
+// the driver's encoder, found once (the library does not link libcuda)
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess || found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// codes [rows][width], `stride` bytes apart, in tiles of box x 128
+bool encode_codes(CUtensorMap *map, const int8_t *p, uint64_t width, uint64_t rows, uint64_t stride, uint32_t box) {
+    const EncodeFn fn = encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {width, rows}, strides[1] = {stride};
+    const cuuint32_t tile[2] = {kMmK, box}, steps[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), dims, strides, tile, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr uint32_t kMmSmem = 227 * 1024 - 4096;  // dynamic, beside the static part
+
+template <typename K>
+cudaError_t allow_all_smem(K kernel) {
+    static std::mutex mu;
+    static std::map<std::pair<const void *, int>, bool> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lk(mu);
+    bool &have = done[{reinterpret_cast<const void *>(kernel), dev}];
+    if (have) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmSmem);
+    have = e == cudaSuccess;
+    return e;
+}
+
+template <typename K, typename... Args>
+cudaError_t launch_clusters(K kernel, dim3 grid, uint32_t cluster, size_t smem, cudaStream_t s, Args... args) {
+    cudaError_t e = allow_all_smem(kernel);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kMmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+
+// how a product is cut up
+struct MmPlan {
+    bool pair;
+    uint32_t nt, splits, stages;
+};
+MmPlan plan_matmul(uint32_t m, uint32_t n, uint32_t kblocks, uint32_t sms) {
+    MmPlan p{};
+    const uint32_t n_tiles = (n + kMmRows - 1) / kMmRows;
+    if (m > 256) {
+        p.pair = true;
+        const uint32_t m_tiles = (m + kPairTokens - 1) / kPairTokens;
+        p.nt = std::max(32u, ((m + m_tiles - 1) / m_tiles + 31) / 32 * 32);
+        return p;
+    }
+    p.nt = (m + 15) / 16 * 16;
+    p.splits = 1;
+    while (p.splits * 2 <= kMaxSplit && p.splits * 2 <= kblocks && n_tiles * p.splits * 2 <= sms) p.splits *= 2;
+    const uint32_t stage = kWBytes + p.nt * kMmK;
+    p.stages = std::min(kMaxStages, (kMmSmem - 1024) / stage);
+    return p;
+}
+
+template <typename T>
+cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, uint64_t x_stride, cudaStream_t s) {
+    const MmPlan p = plan_matmul(a.m, a.n, a.kblocks, (uint32_t)mm.sms);
+    const uint32_t n_tiles = (a.n + kMmRows - 1) / kMmRows;
+    CUtensorMap xmap;
+    if (!encode_codes(&xmap, x, mm.k, a.m, x_stride, p.pair ? p.nt / 2 : p.nt)) return cudaErrorInvalidValue;
+    if (p.pair) {
+        const uint32_t m_tiles = (a.m + p.nt - 1) / p.nt, tiles = (n_tiles + 1) / 2 * m_tiles;
+        const uint32_t pairs = std::min(tiles, (uint32_t)mm.sms / 2);
+        const size_t smem = 1024 + (size_t)kPairStages * (kWBytes + p.nt / 2 * kMmK);
+        return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, mm.wmap, xmap, a, p.nt, m_tiles,
+                               tiles);
+    }
+    uint32_t columns = 32;
+    while (columns < p.nt) columns *= 2;
+    const size_t smem = 1024 + std::max((size_t)p.stages * (kWBytes + p.nt * kMmK),
+                                        p.splits > 1 ? (size_t)p.nt * kMmRows * 4 : 0);
+    return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, (a.m + p.nt - 1) / p.nt), p.splits, smem,
+                           s, mm.wmap, xmap, a, p.nt, p.splits, p.stages, columns);
 }
 
 }  // namespace
@@ -131,6 +459,7 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
     m->n = o->out_features;
     m->k = o->in_features;
     m->kpad = (o->in_features + kMmK - 1) / kMmK * kMmK;
+    cudaDeviceGetAttribute(&m->sms, cudaDevAttrMultiProcessorCount, m->device);
     cudaStream_t s = static_cast<cudaStream_t>(o->stream);
     const size_t wb = (size_t)m->n * m->kpad, fb = (size_t)m->n * sizeof(float);
     if (cudaMalloc(&m->w, wb) != cudaSuccess || cudaMalloc(&m->scales, fb) != cudaSuccess ||
@@ -151,6 +480,11 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
         set_cuda_error("qwn_matmul_q8_create: copy", e);
         matmul_release(m);
         return QWN_CUDA_STATUS_RUNTIME_ERROR;
+    }
+    if (!encode_codes(&m->wmap, m->w, m->kpad, m->n, m->kpad, kMmRows)) {
+        set_error("qwn_matmul_q8_create: the driver has no tensor maps");
+        matmul_release(m);
+        return QWN_CUDA_STATUS_UNSUPPORTED;
     }
     std::memset(out, 0, sizeof(*out));
     qwn_cuda_abi_header_init(&out->header, sizeof(*out));
@@ -184,11 +518,16 @@ QWN_CUDA_ABI_API int qwn_matmul_q8(QwnMatmulQ8Handle *h, const QwnMatmulQ8Reques
     DeviceScope scope(m->device);
     if (!scope.ok) return scope.fail("qwn_matmul_q8");
     MmArgs a{};
-    a.x = r->codes_dev, a.w = m->w;
     a.sx = r->scales_dev, a.sw = m->scales, a.bias = m->bias;
-    a.out = r->out_dev, a.out_stride = os, a.x_stride = xs;
-    a.m = r->rows, a.n = m->n, a.k = m->k, a.kpad = m->kpad, a.out_dtype = r->out_dtype;
-    const cudaError_t e = launch_matmul(a, static_cast<cudaStream_t>(r->stream));
+    a.out = r->out_dev, a.out_stride = os;
+    a.m = r->rows, a.n = m->n, a.kblocks = m->kpad / kMmK;
+    a.status = m->status;
+    cudaStream_t s = static_cast<cudaStream_t>(r->stream);
+    const uint64_t stride = (xs + 15) / 16 * 16;  // of a single row: any
+    cudaError_t e;
+    if (r->out_dtype == QWN_DTYPE_F32) e = launch_matmul<float>(*m, a, r->codes_dev, stride, s);
+    else if (r->out_dtype == QWN_DTYPE_F16) e = launch_matmul<__half>(*m, a, r->codes_dev, stride, s);
+    else e = launch_matmul<__nv_bfloat16>(*m, a, r->codes_dev, stride, s);
     if (e != cudaSuccess) { set_cuda_error("qwn_matmul_q8", e); return QWN_CUDA_STATUS_RUNTIME_ERROR; }
     return QWN_CUDA_STATUS_OK;
 }
