@@ -2633,8 +2633,9 @@ cudaError_t launch_attention(Pool *p, const AttnLaunch &a, cudaStream_t s) {
     // Early start.  Every other kernel of this library is an ordinary launch
     // (the next launch waits for it to finish) -- except seq_append_kernel,
     // which lets the next launch start at once and therefore clears
-    // last_attn, so that the launch after it is never early -- so this
-    // attention kernel can overlap only an attention kernel of the stream that
+    // last_attn, and those that note_early_trigger() counts, after which the
+    // count differs from the last attention launch's: the launch after either
+    // is never early -- so this attention kernel can overlap only an attention kernel of the stream that
     // precedes it directly.  That kernel writes its layer's newest-token tiles, its output
     // rows, the pool's partial slots, counters and plans.  When the previous
     // attention launch of this pool on this stream was of another layer,
@@ -2664,11 +2665,13 @@ cudaError_t launch_attention(Pool *p, const AttnLaunch &a, cudaStream_t s) {
         }
         const Pool::LastAttention &L = p->last_attn;
         auto clear = [&](uintptr_t lo, size_t n) { return lo + n <= L.out_lo || lo >= L.out_hi; };
-        A.early = eligible && L.valid && !L.recorded && L.stream == s && L.layer != a.layer && clear(q0, qbytes) &&
+        const uint64_t triggers = g_early_triggers.load(std::memory_order_relaxed);
+        A.early = eligible && L.valid && L.triggers == triggers && !L.recorded && L.stream == s && L.layer != a.layer && clear(q0, qbytes) &&
                   clear(o0, qbytes) && (!a.new_k || (clear(k0, kvbytes) && clear(v0, kvbytes)));
         p->last_attn.valid = eligible;
         p->last_attn.recorded = records;
         p->last_attn.stream = s;
+        p->last_attn.triggers = triggers;
         p->last_attn.layer = a.layer;
         p->last_attn.out_lo = o0;
         p->last_attn.out_hi = o0 + qbytes;

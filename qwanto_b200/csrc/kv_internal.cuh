@@ -48,6 +48,13 @@ struct DeviceScope {
     }
 };
 
+// Launches of kernels (other than attention) that let the stream's next kernel
+// start before they end.  An attention launch that follows one must not read
+// anything before its dependency wait, so it compares this count with the one
+// its pool's previous attention launch saw.
+extern std::atomic<uint64_t> g_early_triggers;
+inline void note_early_trigger() { g_early_triggers.fetch_add(1, std::memory_order_relaxed); }
+
 inline bool header_ok(const QwnCudaAbiHeader &h, size_t expected) {
     return h.abi_version == QWN_CUDA_ABI_VERSION && h.struct_size >= expected;
 }
@@ -111,6 +118,7 @@ struct Pool {
         cudaStream_t stream = nullptr;
         uint32_t layer = 0;
         uintptr_t out_lo = 0, out_hi = 0;
+        uint64_t triggers = 0;  // g_early_triggers at that launch
     } last_attn;
     // host mirror of the plan records' key: plan_valid is cleared by every
     // launch that changes lengths or tables (the device epoch moves)
@@ -265,6 +273,11 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
+
+// programmatic launches: the stream's next kernel may start; wait until the
+// previous one has finished and its writes are visible
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t atom_add_acq_rel_gpu(uint32_t *p, uint32_t v) {
     uint32_t old;

@@ -13,6 +13,7 @@
 namespace qkv {
 
 std::atomic<uint64_t> g_launches{0};
+std::atomic<uint64_t> g_early_triggers{0};
 static std::mutex g_err_mu;
 static std::string g_last_error;
 

@@ -9,9 +9,16 @@
 // per CTA on TMEM's lanes) and the tokens as B (the columns), so that a few
 // tokens cost a narrow MMA and a warp's lanes write consecutive outputs.
 // Operand tiles are 128 codes deep, loaded by TMA with 128-byte swizzle.
-// Weights are copied once into rows of a multiple of 128 bytes, zero past
-// in_features, so a product never branches on in_features' remainder; TMA
-// fills what lies outside the codes with zeros.
+// The handle keeps the weights as [in/128][out][128], zero past in_features:
+// a tile of any number of outputs is one run of HBM, and a product never
+// branches on in_features' remainder; TMA fills what lies outside the codes
+// with zeros.  A CTA may take fewer than 128 outputs, where that spreads them
+// evenly over the SMs: the MMA then multiplies whatever follows the tile in
+// shared memory into lanes that nobody reads.
+//
+// Both kernels start while the stream's previous kernel still runs
+// (programmatic launch), fetch weights, and wait for it before they read codes
+// or scales or write anything.
 #include <algorithm>
 #include <cstring>
 #include <map>
@@ -27,19 +34,19 @@ namespace qkv {
 namespace {
 
 constexpr uint32_t kMmK = 128;       // codes per operand tile row: one swizzled row
-constexpr uint32_t kMmRows = 128;    // outputs (weight rows) per CTA
-constexpr uint32_t kWBytes = kMmRows * kMmK;
+constexpr uint32_t kMmRows = 128;    // lanes of a CTA's accumulator: at most so many outputs
 constexpr uint32_t kMaxStages = 12;
 constexpr uint32_t kMmThreads = 192; // TMA warp, MMA warp, four warps that read TMEM
 constexpr uint32_t kMaxSplit = 8;    // CTAs of a cluster that share an output tile
 
 struct MatmulQ8 {
     int device = 0, sms = 148;
-    uint32_t n = 0, k = 0, kpad = 0;
+    uint32_t n = 0, k = 0, kblocks = 0;
     int8_t *w = nullptr;
     float *scales = nullptr, *bias = nullptr;
     uint32_t *status = nullptr;
-    CUtensorMap wmap;
+    uint32_t clusters[kMaxSplit + 1] = {};  // clusters of each size that run at once, one CTA per SM
+    CUtensorMap wmap[kMmRows / 8];          // tiles of 8, 16, ... 128 outputs
 };
 
 MatmulQ8 *matmul_from(const QwnMatmulQ8Handle *h) {
@@ -55,11 +62,33 @@ void matmul_release(MatmulQ8 *m) {
     delete m;
 }
 
+// weight [n][k] (rows `stride` apart) into [k / 128][n][128], zeros outside; a thread moves 16 codes
+__global__ void __launch_bounds__(256) pack_weight_kernel(const int8_t *w, uint64_t stride, uint32_t n, uint32_t k,
+                                                          uint64_t chunks, int8_t *out) {
+    const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
+    const bool wide = ((uintptr_t)w | stride) % 16 == 0;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < chunks; i += step) {
+        const uint64_t row = i >> 3;
+        const uint32_t col = (uint32_t)(row / n) * kMmK + (uint32_t)(i & 7) * 16;
+        const int8_t *p = w + (row % n) * stride + col;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (wide && col + 16 <= k) {
+            v = *reinterpret_cast<const uint4 *>(p);
+        } else {
+            uint32_t q[4] = {};
+            for (uint32_t j = 0; j < 16 && col + j < k; j++) q[j >> 2] |= (uint32_t)(uint8_t)p[j] << (8 * (j & 3));
+            v = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+        reinterpret_cast<uint4 *>(out)[i] = v;
+    }
+}
+
 struct MmArgs {
     const float *sx, *sw, *bias;
     void *out;
     uint64_t out_stride;
     uint32_t m, n, kblocks;
+    uint32_t rows;  // outputs per CTA, a multiple of 8
     uint32_t *status;
 };
 
@@ -78,127 +107,164 @@ __device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias)
 // Few tokens: bound by the weights' bytes.  One CTA per 128 outputs, tile of
 // `nt` tokens and share of k; the cluster's CTAs take a share of k each, so
 // that a few hundred outputs already load from every SM.  Their int32 sums
-// meet in shared memory: CTA r adds the partial sums of its share of the
-// tokens over the cluster (exact in any order) and writes them.
+// meet in shared memory: CTA r receives the others' sums of its share of the
+// tokens, adds them (exact in any order) and writes them.
 // ---------------------------------------------------------------------------
+// bytes that CTA r receives: [splits][its tokens][128 outputs]
+__host__ __device__ constexpr uint32_t share_tokens(uint32_t nt, uint32_t splits) { return (nt + splits - 1) / splits; }
+__host__ __device__ constexpr uint32_t share_bytes(uint32_t nt, uint32_t splits) {
+    return splits > 1 ? splits * share_tokens(nt, splits) * kMmRows * 4 : 0;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kMmThreads) matmul_q8_split_kernel(const __grid_constant__ CUtensorMap wmap,
-                                                                     const __grid_constant__ CUtensorMap xmap,
-                                                                     MmArgs a, uint32_t nt, uint32_t splits,
-                                                                     uint32_t stages, uint32_t columns) {
+__global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __grid_constant__ CUtensorMap wmap,
+                                                                        const __grid_constant__ CUtensorMap xmap,
+                                                                        MmArgs a, uint32_t nt, uint32_t splits,
+                                                                        uint32_t stages, uint32_t columns) {
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_at;
-    __shared__ int issued, gave_up;
     __shared__ float sx[256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t rank = splits > 1 ? cluster_rank() : 0;
-    const uint32_t n0 = blockIdx.x / splits * kMmRows, m0 = blockIdx.y * nt;
+    const uint32_t n0 = blockIdx.x / splits * a.rows, m0 = blockIdx.y * nt;
     const uint32_t kb0 = (uint32_t)((uint64_t)a.kblocks * rank / splits);
     const uint32_t kb1 = (uint32_t)((uint64_t)a.kblocks * (rank + 1) / splits);
-    const uint32_t count = kb1 - kb0, stage_bytes = kWBytes + nt * kMmK;
+    const uint32_t w_bytes = a.rows * kMmK, stage_bytes = w_bytes + nt * kMmK, count = kb1 - kb0;
     const uint32_t valid = min(nt, a.m - m0);  // tokens of this tile that exist
+    launch_dependents();
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < stages; i++) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
         mbar_init(&done, 1);
-        issued = gave_up = 0;
         fence_barrier_init();
-        tma_prefetch(&wmap);
-        tma_prefetch(&xmap);
     }
     if (warp == 1) tmem_alloc<1>(&tmem_at, columns);
     tc_fence_before();
     __syncthreads();
+    if (splits > 1) cluster_arrive();  // this CTA runs: the others may write to it from their wait on
     tc_fence_after();
     const uint32_t tmem = tmem_at;
     bool ok = true;
-    if (warp == 0 && lane == 0) {
-        uint32_t i = 0;
+    if (warp == 0) {
+        const bool one = elect_one();
+        const uint32_t ahead = min(count, stages);
+        auto load_w = [&](uint32_t i, uint32_t st) {
+            mbar_expect_tx(&full[st], stage_bytes);
+            tma_load(base + st * stage_bytes, &wmap, 0, (int)((kb0 + i) * a.n + n0), smem_u32(&full[st]));
+        };
+        auto load_x = [&](uint32_t i, uint32_t st) {
+            tma_load(base + st * stage_bytes + w_bytes, &xmap, (int)((kb0 + i) * kMmK), (int)m0, smem_u32(&full[st]));
+        };
+        for (uint32_t i = 0; i < ahead; i++)
+            if (one) load_w(i, i);
+        wait_previous();
+        for (uint32_t i = 0; i < ahead; i++)
+            if (one) load_x(i, i);
+        Ring r;
+        uint32_t i = ahead;
         for (; i < count; i++) {
-            const uint32_t s = i % stages;
-            if (i >= stages && !mbar_wait_bounded(&empty[s], (i / stages - 1) & 1)) { ok = false; break; }
-            mbar_expect_tx(&full[s], stage_bytes);
-            const uint32_t dst = base + s * stage_bytes;
-            const int x = (int)((kb0 + i) * kMmK);
-            tma_load(dst, &wmap, x, (int)n0, smem_u32(&full[s]));
-            tma_load(dst + kWBytes, &xmap, x, (int)m0, smem_u32(&full[s]));
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[r.stage], r.parity));
+            if (!ok) break;
+            if (one) {
+                load_w(i, r.stage);
+                load_x(i, r.stage);
+            }
+            r.next(stages);
         }
-        issued = (int)i;
-    } else if (warp == 1 && lane == 0) {
+        if (!ok && one)  // the copies in flight land before the memory goes
+            for (uint32_t j = i - stages; j < i; j++) mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
+    } else if (warp == 1) {
+        const bool one = elect_one();
         const uint32_t desc = i8_desc(kMmRows, nt);
+        const uint64_t first = smem_desc(base);
+        Ring r;
         for (uint32_t i = 0; i < count; i++) {
-            const uint32_t s = i % stages;
-            if (!mbar_wait_bounded(&full[s], (i / stages) & 1)) { ok = false; break; }
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[r.stage], r.parity));
+            if (!ok) break;
             tc_fence_after();
-            const uint64_t wd = smem_desc(base + s * stage_bytes), xd = smem_desc(base + s * stage_bytes + kWBytes);
-#pragma unroll
-            for (int j = 0; j < (int)kMmK / 32; j++)  // 32 codes further: 32 bytes of the swizzled row
-                mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, desc, i > 0 || j > 0);
-            mma_commit(&empty[s]);
+            const uint64_t wd = first + ((r.stage * stage_bytes) >> 4);
+            if (one) {
+                mma_tile<1>(tmem, wd, wd + (w_bytes >> 4), desc, i > 0);
+                mma_commit(&empty[r.stage]);
+            }
+            r.next(stages);
         }
-        mma_commit(&done);
+        if (one) mma_commit(&done);
     }
+    const uint32_t quarter = warp & 3, feature = quarter * 32 + lane;  // TMEM lanes this warp may read
+    const uint32_t lanes = tmem + (quarter << 21);
+    const uint32_t n = n0 + feature;
+    const bool in = feature < a.rows && n < a.n;
+    float sw = 0.f, bias = 0.f;
+    T *out = static_cast<T *>(a.out) + (uint64_t)m0 * a.out_stride + n;
     if (warp >= 2) {
+        if (in) sw = a.sw[n];
+        if (in && a.bias) bias = a.bias[n];
+        wait_previous();
         for (uint32_t c = threadIdx.x - 64; c < valid; c += 128) sx[c] = a.sx[m0 + c];
         asm volatile("bar.sync 1, 128;" ::: "memory");
         ok = mbar_wait_bounded(&done, 0);
         tc_fence_after();
     }
-    if (!ok) {
-        gave_up = 1;
-        latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
-    }
+    if (!ok) latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
     __syncwarp();
-    const uint32_t quarter = warp & 3, feature = quarter * 32 + lane;  // TMEM lanes this warp may read
-    const uint32_t lanes = tmem + (quarter << 21);
-    const uint32_t n = n0 + feature;
-    const float sw = n < a.n ? a.sw[n] : 0.f, bias = a.bias && n < a.n ? a.bias[n] : 0.f;
-    T *out = static_cast<T *>(a.out) + n;
     if (splits == 1) {
-        if (warp >= 2 && ok) {
-            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
-                uint32_t v[16];
-                tmem_load16(v, lanes + c0);
-#pragma unroll
-                for (uint32_t i = 0; i < 16; i++)
-                    if (c0 + i < valid && n < a.n)
-                        store_out(out + (uint64_t)(m0 + c0 + i) * a.out_stride, scaled((int)v[i], sx[c0 + i], sw, bias));
-            }
-        }
-    } else {
-        // partial sums [token][128 outputs] over the operand tiles, which the MMAs have finished with
         if (warp >= 2) {
             for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
                 uint32_t v[16];
                 tmem_load16(v, lanes + c0);
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i++)
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + ((c0 + i) * kMmRows + feature) * 4), "r"(v[i])
-                                 : "memory");
+                for (uint32_t i = 0; i < 16; i++) {
+                    if (in && c0 + i < valid) store_out(out, scaled((int)v[i], sx[c0 + i], sw, bias));
+                    out += a.out_stride;
+                }
+            }
+        }
+    } else {
+        const uint32_t share = share_tokens(valid, splits);
+        const uint32_t region = base + stages * stage_bytes;
+        cluster_wait();
+        if (warp >= 2) {
+            // this CTA's sums of token c go to the CTA of c's share
+            const uint32_t mine = region + (rank * share * kMmRows + feature) * 4;
+            uint32_t owner = 0, left = share, to = cluster_addr(mine, 0);
+            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
+                uint32_t v[16];
+                tmem_load16(v, lanes + c0);
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++) {
+                    if (c0 + i >= valid) break;
+                    if (left == 0) {
+                        left = share;
+                        to = cluster_addr(mine, ++owner);
+                    }
+                    st_cluster(to, v[i]);
+                    to += kMmRows * 4;
+                    left--;
+                }
             }
         }
         cluster_sync();
-        if (warp >= 2 && n < a.n) {
-            const uint32_t c_end = valid * (rank + 1) / splits;
-            for (uint32_t c = valid * rank / splits; c < c_end; c++) {
-                const uint32_t at = base + (c * kMmRows + feature) * 4;
+        if (warp >= 2 && in) {
+            const uint32_t first = rank * share, mine = first < valid ? min(share, valid - first) : 0;
+            out += (uint64_t)first * a.out_stride;
+            for (uint32_t c = 0; c < mine; c++) {
                 int sum = 0;
-                for (uint32_t p = 0; p < splits; p++) sum += ld_cluster(cluster_addr(at, p));
-                store_out(out + (uint64_t)(m0 + c) * a.out_stride, scaled(sum, sx[c], sw, bias));
+#pragma unroll
+                for (uint32_t p = 0; p < kMaxSplit; p++)
+                    if (p < splits) sum += ld_shared(region + ((p * share + c) * kMmRows + feature) * 4);
+                store_out(out, scaled(sum, sx[first + c], sw, bias));
+                out += a.out_stride;
             }
         }
-        cluster_sync();  // this CTA's partial sums stay until the others have read them
     }
     tc_fence_before();
     __syncwarp();
     __syncthreads();
-    if (gave_up && threadIdx.x == 0)  // copies in flight land before the memory goes
-        for (uint32_t i = issued > (int)stages ? (uint32_t)issued - stages : 0; i < (uint32_t)issued; i++)
-            mbar_wait_bounded(&full[i % stages], (i / stages) & 1);
     if (warp == 1) {
         tc_fence_after();
         tmem_free<1>(tmem, columns);
@@ -226,7 +292,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1;
-    const uint32_t half = nt / 2, stage_bytes = kWBytes + half * kMmK;
+    const uint32_t half = nt / 2, w_bytes = a.rows * kMmK, stage_bytes = w_bytes + half * kMmK;
+    launch_dependents();
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kPairStages; i++) {
             mbar_init(&full[i], 1);
@@ -237,8 +304,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
             mbar_init(&acc_empty[i], 8);  // the TMEM warps of both CTAs
         }
         fence_barrier_init();
-        tma_prefetch(&wmap);
-        tma_prefetch(&xmap);
     }
     if (warp == 1) tmem_alloc<2>(&tmem_at, 512);
     tc_fence_before();
@@ -247,49 +312,75 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     tc_fence_after();
     const uint32_t tmem = tmem_at;
     bool ok = true;
-    if (warp == 0 && lane == 0) {
-        uint32_t i = 0;
-        for (uint32_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
-            const int n0 = (int)(t / m_tiles * 2 * kMmRows + rank * kMmRows);
-            const int m0 = (int)(t % m_tiles * nt + rank * half);
+    if (warp == 0) {
+        const bool one = elect_one();
+        const uint32_t bars = cluster_addr(smem_u32(full), 0);  // the first CTA's barriers count both CTAs' bytes
+        auto load_w = [&](uint32_t kb, uint32_t row, uint32_t st) {
+            if (rank == 0) mbar_expect_tx(&full[st], 2 * stage_bytes);
+            tma_load_pair(base + st * stage_bytes, &wmap, 0, (int)(kb * a.n + row), bars + 8 * st);
+        };
+        auto load_x = [&](uint32_t kb, uint32_t row, uint32_t st) {
+            tma_load_pair(base + st * stage_bytes + w_bytes, &xmap, (int)(kb * kMmK), (int)row, bars + 8 * st);
+        };
+        const uint32_t ahead = min(a.kblocks, kPairStages);  // weights of the first tile
+        uint32_t t = blockIdx.x >> 1, i = 0;
+        uint32_t n0 = (t / m_tiles * 2 + rank) * a.rows, m0 = t % m_tiles * nt + rank * half;
+        for (uint32_t j = 0; j < ahead; j++)
+            if (one) load_w(j, n0, j);
+        wait_previous();
+        Ring r;
+        for (; t < tiles && ok; t += pairs) {
+            n0 = (t / m_tiles * 2 + rank) * a.rows;
+            m0 = t % m_tiles * nt + rank * half;
             for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
-                const uint32_t s = i % kPairStages;
-                if (i >= kPairStages && !mbar_wait_cluster(&empty[s], (i / kPairStages - 1) & 1)) { ok = false; break; }
-                if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);  // this CTA's bytes and the other's
-                const uint32_t bar = cluster_addr(smem_u32(&full[s]), 0);
-                const uint32_t dst = base + s * stage_bytes;
-                tma_load_pair(dst, &wmap, (int)(kb * kMmK), n0, bar);
-                tma_load_pair(dst + kWBytes, &xmap, (int)(kb * kMmK), m0, bar);
+                if (i >= kPairStages) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty[r.stage], r.parity ^ 1));
+                    if (!ok) break;
+                }
+                if (one) {
+                    if (i >= ahead) load_w(kb, n0, r.stage);
+                    load_x(kb, m0, r.stage);
+                }
+                r.next(kPairStages);
             }
         }
-        if (!ok && rank == 0)  // the copies in flight land before the memory goes
-            for (uint32_t j = i > kPairStages ? i - kPairStages : 0; j < i; j++)
+        if (!ok && one && rank == 0)  // the copies in flight land before the memory goes
+            for (uint32_t j = i - kPairStages; j < i; j++)
                 mbar_wait_cluster(&full[j % kPairStages], (j / kPairStages) & 1);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+        const bool one = elect_one();
         const uint32_t desc = i8_desc(2 * kMmRows, nt);
-        uint32_t i = 0, n = 0;
+        const uint64_t first = smem_desc(base);
+        Ring r;
+        uint32_t n = 0;
         for (uint32_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs, n++) {
             const uint32_t buf = n & 1, d = tmem + buf * kPairTokens;
-            if (n >= 2 && !mbar_wait_cluster(&acc_empty[buf], (n / 2 - 1) & 1)) { ok = false; break; }
-            tc_fence_after();
-            for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
-                const uint32_t s = i % kPairStages;
-                if (!mbar_wait_cluster(&full[s], (i / kPairStages) & 1)) { ok = false; break; }
-                tc_fence_after();
-                const uint64_t wd = smem_desc(base + s * stage_bytes), xd = smem_desc(base + s * stage_bytes + kWBytes);
-#pragma unroll
-                for (int j = 0; j < (int)kMmK / 32; j++) mma_i8<2>(d, wd + 2 * j, xd + 2 * j, desc, kb > 0 || j > 0);
-                mma_commit_pair(&empty[s]);
+            if (n >= 2) {
+                ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[buf], (n / 2 - 1) & 1));
+                if (!ok) break;
             }
-            mma_commit_pair(&acc_full[buf]);
+            tc_fence_after();
+            for (uint32_t kb = 0; kb < a.kblocks; kb++) {
+                ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[r.stage], r.parity));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t wd = first + ((r.stage * stage_bytes) >> 4);
+                if (one) {
+                    mma_tile<2>(d, wd, wd + (w_bytes >> 4), desc, kb > 0);
+                    mma_commit_pair(&empty[r.stage]);
+                }
+                r.next(kPairStages);
+            }
+            if (one) mma_commit_pair(&acc_full[buf]);
         }
     } else if (warp >= 2) {
         const uint32_t quarter = warp & 3;
         uint32_t n = 0;
+        wait_previous();
         for (uint32_t t = blockIdx.x >> 1; t < tiles; t += pairs, n++) {
             const uint32_t buf = n & 1, m0 = t % m_tiles * nt, valid = min(nt, a.m - m0);
-            const uint32_t col = t / m_tiles * 2 * kMmRows + rank * kMmRows + quarter * 32 + lane;
-            const bool in = col < a.n;
+            const uint32_t col = (t / m_tiles * 2 + rank) * a.rows + quarter * 32 + lane;
+            const bool in = quarter * 32 + lane < a.rows && col < a.n;
             const float sw = in ? a.sw[col] : 0.f, bias = a.bias && in ? a.bias[col] : 0.f;
             float sx[kPairTokens / 32];
 #pragma unroll
@@ -380,25 +471,31 @@ cudaError_t launch_clusters(K kernel, dim3 grid, uint32_t cluster, size_t smem, 
     cfg.blockDim = dim3(kMmThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    note_early_trigger();
     e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) count_launch();
+    else cudaGetLastError();  // reported here, not by a later launch
     return e;
 }
 
-// how a product is cut up
+// how a product is cut up: outputs per CTA, tokens per tile, and for the split
+// kernel the CTAs that share k and their stages
 struct MmPlan {
-    bool pair;
-    uint32_t nt, splits, stages;
+    bool pair = false;
+    uint32_t rows = kMmRows, nt = 16, splits = 1, stages = 4;
 };
-MmPlan plan_matmul(uint32_t m, uint32_t n, uint32_t kblocks, uint32_t sms) {
+
+MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
     MmPlan p{};
-    const uint32_t n_tiles = (n + kMmRows - 1) / kMmRows;
+    const uint32_t n_tiles = (mm.n + kMmRows - 1) / kMmRows;
     if (m > 256) {
         p.pair = true;
         const uint32_t m_tiles = (m + kPairTokens - 1) / kPairTokens;
@@ -407,31 +504,56 @@ MmPlan plan_matmul(uint32_t m, uint32_t n, uint32_t kblocks, uint32_t sms) {
     }
     p.nt = (m + 15) / 16 * 16;
     p.splits = 1;
-    while (p.splits * 2 <= kMaxSplit && p.splits * 2 <= kblocks && n_tiles * p.splits * 2 <= sms) p.splits *= 2;
-    const uint32_t stage = kWBytes + p.nt * kMmK;
-    p.stages = std::min(kMaxStages, (kMmSmem - 1024) / stage);
+    while (p.splits < kMaxSplit && p.splits < mm.kblocks && n_tiles <= mm.clusters[p.splits + 1]) p.splits++;
     return p;
 }
 
+// shared memory of the split kernel beside its stages: alignment, the other CTAs' sums, and at least what the
+// MMA reads past the last tile
+uint32_t split_extra(const MmPlan &p) {
+    return 1024 + std::max(share_bytes(p.nt, p.splits), (kMmRows - p.rows) * kMmK);
+}
+
 template <typename T>
-cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, uint64_t x_stride, cudaStream_t s) {
-    const MmPlan p = plan_matmul(a.m, a.n, a.kblocks, (uint32_t)mm.sms);
-    const uint32_t n_tiles = (a.n + kMmRows - 1) / kMmRows;
+cudaError_t launch_matmul(const MatmulQ8 &mm, MmArgs a, const int8_t *x, uint64_t x_stride, cudaStream_t s) {
+    MmPlan p = plan_matmul(mm, a.m);
+    a.rows = p.rows;
+    const uint32_t m_tiles = (a.m + p.nt - 1) / p.nt, n_tiles = (a.n + p.rows - 1) / p.rows;
+    const CUtensorMap &wmap = mm.wmap[p.rows / 8 - 1];
     CUtensorMap xmap;
     if (!encode_codes(&xmap, x, mm.k, a.m, x_stride, p.pair ? p.nt / 2 : p.nt)) return cudaErrorInvalidValue;
     if (p.pair) {
-        const uint32_t m_tiles = (a.m + p.nt - 1) / p.nt, tiles = (n_tiles + 1) / 2 * m_tiles;
-        const uint32_t pairs = std::min(tiles, (uint32_t)mm.sms / 2);
-        const size_t smem = 1024 + (size_t)kPairStages * (kWBytes + p.nt / 2 * kMmK);
-        return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, mm.wmap, xmap, a, p.nt, m_tiles,
-                               tiles);
+        const uint32_t tiles = (n_tiles + 1) / 2 * m_tiles, pairs = std::min(tiles, (uint32_t)mm.sms / 2);
+        const size_t smem = 1024 + (size_t)kPairStages * (p.rows + p.nt / 2) * kMmK + (kMmRows - p.rows) * kMmK;
+        return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, wmap, xmap, a, p.nt, m_tiles, tiles);
     }
     uint32_t columns = 32;
     while (columns < p.nt) columns *= 2;
-    const size_t smem = 1024 + std::max((size_t)p.stages * (kWBytes + p.nt * kMmK),
-                                        p.splits > 1 ? (size_t)p.nt * kMmRows * 4 : 0);
-    return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, (a.m + p.nt - 1) / p.nt), p.splits, smem,
-                           s, mm.wmap, xmap, a, p.nt, p.splits, p.stages, columns);
+    const uint32_t stage = (p.rows + p.nt) * kMmK;
+    p.stages = std::min(kMaxStages, (kMmSmem - split_extra(p)) / stage);
+    return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, m_tiles), p.splits,
+                           split_extra(p) + (size_t)p.stages * stage, s, wmap, xmap, a, p.nt, p.splits, p.stages, columns);
+}
+
+// how many clusters of each size the device runs at once with one CTA per SM
+bool count_clusters(MatmulQ8 *mm) {
+    if (allow_all_smem(matmul_q8_split_kernel<float>) != cudaSuccess) return false;
+    for (uint32_t c = 1; c <= kMaxSplit; c++) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(c);
+        cfg.blockDim = dim3(kMmThreads);
+        cfg.dynamicSmemBytes = kMmSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = c;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, matmul_q8_split_kernel<float>, &cfg) != cudaSuccess) return false;
+        mm->clusters[c] = (uint32_t)n;
+    }
+    return true;
 }
 
 }  // namespace
@@ -458,10 +580,15 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
     m->device = o->device_id;
     m->n = o->out_features;
     m->k = o->in_features;
-    m->kpad = (o->in_features + kMmK - 1) / kMmK * kMmK;
+    m->kblocks = (o->in_features + kMmK - 1) / kMmK;
     cudaDeviceGetAttribute(&m->sms, cudaDevAttrMultiProcessorCount, m->device);
     cudaStream_t s = static_cast<cudaStream_t>(o->stream);
-    const size_t wb = (size_t)m->n * m->kpad, fb = (size_t)m->n * sizeof(float);
+    const size_t wb = (size_t)m->kblocks * m->n * kMmK, fb = (size_t)m->n * sizeof(float);
+    if (!count_clusters(m)) {
+        set_cuda_error("qwn_matmul_q8_create", cudaGetLastError());
+        matmul_release(m);
+        return QWN_CUDA_STATUS_RUNTIME_ERROR;
+    }
     if (cudaMalloc(&m->w, wb) != cudaSuccess || cudaMalloc(&m->scales, fb) != cudaSuccess ||
         (o->bias_dev && cudaMalloc(&m->bias, fb) != cudaSuccess) ||
         cudaMalloc(&m->status, sizeof(uint32_t)) != cudaSuccess) {
@@ -469,9 +596,11 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
         matmul_release(m);
         return QWN_CUDA_STATUS_OUT_OF_MEMORY;
     }
-    cudaError_t e = m->kpad == m->k ? cudaSuccess : cudaMemsetAsync(m->w, 0, wb, s);
-    if (e == cudaSuccess)
-        e = cudaMemcpy2DAsync(m->w, m->kpad, o->weight_dev, stride, m->k, m->n, cudaMemcpyDeviceToDevice, s);
+    const uint64_t chunks = wb / 16;
+    pack_weight_kernel<<<(unsigned)std::min<uint64_t>((chunks + 255) / 256, (uint64_t)m->sms * 16), 256, 0, s>>>(
+        o->weight_dev, stride, m->n, m->k, chunks, m->w);
+    count_launch();
+    cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaMemcpyAsync(m->scales, o->scales_dev, fb, cudaMemcpyDeviceToDevice, s);
     if (e == cudaSuccess && m->bias) e = cudaMemcpyAsync(m->bias, o->bias_dev, fb, cudaMemcpyDeviceToDevice, s);
     if (e == cudaSuccess) e = cudaMemsetAsync(m->status, 0, sizeof(uint32_t), s);
@@ -481,7 +610,10 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
         matmul_release(m);
         return QWN_CUDA_STATUS_RUNTIME_ERROR;
     }
-    if (!encode_codes(&m->wmap, m->w, m->kpad, m->n, m->kpad, kMmRows)) {
+    bool maps = true;
+    for (uint32_t i = 0; i < kMmRows / 8; i++)
+        maps = maps && encode_codes(&m->wmap[i], m->w, kMmK, (uint64_t)m->kblocks * m->n, kMmK, 8 * (i + 1));
+    if (!maps) {
         set_error("qwn_matmul_q8_create: the driver has no tensor maps");
         matmul_release(m);
         return QWN_CUDA_STATUS_UNSUPPORTED;
@@ -520,7 +652,7 @@ QWN_CUDA_ABI_API int qwn_matmul_q8(QwnMatmulQ8Handle *h, const QwnMatmulQ8Reques
     MmArgs a{};
     a.sx = r->scales_dev, a.sw = m->scales, a.bias = m->bias;
     a.out = r->out_dev, a.out_stride = os;
-    a.m = r->rows, a.n = m->n, a.kblocks = m->kpad / kMmK;
+    a.m = r->rows, a.n = m->n, a.kblocks = m->kblocks;
     a.status = m->status;
     cudaStream_t s = static_cast<cudaStream_t>(r->stream);
     const uint64_t stride = (xs + 15) / 16 * 16;  // of a single row: any

@@ -19,20 +19,44 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// its two halves
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // the address of another CTA's copy of this CTA's shared variable
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t shared, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(shared), "r"(rank));
     return a;
 }
-__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ int ld_shared(uint32_t addr) {
     int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+    asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
+// true in one lane of a converged warp.  The loops that feed the tensor core
+// run in whole warps with this lane issuing: their counters and descriptors
+// then live in uniform registers, where the instructions take them from.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p;
+}
+// a ring of stages and the parity of its current round
+struct Ring {
+    uint32_t stage = 0, parity = 0;
+    __device__ __forceinline__ void next(uint32_t stages) {
+        if (++stage == stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+    }
+};
 // bounded wait that also sees what the cluster's other CTAs did before they arrived
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
     for (uint32_t it = 0; it < kWaitLimit; ++it) {
@@ -49,9 +73,6 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
 }
 
 // ---- TMA ----------------------------------------------------------------------
-__device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
 // a 2-D tile into this CTA's shared memory; the bytes count on `bar` (a shared::cluster address)
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -130,6 +151,14 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
             smem_u32(bar)),
         "h"((uint16_t)3)
         : "memory");
+}
+// the four MMAs of a 128-code tile: 32 codes further are 32 bytes of the swizzled row
+template <int CTAS>
+__device__ __forceinline__ void mma_tile(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    mma_i8<CTAS>(d, a, b, desc, add);
+    mma_i8<CTAS>(d, a + 2, b + 2, desc, true);
+    mma_i8<CTAS>(d, a + 4, b + 4, desc, true);
+    mma_i8<CTAS>(d, a + 6, b + 6, desc, true);
 }
 // 16 or 32 columns of the warp's 32 lanes, complete on return
 __device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
