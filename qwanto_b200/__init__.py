@@ -49,6 +49,22 @@ def _ptr(x) -> int | None:
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
+def _addr(x) -> int:
+    """_ptr for a packed request, 0 for None."""
+    if x is None:
+        return 0
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
+
+
+_pack_append_rotary = _lib.packer(_lib.AppendRotaryRequest)
+_pack_load_tokens = _lib.packer(_lib.LoadTokensRequest)
+_pack_rmsnorm_q8 = _lib.packer(_lib.RmsNormQ8Request)
+_pack_matmul_q8 = _lib.packer(_lib.MatmulQ8Request)
+
+
 def _stream(s) -> int | None:
     if s is None:
         return None
@@ -100,7 +116,8 @@ class KvPool:
         o.max_query_heads = max_query_heads or 0
         o.permutation_seed, o.memory_budget_bytes = permutation_seed, memory_budget_bytes
         self.h = init(_lib.Handle())
-        check("qwn_kv_pool_create", lib().qwn_kv_pool_create(C.byref(o), C.byref(self.h)))
+        self._href = C.byref(self.h)
+        check("qwn_kv_pool_create", lib().qwn_kv_pool_create(C.byref(o), self._href))
         self.codec, self.layers, self.kv_heads, self.page_tokens = codec, layers, kv_heads, page_tokens
         self.total_pages, self.max_seqs, self.max_pages_per_seq = total_pages, max_seqs, max_pages_per_seq
         self.device = device
@@ -201,27 +218,20 @@ class KvPool:
         their pages and Q in query_out (qwn_kv_append_rotary): one row per
         sequence, or with row_begin [num_seqs + 1] ragged runs of rows.
         Strides are in values between rows (0: contiguous)."""
-        r = init(_lib.AppendRotaryRequest())
-        r.layer, r.num_seqs, r.num_rows, r.dtype = layer, num_seqs, num_rows, dtype
-        r.seq_ids_dev, r.row_begin_dev = _ptr(seq_ids), _ptr(row_begin)
-        r.first_pos_dev, r.rotary_pos_dev = _ptr(first_pos), _ptr(rotary_pos)
-        r.query_heads, r.query_out_dtype, r.rotary_dim = query_heads, query_out_dtype, rotary_dim
-        r.rotary_style, r.max_position, r.rotations_dev = int(neighbours), max_position, _ptr(rotations)
-        r.query_stride, r.key_stride, r.value_stride = query_stride, key_stride, value_stride
-        r.query_dev, r.key_dev, r.value_dev, r.query_out_dev = _ptr(query), _ptr(key), _ptr(value), _ptr(query_out)
-        r.stream = _stream(stream)
-        check("qwn_kv_append_rotary", lib().qwn_kv_append_rotary(C.byref(self.h), C.byref(r)))
+        rc = lib().qwn_kv_append_rotary(self._href, _pack_append_rotary(
+            layer, num_seqs, _addr(seq_ids), _addr(row_begin), _addr(first_pos), _addr(rotary_pos), num_rows, dtype,
+            query_heads, query_out_dtype, rotary_dim, neighbours, max_position, 0, _addr(rotations), query_stride,
+            key_stride, value_stride, _addr(query), _addr(key), _addr(value), _addr(query_out), _stream(stream) or 0))
+        check("qwn_kv_append_rotary", rc)
 
     def load_tokens(self, layer: int, num_seqs: int, num_rows: int, dtype: int, key_out=None, value_out=None,
                     row_begin=None, first_pos=None, seq_ids=None, key_stride: int = 0, value_stride: int = 0,
                     stream=None) -> None:
         """Cached tokens back to rows (qwn_kv_load_tokens), as the values their codes stand for."""
-        r = init(_lib.LoadTokensRequest())
-        r.layer, r.num_seqs, r.num_rows, r.dtype = layer, num_seqs, num_rows, dtype
-        r.seq_ids_dev, r.row_begin_dev, r.first_pos_dev = _ptr(seq_ids), _ptr(row_begin), _ptr(first_pos)
-        r.key_stride, r.value_stride = key_stride, value_stride
-        r.key_out_dev, r.value_out_dev, r.stream = _ptr(key_out), _ptr(value_out), _stream(stream)
-        check("qwn_kv_load_tokens", lib().qwn_kv_load_tokens(C.byref(self.h), C.byref(r)))
+        rc = lib().qwn_kv_load_tokens(self._href, _pack_load_tokens(
+            layer, num_seqs, _addr(seq_ids), _addr(row_begin), _addr(first_pos), num_rows, dtype, key_stride,
+            value_stride, _addr(key_out), _addr(value_out), _stream(stream) or 0))
+        check("qwn_kv_load_tokens", rc)
 
     def prefill_synthetic(self, seq_ids, lens, seed: int, outlier_mask: np.ndarray | None = None,
                           stream=None) -> None:
@@ -255,14 +265,11 @@ def rmsnorm_q8(x, rows: int, width: int, dtype: int, codes, scales, weight=None,
     """Rows to int8 codes with one scale each, after the residual's addition
     and the root-mean-square norm (qwn_rmsnorm_q8); norm=False only quantises.
     Strides are in values between rows (0: width)."""
-    r = init(_lib.RmsNormQ8Request())
-    r.device_id, r.rows, r.width, r.dtype, r.mode, r.eps = device, rows, width, dtype, int(not norm), eps
-    r.rows_dtype = rows_dtype
-    r.x_stride, r.residual_stride, r.residual_out_stride = x_stride, residual_stride, residual_out_stride
-    r.codes_stride, r.rows_stride = codes_stride, rows_stride
-    r.x_dev, r.residual_dev, r.weight_dev, r.residual_out_dev = _ptr(x), _ptr(residual), _ptr(weight), _ptr(residual_out)
-    r.codes_dev, r.scales_dev, r.rows_out_dev, r.stream = _ptr(codes), _ptr(scales), _ptr(rows_out), _stream(stream)
-    check("qwn_rmsnorm_q8", lib().qwn_rmsnorm_q8(C.byref(r)))
+    rc = lib().qwn_rmsnorm_q8(_pack_rmsnorm_q8(
+        device, rows, width, dtype, not norm, eps, rows_dtype, 0, x_stride, residual_stride, residual_out_stride,
+        codes_stride, rows_stride, _addr(x), _addr(residual), _addr(weight), _addr(residual_out), _addr(codes),
+        _addr(scales), _addr(rows_out), _stream(stream) or 0))
+    check("qwn_rmsnorm_q8", rc)
 
 
 class MatmulQ8:
@@ -276,15 +283,15 @@ class MatmulQ8:
         o.device_id, o.out_features, o.in_features, o.weight_stride = device, out_features, in_features, weight_stride
         o.weight_dev, o.scales_dev, o.bias_dev, o.stream = _ptr(weight), _ptr(scales), _ptr(bias), _stream(stream)
         self.h = init(_lib.Handle())
-        check("qwn_matmul_q8_create", lib().qwn_matmul_q8_create(C.byref(o), C.byref(self.h)))
+        self._href = C.byref(self.h)
+        check("qwn_matmul_q8_create", lib().qwn_matmul_q8_create(C.byref(o), self._href))
         self.out_features, self.in_features, self.device = out_features, in_features, device
 
     def __call__(self, codes, scales, rows: int, out, out_dtype: int, codes_stride: int = 0, out_stride: int = 0,
                  stream=None) -> None:
-        r = init(_lib.MatmulQ8Request())
-        r.rows, r.out_dtype, r.codes_stride, r.out_stride = rows, out_dtype, codes_stride, out_stride
-        r.codes_dev, r.scales_dev, r.out_dev, r.stream = _ptr(codes), _ptr(scales), _ptr(out), _stream(stream)
-        check("qwn_matmul_q8", lib().qwn_matmul_q8(C.byref(self.h), C.byref(r)))
+        rc = lib().qwn_matmul_q8(self._href, _pack_matmul_q8(rows, out_dtype, codes_stride, out_stride, _addr(codes),
+                                                              _addr(scales), _addr(out), _stream(stream) or 0))
+        check("qwn_matmul_q8", rc)
 
     def check(self) -> int:
         bits = C.c_uint32(0)

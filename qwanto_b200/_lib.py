@@ -7,7 +7,9 @@ fallback.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "qwn_cuda.so")
@@ -237,6 +239,18 @@ class MatmulQ8Request(C.Structure):
                 ("out_dev", C.c_void_p), ("stream", C.c_void_p)]
 
 
+_FORMATS = {C.c_uint32: "I", C.c_int32: "i", C.c_float: "f", C.c_uint64: "Q", C.c_void_p: "Q"}
+
+
+def packer(cls):
+    """A function from the values of a request's fields after its header to the
+    request's bytes, which a call takes as the structure.  Writing a structure
+    field by field costs more than the small kernels behind these calls."""
+    s = struct.Struct("@6I" + "".join(_FORMATS[t] for _, t in cls._fields_[1:]) + "0Q")
+    assert s.size == C.sizeof(cls), cls
+    return functools.partial(s.pack, s.size, ABI_VERSION, 0, 0, 0, 0)
+
+
 _P = C.POINTER
 _SIGS = {
     "qwn_cuda_abi_query": (C.c_int, [_P(AbiInfo)]),
@@ -277,12 +291,13 @@ _SIGS = {
     "qwn_kv_decode_split": (C.c_int, [_P(Handle), _P(SplitRequest)]),
     "qwn_kv_store_tokens": (C.c_int, [_P(Handle), C.c_int32, C.c_uint32, C.c_uint32, C.c_uint32,
                                       C.c_void_p, C.c_void_p, C.c_void_p]),
-    "qwn_kv_append_rotary": (C.c_int, [_P(Handle), _P(AppendRotaryRequest)]),
-    "qwn_kv_load_tokens": (C.c_int, [_P(Handle), _P(LoadTokensRequest)]),
-    "qwn_rmsnorm_q8": (C.c_int, [_P(RmsNormQ8Request)]),
+    # requests as bytes: see packer()
+    "qwn_kv_append_rotary": (C.c_int, [_P(Handle), C.c_void_p]),
+    "qwn_kv_load_tokens": (C.c_int, [_P(Handle), C.c_void_p]),
+    "qwn_rmsnorm_q8": (C.c_int, [C.c_void_p]),
     "qwn_matmul_q8_create": (C.c_int, [_P(MatmulQ8Options), _P(Handle)]),
     "qwn_matmul_q8_destroy": (C.c_int, [_P(Handle)]),
-    "qwn_matmul_q8": (C.c_int, [_P(Handle), _P(MatmulQ8Request)]),
+    "qwn_matmul_q8": (C.c_int, [_P(Handle), C.c_void_p]),
     "qwn_matmul_q8_check": (C.c_int, [_P(Handle), _P(C.c_uint32)]),
     "qwn_kv_generate_rows": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64,
                                        C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -10,11 +10,10 @@
 // tokens cost a narrow MMA and a warp's lanes write consecutive outputs.
 // Operand tiles are 128 codes deep, loaded by TMA with 128-byte swizzle.
 // The handle keeps the weights as [in/128][out][128], zero past in_features:
-// a tile of any number of outputs is one run of HBM, and a product never
-// branches on in_features' remainder; TMA fills what lies outside the codes
-// with zeros.  A CTA may take fewer than 128 outputs, where that spreads them
-// evenly over the SMs: the MMA then multiplies whatever follows the tile in
-// shared memory into lanes that nobody reads.
+// a tile is 16 KB in a row of HBM (with the caller's row order its 128-byte
+// pieces are in_features apart, and a large weight streamed at 4.7 TB/s
+// instead of 6.6), and a product never branches on in_features' remainder;
+// TMA fills what lies outside the codes with zeros.
 //
 // Both kernels start while the stream's previous kernel still runs
 // (programmatic launch), fetch weights, and wait for it before they read codes
@@ -34,9 +33,11 @@ namespace qkv {
 namespace {
 
 constexpr uint32_t kMmK = 128;       // codes per operand tile row: one swizzled row
-constexpr uint32_t kMmRows = 128;    // lanes of a CTA's accumulator: at most so many outputs
+constexpr uint32_t kMmRows = 128;    // outputs per CTA: the lanes of its accumulator
+constexpr uint32_t kWBytes = kMmRows * kMmK;
 constexpr uint32_t kMaxStages = 12;
-constexpr uint32_t kMmThreads = 192; // TMA warp, MMA warp, four warps that read TMEM
+constexpr uint32_t kOutWarps = 8;    // read TMEM and write: two for each quarter of its lanes
+constexpr uint32_t kMmThreads = 64 + 32 * kOutWarps; // TMA warp, MMA warp, those
 constexpr uint32_t kMaxSplit = 8;    // CTAs of a cluster that share an output tile
 
 struct MatmulQ8 {
@@ -46,7 +47,7 @@ struct MatmulQ8 {
     float *scales = nullptr, *bias = nullptr;
     uint32_t *status = nullptr;
     uint32_t clusters[kMaxSplit + 1] = {};  // clusters of each size that run at once, one CTA per SM
-    CUtensorMap wmap[kMmRows / 8];          // tiles of 8, 16, ... 128 outputs
+    CUtensorMap wmap;
 };
 
 MatmulQ8 *matmul_from(const QwnMatmulQ8Handle *h) {
@@ -88,7 +89,6 @@ struct MmArgs {
     void *out;
     uint64_t out_stride;
     uint32_t m, n, kblocks;
-    uint32_t rows;  // outputs per CTA, a multiple of 8
     uint32_t *status;
 };
 
@@ -128,10 +128,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t rank = splits > 1 ? cluster_rank() : 0;
-    const uint32_t n0 = blockIdx.x / splits * a.rows, m0 = blockIdx.y * nt;
+    const uint32_t n0 = blockIdx.x / splits * kMmRows, m0 = blockIdx.y * nt;
     const uint32_t kb0 = (uint32_t)((uint64_t)a.kblocks * rank / splits);
     const uint32_t kb1 = (uint32_t)((uint64_t)a.kblocks * (rank + 1) / splits);
-    const uint32_t w_bytes = a.rows * kMmK, stage_bytes = w_bytes + nt * kMmK, count = kb1 - kb0;
+    const uint32_t stage_bytes = kWBytes + nt * kMmK, count = kb1 - kb0;
     const uint32_t valid = min(nt, a.m - m0);  // tokens of this tile that exist
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
             tma_load(base + st * stage_bytes, &wmap, 0, (int)((kb0 + i) * a.n + n0), smem_u32(&full[st]));
         };
         auto load_x = [&](uint32_t i, uint32_t st) {
-            tma_load(base + st * stage_bytes + w_bytes, &xmap, (int)((kb0 + i) * kMmK), (int)m0, smem_u32(&full[st]));
+            tma_load(base + st * stage_bytes + kWBytes, &xmap, (int)((kb0 + i) * kMmK), (int)m0, smem_u32(&full[st]));
         };
         for (uint32_t i = 0; i < ahead; i++)
             if (one) load_w(i, i);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
             tc_fence_after();
             const uint64_t wd = first + ((r.stage * stage_bytes) >> 4);
             if (one) {
-                mma_tile<1>(tmem, wd, wd + (w_bytes >> 4), desc, i > 0);
+                mma_tile<1>(tmem, wd, wd + (kWBytes >> 4), desc, i > 0);
                 mma_commit(&empty[r.stage]);
             }
             r.next(stages);
@@ -197,16 +197,17 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     }
     const uint32_t quarter = warp & 3, feature = quarter * 32 + lane;  // TMEM lanes this warp may read
     const uint32_t lanes = tmem + (quarter << 21);
+    const uint32_t second = warp >= 2 ? (uint32_t)(warp - 2) >> 2 : 0;  // every other 16 tokens
     const uint32_t n = n0 + feature;
-    const bool in = feature < a.rows && n < a.n;
+    const bool in = n < a.n;
     float sw = 0.f, bias = 0.f;
     T *out = static_cast<T *>(a.out) + (uint64_t)m0 * a.out_stride + n;
     if (warp >= 2) {
         if (in) sw = a.sw[n];
         if (in && a.bias) bias = a.bias[n];
         wait_previous();
-        for (uint32_t c = threadIdx.x - 64; c < valid; c += 128) sx[c] = a.sx[m0 + c];
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (uint32_t c = threadIdx.x - 64; c < valid; c += 32 * kOutWarps) sx[c] = a.sx[m0 + c];
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
         ok = mbar_wait_bounded(&done, 0);
         tc_fence_after();
     }
@@ -214,13 +215,14 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     __syncwarp();
     if (splits == 1) {
         if (warp >= 2) {
-            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
+            for (uint32_t c0 = 16 * second; c0 < valid; c0 += 32) {
                 uint32_t v[16];
                 tmem_load16(v, lanes + c0);
+                T *to = out + c0 * a.out_stride;
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i++) {
-                    if (in && c0 + i < valid) store_out(out, scaled((int)v[i], sx[c0 + i], sw, bias));
-                    out += a.out_stride;
+                    if (in && c0 + i < valid) store_out(to, scaled((int)v[i], sx[c0 + i], sw, bias));
+                    to += a.out_stride;
                 }
             }
         }
@@ -231,34 +233,30 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
         if (warp >= 2) {
             // this CTA's sums of token c go to the CTA of c's share
             const uint32_t mine = region + (rank * share * kMmRows + feature) * 4;
-            uint32_t owner = 0, left = share, to = cluster_addr(mine, 0);
-            for (uint32_t c0 = 0; c0 < valid; c0 += 16) {
+            for (uint32_t c0 = 16 * second; c0 < valid; c0 += 32) {
                 uint32_t v[16];
                 tmem_load16(v, lanes + c0);
+                uint32_t owner = c0 / share, at = c0 - owner * share, to = cluster_addr(mine, owner);
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i++) {
                     if (c0 + i >= valid) break;
-                    if (left == 0) {
-                        left = share;
+                    if (at == share) {
+                        at = 0;
                         to = cluster_addr(mine, ++owner);
                     }
-                    st_cluster(to, v[i]);
-                    to += kMmRows * 4;
-                    left--;
+                    st_cluster(to + at++ * kMmRows * 4, v[i]);
                 }
             }
         }
         cluster_sync();
         if (warp >= 2 && in) {
             const uint32_t first = rank * share, mine = first < valid ? min(share, valid - first) : 0;
-            out += (uint64_t)first * a.out_stride;
-            for (uint32_t c = 0; c < mine; c++) {
+            for (uint32_t c = second; c < mine; c += 2) {
                 int sum = 0;
 #pragma unroll
                 for (uint32_t p = 0; p < kMaxSplit; p++)
                     if (p < splits) sum += ld_shared(region + ((p * share + c) * kMmRows + feature) * 4);
-                store_out(out, scaled(sum, sx[first + c], sw, bias));
-                out += a.out_stride;
+                store_out(out + (first + c) * a.out_stride, scaled(sum, sx[first + c], sw, bias));
             }
         }
     }
@@ -292,7 +290,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1;
-    const uint32_t half = nt / 2, w_bytes = a.rows * kMmK, stage_bytes = w_bytes + half * kMmK;
+    const uint32_t half = nt / 2, stage_bytes = kWBytes + half * kMmK;
     launch_dependents();
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kPairStages; i++) {
@@ -301,7 +299,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);  // the TMEM warps of both CTAs
+            mbar_init(&acc_empty[i], 2 * kOutWarps);  // of both CTAs
         }
         fence_barrier_init();
     }
@@ -320,17 +318,17 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
             tma_load_pair(base + st * stage_bytes, &wmap, 0, (int)(kb * a.n + row), bars + 8 * st);
         };
         auto load_x = [&](uint32_t kb, uint32_t row, uint32_t st) {
-            tma_load_pair(base + st * stage_bytes + w_bytes, &xmap, (int)(kb * kMmK), (int)row, bars + 8 * st);
+            tma_load_pair(base + st * stage_bytes + kWBytes, &xmap, (int)(kb * kMmK), (int)row, bars + 8 * st);
         };
         const uint32_t ahead = min(a.kblocks, kPairStages);  // weights of the first tile
         uint32_t t = blockIdx.x >> 1, i = 0;
-        uint32_t n0 = (t / m_tiles * 2 + rank) * a.rows, m0 = t % m_tiles * nt + rank * half;
+        uint32_t n0 = (t / m_tiles * 2 + rank) * kMmRows, m0 = t % m_tiles * nt + rank * half;
         for (uint32_t j = 0; j < ahead; j++)
             if (one) load_w(j, n0, j);
         wait_previous();
         Ring r;
         for (; t < tiles && ok; t += pairs) {
-            n0 = (t / m_tiles * 2 + rank) * a.rows;
+            n0 = (t / m_tiles * 2 + rank) * kMmRows;
             m0 = t % m_tiles * nt + rank * half;
             for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
                 if (i >= kPairStages) {
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
                 tc_fence_after();
                 const uint64_t wd = first + ((r.stage * stage_bytes) >> 4);
                 if (one) {
-                    mma_tile<2>(d, wd, wd + (w_bytes >> 4), desc, kb > 0);
+                    mma_tile<2>(d, wd, wd + (kWBytes >> 4), desc, kb > 0);
                     mma_commit_pair(&empty[r.stage]);
                 }
                 r.next(kPairStages);
@@ -374,30 +372,36 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
             if (one) mma_commit_pair(&acc_full[buf]);
         }
     } else if (warp >= 2) {
-        const uint32_t quarter = warp & 3;
+        const uint32_t quarter = warp & 3, second = (uint32_t)(warp - 2) >> 2;
         uint32_t n = 0;
         wait_previous();
         for (uint32_t t = blockIdx.x >> 1; t < tiles; t += pairs, n++) {
             const uint32_t buf = n & 1, m0 = t % m_tiles * nt, valid = min(nt, a.m - m0);
-            const uint32_t col = (t / m_tiles * 2 + rank) * a.rows + quarter * 32 + lane;
-            const bool in = quarter * 32 + lane < a.rows && col < a.n;
+            const uint32_t col = (t / m_tiles * 2 + rank) * kMmRows + quarter * 32 + lane;
+            const bool in = col < a.n;
             const float sw = in ? a.sw[col] : 0.f, bias = a.bias && in ? a.bias[col] : 0.f;
-            float sx[kPairTokens / 32];
+            constexpr uint32_t kChunks = kPairTokens / 64;  // this warp's: every other 32 tokens
+            float sx[kChunks];
 #pragma unroll
-            for (uint32_t j = 0; j < kPairTokens / 32; j++) sx[j] = j * 32 + lane < valid ? a.sx[m0 + j * 32 + lane] : 0.f;
+            for (uint32_t j = 0; j < kChunks; j++) {
+                const uint32_t c = (2 * j + second) * 32 + lane;
+                sx[j] = c < valid ? a.sx[m0 + c] : 0.f;
+            }
             if (!mbar_wait_cluster(&acc_full[buf], (n / 2) & 1)) { ok = false; break; }
             tc_fence_after();
             T *out = static_cast<T *>(a.out) + (uint64_t)m0 * a.out_stride + col;
 #pragma unroll
-            for (uint32_t j = 0; j < kPairTokens / 32; j++) {
-                if (j * 32 < valid) {
+            for (uint32_t j = 0; j < kChunks; j++) {
+                const uint32_t c0 = (2 * j + second) * 32;
+                if (c0 < valid) {
                     uint32_t v[32];
-                    tmem_load32(v, tmem + (quarter << 21) + buf * kPairTokens + j * 32);
+                    tmem_load32(v, tmem + (quarter << 21) + buf * kPairTokens + c0);
+                    T *to = out + c0 * a.out_stride;
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i++) {
                         const float s = __shfl_sync(0xffffffffu, sx[j], i);
-                        if (in && j * 32 + i < valid) store_out(out, scaled((int)v[i], s, sw, bias));
-                        out += a.out_stride;
+                        if (in && c0 + i < valid) store_out(to, scaled((int)v[i], s, sw, bias));
+                        to += a.out_stride;
                     }
                 }
             }
@@ -486,53 +490,86 @@ cudaError_t launch_clusters(K kernel, dim3 grid, uint32_t cluster, size_t smem, 
     return e;
 }
 
-// how a product is cut up: outputs per CTA, tokens per tile, and for the split
-// kernel the CTAs that share k and their stages
+// how a product is cut up: tokens per tile, and for the split kernel the CTAs
+// that share k
 struct MmPlan {
-    bool pair = false;
-    uint32_t rows = kMmRows, nt = 16, splits = 1, stages = 4;
+    bool pair;
+    uint32_t nt, splits;
 };
 
+// The cut with the lowest estimate of its microseconds.  What the estimates are
+// made of, measured on B200:
+//  - the weights come out of HBM at 6.5 KB per ns at best, and all SMs together
+//    read 11 KB per ns out of L2: a tile's weights once per token tile, its
+//    tokens once per 128 outputs;
+//  - the split kernel spends 0.14 us on 128 codes of a CTA's share of k (four
+//    narrow MMAs), 0.2 when the CTAs fill the GPU, starts and ends in 2.2 us, writes a token in 20 ns, and joins
+//    a cluster's sums in 1.3 us (0.1 for one token) and 17 ns per token.  Shares
+//    only as long as all clusters run at once (74 of two CTAs, 45 of three, 33
+//    of four, 15 of eight): 48 clusters of three took 15.7 us where 48 of two
+//    took 10.1;
+//  - a pair spends 0.13 us + 1.05 ns per token of its tile on 128 codes, at
+//    least 10.5 ns per token on a tile (its output), and starts and ends in
+//    2.6 us.
+// A few tokens thus go to the split kernel with as many shares as run at once
+// (1 x 1536 x 2048: 2.7 us in 4 shares, 4.3 in one), more to pairs with the
+// widest tile that still reaches all of them (257 x 4099 x 4095: 10.7 us with
+// 96 tokens a tile, 14.1 with 256; 8192 x 6144 x 8192: 260 us with 256, 278
+// with 192).
 MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
-    MmPlan p{};
-    const uint32_t n_tiles = (mm.n + kMmRows - 1) / kMmRows;
-    if (m > 256) {
-        p.pair = true;
-        const uint32_t m_tiles = (m + kPairTokens - 1) / kPairTokens;
-        p.nt = std::max(32u, ((m + m_tiles - 1) / m_tiles + 31) / 32 * 32);
-        return p;
+    MmPlan best{};
+    float least = INFINITY;
+    const uint32_t n_tiles = (mm.n + kMmRows - 1) / kMmRows, n_pairs = (n_tiles + 1) / 2, pairs = (uint32_t)mm.sms / 2;
+    const float kb = (float)mm.kblocks, hbm = (float)mm.n * kb * (float)kMmK / 6.5e6f;
+    auto l2 = [&](uint64_t ctas, uint32_t tokens) { return (float)ctas * kb * (float)((kMmRows + tokens) * kMmK) / 11e6f; };
+    for (uint32_t nt = 32; nt <= kPairTokens; nt += 32) {
+        const uint64_t tiles = (uint64_t)n_pairs * ((m + nt - 1) / nt), waves = (tiles + pairs - 1) / pairs;
+        const float w = (float)nt, tile = std::max(kb * (0.13f + 0.00105f * w), 0.25f + 0.0105f * w);
+        const float t = 2.6f + std::max({(float)waves * tile, l2(2 * tiles, nt / 2), hbm}) + 0.006f * w;
+        if (t < least) {
+            least = t;
+            best = {true, nt, 1};
+        }
     }
-    p.nt = (m + 15) / 16 * 16;
-    p.splits = 1;
-    while (p.splits < kMaxSplit && p.splits < mm.kblocks && n_tiles <= mm.clusters[p.splits + 1]) p.splits++;
-    return p;
-}
-
-// shared memory of the split kernel beside its stages: alignment, the other CTAs' sums, and at least what the
-// MMA reads past the last tile
-uint32_t split_extra(const MmPlan &p) {
-    return 1024 + std::max(share_bytes(p.nt, p.splits), (kMmRows - p.rows) * kMmK);
+    if (m > 1024) return best;
+    for (uint32_t m_tiles = (m + 127) / 128; m_tiles <= 8 && (m_tiles - 1) * 16 < m; m_tiles++) {
+        const uint32_t nt = ((m + m_tiles - 1) / m_tiles + 15) / 16 * 16, count = (m + nt - 1) / nt;
+        const uint64_t tiles = (uint64_t)n_tiles * count;
+        const float tokens = (float)std::min(m, nt);
+        for (uint32_t splits = 1; splits <= kMaxSplit && splits <= mm.kblocks; splits++) {
+            if (splits > 1 && tiles > mm.clusters[splits]) break;
+            const uint64_t waves = splits > 1 ? 1 : (tiles + mm.sms - 1) / mm.sms;
+            const float busy = (float)std::min<uint64_t>(tiles * splits, (uint64_t)mm.sms);
+            float cta = (float)((mm.kblocks + splits - 1) / splits) * (0.14f + 0.0004f * (float)nt + 0.0005f * busy);
+            if (waves > 1) cta += 1.f + 0.02f * tokens;
+            const float out = splits > 1 ? std::min(0.1f * tokens, 1.3f) + 0.017f * tokens : 0.02f * tokens;
+            const float t = 2.2f + std::max({(float)waves * cta, l2(tiles, nt), hbm}) + out;
+            if (t < least) {
+                least = t;
+                best = {false, nt, splits};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T>
-cudaError_t launch_matmul(const MatmulQ8 &mm, MmArgs a, const int8_t *x, uint64_t x_stride, cudaStream_t s) {
-    MmPlan p = plan_matmul(mm, a.m);
-    a.rows = p.rows;
-    const uint32_t m_tiles = (a.m + p.nt - 1) / p.nt, n_tiles = (a.n + p.rows - 1) / p.rows;
-    const CUtensorMap &wmap = mm.wmap[p.rows / 8 - 1];
+cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, uint64_t x_stride, cudaStream_t s) {
+    const MmPlan p = plan_matmul(mm, a.m);
+    const uint32_t m_tiles = (a.m + p.nt - 1) / p.nt, n_tiles = (a.n + kMmRows - 1) / kMmRows;
     CUtensorMap xmap;
     if (!encode_codes(&xmap, x, mm.k, a.m, x_stride, p.pair ? p.nt / 2 : p.nt)) return cudaErrorInvalidValue;
     if (p.pair) {
         const uint32_t tiles = (n_tiles + 1) / 2 * m_tiles, pairs = std::min(tiles, (uint32_t)mm.sms / 2);
-        const size_t smem = 1024 + (size_t)kPairStages * (p.rows + p.nt / 2) * kMmK + (kMmRows - p.rows) * kMmK;
-        return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, wmap, xmap, a, p.nt, m_tiles, tiles);
+        const size_t smem = 1024 + (size_t)kPairStages * (kWBytes + p.nt / 2 * kMmK);
+        return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, mm.wmap, xmap, a, p.nt, m_tiles, tiles);
     }
     uint32_t columns = 32;
     while (columns < p.nt) columns *= 2;
-    const uint32_t stage = (p.rows + p.nt) * kMmK;
-    p.stages = std::min(kMaxStages, (kMmSmem - split_extra(p)) / stage);
+    const uint32_t stage = kWBytes + p.nt * kMmK, extra = 1024 + share_bytes(p.nt, p.splits);
+    const uint32_t stages = std::min({kMaxStages, (kMmSmem - extra) / stage, (mm.kblocks + p.splits - 1) / p.splits});
     return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, m_tiles), p.splits,
-                           split_extra(p) + (size_t)p.stages * stage, s, wmap, xmap, a, p.nt, p.splits, p.stages, columns);
+                           extra + (size_t)stages * stage, s, mm.wmap, xmap, a, p.nt, p.splits, stages, columns);
 }
 
 // how many clusters of each size the device runs at once with one CTA per SM
@@ -610,10 +647,7 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
         matmul_release(m);
         return QWN_CUDA_STATUS_RUNTIME_ERROR;
     }
-    bool maps = true;
-    for (uint32_t i = 0; i < kMmRows / 8; i++)
-        maps = maps && encode_codes(&m->wmap[i], m->w, kMmK, (uint64_t)m->kblocks * m->n, kMmK, 8 * (i + 1));
-    if (!maps) {
+    if (!encode_codes(&m->wmap, m->w, kMmK, (uint64_t)m->kblocks * m->n, kMmK, kMmRows)) {
         set_error("qwn_matmul_q8_create: the driver has no tensor maps");
         matmul_release(m);
         return QWN_CUDA_STATUS_UNSUPPORTED;

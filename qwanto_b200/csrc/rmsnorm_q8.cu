@@ -8,6 +8,15 @@
 // One CTA per row keeps the row in registers between its two reductions (the
 // sum of squares, then the largest |y|), so x and r are read once and each
 // output is written once; bound by HBM, or by the launch for a few rows.
+// Codes come from y x (127 / max|y|) by adding 1.5 x 2^23: the sum's low byte
+// is the rounded code, and the sum less that number the code in fp32, with no
+// division or conversion per value.  All loads of a row, the weight's among
+// them, are issued before the first is used: 8191 x 6144 fp16 with residual and
+// rows_out takes 69 us, 6.5 TB/s (131 us with divisions and loads as they are
+// needed).  Rows over 8192 wide leave two CTAs' registers per SM and reach 4.1
+// TB/s.
+#include <type_traits>
+
 #include "kv_internal.cuh"
 #include "rows.cuh"
 
@@ -25,43 +34,67 @@ struct NormArgs {
     bool norm;
 };
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float &d, float x) { d = x; }
-__device__ __forceinline__ void from_f(__half &d, float x) { d = __float2half_rn(x); }
-__device__ __forceinline__ void from_f(__nv_bfloat16 &d, float x) { d = __float2bfloat16_rn(x); }
-
-// the n values from p on (n < V at the row's end), V in one access where VEC
-template <bool VEC, int V, typename T>
-__device__ __forceinline__ void load_chunk(float (&v)[V], const T *p, int n) {
-    if (VEC && n >= V) {
-        T t[V];
-        *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(p);
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = to_f(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = i < n ? to_f(p[i]) : 0.f;
+// the V values from `at` on, 16 bytes; beyond the row's end any values of it.
+// No branch: the loads of all chunks are in flight together.
+template <typename T>
+struct Chunk {
+    uint32_t w[4];
+    __device__ __forceinline__ float get(int i) const {  // i is known at compile time
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __half>) return h2f((uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]));
+        else return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
     }
+};
+__device__ __forceinline__ uint32_t raw_bits(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t raw_bits(__half x) { return __half_as_ushort(x); }
+__device__ __forceinline__ uint32_t raw_bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+template <bool VEC, typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T *p, int at, int width) {
+    Chunk<T> c;
+    if constexpr (VEC) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p + (at < width ? at : 0));
+        c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
+    } else {
+        constexpr int V = 16 / (int)sizeof(T), per = V / 4;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const uint32_t b = raw_bits(p[min(at + i, width - 1)]);
+            if (i % per == 0) c.w[i / per] = b;
+            else c.w[i / per] |= b << 16;
+        }
+    }
+    return c;
 }
+__device__ __forceinline__ uint32_t pack2(const float *, float a, float) { return __float_as_uint(a); }
+__device__ __forceinline__ uint32_t pack2(const __half *, float a, float b) { return pack_h2(a, b); }
+__device__ __forceinline__ uint32_t pack2(const __nv_bfloat16 *, float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+// the first n of V values, all in 16-byte (or one 8-byte) accesses where VEC
 template <bool VEC, int V, typename T>
 __device__ __forceinline__ void store_chunk(T *p, const float (&v)[V], int n) {
-    T t[V];
+    constexpr int per = 4 / (int)sizeof(T), W = V / per;
+    uint32_t w[W];
 #pragma unroll
-    for (int i = 0; i < V; i++) from_f(t[i], v[i]);
-    if (VEC && n >= V) {
-        constexpr int W = V * (int)sizeof(T) / 4;
-        if constexpr (W % 4 == 0) {
+    for (int i = 0; i < W; i++) w[i] = pack2(p, v[per * i], v[per * i + per - 1]);
+    if (VEC) {
+        if (n > 0) {
+            if constexpr (W % 4 == 0) {
 #pragma unroll
-            for (int i = 0; i < W / 4; i++) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(t)[i];
-        } else {
-            *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(t);
+                for (int i = 0; i < W; i += 4)
+                    *reinterpret_cast<uint4 *>(p + per * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            } else {
+                *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i < n) p[i] = t[i];
+        for (int i = 0; i < V; i++) {
+            if (i >= n) break;
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+            else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+        }
     }
 }
 
@@ -86,37 +119,50 @@ __device__ __forceinline__ float block_reduce(float v, float *sm) {
     return v;
 }
 
-// CH chunks of 16 bytes per thread hold the row; VEC: every row and the weight
-// start on 16 bytes (codes and rows_out on a chunk's part)
+// CH chunks of 16 bytes per thread hold the row; VEC: rows are whole chunks, and
+// every row and the weight start on 16 bytes (codes and rows_out on a chunk's part)
 template <typename T, int CH, bool VEC>
-__global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(NormArgs a) {
+__global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     __shared__ float sm[2][32];
     const int width = (int)a.width;
     const size_t row = blockIdx.x;
+    auto at = [](int c) { return ((int)threadIdx.x + c * (int)blockDim.x) * V; };
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+    const T *w = static_cast<const T *>(a.weight);
     float h[CH][V];
+    Chunk<T> wc[CH];
     float ss = 0.f;
+    launch_dependents();
+    wait_previous();
+    {
+        Chunk<T> xc[CH], rc[CH];
 #pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int at = ((int)threadIdx.x + c * (int)blockDim.x) * V;
-        load_chunk<VEC>(h[c], x + at, width - at);
+        for (int c = 0; c < CH; c++) xc[c] = load_chunk<VEC>(x, at(c), width);
         if (r) {
-            float d[V];
-            load_chunk<VEC>(d, r + at, width - at);
 #pragma unroll
-            for (int i = 0; i < V; i++) h[c][i] += d[i];
+            for (int c = 0; c < CH; c++) rc[c] = load_chunk<VEC>(r, at(c), width);
+        }
+        if (w) {
+#pragma unroll
+            for (int c = 0; c < CH; c++) wc[c] = load_chunk<VEC>(w, at(c), width);
         }
 #pragma unroll
-        for (int i = 0; i < V; i++) ss = fmaf(h[c][i], h[c][i], ss);
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                float v = xc[c].get(i);
+                if (r) v += rc[c].get(i);
+                h[c][i] = at(c) + (VEC ? 0 : i) < width ? v : 0.f;
+                ss = fmaf(h[c][i], h[c][i], ss);
+            }
     }
     if (a.residual_out) {
         T *out = static_cast<T *>(a.residual_out) + row * a.residual_out_stride;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int at = ((int)threadIdx.x + c * (int)blockDim.x) * V;
-            store_chunk<VEC>(out + at, h[c], width - at);
+            store_chunk<VEC>(out + at(c), h[c], width - at(c));
         }
     }
     float inv = 1.f;
@@ -124,44 +170,50 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(NormArgs a) {
     float top = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-        const int at = ((int)threadIdx.x + c * (int)blockDim.x) * V;
-        float w[V];
-        if (a.weight) load_chunk<VEC>(w, static_cast<const T *>(a.weight) + at, width - at);
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            h[c][i] = h[c][i] * inv;
-            if (a.weight) h[c][i] *= w[i];
-            const float m = fabsf(h[c][i]);
-            if (m < INFINITY) top = fmaxf(top, m);
+            float y = h[c][i] * inv;
+            if (w) y *= wc[c].get(i);
+            y = fabsf(y) < INFINITY ? y : 0.f;  // what is no number has code 0
+            top = fmaxf(top, fabsf(y));
+            h[c][i] = y;
         }
     }
     top = block_reduce<true>(top, sm[1]);
-    const float scale = top > 0.f ? __fdiv_rn(top, 127.f) : 1.f;
+    float scale = __fdiv_rn(top, 127.f);
+    // 127 / top as two factors, so that a row of values near the smallest ones does not overflow it
+    const float lift = top < 0x1p-100f ? 0x1p60f : 1.f;
+    const float per = scale > 0.f ? __fdiv_rn(127.f, top * lift) : 0.f;
+    if (scale == 0.f) scale = 1.f;
     if (threadIdx.x == 0) a.scales[row] = scale;
     int8_t *codes = a.codes + row * a.codes_stride;
+    const float magic = 12582912.f;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-        const int at = ((int)threadIdx.x + c * (int)blockDim.x) * V, n = width - at;
+        const int first = at(c), n = width - first;
         uint32_t q[V / 4];
         float back[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float m = fabsf(h[c][i]);
-            const int code = m < INFINITY ? max(-127, min(127, __float2int_rn(__fdiv_rn(h[c][i], scale)))) : 0;
-            back[i] = (float)code * scale;
-            if (i % 4 == 0) q[i / 4] = (uint32_t)code & 0xFFu;
-            else q[i / 4] |= ((uint32_t)code & 0xFFu) << (8 * (i % 4));
+        for (int i = 0; i < V; i += 4) {
+            uint32_t bits[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float t = __fadd_rn(__fmul_rn(h[c][i + j] * lift, per), magic);
+                bits[j] = __float_as_uint(t);
+                back[i + j] = (t - magic) * scale;
+            }
+            q[i / 4] = prmt(prmt(bits[0], bits[1], 0x0040u), prmt(bits[2], bits[3], 0x0040u), 0x5410u);
         }
-        if (VEC && n >= V) {
-            if constexpr (V == 8) *reinterpret_cast<uint2 *>(codes + at) = make_uint2(q[0], q[1]);
-            else *reinterpret_cast<uint32_t *>(codes + at) = q[0];
-        } else {
+        if (VEC && n > 0) {
+            if constexpr (V == 8) *reinterpret_cast<uint2 *>(codes + first) = make_uint2(q[0], q[1]);
+            else *reinterpret_cast<uint32_t *>(codes + first) = q[0];
+        } else if (!VEC) {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (i < n) codes[at + i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
+                if (i < n) codes[first + i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
         }
         if (a.rows_out) {
-            const size_t o = row * a.rows_stride + at;
+            const size_t o = row * a.rows_stride + first;
             if (a.rows_dtype == QWN_DTYPE_F32) store_chunk<VEC>(static_cast<float *>(a.rows_out) + o, back, n);
             else if (a.rows_dtype == QWN_DTYPE_F16) store_chunk<VEC>(static_cast<__half *>(a.rows_out) + o, back, n);
             else store_chunk<VEC>(static_cast<__nv_bfloat16 *>(a.rows_out) + o, back, n);
@@ -174,12 +226,17 @@ cudaError_t launch_norm(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
     const uint32_t chunks = (a.width + V - 1) / V;
     auto threads = [&](uint32_t ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
-    if (threads(1) <= 256) rmsnorm_q8_kernel<T, 1, VEC><<<rows, threads(1), 0, s>>>(a);
-    else if (threads(2) <= 256) rmsnorm_q8_kernel<T, 2, VEC><<<rows, threads(2), 0, s>>>(a);
-    else if (threads(4) <= 512) rmsnorm_q8_kernel<T, 4, VEC><<<rows, threads(4), 0, s>>>(a);
-    else rmsnorm_q8_kernel<T, 8, VEC><<<rows, threads(8), 0, s>>>(a);
-    count_launch();
-    return cudaGetLastError();
+    // Up to two rows per SM: wide CTAs answer sooner (1 x 1536 fp32: 1.9 us with
+    // one chunk per thread, 2.3 with four).  More: small CTAs with several
+    // chunks each keep more loads in flight per SM (8191 x 6144 fp16: 69 us with
+    // four chunks, 94 with one; 4096 x 1536 bf16: 10.2 with two, 11.2 with one).
+    const bool few = rows <= 296;
+    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, VEC>, dim3(rows), threads(1), s, a);
+    if (threads(2) <= (few ? 1024u : 256u))
+        return launch_next(rmsnorm_q8_kernel<T, 2, VEC>, dim3(rows), threads(2), s, a);
+    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, VEC>, dim3(rows), threads(4), s, a);
+    if (V == 8 || threads(8) <= 512) return launch_next(rmsnorm_q8_kernel<T, 8, VEC>, dim3(rows), threads(8), s, a);
+    return launch_next(rmsnorm_q8_kernel<T, 64 / V, VEC>, dim3(rows), threads(64 / V), s, a);
 }
 
 template <typename T>
@@ -230,7 +287,7 @@ QWN_CUDA_ABI_API int qwn_rmsnorm_q8(const QwnRmsNormQ8Request *r) {
         return !p || ((uintptr_t)p % bytes == 0 && s % bytes == 0);
     };
     const uint64_t ro = v * re < 16 ? v * re : 16;
-    const bool vec = on(r->x_dev, a.x_stride * es, 16) && on(r->residual_dev, a.residual_stride * es, 16) &&
+    const bool vec = r->width % v == 0 && on(r->x_dev, a.x_stride * es, 16) && on(r->residual_dev, a.residual_stride * es, 16) &&
                      on(r->residual_out_dev, a.residual_out_stride * es, 16) && on(r->weight_dev, 0, 16) &&
                      on(r->codes_dev, a.codes_stride, v) && on(r->rows_out_dev, a.rows_stride * re, ro);
     DeviceScope scope(r->device_id);

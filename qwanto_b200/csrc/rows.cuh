@@ -29,6 +29,26 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
 }
 
+// launch a kernel that may start while the stream's previous one still runs (it
+// waits for it itself) and lets the next one start
+template <typename K, typename... Args>
+cudaError_t launch_next(K kernel, dim3 grid, uint32_t threads, cudaStream_t s, const Args &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    note_early_trigger();
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e == cudaSuccess) count_launch();
+    else cudaGetLastError();  // reported here, not by a later launch
+    return e;
+}
+
 inline bool dtype_ok(uint32_t d) { return d == QWN_DTYPE_F32 || d == QWN_DTYPE_F16 || d == QWN_DTYPE_BF16; }
 inline int invalid(const char *msg) {
     set_error(msg);
