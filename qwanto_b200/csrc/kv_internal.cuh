@@ -59,7 +59,7 @@ inline bool header_ok(const QwnCudaAbiHeader &h, size_t expected) {
     return h.abi_version == QWN_CUDA_ABI_VERSION && h.struct_size >= expected;
 }
 
-inline size_t tile_bytes_of(uint32_t codec) {
+__host__ __device__ constexpr size_t tile_bytes_of(uint32_t codec) {
     switch (codec) {
         case QWN_KV_CODEC_Q8_B64_F32: return 4352;
         case QWN_KV_CODEC_Q8_HEAD_F16: return 4160;
@@ -293,6 +293,13 @@ __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t by
         "l"(src), "r"(bytes), "r"(smem_u32(bar))
         : "memory");
 }
+// asynchronous 16-byte copies global -> shared memory, in groups
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    const uint32_t a = smem_u32(dst);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t d;
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));

@@ -12,6 +12,16 @@
 //     x'[i] = x[i] c[p] - x[j] s[p],   x'[j] = x[j] c[p] + x[i] s[p]
 // in fp32 with every product and sum rounded by itself, so that K's codes do
 // not depend on how the compiler contracts.
+//
+// Bound by HBM: rows in, rotated Q and pages out (prompts), by the launch for
+// one token per sequence.  Two ways through the data:
+//  - one warp per row and head, four dims per lane (store_token's layout): one
+//    token per sequence, and the tiles that a prompt fills in part;
+//  - one CTA per tile and kv head where all 16 tokens of the tile are new: 8
+//    lanes per row, which hold dims 8j.. and 64 + 8j.., so that a pair of
+//    halves meets in one lane and a maximum over a head takes 3 shuffles for 4
+//    rows (with 4 dims per lane, 4 + 5 per row); the tile is put together in
+//    shared memory and leaves in 16-byte stores.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,12 +40,24 @@ struct RowMap {
     uint32_t num_seqs, num_rows;
 };
 
-// the position in the cache of row r and its sequence; false (and the status
-// latched) when the row belongs to none or lies outside its sequence
-__device__ __forceinline__ bool find_row(const StoreGeo &g, const RowMap &m, uint32_t row, int32_t &seq, int32_t &pos,
+// whether a position of a sequence holds a token; latches what is wrong with it
+__device__ __forceinline__ bool place_ok(const StoreGeo &g, int32_t seq, int64_t pos, bool tell) {
+    if (seq < 0 || (uint32_t)seq >= g.max_seqs) {
+        if (tell) latch(g.status, QWN_KV_STATUS_BAD_SEQUENCE);
+        return false;
+    }
+    if (pos < 0 || pos >= g.seq_lens[seq]) {
+        if (tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
+        return false;
+    }
+    return true;
+}
+
+// the sequence of a row and its position in the cache; false where there is none
+__device__ __forceinline__ bool find_row(const StoreGeo &g, const RowMap &m, uint32_t row, int32_t &seq, int64_t &pos,
                                          bool tell) {
     uint32_t i = row;
-    int32_t b = (int32_t)row, e = b + 1;
+    int64_t b = row, e = b + 1;
     if (m.row_begin) {
         uint32_t lo = 0, hi = m.num_seqs;  // the last i with row_begin[i] <= row
         while (hi - lo > 1) {
@@ -46,24 +68,15 @@ __device__ __forceinline__ bool find_row(const StoreGeo &g, const RowMap &m, uin
         i = lo;
         b = m.row_begin[i];
         e = m.row_begin[i + 1];
-        if ((int32_t)row < b || (int32_t)row >= e) {
+        if ((int64_t)row < b || (int64_t)row >= e) {
             if (tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
             return false;
         }
     }
     seq = m.seq_ids ? m.seq_ids[i] : (int32_t)i;
-    if (seq < 0 || (uint32_t)seq >= g.max_seqs) {
-        if (tell) latch(g.status, QWN_KV_STATUS_BAD_SEQUENCE);
-        return false;
-    }
-    const int32_t len = g.seq_lens[seq];
-    const int64_t p = (m.first_pos ? (int64_t)m.first_pos[i] : (int64_t)len - ((int64_t)e - b)) + ((int64_t)row - b);
-    if (p < 0 || p >= len) {
-        if (tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
-        return false;
-    }
-    pos = (int32_t)p;
-    return true;
+    const bool known = seq >= 0 && (uint32_t)seq < g.max_seqs;
+    pos = (m.first_pos ? (int64_t)m.first_pos[i] : known ? (int64_t)g.seq_lens[seq] - (e - b) : 0) + (row - b);
+    return place_ok(g, seq, pos, tell);
 }
 
 // the lane's part of a position's rotation: its four dims' cosines and sines,
@@ -120,6 +133,312 @@ __device__ __forceinline__ float4 rotate(float4 x, const Turn &t, bool neighbour
                        turn_first(x.z, y.z, t.c[2], t.s[2]), turn_first(x.w, y.w, t.c[3], t.s[3]));
 }
 
+// ---------------------------------------------------------------------------
+// whole tiles: 8 lanes per row, lane j holds dims 8j..8j+7 and 64+8j..64+8j+7
+// ---------------------------------------------------------------------------
+struct Row16 {
+    float v[16];
+    __device__ __forceinline__ static int dim(int i, int j) { return i < 8 ? 8 * j + i : 56 + 8 * j + i; }
+};
+// the same as it is in memory: loads that are issued long before their use
+template <typename T>
+struct Raw16 {
+    uint4 w[sizeof(T) == 4 ? 4 : 2];
+    __device__ __forceinline__ void load(const T *row, int j) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = *reinterpret_cast<const uint4 *>(row + Row16::dim(4 * q, j));
+        } else {
+            w[0] = *reinterpret_cast<const uint4 *>(row + 8 * j);
+            w[1] = *reinterpret_cast<const uint4 *>(row + 64 + 8 * j);
+        }
+    }
+    __device__ __forceinline__ Row16 row() const {
+        Row16 r;
+#pragma unroll
+        for (int q = 0; q < (int)(sizeof(w) / 16); q++) {
+            const uint32_t u[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (sizeof(T) == 4) {
+                    r.v[4 * q + i] = __uint_as_float(u[i]);
+                } else if constexpr (std::is_same_v<T, __half>) {
+                    r.v[8 * q + 2 * i] = h2f((uint16_t)u[i]);
+                    r.v[8 * q + 2 * i + 1] = h2f((uint16_t)(u[i] >> 16));
+                } else {
+                    r.v[8 * q + 2 * i] = __uint_as_float(u[i] << 16);
+                    r.v[8 * q + 2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                }
+            }
+        }
+        return r;
+    }
+};
+template <typename T>
+__device__ __forceinline__ void store16(T *row, int j, const Row16 &r) {
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        store4(row + Row16::dim(4 * q, j), make_float4(r.v[4 * q], r.v[4 * q + 1], r.v[4 * q + 2], r.v[4 * q + 3]));
+}
+__device__ __forceinline__ void store16(__half *row, int j, const Row16 &r) {
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+        *reinterpret_cast<uint4 *>(row + 64 * q + 8 * j) =
+            make_uint4(pack_h2(r.v[8 * q], r.v[8 * q + 1]), pack_h2(r.v[8 * q + 2], r.v[8 * q + 3]),
+                       pack_h2(r.v[8 * q + 4], r.v[8 * q + 5]), pack_h2(r.v[8 * q + 6], r.v[8 * q + 7]));
+}
+__device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16 *row, int j, const Row16 &r) {
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+        *reinterpret_cast<uint4 *>(row + 64 * q + 8 * j) =
+            make_uint4(pack_b2(r.v[8 * q], r.v[8 * q + 1]), pack_b2(r.v[8 * q + 2], r.v[8 * q + 3]),
+                       pack_b2(r.v[8 * q + 4], r.v[8 * q + 5]), pack_b2(r.v[8 * q + 6], r.v[8 * q + 7]));
+}
+
+// a row's rotation for this lane.  WHOLE: all 128 dims as halves, the pairs are
+// (v[i], v[i + 8]); otherwise the partner's values are read again (from L1).
+template <bool WHOLE>
+struct Turn16 {
+    float c[8], s[8];
+    const float *row;
+    __device__ __forceinline__ void load(const float *r, int j) {
+        row = r;
+        if (WHOLE) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const float4 x = *reinterpret_cast<const float4 *>(r + 8 * j + 4 * q);
+                const float4 y = *reinterpret_cast<const float4 *>(r + 64 + 8 * j + 4 * q);
+                c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
+                s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
+            }
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot, bool neighbours) const {
+        if (WHOLE) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float a = x.v[i], b = x.v[i + 8];
+                x.v[i] = turn_first(a, b, c[i], s[i]);
+                x.v[i + 8] = turn_second(b, a, c[i], s[i]);
+            }
+            return;
+        }
+        const int half = rot >> 1;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            float *v = x.v + 4 * q;
+            const int d = Row16::dim(4 * q, j);
+            if (d >= rot) continue;
+            if (neighbours) {
+                const float2 cc = *reinterpret_cast<const float2 *>(row + (d >> 1));
+                const float2 ss = *reinterpret_cast<const float2 *>(row + half + (d >> 1));
+                const float a = v[0], b = v[1], e = v[2], f = v[3];
+                v[0] = turn_first(a, b, cc.x, ss.x), v[1] = turn_second(b, a, cc.x, ss.x);
+                v[2] = turn_first(e, f, cc.y, ss.y), v[3] = turn_second(f, e, cc.y, ss.y);
+            } else {
+                const bool second = d >= half;
+                const int p = second ? d - half : d;
+                const float4 cc = *reinterpret_cast<const float4 *>(row + p);
+                const float4 ss = *reinterpret_cast<const float4 *>(row + half + p);
+                const float4 o = load4(from + (second ? p : d + half));
+                const float cs[4] = {cc.x, cc.y, cc.z, cc.w}, sn[4] = {ss.x, ss.y, ss.z, ss.w}, y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    v[i] = second ? turn_second(v[i], y[i], cs[i], sn[i]) : turn_first(v[i], y[i], cs[i], sn[i]);
+            }
+        }
+    }
+};
+
+template <int LANES, bool MIN>
+__device__ __forceinline__ float lanes_extreme(float v) {
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MIN ? fminf(v, u) : fmaxf(v, u);
+    }
+    return v;
+}
+__device__ __forceinline__ void put2(uint8_t *p, uint32_t a, uint32_t b) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(a, b);
+}
+
+// K (which 0) or V of the row of token t into the tile's image, by
+// store_token's rules and layout.  Returns false, in every lane that sees it,
+// for what those rules take in an order of their own: a NaN, or a minimum of
+// zero (whose sign is the first zero's); the tile then goes row by row.
+template <int CODEC>
+__device__ bool put_row(uint8_t *tile, int t, int which, const Row16 &x, int j);
+
+__device__ __forceinline__ void put_q8(uint8_t *tile, int t, int which, const Row16 &x, int j, float s0, float s1) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float s = h ? s1 : s0;
+        const float *v = x.v + 8 * h;
+        const uint32_t lo = q8_pack4(make_float4(v[0], v[1], v[2], v[3]), s);
+        const uint32_t hi = q8_pack4(make_float4(v[4], v[5], v[6], v[7]), s);
+        const int d = 64 * h + 8 * j;
+        if (!which) {
+            put2(tile + k8_off(t, d), lo, hi);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) tile[v8_off(t, d + i)] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        }
+    }
+}
+__device__ __forceinline__ float finite_top(const float *v) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float a = fabsf(v[i]);
+        if (a < INFINITY) m = fmaxf(m, a);
+    }
+    return m;
+}
+template <>
+__device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q8_HEAD_F16>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
+    const uint16_t h = head_scale16(lanes_extreme<8, false>(fmaxf(finite_top(x.v), finite_top(x.v + 8))));
+    const float s = h2f(h);
+    put_q8(tile, t, which, x, j, s, s);
+    if (j == 0) *reinterpret_cast<uint16_t *>(tile + (which ? 4128 : 4096) + s16_off(t)) = h;
+    return true;
+}
+template <>
+__device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q8_B64_F32>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
+    float s[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float m = lanes_extreme<8, false>(finite_top(x.v + 8 * h));
+        s[h] = m > 0.f ? __fdiv_rn(m, 127.f) : 1.f;
+    }
+    put_q8(tile, t, which, x, j, s[0], s[1]);
+    if (j < 2) *reinterpret_cast<float *>(tile + (which ? 4224 : 4096) + s32_off(t, j)) = j ? s[1] : s[0];
+    return true;
+}
+template <>
+__device__ __forceinline__ bool put_row<QWN_KV_CODEC_F16>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float *v = x.v + 8 * h;
+        *reinterpret_cast<uint4 *>(tile + f16_off(which, t, 64 * h + 8 * j)) =
+            make_uint4(f16_bits(v[0]) | (f16_bits(v[1]) << 16), f16_bits(v[2]) | (f16_bits(v[3]) << 16),
+                       f16_bits(v[4]) | (f16_bits(v[5]) << 16), f16_bits(v[6]) | (f16_bits(v[7]) << 16));
+    }
+    return true;
+}
+// smallest and largest of a group held by LANES lanes' halves h, range and its
+// inverse; false where the row-by-row order matters
+struct Span {
+    float mn, range, inv;
+};
+template <int LANES>
+__device__ __forceinline__ bool group_span(const float *v, Span &g) {
+    float mn = v[0], mx = v[0];
+    bool nan = v[0] != v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        mn = fminf(mn, v[i]);
+        mx = fmaxf(mx, v[i]);
+        nan |= v[i] != v[i];
+    }
+    g.mn = lanes_extreme<LANES, true>(mn);
+    g.range = __fsub_rn(lanes_extreme<LANES, false>(mx), g.mn);
+    g.inv = g.range > 1e-8f ? __fdiv_rn(1.0f, g.range) : 0.f;
+    return !nan && g.mn != 0.f;
+}
+__device__ __forceinline__ uint32_t span_params(const Span &g) {
+    return (uint32_t)tq_f32_to_f16(g.range) | ((uint32_t)tq_f32_to_f16(g.mn) << 16);
+}
+template <>
+__device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q4_G32>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
+    bool ok = true;
+    uint32_t nib[2];  // the half's eight codes, dim i in nibble i
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float *v = x.v + 8 * h;
+        Span g;
+        ok &= group_span<4>(v, g);
+        nib[h] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) nib[h] |= tq_code(v[i], g.mn, g.inv, 15.f) << (4 * i);
+        const int c = 2 * h + (j >> 2);
+        if ((j & 3) == 0)
+            *reinterpret_cast<uint32_t *>(tile + (which ? 2304 : 2048) + 32 * (t & 7) + 8 * c + 4 * (t >> 3)) =
+                span_params(g);
+    }
+    if (!which) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // byte i: dims i and i + 4
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                w |= (((nib[h] >> (4 * i)) & 15u) | (((nib[h] >> (4 * i + 16)) & 15u) << 4)) << (8 * i);
+            *reinterpret_cast<uint32_t *>(tile + 64 * t + 16 * (j & 3) + 4 * (2 * h + (j >> 2))) = w;
+        }
+    } else {
+        // a byte holds dims gid and gid + 8 of a block of 16: lanes j and j + 1; the even one writes half 0
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, j & 1 ? nib[0] : nib[1], 1);
+        const int h = j & 1, mb = 4 * h + (j >> 1);
+        const uint32_t low = h ? other : nib[0], high = h ? nib[1] : other;
+#pragma unroll
+        for (int gid = 0; gid < 8; gid++) {
+            const int lv = 4 * gid + ((t & 7) >> 1);
+            const int chunk = (mb >> 2) ^ ((lv >> 2) & 1);
+            tile[1024 + 32 * lv + 16 * chunk + 4 * (mb & 3) + (t >> 3) + 2 * (t & 1)] =
+                (uint8_t)(((low >> (4 * gid)) & 15u) | (((high >> (4 * gid)) & 15u) << 4));
+        }
+    }
+    return ok;
+}
+// where the codes of dims 2m, 2m + 1 of both halves are (tq35_put's layout): the
+// even ones in nibble n of words `even` and `even + even_step`, the odd ones' low
+// bits in nibble n of word `odd`, half 1's two high bits in field n of `plane`
+struct TqPlace {
+    uint32_t even, even_step, odd, plane, n;
+};
+__device__ __forceinline__ TqPlace tq_place(int which, int t, int m) {
+    if (!which) {
+        const uint32_t tig = m >> 3;
+        return {32u * t + 8 * tig, 4, 512u + 16 * t + 4 * tig, 768u + 8 * t + 2 * tig, (uint32_t)lb_k_nibble(m)};
+    }
+    const int r = m & 15;
+    const uint32_t lv = ((r & 7) << 2) | ((t & 7) >> 1), b = m >> 4;
+    return {16 * lv + 4 * b, 8, 512 + 8 * lv + 4 * b, 768 + 4 * lv + 2 * b,
+            (uint32_t)((r >> 3) + 2 * (t >> 3) + 4 * (t & 1))};
+}
+// the image starts as zeros: a word holds codes of several lanes
+template <>
+__device__ __forceinline__ bool put_row<QWN_KV_CODEC_TQ35_G64>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
+    uint8_t *half = tile + which * 1024;
+    bool ok = true;
+    uint32_t code[16];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        Span g;
+        ok &= group_span<8>(x.v + 8 * h, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) code[8 * h + i] = tq_code(x.v[8 * h + i], g.mn, g.inv, i & 1 ? 7.f : 15.f);
+        if (j == 0)
+            *reinterpret_cast<uint32_t *>(half + 896 + 16 * (t & 7) + 8 * h + 4 * (t >> 3)) = span_params(g);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {  // dims 2i and 2i + 1 of both halves
+        const TqPlace p = tq_place(which, t, 4 * j + i);
+        auto put = [&](uint32_t at, uint32_t v) { atomicOr(reinterpret_cast<uint32_t *>(half + at), v); };
+        const uint32_t o0 = code[2 * i + 1], o1 = code[9 + 2 * i];
+        put(p.even, code[2 * i] << (4 * p.n));
+        put(p.even + p.even_step, code[8 + 2 * i] << (4 * p.n));
+        put(p.odd, (o0 | ((o1 & 1u) << 3)) << (4 * p.n));
+        put(p.plane & ~3u, (o1 >> 1) << (2 * p.n + 8 * (p.plane & 3u)));
+    }
+    return ok;
+}
+
 struct RotaryArgs {
     RowMap rows;
     const int32_t *rotary_pos;
@@ -129,10 +448,40 @@ struct RotaryArgs {
     uint64_t query_stride, key_stride, value_stride;
 };
 
+// place_ok with the row's angles
+__device__ __forceinline__ bool row_ok(const StoreGeo &g, const RotaryArgs &a, int32_t seq, int64_t pos, uint32_t row,
+                                       int32_t &angle, bool tell) {
+    if (!place_ok(g, seq, pos, tell)) return false;
+    if (!a.rot) return true;
+    angle = a.rotary_pos ? a.rotary_pos[row] : (int32_t)pos;
+    if (angle >= 0 && (uint32_t)angle < a.max_position) return true;
+    if (tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
+    return false;
+}
+
 __device__ __forceinline__ void store_any(void *out, uint32_t dtype, size_t at, float4 v) {
     if (dtype == QWN_DTYPE_F32) store4(static_cast<float *>(out) + at, v);
     else if (dtype == QWN_DTYPE_F16) store4(static_cast<__half *>(out) + at, v);
     else store4(static_cast<__nv_bfloat16 *>(out) + at, v);
+}
+
+// one row and head by a warp: rotate and store
+template <int CODEC, typename T>
+__device__ __forceinline__ void append_row(const StoreGeo &g, const RotaryArgs &a, bool ok, int32_t seq, int32_t pos,
+                                           int32_t angle, uint32_t row, uint32_t slot, float4 x, float4 v,
+                                           void *query_out, int lane) {
+    if (ok && a.rot) {
+        const Turn t = load_turn(a.table + (size_t)angle * a.rot, (int)a.rot, a.neighbours, lane);
+        x = rotate(x, t, a.neighbours);
+    }
+    if (slot < g.kv_heads) {
+        uint8_t *tile = ok ? tile_for(g, seq, a.layer, slot, pos) : nullptr;
+        if (tile) store_token<CODEC>(tile, pos & 15, x, v, lane);
+    } else {
+        store_any(query_out, a.query_out_dtype,
+                  ((size_t)row * a.query_heads + slot - g.kv_heads) * kHeadDim + 4 * lane,
+                  ok ? x : make_float4(0.f, 0.f, 0.f, 0.f));
+    }
 }
 
 // one warp per (row, head): the kv heads (K and V together), then the query heads
@@ -143,53 +492,333 @@ __global__ void __launch_bounds__(128) append_rotary_kernel(StoreGeo g, RotaryAr
     const int lane = threadIdx.x & 31;
     const uint32_t slots = g.kv_heads + a.query_heads;
     const uint32_t row = (uint32_t)(wg / slots), slot = (uint32_t)(wg % slots);
+    launch_dependents();
+    wait_previous();
     if (row >= a.rows.num_rows) return;
-    int32_t seq, pos = 0;
-    bool ok = find_row(g, a.rows, row, seq, pos, lane == 0 && slot == 0);
-    const int32_t angle = ok && a.rotary_pos ? a.rotary_pos[row] : pos;
-    if (ok && a.rot && (angle < 0 || (uint32_t)angle >= a.max_position)) {
-        if (lane == 0 && slot == 0) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
-        ok = false;
+    const bool is_kv = slot < g.kv_heads;
+    const float4 x = is_kv ? load4(key + (size_t)row * a.key_stride + slot * kHeadDim + 4 * lane)
+                           : load4(query + (size_t)row * a.query_stride + (slot - g.kv_heads) * kHeadDim + 4 * lane);
+    const float4 v = is_kv ? load4(value + (size_t)row * a.value_stride + slot * kHeadDim + 4 * lane) : x;
+    int32_t seq = 0, angle = 0;
+    int64_t pos = 0;
+    const bool tell = lane == 0 && slot == 0;
+    const bool ok = find_row(g, a.rows, row, seq, pos, tell) && row_ok(g, a, seq, pos, row, angle, tell);
+    append_row<CODEC, T>(g, a, ok, seq, (int32_t)pos, angle, row, slot, x, v, query_out, lane);
+}
+
+// the rows of a batch by tiles of the cache: unit u is tile u - base_i of
+// sequence i, base_i = row_begin[i] / 16 + 2 i.  n rows touch at most n / 16 + 2
+// tiles, so that num_rows / 16 + 2 num_seqs units cover them all without a
+// table; some stay empty.
+struct Unit {
+    uint32_t first, count;  // rows
+    int32_t seq;            // -1: none such
+    int64_t pos;            // of the first row
+};
+__device__ __forceinline__ bool find_unit(const StoreGeo &g, const RowMap &m, uint32_t u, Unit &t) {
+    uint32_t lo = 0, hi = m.num_seqs;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if ((uint32_t)max(m.row_begin[mid], 0) / 16 + 2 * mid <= u) lo = mid;
+        else hi = mid;
     }
-    Turn t;
-    if (ok && a.rot) t = load_turn(a.table + (size_t)angle * a.rot, (int)a.rot, a.neighbours, lane);
-    if (slot < g.kv_heads) {
-        if (!ok) return;
-        uint8_t *tile = tile_for(g, seq, a.layer, slot, pos);
-        if (!tile) return;
-        float4 k = load4(key + (size_t)row * a.key_stride + slot * kHeadDim + 4 * lane);
-        const float4 v = load4(value + (size_t)row * a.value_stride + slot * kHeadDim + 4 * lane);
-        if (a.rot) k = rotate(k, t, a.neighbours);
-        store_token<CODEC>(tile, pos & 15, k, v, lane);
-    } else {
-        const uint32_t h = slot - g.kv_heads;
-        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ok) {
-            q = load4(query + (size_t)row * a.query_stride + h * kHeadDim + 4 * lane);
-            if (a.rot) q = rotate(q, t, a.neighbours);
+    const int64_t b = max(m.row_begin[lo], 0), e = min((int64_t)m.row_begin[lo + 1], (int64_t)m.num_rows);
+    const int64_t base = b / 16 + 2 * (int64_t)lo;
+    if (e <= b || (int64_t)u < base) return false;
+    t.seq = m.seq_ids ? m.seq_ids[lo] : (int32_t)lo;
+    if (t.seq < 0 || (uint32_t)t.seq >= g.max_seqs) t.seq = -1;
+    const int64_t p0 = m.first_pos ? (int64_t)m.first_pos[lo] : t.seq < 0 ? 0 : (int64_t)g.seq_lens[t.seq] - (e - b);
+    const int64_t tile = (p0 >> 4) + ((int64_t)u - base);
+    const int64_t from = max(p0, tile << 4), to = min(p0 + (e - b), (tile + 1) << 4);
+    if (from >= to) return false;
+    t.first = (uint32_t)(b + (from - p0));
+    t.count = (uint32_t)(to - from);
+    t.pos = from;
+    return true;
+}
+// rows before the first sequence's and after the last one's: unit 0 looks at them
+struct Gaps {
+    int64_t before, after, count;
+    __device__ __forceinline__ explicit Gaps(const RowMap &m) {
+        const int64_t n = m.num_rows;
+        before = min(max((int64_t)m.row_begin[0], (int64_t)0), n);
+        after = min(max((int64_t)m.row_begin[m.num_seqs], before), n);
+        count = before + n - after;
+    }
+    __device__ __forceinline__ uint32_t row(int64_t i) const { return (uint32_t)(i < before ? i : after + i - before); }
+};
+
+constexpr int kTileThreads = 128;  // 16 rows of 8 lanes
+
+// one CTA per (tile, kv head): its K and V, and the query heads that read it
+template <int CODEC, typename T, bool WHOLE>
+__global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, RotaryArgs a, const T *query,
+                                                                    const T *key, const T *value, void *query_out) {
+    constexpr int kImage = (int)tile_bytes_of(CODEC), kAhead = sizeof(T) == 4 ? 2 : 4;  // query heads in flight
+    __shared__ __align__(16) uint8_t buf[2 * 16 * kHeadDim * 4];  // the tile's image, or K and V of its rows in fp32
+    __shared__ uint8_t stored[16];
+    const uint32_t head = blockIdx.y, group = a.query_heads / g.kv_heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int j = threadIdx.x & 7, r = threadIdx.x >> 3;
+    launch_dependents();
+    wait_previous();
+    const Row16 zero = {};
+    auto put_query = [&](uint32_t row, uint32_t q, const Row16 &x) {
+        const size_t at = ((size_t)row * a.query_heads + head * group + q) * kHeadDim;
+        if (a.query_out_dtype == QWN_DTYPE_F32) store16(static_cast<float *>(query_out) + at, j, x);
+        else if (a.query_out_dtype == QWN_DTYPE_F16) store16(static_cast<__half *>(query_out) + at, j, x);
+        else store16(static_cast<__nv_bfloat16 *>(query_out) + at, j, x);
+    };
+    if (blockIdx.x == 0) {  // rows of no sequence
+        const Gaps gaps(a.rows);
+        if (gaps.count > 0 && head == 0 && threadIdx.x == 0) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
+        for (int64_t i = r; i < gaps.count; i += 16)
+            for (uint32_t q = 0; q < group; q++) put_query(gaps.row(i), q, zero);
+    }
+    Unit u;
+    if (!find_unit(g, a.rows, blockIdx.x, u)) return;
+    const bool have = (uint32_t)r < u.count;
+    const uint32_t row = u.first + (have ? (uint32_t)r : 0);
+    const T *kr = key + (size_t)row * a.key_stride + head * kHeadDim;
+    const T *vr = value + (size_t)row * a.value_stride + head * kHeadDim;
+    const T *qr = query + (size_t)row * a.query_stride + (size_t)head * group * kHeadDim;
+    Raw16<T> kw, vw, qw[kAhead];
+    kw.load(kr, j);
+    vw.load(vr, j);
+#pragma unroll
+    for (uint32_t q = 0; q < kAhead; q++)
+        if (q < group) qw[q].load(qr + q * kHeadDim, j);
+    // the rows share a tile, whose page one of their positions finds
+    const int64_t some = max(u.pos, (int64_t)0);
+    uint8_t *tile = nullptr;
+    if (u.seq >= 0 && some < min(u.pos + u.count, (int64_t)g.seq_lens[u.seq]))
+        tile = tile_for(g, u.seq, a.layer, head, (int32_t)some);
+    int32_t angle = 0;
+    const bool ok = have && row_ok(g, a, u.seq, u.pos + r, row, angle, j == 0 && head == 0);
+    const bool turns = ok && (WHOLE || a.rot);
+    Turn16<WHOLE> turn;
+    if (turns) turn.load(a.table + (size_t)angle * a.rot, j);
+    for (uint32_t q0 = 0; q0 < group; q0 += kAhead) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const uint32_t q = q0 + i;
+            if (q >= group) break;
+            Row16 x = ok ? qw[i].row() : zero;
+            if (turns) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot, a.neighbours);
+            if (!WHOLE) __syncwarp();  // query_out may be query: every lane has read its partner's values
+            if (have) put_query(row, q, x);
+            if (q + kAhead < group) qw[i].load(qr + (q + kAhead) * kHeadDim, j);
         }
-        store_any(query_out, a.query_out_dtype, ((size_t)row * a.query_heads + h) * kHeadDim + 4 * lane, q);
+    }
+    Row16 k = kw.row();
+    const Row16 v = vw.row();
+    if (turns) turn.apply(k, kr, j, (int)a.rot, a.neighbours);
+    if (CODEC == QWN_KV_CODEC_TQ35_G64)
+        for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
+            reinterpret_cast<uint4 *>(buf)[i] = make_uint4(0, 0, 0, 0);
+    // 16 new tokens: the whole tile is put together here
+    if (__syncthreads_and(ok && u.count == 16 && tile)) {
+        const bool fine = put_row<CODEC>(buf, r, 0, k, j) & put_row<CODEC>(buf, r, 1, v, j);
+        if (__syncthreads_and(fine)) {
+            for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
+                reinterpret_cast<uint4 *>(tile)[i] = reinterpret_cast<const uint4 *>(buf)[i];
+            return;
+        }
+    }
+    // a tile filled in part, or one whose codes depend on its values' order: token by token
+    if (j == 0) stored[r] = ok;
+    float *rows = reinterpret_cast<float *>(buf);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int d = Row16::dim(4 * q, j);
+        store4(rows + r * kHeadDim + d, make_float4(k.v[4 * q], k.v[4 * q + 1], k.v[4 * q + 2], k.v[4 * q + 3]));
+        store4(rows + (16 + r) * kHeadDim + d, make_float4(v.v[4 * q], v.v[4 * q + 1], v.v[4 * q + 2], v.v[4 * q + 3]));
+    }
+    __syncthreads();
+    if (!tile) return;
+    for (uint32_t i = warp; i < u.count; i += kTileThreads / 32)
+        if (stored[i])
+            store_token<CODEC>(tile, (int)((u.pos + i) & 15), load4(rows + i * kHeadDim + 4 * lane),
+                               load4(rows + (16 + i) * kHeadDim + 4 * lane), lane);
+}
+
+// ---------------------------------------------------------------------------
+// the way back, by tiles: the tile into shared memory in 16-byte loads, its
+// rows out of it by 8 lanes each
+// ---------------------------------------------------------------------------
+template <int CODEC>
+__device__ Row16 take_row(const uint8_t *tile, int t, int which, int j);
+
+__device__ __forceinline__ Row16 take_q8(const uint8_t *tile, int t, int which, int j, float s0, float s1) {
+    Row16 x;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int d = 64 * h + 8 * j;
+        uint32_t b[8];
+        if (!which) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(tile + k8_off(t, d));
+#pragma unroll
+            for (int i = 0; i < 8; i++) b[i] = prmt(i < 4 ? w.x : w.y, 0x4B000000u, 0x7650u | (uint32_t)(i & 3));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) b[i] = 0x4B000000u | tile[v8_off(t, d + i)];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)  // 2^23 + code + 128, less that
+            x.v[8 * h + i] = (__uint_as_float(b[i]) - 8388736.f) * (h ? s1 : s0);
+    }
+    return x;
+}
+template <>
+__device__ __forceinline__ Row16 take_row<QWN_KV_CODEC_Q8_HEAD_F16>(const uint8_t *tile, int t, int which, int j) {
+    const float s = h2f(*reinterpret_cast<const uint16_t *>(tile + (which ? 4128 : 4096) + s16_off(t)));
+    return take_q8(tile, t, which, j, s, s);
+}
+template <>
+__device__ __forceinline__ Row16 take_row<QWN_KV_CODEC_Q8_B64_F32>(const uint8_t *tile, int t, int which, int j) {
+    const uint8_t *s = tile + (which ? 4224 : 4096);
+    return take_q8(tile, t, which, j, *reinterpret_cast<const float *>(s + s32_off(t, 0)),
+                   *reinterpret_cast<const float *>(s + s32_off(t, 1)));
+}
+template <>
+__device__ __forceinline__ Row16 take_row<QWN_KV_CODEC_F16>(const uint8_t *tile, int t, int which, int j) {
+    Row16 x;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(tile + f16_off(which, t, 64 * h + 8 * j));
+        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) x.v[8 * h + i] = h2f((uint16_t)(q[i >> 1] >> (16 * (i & 1))));
+    }
+    return x;
+}
+__device__ __forceinline__ float code_value(uint32_t code, float step, float mn) {
+    return fmaf(__uint_as_float(0x4B000000u | code) - 8388608.f, step, mn);
+}
+template <>
+__device__ __forceinline__ Row16 take_row<QWN_KV_CODEC_Q4_G32>(const uint8_t *tile, int t, int which, int j) {
+    Row16 x;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int c = 2 * h + (j >> 2), mb = 4 * h + (j >> 1);
+        const uint32_t par = *reinterpret_cast<const uint32_t *>(tile + (which ? 2304 : 2048) + 32 * (t & 7) + 8 * c +
+                                                                 4 * (t >> 3));
+        const float step = __fdiv_rn(h2f((uint16_t)par), 15.f), mn = h2f((uint16_t)(par >> 16));
+        const uint32_t w = which ? 0u : *reinterpret_cast<const uint32_t *>(tile + 64 * t + 16 * (j & 3) + 4 * c);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            uint32_t q;
+            if (!which) {
+                q = w >> (8 * (i & 3) + 4 * (i >> 2));
+            } else {
+                const int lv = 4 * i + ((t & 7) >> 1), chunk = (mb >> 2) ^ ((lv >> 2) & 1);
+                q = (uint32_t)tile[1024 + 32 * lv + 16 * chunk + 4 * (mb & 3) + (t >> 3) + 2 * (t & 1)] >> (4 * (j & 1));
+            }
+            x.v[8 * h + i] = code_value(q & 15u, step, mn);
+        }
+    }
+    return x;
+}
+template <>
+__device__ __forceinline__ Row16 take_row<QWN_KV_CODEC_TQ35_G64>(const uint8_t *tile, int t, int which, int j) {
+    const uint8_t *half = tile + which * 1024;
+    float mn[2], even[2], odd[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t par = *reinterpret_cast<const uint32_t *>(half + 896 + 16 * (t & 7) + 8 * h + 4 * (t >> 3));
+        mn[h] = h2f((uint16_t)(par >> 16));
+        even[h] = __fdiv_rn(h2f((uint16_t)par), 15.f);
+        odd[h] = __fdiv_rn(h2f((uint16_t)par), 7.f);
+    }
+    auto word = [&](uint32_t at) { return *reinterpret_cast<const uint32_t *>(half + at); };
+    Row16 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const TqPlace p = tq_place(which, t, 4 * j + i);
+        const uint32_t o = word(p.odd) >> (4 * p.n), hi = word(p.plane & ~3u) >> (2 * p.n + 8 * (p.plane & 3u));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t code = h ? ((o >> 3) & 1u) | ((hi & 3u) << 1) : o & 7u;
+            x.v[8 * h + 2 * i] = code_value((word(p.even + h * p.even_step) >> (4 * p.n)) & 15u, even[h], mn[h]);
+            x.v[8 * h + 2 * i + 1] = code_value(code, odd[h], mn[h]);
+        }
+    }
+    return x;
+}
+
+// one CTA per tile and `heads` kv heads: the next head's tile is on its way into
+// shared memory while this one's rows go out
+template <int CODEC, typename T>
+__global__ void __launch_bounds__(kTileThreads) load_tiles_kernel(StoreGeo g, RowMap m, uint32_t layer, uint32_t heads,
+                                                                  uint64_t key_stride, uint64_t value_stride, T *key,
+                                                                  T *value) {
+    constexpr int kImage = (int)tile_bytes_of(CODEC);
+    __shared__ __align__(16) uint8_t image[2][kImage];
+    const uint32_t h0 = blockIdx.y * heads, h1 = min(h0 + heads, g.kv_heads);
+    launch_dependents();
+    wait_previous();
+    const int j = threadIdx.x & 7, r = threadIdx.x >> 3;
+    const Row16 zero = {};
+    auto put = [&](uint32_t row, uint32_t head, const Row16 &k, const Row16 &v) {
+        if (key) store16(key + (size_t)row * key_stride + head * kHeadDim, j, k);
+        if (value) store16(value + (size_t)row * value_stride + head * kHeadDim, j, v);
+    };
+    if (blockIdx.x == 0) {  // rows of no sequence
+        const Gaps gaps(m);
+        if (gaps.count > 0 && h0 == 0 && threadIdx.x == 0) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
+        for (int64_t i = r; i < gaps.count; i += 16)
+            for (uint32_t h = h0; h < h1; h++) put(gaps.row(i), h, zero, zero);
+    }
+    Unit u;
+    if (!find_unit(g, m, blockIdx.x, u)) return;
+    // the rows share a tile of each head, whose page one of their positions finds
+    const int64_t some = max(u.pos, (int64_t)0);
+    const uint8_t *tile = nullptr;
+    if (u.seq >= 0 && some < min(u.pos + u.count, (int64_t)g.seq_lens[u.seq]))
+        tile = tile_for(g, u.seq, layer, h0, (int32_t)some);
+    const size_t next = (size_t)g.tpp * g.tile_bytes;  // the following head's tile
+    auto fetch = [&](uint32_t h) {
+        if (tile && h < h1)
+            for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
+                cp_async16(image[(h - h0) & 1] + 16 * i, tile + (h - h0) * next + 16 * i);
+        cp_async_commit();
+    };
+    fetch(h0);
+    const int64_t pos = u.pos + r;
+    const bool have = (uint32_t)r < u.count;
+    const bool ok = have && place_ok(g, u.seq, pos, j == 0 && h0 == 0) && tile;
+    const int t = (int)(pos & 15);
+    for (uint32_t h = h0; h < h1; h++) {
+        fetch(h + 1);
+        cp_async_wait1();
+        __syncthreads();
+        const uint8_t *in = image[(h - h0) & 1];
+        if (ok) put(u.first + r, h, take_row<CODEC>(in, t, 0, j), take_row<CODEC>(in, t, 1, j));
+        else if (have) put(u.first + r, h, zero, zero);
+        __syncthreads();  // before the tile after the next lands here
     }
 }
 
-// one warp per (row, head): K and V of a cached token back to rows
+// one warp per (row, head): K and V of a cached token back to rows (one token
+// per sequence, and rows that are not 16-byte aligned)
 template <int CODEC, typename T>
-__global__ void __launch_bounds__(128) load_tokens_kernel(StoreGeo g, RowMap m, uint32_t layer, uint64_t key_stride,
-                                                          uint64_t value_stride, T *key, T *value) {
+__global__ void __launch_bounds__(128) load_rows_kernel(StoreGeo g, RowMap m, uint32_t layer, uint64_t key_stride,
+                                                        uint64_t value_stride, T *key, T *value) {
     const uint64_t wg = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const uint32_t row = (uint32_t)(wg / g.kv_heads), h = (uint32_t)(wg % g.kv_heads);
+    launch_dependents();
+    wait_previous();
     if (row >= m.num_rows) return;
-    int32_t seq, pos;
+    int32_t seq = 0;
+    int64_t pos = 0;
     const uint8_t *tile = nullptr;
-    if (find_row(g, m, row, seq, pos, lane == 0 && h == 0)) tile = tile_for(g, seq, layer, h, pos);
+    if (find_row(g, m, row, seq, pos, lane == 0 && h == 0)) tile = tile_for(g, seq, layer, h, (int32_t)pos);
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (key)
-        store4(key + (size_t)row * key_stride + h * kHeadDim + 4 * lane,
-               tile ? load_token<CODEC>(tile, pos & 15, 0, lane) : zero);
-    if (value)
-        store4(value + (size_t)row * value_stride + h * kHeadDim + 4 * lane,
-               tile ? load_token<CODEC>(tile, pos & 15, 1, lane) : zero);
+    const size_t at = h * kHeadDim + 4 * lane;
+    const int t = (int)(pos & 15);
+    if (key) store4(key + (size_t)row * key_stride + at, tile ? load_token<CODEC>(tile, t, 0, lane) : zero);
+    if (value) store4(value + (size_t)row * value_stride + at, tile ? load_token<CODEC>(tile, t, 1, lane) : zero);
 }
 
 // f.operator()<CODEC, T>() for the pool's codec and the rows' type
@@ -214,10 +843,17 @@ cudaError_t with_codec(uint32_t codec, uint32_t dtype, F &&f) {
     }
 }
 
-// four values of a row are one access: rows start on four values
-bool rows_aligned(const void *p, uint64_t stride, uint32_t dtype) {
-    return (uintptr_t)p % (dtype == QWN_DTYPE_F32 ? 16 : 8) == 0 && stride % 4 == 0;
+uint64_t value_bytes(uint32_t dtype) { return dtype == QWN_DTYPE_F32 ? 4 : 2; }
+// rows start on `values` values
+bool rows_aligned(const void *p, uint64_t stride, uint32_t dtype, uint64_t values = 4) {
+    return (uintptr_t)p % (value_bytes(dtype) * values) == 0 && stride % values == 0;
 }
+// 16-byte accesses, which the tile kernels make
+bool rows_wide(const void *p, uint64_t stride, uint32_t dtype) {
+    return rows_aligned(p, stride, dtype, 16 / value_bytes(dtype));
+}
+// units of find_unit for a batch
+uint64_t unit_count(uint32_t rows, uint32_t seqs) { return (uint64_t)rows / 16 + 2 * (uint64_t)seqs; }
 }  // namespace
 }  // namespace qkv
 
@@ -265,17 +901,27 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
     a.query_stride = qs;
     a.key_stride = ks;
     a.value_stride = vs;
-    const uint64_t ctas = ((uint64_t)r->num_rows * (p->kv_heads + r->query_heads) + 3) / 4;
-    if (ctas > 0x7FFFFFFFull) return invalid("qwn_kv_append_rotary: too many rows for one call");
     const StoreGeo g = store_geo(p);
     cudaStream_t s = stream_of(p, r->stream);
+    // runs of rows go by tiles; one row per sequence, or rows off the 16-byte grid, one by one
+    // (16384 rows of 32 + 2 x 8 bf16 heads into 4-bit pages: TILES_US by tiles, ROWS_US one by one)
+    const bool tiles = r->row_begin_dev && rows_wide(r->key_dev, ks, r->dtype) && rows_wide(r->value_dev, vs, r->dtype) &&
+                       (!r->query_heads || (rows_wide(r->query_dev, qs, r->dtype) &&
+                                            rows_wide(r->query_out_dev, q_width, r->query_out_dtype)));
+    const uint64_t ctas = tiles ? unit_count(r->num_rows, r->num_seqs)
+                                : ((uint64_t)r->num_rows * (p->kv_heads + r->query_heads) + 3) / 4;
+    if (ctas > 0x7FFFFFFFull || (tiles && p->kv_heads > 65535u))
+        return invalid("qwn_kv_append_rotary: too many rows for one call");
     const cudaError_t e = with_codec(p->codec, r->dtype, [&](auto codec, auto *type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        append_rotary_kernel<decltype(codec)::value, T><<<(unsigned)ctas, 128, 0, s>>>(
-            g, a, static_cast<const T *>(r->query_dev), static_cast<const T *>(r->key_dev),
-            static_cast<const T *>(r->value_dev), r->query_out_dev);
-        count_launch();
-        return cudaGetLastError();
+        constexpr int C = decltype(codec)::value;
+        const T *q = static_cast<const T *>(r->query_dev), *k = static_cast<const T *>(r->key_dev),
+                *v = static_cast<const T *>(r->value_dev);
+        const dim3 grid((unsigned)ctas, tiles ? p->kv_heads : 1);
+        if (!tiles) return launch_next(append_rotary_kernel<C, T>, grid, 128, s, g, a, q, k, v, r->query_out_dev);
+        if (a.rot == (uint32_t)kHeadDim && !a.neighbours)
+            return launch_next(append_tiles_kernel<C, T, true>, grid, kTileThreads, s, g, a, q, k, v, r->query_out_dev);
+        return launch_next(append_tiles_kernel<C, T, false>, grid, kTileThreads, s, g, a, q, k, v, r->query_out_dev);
     });
     if (e != cudaSuccess) { set_cuda_error("qwn_kv_append_rotary", e); return QWN_CUDA_STATUS_RUNTIME_ERROR; }
     return QWN_CUDA_STATUS_OK;
@@ -301,16 +947,23 @@ QWN_CUDA_ABI_API int qwn_kv_load_tokens(QwnKvPoolHandle *h, const QwnKvLoadToken
         return invalid("qwn_kv_load_tokens: rows must start on four values (pointers and strides)");
     cudaSetDevice(p->device);
     const RowMap m = {r->seq_ids_dev, r->row_begin_dev, r->first_pos_dev, r->num_seqs, r->num_rows};
-    const uint64_t ctas = ((uint64_t)r->num_rows * p->kv_heads + 3) / 4;
-    if (ctas > 0x7FFFFFFFull) return invalid("qwn_kv_load_tokens: too many rows for one call");
+    const bool tiles = r->row_begin_dev && rows_wide(r->key_out_dev, ks, r->dtype) &&
+                       rows_wide(r->value_out_dev, vs, r->dtype);
+    const uint64_t ctas = tiles ? unit_count(r->num_rows, r->num_seqs) : ((uint64_t)r->num_rows * p->kv_heads + 3) / 4;
+    if (ctas > 0x7FFFFFFFull || (tiles && p->kv_heads > 65535u))
+        return invalid("qwn_kv_load_tokens: too many rows for one call");
     const StoreGeo g = store_geo(p);
     cudaStream_t s = stream_of(p, r->stream);
     const cudaError_t e = with_codec(p->codec, r->dtype, [&](auto codec, auto *type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        load_tokens_kernel<decltype(codec)::value, T><<<(unsigned)ctas, 128, 0, s>>>(
-            g, m, r->layer, ks, vs, static_cast<T *>(r->key_out_dev), static_cast<T *>(r->value_out_dev));
-        count_launch();
-        return cudaGetLastError();
+        constexpr int C = decltype(codec)::value;
+        T *k = static_cast<T *>(r->key_out_dev), *v = static_cast<T *>(r->value_out_dev);
+        // as many heads per CTA as leave every SM a few CTAs
+        uint32_t heads = p->kv_heads;
+        while (heads > 1 && ctas * ((p->kv_heads + heads - 1) / heads) < 16 * 148) heads = (heads + 1) / 2;
+        const dim3 grid((unsigned)ctas, tiles ? (p->kv_heads + heads - 1) / heads : 1);
+        if (tiles) return launch_next(load_tiles_kernel<C, T>, grid, kTileThreads, s, g, m, r->layer, heads, ks, vs, k, v);
+        return launch_next(load_rows_kernel<C, T>, grid, 128, s, g, m, r->layer, ks, vs, k, v);
     });
     if (e != cudaSuccess) { set_cuda_error("qwn_kv_load_tokens", e); return QWN_CUDA_STATUS_RUNTIME_ERROR; }
     return QWN_CUDA_STATUS_OK;

@@ -192,13 +192,6 @@ __device__ __forceinline__ void cp_async4(float *dst, const float *src) {
     const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(a), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async16(float *dst, const float *src) {
-    const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-
 // One group of P tokens for one warp of the prefill pipeline: update the
 // warp's rows with each token's k and v, then continue each token's output
 // chain over them, for each of the thread's CPT columns (lane, lane + 32, ...).

@@ -31,8 +31,8 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
 
 // launch a kernel that may start while the stream's previous one still runs (it
 // waits for it itself) and lets the next one start
-template <typename K, typename... Args>
-cudaError_t launch_next(K kernel, dim3 grid, uint32_t threads, cudaStream_t s, const Args &...args) {
+template <typename... Params, typename... Args>
+cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, uint32_t threads, cudaStream_t s, Args &&...args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -43,7 +43,7 @@ cudaError_t launch_next(K kernel, dim3 grid, uint32_t threads, cudaStream_t s, c
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     note_early_trigger();
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
     if (e == cudaSuccess) count_launch();
     else cudaGetLastError();  // reported here, not by a later launch
     return e;

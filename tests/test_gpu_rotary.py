@@ -105,7 +105,7 @@ class Batch:
     """A pool, and the rows of one call over some of its sequences."""
 
     def __init__(self, torch, codec, kind, counts, starts, kv=2, group=3, page=16, layers=2, seed=0, max_query=None,
-                 spare=5, lens=None):
+                 spare=5, lens=None, lead=4):
         import qwanto_b200 as qb
         self.torch, self.qb = torch, qb
         self.counts, self.starts = counts, starts
@@ -122,10 +122,14 @@ class Batch:
         for p in (self.pool, self.twin):
             p.seq_append(n, counts=self.lens)
         g = torch.Generator("cuda").manual_seed(seed)
-        self.wide = (self.hq + 2 * kv) * 128 + 12
+        # rows of the projection's output: `lead` values before the heads, as many and 4 more after (lead 4: rows
+        # start on 4 values, lead 8 and no more after: on 16 bytes)
+        self.lead = lead
+        width = (self.hq + 2 * kv) * 128
+        self.wide = width + 2 * lead + (4 if lead == 4 else 0)
         self.qkv = torch.full((self.rows, self.wide), float("nan"), device="cuda", dtype=_type(torch, kind))
-        self.qkv[:, 4:self.wide - 8] = torch.randn((self.rows, self.wide - 12), device="cuda", generator=g).to(self.qkv.dtype)
-        x = self.qkv[:, 4:self.wide - 8].view(self.rows, -1, 128) if self.rows else self.qkv.new_zeros((0, self.hq + 2 * kv, 128))
+        self.qkv[:, lead:lead + width] = torch.randn((self.rows, width), device="cuda", generator=g).to(self.qkv.dtype)
+        x = self.qkv[:, lead:lead + width].view(self.rows, -1, 128) if self.rows else self.qkv.new_zeros((0, self.hq + 2 * kv, 128))
         self.q, self.k, self.v = x[:, :self.hq], x[:, self.hq:self.hq + kv], x[:, self.hq + kv:]
         self.begin = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device="cuda")
         self.first = torch.tensor(starts, dtype=torch.int32, device="cuda")
@@ -134,7 +138,8 @@ class Batch:
 
     def parts(self):
         """query, key, value where the rows' heads begin."""
-        return self.qkv[:, 4:], self.qkv[:, 4 + self.hq * 128:], self.qkv[:, 4 + (self.hq + self.kv) * 128:]
+        at = self.lead
+        return self.qkv[:, at:], self.qkv[:, at + self.hq * 128:], self.qkv[:, at + (self.hq + self.kv) * 128:]
 
     def append(self, layer, rot, neighbours, table, out, out_kind, **over):
         q, k, v = self.parts()
@@ -173,9 +178,10 @@ COUNTS = ([1, 0, 15, 16, 17, 40, 3], [0, 5, 16, 3, 31, 12, 47])  # rows of each 
     ("f32", "f32", 128, False, 16), ("bf16", "f32", 128, True, 32), ("f16", "bf16", 64, False, 64),
     ("bf16", "f16", 8, True, 16), ("f32", "bf16", 96, False, 16), ("f16", "f16", 0, False, 48),
     ("bf16", "bf16", 40, False, 16)])
-def test_ragged_rows(cuda, codec, kind, out_kind, rot, neighbours, page):
+@pytest.mark.parametrize("lead", [4, 8])
+def test_ragged_rows(cuda, codec, kind, out_kind, rot, neighbours, page, lead):
     torch = cuda
-    b = Batch(torch, codec, kind, *COUNTS, page=page, seed=codec * 10 + rot)
+    b = Batch(torch, codec, kind, *COUNTS, page=page, seed=codec * 10 + rot, lead=lead)
     try:
         # tokens that are there already must stay: fill everything first
         old = torch.randn((200, b.kv, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(77))
@@ -248,10 +254,11 @@ def test_one_token_each_then_attention(cuda, codec, kv, group, kind):
         b.close()
 
 
-def test_sequence_ids_in_any_order_and_newest_rows(cuda):
+@pytest.mark.parametrize("lead", [4, 8])
+def test_sequence_ids_in_any_order_and_newest_rows(cuda, lead):
     """seq_ids picks the sequences; without first_pos the rows are each one's newest."""
     torch = cuda
-    b = Batch(torch, 2, "f32", [5, 20, 1], [30, 7, 16], seed=3)
+    b = Batch(torch, 2, "f32", [5, 20, 1], [30, 7, 16], seed=3, lead=lead)
     try:
         ids = torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda")
         order = [1, 20, 5]  # rows per entry: sequence 2's 1, 0's ... in the order of ids
@@ -285,7 +292,7 @@ def test_sequence_ids_in_any_order_and_newest_rows(cuda):
 def test_angles_apart_from_cache_positions(cuda):
     """After an eviction a token's place in the cache is not its position."""
     torch = cuda
-    b = Batch(torch, 5, "f32", [9, 9], [0, 20], seed=6)
+    b = Batch(torch, 5, "f32", [9, 39], [0, 20], seed=6, lead=8)
     try:
         table = _table(torch, 5000, 128)
         angles = torch.randint(0, 5000, (b.rows,), device="cuda", dtype=torch.int32)
@@ -299,46 +306,57 @@ def test_angles_apart_from_cache_positions(cuda):
         b.close()
 
 
-def test_query_in_place_and_no_query(cuda):
+@pytest.mark.parametrize("rot,neighbours", [(128, False), (64, True), (64, False), (40, False)])
+@pytest.mark.parametrize("lead", [4, 8])
+def test_query_in_place_and_no_query(cuda, rot, neighbours, lead):
     torch = cuda
-    b = Batch(torch, 4, "f32", [33], [2], seed=9)
+    b = Batch(torch, 4, "f32", [63], [2], seed=9, lead=lead)
     try:
-        table = _table(torch, 64, 64)
+        table = _table(torch, 70, rot)
         q = b.q.contiguous().clone()
-        want = _rotated(torch, q, table[b.pos], 64, True)
-        b.append(0, 64, True, table, q, "f32", query=q, query_stride=0)
-        b.append(0, 64, True, table, None, "f32", query=None, query_heads=0)
+        want = _rotated(torch, q, table[b.pos], rot, neighbours)
+        b.append(0, rot, neighbours, table, q, "f32", query=q, query_stride=0)
+        b.append(0, rot, neighbours, table, None, "f32", query=None, query_heads=0)
         assert b.pool.check() == 0
         assert torch.equal(q, want)
     finally:
         b.close()
 
 
-@pytest.mark.parametrize("codec", [1, 3, 4, 5])
-def test_beyond_numbers_in_other_rows(cuda, codec):
-    """NaN and infinities of one row leave the other rows of its tile alone."""
+@pytest.mark.parametrize("lead", [4, 8])
+@pytest.mark.parametrize("codec", [1, 2, 3, 4, 5])
+def test_beyond_numbers_in_other_rows(cuda, codec, lead):
+    """NaN and infinities of one row leave the other rows of its tile alone, and
+    are stored as the fp32 entry point stores them; so is a row of zeros with a
+    negative one among them."""
     torch = cuda
-    b = Batch(torch, codec, "f32", [24], [3], seed=2)
+    b = Batch(torch, codec, "f32", [44], [3], seed=2, lead=lead)
     try:
         b.k[5, 0, 3], b.k[9, 1, 77], b.v[5, 1, 0] = float("nan"), float("inf"), float("-inf")
+        b.k[20, 0], b.v[21, 1] = 0.0, 0.0
+        b.v[21, 1, 40], b.v[21, 1, 100] = -0.0, 2.0
+        b.v[20, 0, 64:] = float("nan")
         table = _table(torch, 64, 128)
         out = torch.empty((b.rows, b.hq, 128), device="cuda")
         b.append(0, 128, False, table, out, "f32")
         assert b.pool.check() == 0
         bk, bv = (torch.empty((b.rows, b.kv, 128), device="cuda") for _ in range(2))
         b.pool.load_tokens(0, 1, b.rows, 1, bk, bv, row_begin=b.begin, first_pos=b.first)
-        keep = torch.tensor([i for i in range(24) if i not in (5, 9)], device="cuda")
+        keep = torch.tensor([i for i in range(44) if i not in (5, 9, 20, 21)], device="cuda")
         for got, x in ((bk, _rotated(torch, b.k, table[b.pos], 128, False)), (bv, b.v.float())):
             want, far = _held64(torch, codec, x[keep])
             _assert_within((got[keep].double() - want).abs(), far + U * want.abs() + 2.0 ** -25, "other rows")
+        b.store_twin(0, _rotated(torch, b.k, table[b.pos], 128, False), b.v.float())
+        b.assert_pages_equal()
     finally:
         b.close()
 
 
-def test_rows_that_cannot_be_stored(cuda):
+@pytest.mark.parametrize("lead", [4, 8])
+def test_rows_that_cannot_be_stored(cuda, lead):
     """A bad sequence id, position, angle or run: latched, nothing stored, zero rows out; the others go on."""
     torch = cuda
-    b = Batch(torch, 2, "f32", [4, 4, 4], [0, 3, 10], seed=1)
+    b = Batch(torch, 2, "f32", [4, 4, 4], [0, 3, 10], seed=1, lead=lead)
     try:
         table = _table(torch, 13, 128)  # positions 13 of sequence 2 are outside
         out = torch.full((b.rows, b.hq, 128), float("nan"), device="cuda")
@@ -407,14 +425,14 @@ def test_long_cache_offsets_pass_32_bits(cuda):
 
 def test_a_stream_of_its_own(cuda):
     torch = cuda
-    b = Batch(torch, 1, "bf16", [300, 200], [0, 40], seed=12)
+    b = Batch(torch, 1, "bf16", [300, 200], [0, 40], seed=12, lead=8)
     try:
         table = _table(torch, 512, 128)
         out = torch.empty((b.rows, b.hq, 128), device="cuda")
         s = torch.cuda.Stream()
         torch.cuda.synchronize()
         with torch.cuda.stream(s):
-            b.qkv[:, 4:b.wide - 8] *= 2  # written on the stream that the call reads on
+            b.qkv *= 2  # written on the stream that the call reads on
             b.append(0, 128, False, table, out, "f32", stream=s)
             bk, bv = (torch.empty((b.rows, b.kv, 128), device="cuda") for _ in range(2))
             b.pool.load_tokens(0, 2, b.rows, 1, bk, bv, row_begin=b.begin, first_pos=b.first, stream=s)
