@@ -140,6 +140,35 @@ struct Row16 {
     float v[16];
     __device__ __forceinline__ static int dim(int i, int j) { return i < 8 ? 8 * j + i : 56 + 8 * j + i; }
 };
+// Two fp32 values in one instruction.  A packed sum of packed products may be
+// contracted to one rounding, so sums that must not be are made one by one.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ void unpair(uint64_t p, uint32_t &lo, uint32_t &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2_down(uint64_t a, uint64_t b) {  // towards zero
+    uint64_t r;
+    asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // the same as it is in memory: loads that are issued long before their use
 template <typename T>
 struct Raw16 {
@@ -219,12 +248,21 @@ struct Turn16 {
     }
     template <typename T>
     __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot, bool neighbours) const {
-        if (WHOLE) {
+        if (WHOLE) {  // turn_first and turn_second, the products two at a time
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float a = x.v[i], b = x.v[i + 8];
-                x.v[i] = turn_first(a, b, c[i], s[i]);
-                x.v[i + 8] = turn_second(b, a, c[i], s[i]);
+            for (int i = 0; i < 8; i += 2) {
+                const uint64_t a = pair(x.v[i], x.v[i + 1]), b = pair(x.v[i + 8], x.v[i + 9]);
+                const uint64_t cc = pair(c[i], c[i + 1]), ss = pair(s[i], s[i + 1]);
+                float ac[2], bs[2], bc[2], as[2];
+                unpair(mul2(a, cc), ac[0], ac[1]);
+                unpair(mul2(b, ss), bs[0], bs[1]);
+                unpair(mul2(b, cc), bc[0], bc[1]);
+                unpair(mul2(a, ss), as[0], as[1]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    x.v[i + e] = __fsub_rn(ac[e], bs[e]);
+                    x.v[i + 8 + e] = __fadd_rn(bc[e], as[e]);
+                }
             }
             return;
         }
@@ -275,13 +313,41 @@ __device__ __forceinline__ void put2(uint8_t *p, uint32_t a, uint32_t b) {
 template <int CODEC>
 __device__ bool put_row(uint8_t *tile, int t, int which, const Row16 &x, int j);
 
-__device__ __forceinline__ void put_q8(uint8_t *tile, int t, int which, const Row16 &x, int j, float s0, float s1) {
+// Eight codes as two words of biased bytes.  q8_pack4 divides; here the product
+// with 1 / s decides unless it lies within 1e-4 of a tie or no number is (then
+// false): its error is below 127 x 2^-22.  The sum with 1.5 x 2^23 + 128 rounds
+// to the nearest whole number, ties to even, and has the byte at its low end.
+__device__ __forceinline__ bool q8_words(const float *v, float per, uint32_t &lo, uint32_t &hi) {
+    const float magic = 12583040.f;
+    const uint64_t m2 = pair(magic, magic), n2 = pair(-magic, -magic), r2 = pair(per, per);
+    uint32_t bits[8];
+    bool sure = true;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t y = mul2(pair(v[i], v[i + 1]), r2), t = add2(y, m2);
+        float y0, y1, n0, n1;
+        unpair(y, y0, y1);
+        unpair(add2(t, n2), n0, n1);
+        sure &= fabsf(y0 - n0) < 0.4999f && fabsf(y1 - n1) < 0.4999f;
+        unpair(t, bits[i], bits[i + 1]);
+    }
+    lo = prmt(prmt(bits[0], bits[1], 0x0040u), prmt(bits[2], bits[3], 0x0040u), 0x5410u);
+    hi = prmt(prmt(bits[4], bits[5], 0x0040u), prmt(bits[6], bits[7], 0x0040u), 0x5410u);
+    return sure;
+}
+// `top` is the largest finite value that s was made for
+__device__ __forceinline__ void put_q8(uint8_t *tile, int t, int which, const Row16 &x, int j, float s0, float s1,
+                                       float top0, float top1) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const float s = h ? s1 : s0;
+        const float s = h ? s1 : s0, top = h ? top1 : top0;
         const float *v = x.v + 8 * h;
-        const uint32_t lo = q8_pack4(make_float4(v[0], v[1], v[2], v[3]), s);
-        const uint32_t hi = q8_pack4(make_float4(v[4], v[5], v[6], v[7]), s);
+        const float per = __fdiv_rn(1.f, s);
+        uint32_t lo, hi;
+        if (!q8_words(v, per, lo, hi) || !(top * per < 127.4f)) {
+            lo = q8_pack4(make_float4(v[0], v[1], v[2], v[3]), s);
+            hi = q8_pack4(make_float4(v[4], v[5], v[6], v[7]), s);
+        }
         const int d = 64 * h + 8 * j;
         if (!which) {
             put2(tile + k8_off(t, d), lo, hi);
@@ -302,21 +368,22 @@ __device__ __forceinline__ float finite_top(const float *v) {
 }
 template <>
 __device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q8_HEAD_F16>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
-    const uint16_t h = head_scale16(lanes_extreme<8, false>(fmaxf(finite_top(x.v), finite_top(x.v + 8))));
+    const float top = lanes_extreme<8, false>(fmaxf(finite_top(x.v), finite_top(x.v + 8)));
+    const uint16_t h = head_scale16(top);
     const float s = h2f(h);
-    put_q8(tile, t, which, x, j, s, s);
+    put_q8(tile, t, which, x, j, s, s, top, top);
     if (j == 0) *reinterpret_cast<uint16_t *>(tile + (which ? 4128 : 4096) + s16_off(t)) = h;
     return true;
 }
 template <>
 __device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q8_B64_F32>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
-    float s[2];
+    float s[2], m[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const float m = lanes_extreme<8, false>(finite_top(x.v + 8 * h));
-        s[h] = m > 0.f ? __fdiv_rn(m, 127.f) : 1.f;
+        m[h] = lanes_extreme<8, false>(finite_top(x.v + 8 * h));
+        s[h] = m[h] > 0.f ? __fdiv_rn(m[h], 127.f) : 1.f;
     }
-    put_q8(tile, t, which, x, j, s[0], s[1]);
+    put_q8(tile, t, which, x, j, s[0], s[1], m[0], m[1]);
     if (j < 2) *reinterpret_cast<float *>(tile + (which ? 4224 : 4096) + s32_off(t, j)) = j ? s[1] : s[0];
     return true;
 }
@@ -331,66 +398,93 @@ __device__ __forceinline__ bool put_row<QWN_KV_CODEC_F16>(uint8_t *tile, int t, 
     }
     return true;
 }
-// smallest and largest of a group held by LANES lanes' halves h, range and its
-// inverse; false where the row-by-row order matters
+// smallest value and range of a group held by LANES lanes' halves, and the
+// range's inverse.  False where store_token's order or special cases matter: a
+// NaN, a minimum of zero (its sign is the first zero's), parameters beyond fp16.
 struct Span {
     float mn, range, inv;
 };
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN where either is one
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 template <int LANES>
 __device__ __forceinline__ bool group_span(const float *v, Span &g) {
     float mn = v[0], mx = v[0];
-    bool nan = v[0] != v[0];
 #pragma unroll
     for (int i = 1; i < 8; i++) {
-        mn = fminf(mn, v[i]);
+        mn = min_nan(mn, v[i]);
         mx = fmaxf(mx, v[i]);
-        nan |= v[i] != v[i];
     }
-    g.mn = lanes_extreme<LANES, true>(mn);
-    g.range = __fsub_rn(lanes_extreme<LANES, false>(mx), g.mn);
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    g.mn = mn;
+    g.range = __fsub_rn(mx, mn);
     g.inv = g.range > 1e-8f ? __fdiv_rn(1.0f, g.range) : 0.f;
-    return !nan && g.mn != 0.f;
+    return fabsf(mn) > 0.f && fabsf(mn) < 65536.f && g.range < 65536.f;
 }
+// both parameters cut off to fp16 (as tq_f32_to_f16 does below 65536): range low, minimum high
 __device__ __forceinline__ uint32_t span_params(const Span &g) {
-    return (uint32_t)tq_f32_to_f16(g.range) | ((uint32_t)tq_f32_to_f16(g.mn) << 16);
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(g.mn), "f"(g.range));
+    return r;
 }
+// tq_code of eight numbers of the span's group: the two sums towards zero are
+// floor(y + 1/2) without roundf's exceptions (y is in [0, levels + 2^-19]), left
+// in the low bits; the number on top of them is 0x4B000000
+__device__ __forceinline__ void span_codes(const float *v, const Span &g, float even, float odd, uint32_t (&c)[8]) {
+    const uint64_t mn = pair(-g.mn, -g.mn), inv = pair(g.inv, g.inv), levels = pair(even, odd);
+    const uint64_t whole = pair(8388608.f, 8388608.f);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float y0, y1;
+        unpair(mul2(mul2(add2(pair(v[i], v[i + 1]), mn), inv), levels), y0, y1);
+        unpair(add2_down(pair(__fadd_rz(y0, 0.5f), __fadd_rz(y1, 0.5f)), whole), c[i], c[i + 1]);
+    }
+}
+constexpr uint32_t kCodeBase = 0x4B000000u;
 template <>
 __device__ __forceinline__ bool put_row<QWN_KV_CODEC_Q4_G32>(uint8_t *tile, int t, int which, const Row16 &x, int j) {
     bool ok = true;
-    uint32_t nib[2];  // the half's eight codes, dim i in nibble i
+    uint32_t nib[2];  // the half's eight codes: K in byte i dims i and i + 4, V in nibble i dim i
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const float *v = x.v + 8 * h;
         Span g;
-        ok &= group_span<4>(v, g);
+        uint32_t code[8];
+        ok &= group_span<4>(x.v + 8 * h, g);
+        span_codes(x.v + 8 * h, g, 15.f, 15.f, code);
         nib[h] = 0;
+        uint32_t base = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) nib[h] |= tq_code(v[i], g.mn, g.inv, 15.f) << (4 * i);
+        for (int i = 0; i < 8; i++) {
+            const int at = which ? 4 * i : i < 4 ? 8 * i : 8 * (i - 4) + 4;
+            nib[h] += code[i] << at;
+            base += kCodeBase << at;
+        }
+        nib[h] -= base;
         const int c = 2 * h + (j >> 2);
         if ((j & 3) == 0)
             *reinterpret_cast<uint32_t *>(tile + (which ? 2304 : 2048) + 32 * (t & 7) + 8 * c + 4 * (t >> 3)) =
                 span_params(g);
+        if (!which) *reinterpret_cast<uint32_t *>(tile + 64 * t + 16 * (j & 3) + 4 * c) = nib[h];
     }
-    if (!which) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {  // byte i: dims i and i + 4
-            uint32_t w = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                w |= (((nib[h] >> (4 * i)) & 15u) | (((nib[h] >> (4 * i + 16)) & 15u) << 4)) << (8 * i);
-            *reinterpret_cast<uint32_t *>(tile + 64 * t + 16 * (j & 3) + 4 * (2 * h + (j >> 2))) = w;
-        }
-    } else {
+    if (which) {
         // a byte holds dims gid and gid + 8 of a block of 16: lanes j and j + 1; the even one writes half 0
         const uint32_t other = __shfl_xor_sync(0xffffffffu, j & 1 ? nib[0] : nib[1], 1);
         const int h = j & 1, mb = 4 * h + (j >> 1);
         const uint32_t low = h ? other : nib[0], high = h ? nib[1] : other;
+        const uint32_t even = (low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u);
+        const uint32_t odd = ((low >> 4) & 0x0F0F0F0Fu) | (high & 0xF0F0F0F0u);
 #pragma unroll
         for (int gid = 0; gid < 8; gid++) {
             const int lv = 4 * gid + ((t & 7) >> 1);
             const int chunk = (mb >> 2) ^ ((lv >> 2) & 1);
             tile[1024 + 32 * lv + 16 * chunk + 4 * (mb & 3) + (t >> 3) + 2 * (t & 1)] =
-                (uint8_t)(((low >> (4 * gid)) & 15u) | (((high >> (4 * gid)) & 15u) << 4));
+                (uint8_t)((gid & 1 ? odd : even) >> (8 * (gid >> 1)));
         }
     }
     return ok;
@@ -420,9 +514,11 @@ __device__ __forceinline__ bool put_row<QWN_KV_CODEC_TQ35_G64>(uint8_t *tile, in
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         Span g;
+        uint32_t c[8];
         ok &= group_span<8>(x.v + 8 * h, g);
+        span_codes(x.v + 8 * h, g, 15.f, 7.f, c);
 #pragma unroll
-        for (int i = 0; i < 8; i++) code[8 * h + i] = tq_code(x.v[8 * h + i], g.mn, g.inv, i & 1 ? 7.f : 15.f);
+        for (int i = 0; i < 8; i++) code[8 * h + i] = c[i] & 15u;
         if (j == 0)
             *reinterpret_cast<uint32_t *>(half + 896 + 16 * (t & 7) + 8 * h + 4 * (t >> 3)) = span_params(g);
     }
