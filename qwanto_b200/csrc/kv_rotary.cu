@@ -53,6 +53,13 @@ __device__ __forceinline__ bool place_ok(const StoreGeo &g, int32_t seq, int64_t
     return true;
 }
 
+// the same for a unit's row
+__device__ __forceinline__ bool unit_row_ok(const StoreGeo &g, int32_t seq, int32_t len, int64_t pos, bool tell) {
+    if (seq >= 0 && pos >= 0 && pos < len) return true;
+    if (tell) latch(g.status, seq < 0 ? QWN_KV_STATUS_BAD_SEQUENCE : QWN_KV_STATUS_BAD_LENGTH);
+    return false;
+}
+
 // the sequence of a row and its position in the cache; false where there is none
 __device__ __forceinline__ bool find_row(const StoreGeo &g, const RowMap &m, uint32_t row, int32_t &seq, int64_t &pos,
                                          bool tell) {
@@ -544,10 +551,9 @@ struct RotaryArgs {
     uint64_t query_stride, key_stride, value_stride;
 };
 
-// place_ok with the row's angles
-__device__ __forceinline__ bool row_ok(const StoreGeo &g, const RotaryArgs &a, int32_t seq, int64_t pos, uint32_t row,
-                                       int32_t &angle, bool tell) {
-    if (!place_ok(g, seq, pos, tell)) return false;
+// whether a row's angles are in the table
+__device__ __forceinline__ bool angle_ok(const StoreGeo &g, const RotaryArgs &a, int64_t pos, uint32_t row,
+                                         int32_t &angle, bool tell) {
     if (!a.rot) return true;
     angle = a.rotary_pos ? a.rotary_pos[row] : (int32_t)pos;
     if (angle >= 0 && (uint32_t)angle < a.max_position) return true;
@@ -598,7 +604,7 @@ __global__ void __launch_bounds__(128) append_rotary_kernel(StoreGeo g, RotaryAr
     int32_t seq = 0, angle = 0;
     int64_t pos = 0;
     const bool tell = lane == 0 && slot == 0;
-    const bool ok = find_row(g, a.rows, row, seq, pos, tell) && row_ok(g, a, seq, pos, row, angle, tell);
+    const bool ok = find_row(g, a.rows, row, seq, pos, tell) && angle_ok(g, a, pos, row, angle, tell);
     append_row<CODEC, T>(g, a, ok, seq, (int32_t)pos, angle, row, slot, x, v, query_out, lane);
 }
 
@@ -607,30 +613,47 @@ __global__ void __launch_bounds__(128) append_rotary_kernel(StoreGeo g, RotaryAr
 // tiles, so that num_rows / 16 + 2 num_seqs units cover them all without a
 // table; some stay empty.
 struct Unit {
-    uint32_t first, count;  // rows
-    int32_t seq;            // -1: none such
+    uint32_t first, count;  // rows; none where count is 0
+    int32_t seq, len;       // -1 and 0: no such sequence
     int64_t pos;            // of the first row
 };
-__device__ __forceinline__ bool find_unit(const StoreGeo &g, const RowMap &m, uint32_t u, Unit &t) {
-    uint32_t lo = 0, hi = m.num_seqs;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if ((uint32_t)max(m.row_begin[mid], 0) / 16 + 2 * mid <= u) lo = mid;
-        else hi = mid;
+// by one warp; the other warps of the CTA wait for it (with every warp doing
+// this, half of the kernel's instructions were these)
+__device__ __forceinline__ Unit find_unit(const StoreGeo &g, const RowMap &m, uint32_t u) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, n = m.num_seqs;  // the last of sequences lo .. lo + n - 1 whose base is not beyond u
+    while (n > 1) {                   // 32 at a time
+        const uint32_t step = (n + 31) / 32, i = lo + lane * step;
+        const bool below = lane * step < n && (uint32_t)max(m.row_begin[i], 0) / 16 + 2 * i <= u;
+        const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+        n = min(step, n - last * step);
+        lo += last * step;
     }
-    const int64_t b = max(m.row_begin[lo], 0), e = min((int64_t)m.row_begin[lo + 1], (int64_t)m.num_rows);
-    const int64_t base = b / 16 + 2 * (int64_t)lo;
-    if (e <= b || (int64_t)u < base) return false;
-    t.seq = m.seq_ids ? m.seq_ids[lo] : (int32_t)lo;
-    if (t.seq < 0 || (uint32_t)t.seq >= g.max_seqs) t.seq = -1;
-    const int64_t p0 = m.first_pos ? (int64_t)m.first_pos[lo] : t.seq < 0 ? 0 : (int64_t)g.seq_lens[t.seq] - (e - b);
-    const int64_t tile = (p0 >> 4) + ((int64_t)u - base);
+    Unit t = {0, 0, -1, 0, 0};
+    const int32_t b = max(m.row_begin[lo], 0);
+    const int32_t e = (int32_t)min((int64_t)m.row_begin[lo + 1], (int64_t)m.num_rows);
+    const uint32_t base = (uint32_t)b / 16 + 2 * lo;
+    const int32_t seq = m.seq_ids ? m.seq_ids[lo] : (int32_t)lo;
+    if (seq >= 0 && (uint32_t)seq < g.max_seqs) {
+        t.seq = seq;
+        t.len = g.seq_lens[seq];
+    }
+    if (e <= b || u < base) return t;
+    const int64_t p0 = m.first_pos ? m.first_pos[lo] : t.seq < 0 ? 0 : (int64_t)t.len - (e - b);
+    const int64_t tile = (p0 >> 4) + (u - base);
     const int64_t from = max(p0, tile << 4), to = min(p0 + (e - b), (tile + 1) << 4);
-    if (from >= to) return false;
+    if (from >= to) return t;
     t.first = (uint32_t)(b + (from - p0));
     t.count = (uint32_t)(to - from);
     t.pos = from;
-    return true;
+    return t;
+}
+// the tile of a unit's rows for one head and the layer, whose page one of their
+// positions finds; null where none of them exists
+__device__ __forceinline__ uint8_t *unit_tile(const StoreGeo &g, const Unit &u, uint32_t layer, uint32_t head) {
+    const int64_t some = max(u.pos, (int64_t)0);
+    if (u.seq < 0 || some >= min(u.pos + u.count, (int64_t)u.len)) return nullptr;
+    return tile_for(g, u.seq, layer, head, (int32_t)some);
 }
 // rows before the first sequence's and after the last one's: unit 0 looks at them
 struct Gaps {
@@ -648,7 +671,7 @@ constexpr int kTileThreads = 128;  // 16 rows of 8 lanes
 
 // one CTA per (tile, kv head): its K and V, and the query heads that read it
 template <int CODEC, typename T, bool WHOLE>
-__global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, RotaryArgs a, const T *query,
+__global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo g, RotaryArgs a, const T *query,
                                                                     const T *key, const T *value, void *query_out) {
     constexpr int kImage = (int)tile_bytes_of(CODEC), kAhead = sizeof(T) == 4 ? 2 : 4;  // query heads in flight
     __shared__ __align__(16) uint8_t buf[2 * 16 * kHeadDim * 4];  // the tile's image, or K and V of its rows in fp32
@@ -671,8 +694,15 @@ __global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, 
         for (int64_t i = r; i < gaps.count; i += 16)
             for (uint32_t q = 0; q < group; q++) put_query(gaps.row(i), q, zero);
     }
-    Unit u;
-    if (!find_unit(g, a.rows, blockIdx.x, u)) return;
+    __shared__ Unit unit;
+    __shared__ uint8_t *unit_at;
+    if (warp == 0) {
+        const Unit t = find_unit(g, a.rows, blockIdx.x);
+        if (lane == 0) unit = t;
+    }
+    __syncthreads();
+    const Unit u = unit;
+    if (u.count == 0) return;
     const bool have = (uint32_t)r < u.count;
     const uint32_t row = u.first + (have ? (uint32_t)r : 0);
     const T *kr = key + (size_t)row * a.key_stride + head * kHeadDim;
@@ -684,13 +714,10 @@ __global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, 
 #pragma unroll
     for (uint32_t q = 0; q < kAhead; q++)
         if (q < group) qw[q].load(qr + q * kHeadDim, j);
-    // the rows share a tile, whose page one of their positions finds
-    const int64_t some = max(u.pos, (int64_t)0);
-    uint8_t *tile = nullptr;
-    if (u.seq >= 0 && some < min(u.pos + u.count, (int64_t)g.seq_lens[u.seq]))
-        tile = tile_for(g, u.seq, a.layer, head, (int32_t)some);
+    if (threadIdx.x == 0) unit_at = unit_tile(g, u, a.layer, head);
     int32_t angle = 0;
-    const bool ok = have && row_ok(g, a, u.seq, u.pos + r, row, angle, j == 0 && head == 0);
+    const bool tell = have && j == 0 && head == 0;
+    const bool ok = have && unit_row_ok(g, u.seq, u.len, u.pos + r, tell) && angle_ok(g, a, u.pos + r, row, angle, tell);
     const bool turns = ok && (WHOLE || a.rot);
     Turn16<WHOLE> turn;
     if (turns) turn.load(a.table + (size_t)angle * a.rot, j);
@@ -699,10 +726,15 @@ __global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, 
         for (uint32_t i = 0; i < kAhead; i++) {
             const uint32_t q = q0 + i;
             if (q >= group) break;
-            Row16 x = ok ? qw[i].row() : zero;
-            if (turns) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot, a.neighbours);
-            if (!WHOLE) __syncwarp();  // query_out may be query: every lane has read its partner's values
-            if (have) put_query(row, q, x);
+            if (ok) {
+                Row16 x = qw[i].row();
+                if (WHOLE || a.rot) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot, a.neighbours);
+                // query_out may be query: the row's lanes have read their partners' values
+                if (!WHOLE) __syncwarp(0xFFu << (8 * (lane >> 3)));
+                put_query(row, q, x);
+            } else if (have) {
+                put_query(row, q, zero);
+            }
             if (q + kAhead < group) qw[i].load(qr + (q + kAhead) * kHeadDim, j);
         }
     }
@@ -713,7 +745,9 @@ __global__ void __launch_bounds__(kTileThreads) append_tiles_kernel(StoreGeo g, 
         for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
             reinterpret_cast<uint4 *>(buf)[i] = make_uint4(0, 0, 0, 0);
     // 16 new tokens: the whole tile is put together here
-    if (__syncthreads_and(ok && u.count == 16 && tile)) {
+    const bool whole = __syncthreads_and(ok && u.count == 16);
+    uint8_t *tile = unit_at;
+    if (whole && tile) {
         const bool fine = put_row<CODEC>(buf, r, 0, k, j) & put_row<CODEC>(buf, r, 1, v, j);
         if (__syncthreads_and(fine)) {
             for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
@@ -865,13 +899,19 @@ __global__ void __launch_bounds__(kTileThreads) load_tiles_kernel(StoreGeo g, Ro
         for (int64_t i = r; i < gaps.count; i += 16)
             for (uint32_t h = h0; h < h1; h++) put(gaps.row(i), h, zero, zero);
     }
-    Unit u;
-    if (!find_unit(g, m, blockIdx.x, u)) return;
-    // the rows share a tile of each head, whose page one of their positions finds
-    const int64_t some = max(u.pos, (int64_t)0);
-    const uint8_t *tile = nullptr;
-    if (u.seq >= 0 && some < min(u.pos + u.count, (int64_t)g.seq_lens[u.seq]))
-        tile = tile_for(g, u.seq, layer, h0, (int32_t)some);
+    __shared__ Unit unit;
+    __shared__ const uint8_t *unit_at;
+    if (threadIdx.x < 32) {
+        const Unit t = find_unit(g, m, blockIdx.x);
+        if (threadIdx.x == 0) {
+            unit = t;
+            unit_at = t.count ? unit_tile(g, t, layer, h0) : nullptr;
+        }
+    }
+    __syncthreads();
+    const Unit u = unit;
+    if (u.count == 0) return;
+    const uint8_t *tile = unit_at;
     const size_t next = (size_t)g.tpp * g.tile_bytes;  // the following head's tile
     auto fetch = [&](uint32_t h) {
         if (tile && h < h1)
@@ -882,7 +922,7 @@ __global__ void __launch_bounds__(kTileThreads) load_tiles_kernel(StoreGeo g, Ro
     fetch(h0);
     const int64_t pos = u.pos + r;
     const bool have = (uint32_t)r < u.count;
-    const bool ok = have && place_ok(g, u.seq, pos, j == 0 && h0 == 0) && tile;
+    const bool ok = have && unit_row_ok(g, u.seq, u.len, pos, j == 0 && h0 == 0) && tile;
     const int t = (int)(pos & 15);
     for (uint32_t h = h0; h < h1; h++) {
         fetch(h + 1);
