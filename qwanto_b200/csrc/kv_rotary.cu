@@ -235,27 +235,31 @@ __device__ __forceinline__ void store16(__nv_bfloat16 *row, int j, const Row16 &
                        pack_b2(r.v[8 * q + 4], r.v[8 * q + 5]), pack_b2(r.v[8 * q + 6], r.v[8 * q + 7]));
 }
 
-// a row's rotation for this lane.  WHOLE: all 128 dims as halves, the pairs are
-// (v[i], v[i + 8]); otherwise the partner's values are read again (from L1).
-template <bool WHOLE>
+// A row's rotation for this lane.  All 128 dims as halves: the pairs are (v[i],
+// v[i + 8]).  Neighbours: (v[2i], v[2i + 1]), where the eight dims are below
+// rotary_dim.  Both keep their angles for all heads of the row; halves of fewer
+// dims read angles and the partner's values again for each head (from L1).
+enum { kTurnWhole, kTurnNeighbours, kTurnPart };
+template <int MODE>
 struct Turn16 {
     float c[8], s[8];
     const float *row;
-    __device__ __forceinline__ void load(const float *r, int j) {
+    __device__ __forceinline__ void load(const float *r, int j, int rot) {
         row = r;
-        if (WHOLE) {
+        if (MODE == kTurnPart) return;
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const float4 x = *reinterpret_cast<const float4 *>(r + 8 * j + 4 * q);
-                const float4 y = *reinterpret_cast<const float4 *>(r + 64 + 8 * j + 4 * q);
-                c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
-                s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
-            }
+        for (int q = 0; q < 2; q++) {
+            if (MODE == kTurnNeighbours && 64 * q + 8 * j >= rot) continue;
+            const float *at = MODE == kTurnWhole ? r + 8 * j + 4 * q : r + 32 * q + 4 * j;
+            const float4 x = *reinterpret_cast<const float4 *>(at);
+            const float4 y = *reinterpret_cast<const float4 *>(at + (rot >> 1));
+            c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
+            s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
         }
     }
     template <typename T>
-    __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot, bool neighbours) const {
-        if (WHOLE) {  // turn_first and turn_second, the products two at a time
+    __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot) const {
+        if (MODE == kTurnWhole) {  // turn_first and turn_second, the products two at a time
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 const uint64_t a = pair(x.v[i], x.v[i + 1]), b = pair(x.v[i + 8], x.v[i + 9]);
@@ -273,29 +277,37 @@ struct Turn16 {
             }
             return;
         }
+        if (MODE == kTurnNeighbours) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                if (64 * q + 8 * j >= rot) continue;
+#pragma unroll
+                for (int i = 4 * q; i < 4 * q + 4; i++) {
+                    const uint64_t ab = pair(x.v[2 * i], x.v[2 * i + 1]);
+                    float ac, bc, as, bs;
+                    unpair(mul2(ab, pair(c[i], c[i])), ac, bc);
+                    unpair(mul2(ab, pair(s[i], s[i])), as, bs);
+                    x.v[2 * i] = __fsub_rn(ac, bs);
+                    x.v[2 * i + 1] = __fadd_rn(bc, as);
+                }
+            }
+            return;
+        }
         const int half = rot >> 1;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             float *v = x.v + 4 * q;
             const int d = Row16::dim(4 * q, j);
             if (d >= rot) continue;
-            if (neighbours) {
-                const float2 cc = *reinterpret_cast<const float2 *>(row + (d >> 1));
-                const float2 ss = *reinterpret_cast<const float2 *>(row + half + (d >> 1));
-                const float a = v[0], b = v[1], e = v[2], f = v[3];
-                v[0] = turn_first(a, b, cc.x, ss.x), v[1] = turn_second(b, a, cc.x, ss.x);
-                v[2] = turn_first(e, f, cc.y, ss.y), v[3] = turn_second(f, e, cc.y, ss.y);
-            } else {
-                const bool second = d >= half;
-                const int p = second ? d - half : d;
-                const float4 cc = *reinterpret_cast<const float4 *>(row + p);
-                const float4 ss = *reinterpret_cast<const float4 *>(row + half + p);
-                const float4 o = load4(from + (second ? p : d + half));
-                const float cs[4] = {cc.x, cc.y, cc.z, cc.w}, sn[4] = {ss.x, ss.y, ss.z, ss.w}, y[4] = {o.x, o.y, o.z, o.w};
+            const bool second = d >= half;
+            const int p = second ? d - half : d;
+            const float4 cc = *reinterpret_cast<const float4 *>(row + p);
+            const float4 ss = *reinterpret_cast<const float4 *>(row + half + p);
+            const float4 o = load4(from + (second ? p : d + half));
+            const float cs[4] = {cc.x, cc.y, cc.z, cc.w}, sn[4] = {ss.x, ss.y, ss.z, ss.w}, y[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    v[i] = second ? turn_second(v[i], y[i], cs[i], sn[i]) : turn_first(v[i], y[i], cs[i], sn[i]);
-            }
+            for (int i = 0; i < 4; i++)
+                v[i] = second ? turn_second(v[i], y[i], cs[i], sn[i]) : turn_first(v[i], y[i], cs[i], sn[i]);
         }
     }
 };
@@ -670,7 +682,7 @@ struct Gaps {
 constexpr int kTileThreads = 128;  // 16 rows of 8 lanes
 
 // one CTA per (tile, kv head): its K and V, and the query heads that read it
-template <int CODEC, typename T, bool WHOLE>
+template <int CODEC, typename T, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo g, RotaryArgs a, const T *query,
                                                                     const T *key, const T *value, void *query_out) {
     constexpr int kImage = (int)tile_bytes_of(CODEC), kAhead = sizeof(T) == 4 ? 2 : 4;  // query heads in flight
@@ -718,9 +730,9 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
     int32_t angle = 0;
     const bool tell = have && j == 0 && head == 0;
     const bool ok = have && unit_row_ok(g, u.seq, u.len, u.pos + r, tell) && angle_ok(g, a, u.pos + r, row, angle, tell);
-    const bool turns = ok && (WHOLE || a.rot);
-    Turn16<WHOLE> turn;
-    if (turns) turn.load(a.table + (size_t)angle * a.rot, j);
+    const bool turns = ok && (MODE != kTurnPart || a.rot);
+    Turn16<MODE> turn;
+    if (turns) turn.load(a.table + (size_t)angle * a.rot, j, (int)a.rot);
     for (uint32_t q0 = 0; q0 < group; q0 += kAhead) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; i++) {
@@ -728,9 +740,9 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
             if (q >= group) break;
             if (ok) {
                 Row16 x = qw[i].row();
-                if (WHOLE || a.rot) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot, a.neighbours);
+                if (MODE != kTurnPart || a.rot) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot);
                 // query_out may be query: the row's lanes have read their partners' values
-                if (!WHOLE) __syncwarp(0xFFu << (8 * (lane >> 3)));
+                if (MODE == kTurnPart) __syncwarp(0xFFu << (8 * (lane >> 3)));
                 put_query(row, q, x);
             } else if (have) {
                 put_query(row, q, zero);
@@ -740,7 +752,7 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
     }
     Row16 k = kw.row();
     const Row16 v = vw.row();
-    if (turns) turn.apply(k, kr, j, (int)a.rot, a.neighbours);
+    if (turns) turn.apply(k, kr, j, (int)a.rot);
     if (CODEC == QWN_KV_CODEC_TQ35_G64)
         for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
             reinterpret_cast<uint4 *>(buf)[i] = make_uint4(0, 0, 0, 0);
@@ -1055,9 +1067,10 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
                 *v = static_cast<const T *>(r->value_dev);
         const dim3 grid((unsigned)ctas, tiles ? p->kv_heads : 1);
         if (!tiles) return launch_next(append_rotary_kernel<C, T>, grid, 128, s, g, a, q, k, v, r->query_out_dev);
-        if (a.rot == (uint32_t)kHeadDim && !a.neighbours)
-            return launch_next(append_tiles_kernel<C, T, true>, grid, kTileThreads, s, g, a, q, k, v, r->query_out_dev);
-        return launch_next(append_tiles_kernel<C, T, false>, grid, kTileThreads, s, g, a, q, k, v, r->query_out_dev);
+        const auto kernel = a.neighbours && a.rot                 ? append_tiles_kernel<C, T, kTurnNeighbours>
+                            : a.rot == (uint32_t)kHeadDim ? append_tiles_kernel<C, T, kTurnWhole>
+                                                          : append_tiles_kernel<C, T, kTurnPart>;
+        return launch_next(kernel, grid, kTileThreads, s, g, a, q, k, v, r->query_out_dev);
     });
     if (e != cudaSuccess) { set_cuda_error("qwn_kv_append_rotary", e); return QWN_CUDA_STATUS_RUNTIME_ERROR; }
     return QWN_CUDA_STATUS_OK;
