@@ -473,7 +473,8 @@ QWN_CUDA_ABI_API int qwn_kv_load_tokens(QwnKvPoolHandle *pool, const QwnKvLoadTo
  *     code = y / scale rounded to nearest even, 0 where y is not finite
  * the rules of the pool's Q8 codecs (c/qwanto_turboquant.c:555-586) over a
  * whole row.  residual_out receives h in the rows' type; y comes from h before
- * that rounding.  rows_out, where given, receives code x scale: what a product
+ * that rounding.  A mean of squares beyond fp32 is not finite: such a row's codes
+ * are 0.  rows_out, where given, receives code x scale: what a product
  * that stays in 16 bits must see to agree with the int8 ones. */
 enum { QWN_NORM_RMS = 0, QWN_NORM_NONE = 1 };
 #define QWN_RMSNORM_MAX_WIDTH 32768u

@@ -20,7 +20,6 @@
 // or scales or write anything.
 #include <algorithm>
 #include <cstring>
-#include <map>
 #include <new>
 #include <type_traits>
 #include <utility>
@@ -452,24 +451,19 @@ bool encode_codes(CUtensorMap *map, const int8_t *p, uint64_t width, uint64_t ro
 
 constexpr uint32_t kMmSmem = 227 * 1024 - 4096;  // dynamic, beside the static part
 
+// dynamic shared memory above 48 KB is opted into per kernel and device, when a handle is made there
 template <typename K>
 cudaError_t allow_all_smem(K kernel) {
-    static std::mutex mu;
-    static std::map<std::pair<const void *, int>, bool> done;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lk(mu);
-    bool &have = done[{reinterpret_cast<const void *>(kernel), dev}];
-    if (have) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmSmem);
-    have = e == cudaSuccess;
-    return e;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmSmem);
+}
+template <typename T>
+cudaError_t allow_all_smem() {
+    const cudaError_t e = allow_all_smem(matmul_q8_split_kernel<T>);
+    return e == cudaSuccess ? allow_all_smem(matmul_q8_pair_kernel<T>) : e;
 }
 
 template <typename K, typename... Args>
 cudaError_t launch_clusters(K kernel, dim3 grid, uint32_t cluster, size_t smem, cudaStream_t s, Args... args) {
-    cudaError_t e = allow_all_smem(kernel);
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kMmThreads);
@@ -484,7 +478,7 @@ cudaError_t launch_clusters(K kernel, dim3 grid, uint32_t cluster, size_t smem, 
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     note_early_trigger();
-    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) count_launch();
     else cudaGetLastError();  // reported here, not by a later launch
     return e;
@@ -572,9 +566,12 @@ cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, 
                            extra + (size_t)stages * stage, s, mm.wmap, xmap, a, p.nt, p.splits, stages, columns);
 }
 
-// how many clusters of each size the device runs at once with one CTA per SM
+// prepares the kernels on the current device; how many clusters of each size it
+// runs at once with one CTA per SM
 bool count_clusters(MatmulQ8 *mm) {
-    if (allow_all_smem(matmul_q8_split_kernel<float>) != cudaSuccess) return false;
+    if (allow_all_smem<float>() != cudaSuccess || allow_all_smem<__half>() != cudaSuccess ||
+        allow_all_smem<__nv_bfloat16>() != cudaSuccess)
+        return false;
     for (uint32_t c = 1; c <= kMaxSplit; c++) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(c);
