@@ -2075,9 +2075,12 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32, 3) attn_kernel(const AttnAr
     __syncwarp();
     // let the stream's next kernel start its CTAs as SMs free up; wait for the
     // previous kernel's results before the first global access -- or, in the
-    // early mode, before the first write that kernel could race with
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // early mode, before the first write that kernel could race with.  Outside
+    // the early mode the wait comes first: the next launch may be early, and what
+    // it reads must not still be in the making by the kernel before this one,
+    // which may have let this one start.
     if (!A.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // (returns at once once the previous kernel has finished; reading the flag
     // from the parameter bank keeps it out of the registers)
     auto dep_wait = [&]() {

@@ -176,3 +176,38 @@ def test_attention_after_these_calls_waits_for_them(cuda):
         assert pool.check() == 0 and mm.check() == 0 and wq.check() == 0
     finally:
         pool.close()
+
+
+def test_one_product_writes_the_queries_of_several_layers(cuda):
+    """The second of two attention launches starts behind the first one's start,
+    not behind its end: the first lets it start only once what came before both
+    has ended."""
+    import qwanto_b200 as qb
+    torch = cuda
+    layers, hq, hk, seqs, k = 6, 8, 2, 2, 131056
+    pool = qb.KvPool(2, layers, hk, 16, 64, seqs, 16, max_query_heads=hq)
+    try:
+        g = torch.Generator("cuda").manual_seed(2)
+        pool.prefill_synthetic(list(range(seqs)), [100, 17], 5)
+        ids = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+        w = torch.randint(-127, 128, (hq * 128, k), device="cuda", generator=g).to(torch.int8)
+        mm = qb.MatmulQ8(w, hq * 128, k, torch.full((hq * 128,), 1e-7, device="cuda"))
+        codes = torch.randint(-127, 128, (layers * seqs, k), device="cuda", generator=g).to(torch.int8)
+        scales = torch.rand(layers * seqs, device="cuda", generator=g)
+        got = []
+        for wait in (True, False):
+            for seq_ids in (None, ids):
+                q = torch.zeros((layers, seqs, hq * 128), device="cuda")
+                outs = torch.zeros((layers, seqs, hq, 128), device="cuda")
+                torch.cuda.synchronize()
+                mm(codes, scales, layers * seqs, q, 1)
+                for layer in range(layers):
+                    if wait:
+                        torch.cuda.synchronize()
+                    pool.decode(layer, seqs, hq, q[layer], outs[layer], seq_ids=seq_ids)
+                torch.cuda.synchronize()
+                got.append(outs)
+        assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3])
+        assert pool.check() == 0 and mm.check() == 0
+    finally:
+        pool.close()
