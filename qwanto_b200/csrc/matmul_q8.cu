@@ -278,6 +278,19 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
 constexpr uint32_t kPairStages = 6;
 constexpr uint32_t kPairTokens = 256;
 
+// Tile t of a walk in groups of 16 token tiles, the outputs outside them: the
+// pairs that run together share 16 tiles of tokens and a few of weights
+// (8192 x 6144 x 8192: 246 us, 253 with all 32 token tiles in one group).
+struct PairTile {
+    uint32_t n, m;
+};
+__device__ __forceinline__ PairTile pair_tile(uint32_t t, uint32_t m_tiles, uint32_t n_tiles) {
+    constexpr uint32_t kGroup = 16;
+    const uint32_t group = t / (kGroup * n_tiles), in = t - group * kGroup * n_tiles;
+    const uint32_t wide = min(kGroup, m_tiles - group * kGroup);
+    return {in / wide, group * kGroup + in % wide};
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __grid_constant__ CUtensorMap wmap,
                                                                        const __grid_constant__ CUtensorMap xmap,
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     __shared__ uint32_t tmem_at;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-    const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1;
+    const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1, n_tiles = tiles / m_tiles;
     const uint32_t half = nt / 2, stage_bytes = kWBytes + half * kMmK;
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -321,14 +334,14 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
         };
         const uint32_t ahead = min(a.kblocks, kPairStages);  // weights of the first tile
         uint32_t t = blockIdx.x >> 1, i = 0;
-        uint32_t n0 = (t / m_tiles * 2 + rank) * kMmRows, m0 = t % m_tiles * nt + rank * half;
+        const uint32_t first = (pair_tile(t, m_tiles, n_tiles).n * 2 + rank) * kMmRows;
         for (uint32_t j = 0; j < ahead; j++)
-            if (one) load_w(j, n0, j);
+            if (one) load_w(j, first, j);
         wait_previous();
         Ring r;
         for (; t < tiles && ok; t += pairs) {
-            n0 = (t / m_tiles * 2 + rank) * kMmRows;
-            m0 = t % m_tiles * nt + rank * half;
+            const PairTile tile = pair_tile(t, m_tiles, n_tiles);
+            const uint32_t n0 = (tile.n * 2 + rank) * kMmRows, m0 = tile.m * nt + rank * half;
             for (uint32_t kb = 0; kb < a.kblocks; kb++, i++) {
                 if (i >= kPairStages) {
                     ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty[r.stage], r.parity ^ 1));
@@ -375,8 +388,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
         uint32_t n = 0;
         wait_previous();
         for (uint32_t t = blockIdx.x >> 1; t < tiles; t += pairs, n++) {
-            const uint32_t buf = n & 1, m0 = t % m_tiles * nt, valid = min(nt, a.m - m0);
-            const uint32_t col = (t / m_tiles * 2 + rank) * kMmRows + quarter * 32 + lane;
+            const PairTile tile = pair_tile(t, m_tiles, n_tiles);
+            const uint32_t buf = n & 1, m0 = tile.m * nt, valid = min(nt, a.m - m0);
+            const uint32_t col = (tile.n * 2 + rank) * kMmRows + quarter * 32 + lane;
             const bool in = col < a.n;
             const float sw = in ? a.sw[col] : 0.f, bias = a.bias && in ? a.bias[col] : 0.f;
             constexpr uint32_t kChunks = kPairTokens / 64;  // this warp's: every other 32 tokens
@@ -508,7 +522,7 @@ struct MmPlan {
 // A few tokens thus go to the split kernel with as many shares as run at once
 // (1 x 1536 x 2048: 2.7 us in 4 shares, 4.3 in one), more to pairs with the
 // widest tile that still reaches all of them (257 x 4099 x 4095: 10.7 us with
-// 96 tokens a tile, 14.1 with 256; 8192 x 6144 x 8192: 260 us with 256, 278
+// 96 tokens a tile, 14.1 with 256; 8192 x 6144 x 8192: 253 us with 256, 278
 // with 192).
 MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
     MmPlan best{};

@@ -265,6 +265,21 @@ def test_matmul_two_streams_share_a_handle(cuda):
         _check_matmul(torch, x[:, :k], w, sx, sw, None, "f32", out)
 
 
+@pytest.mark.parametrize("k", [1, 100, 1000, 4097])
+def test_matmul_of_one_row_needs_no_aligned_stride(cuda, k):
+    import qwanto_b200 as qb
+    torch = cuda
+    g = torch.Generator("cuda").manual_seed(k)
+    x = torch.randint(-128, 128, (1, k), device="cuda", generator=g).to(torch.int8)
+    w = torch.randint(-128, 128, (70, k), device="cuda", generator=g).to(torch.int8)
+    sx, sw = torch.rand(1, device="cuda", generator=g), torch.rand(70, device="cuda", generator=g) * 0.01
+    out = torch.full((1, 70), float("nan"), device="cuda")
+    mm = qb.MatmulQ8(w, 70, k, sw)
+    mm(x, sx, 1, out, 1)
+    assert mm.check() == 0
+    _check_matmul(torch, x, w, sx, sw, None, "f32", out)
+
+
 def test_matmul_refusals(cuda):
     import qwanto_b200 as qb
     from qwanto_b200 import _lib
