@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     const uint32_t n0 = blockIdx.x / splits * kMmRows, m0 = blockIdx.y * nt;
     const uint32_t kb0 = (uint32_t)((uint64_t)a.kblocks * rank / splits);
     const uint32_t kb1 = (uint32_t)((uint64_t)a.kblocks * (rank + 1) / splits);
-    const uint32_t stage_bytes = kWBytes + nt * kMmK, count = kb1 - kb0;
+    const uint32_t stage_bytes = 2 * (kWBytes + nt * kMmK), count = kb1 - kb0;
     const uint32_t valid = min(nt, a.m - m0);  // tokens of this tile that exist
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -148,15 +148,24 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     tc_fence_after();
     const uint32_t tmem = tmem_at;
     bool ok = true;
+    // a stage is two tiles of 128 codes, the last one perhaps one: a barrier's round trip per eight MMAs
+    // (1 x 4096 x 6144: 6.4 us with one tile per stage, 5.5 with two)
+    const uint32_t steps = (count + 1) / 2, tile_bytes = kWBytes + nt * kMmK;
     if (warp == 0) {
         const bool one = elect_one();
-        const uint32_t ahead = min(count, stages);
+        const uint32_t ahead = min(steps, stages);
         auto load_w = [&](uint32_t i, uint32_t st) {
-            mbar_expect_tx(&full[st], stage_bytes);
-            tma_load(base + st * stage_bytes, &wmap, 0, (int)((kb0 + i) * a.n + n0), smem_u32(&full[st]));
+            const uint32_t two = min(count - 2 * i, 2u);
+            mbar_expect_tx(&full[st], two * tile_bytes);
+            for (uint32_t e = 0; e < two; e++)
+                tma_load(base + st * stage_bytes + e * tile_bytes, &wmap, 0, (int)((kb0 + 2 * i + e) * a.n + n0),
+                         smem_u32(&full[st]));
         };
         auto load_x = [&](uint32_t i, uint32_t st) {
-            tma_load(base + st * stage_bytes + kWBytes, &xmap, (int)((kb0 + i) * kMmK), (int)m0, smem_u32(&full[st]));
+            const uint32_t two = min(count - 2 * i, 2u);
+            for (uint32_t e = 0; e < two; e++)
+                tma_load(base + st * stage_bytes + e * tile_bytes + kWBytes, &xmap, (int)((kb0 + 2 * i + e) * kMmK), (int)m0,
+                         smem_u32(&full[st]));
         };
         for (uint32_t i = 0; i < ahead; i++)
             if (one) load_w(i, i);
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
             if (one) load_x(i, i);
         Ring r;
         uint32_t i = ahead;
-        for (; i < count; i++) {
+        for (; i < steps; i++) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[r.stage], r.parity));
             if (!ok) break;
             if (one) {
@@ -181,13 +190,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
         const uint32_t desc = i8_desc(kMmRows, nt);
         const uint64_t first = smem_desc(base);
         Ring r;
-        for (uint32_t i = 0; i < count; i++) {
+        for (uint32_t i = 0; i < steps; i++) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[r.stage], r.parity));
             if (!ok) break;
             tc_fence_after();
             const uint64_t wd = first + ((r.stage * stage_bytes) >> 4);
             if (one) {
                 mma_tile<1>(tmem, wd, wd + (kWBytes >> 4), desc, i > 0);
+                if (2 * i + 1 < count)
+                    mma_tile<1>(tmem, wd + (tile_bytes >> 4), wd + ((tile_bytes + kWBytes) >> 4), desc, true);
                 mma_commit(&empty[r.stage]);
             }
             r.next(stages);
@@ -510,17 +521,18 @@ struct MmPlan {
 //  - the weights come out of HBM at 6.5 KB per ns at best, and all SMs together
 //    read 11 KB per ns out of L2: a tile's weights once per token tile, its
 //    tokens once per 128 outputs;
-//  - the split kernel spends 0.14 us on 128 codes of a CTA's share of k (four
-//    narrow MMAs), 0.2 when the CTAs fill the GPU, starts and ends in 2.2 us, writes a token in 20 ns, and joins
-//    a cluster's sums in 1.3 us (0.1 for one token) and 17 ns per token.  Shares
-//    only as long as all clusters run at once (74 of two CTAs, 45 of three, 33
-//    of four, 15 of eight): 48 clusters of three took 15.7 us where 48 of two
-//    took 10.1;
+//  - the split kernel spends 0.12 us on 128 codes of a CTA's share of k (four
+//    narrow MMAs), 0.18 when the CTAs fill the GPU, starts and ends in 2.2 us,
+//    writes a token in 20 ns, and joins a cluster's sums in 0.1 us and 25 ns per
+//    token.  Shares only as long as all clusters run at once (74 of two CTAs,
+//    45 of three, 33 of four, 15 of eight): beyond, a share costs a whole CTA's
+//    time (48 clusters of three took 1.5 times what 48 of two took);
 //  - a pair spends 0.13 us + 1.05 ns per token of its tile on 128 codes, at
 //    least 10.5 ns per token on a tile (its output), and starts and ends in
 //    2.6 us.
 // A few tokens thus go to the split kernel with as many shares as run at once
-// (1 x 1536 x 2048: 2.7 us in 4 shares, 4.3 in one), more to pairs with the
+// (1 x 1536 x 2048: 2.6 us in 4 shares, 4.3 in one; 32 x 4096 x 6144: 6.6 us
+// in 2 shares, 7.3 in one), more to pairs with the
 // widest tile that still reaches all of them (257 x 4099 x 4095: 10.7 us with
 // 96 tokens a tile, 14.1 with 256; 8192 x 6144 x 8192: 253 us with 256, 278
 // with 192).
@@ -548,9 +560,9 @@ MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
             if (splits > 1 && tiles > mm.clusters[splits]) break;
             const uint64_t waves = splits > 1 ? 1 : (tiles + mm.sms - 1) / mm.sms;
             const float busy = (float)std::min<uint64_t>(tiles * splits, (uint64_t)mm.sms);
-            float cta = (float)((mm.kblocks + splits - 1) / splits) * (0.14f + 0.0004f * (float)nt + 0.0005f * busy);
+            float cta = (float)((mm.kblocks + splits - 1) / splits) * (0.12f + 0.0004f * (float)nt + 0.0004f * busy);
             if (waves > 1) cta += 1.f + 0.02f * tokens;
-            const float out = splits > 1 ? std::min(0.1f * tokens, 1.3f) + 0.017f * tokens : 0.02f * tokens;
+            const float out = splits > 1 ? 0.1f + 0.025f * tokens : 0.02f * tokens;
             const float t = 2.2f + std::max({(float)waves * cta, l2(tiles, nt), hbm}) + out;
             if (t < least) {
                 least = t;
@@ -574,8 +586,8 @@ cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, 
     }
     uint32_t columns = 32;
     while (columns < p.nt) columns *= 2;
-    const uint32_t stage = kWBytes + p.nt * kMmK, extra = 1024 + share_bytes(p.nt, p.splits);
-    const uint32_t stages = std::min({kMaxStages, (kMmSmem - extra) / stage, (mm.kblocks + p.splits - 1) / p.splits});
+    const uint32_t stage = 2 * (kWBytes + p.nt * kMmK), extra = 1024 + share_bytes(p.nt, p.splits);
+    const uint32_t stages = std::min({kMaxStages, (kMmSmem - extra) / stage, (mm.kblocks + 2 * p.splits - 1) / (2 * p.splits)});
     return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, m_tiles), p.splits,
                            extra + (size_t)stages * stage, s, mm.wmap, xmap, a, p.nt, p.splits, stages, columns);
 }
