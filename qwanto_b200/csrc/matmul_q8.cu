@@ -20,6 +20,7 @@
 // or scales or write anything.
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 #include <new>
 #include <type_traits>
 #include <utility>
@@ -56,9 +57,6 @@ MatmulQ8 *matmul_from(const QwnMatmulQ8Handle *h) {
 
 void matmul_release(MatmulQ8 *m) {
     cudaFree(m->w);
-    cudaFree(m->scales);
-    cudaFree(m->bias);
-    cudaFree(m->status);
     delete m;
 }
 
@@ -476,7 +474,7 @@ bool encode_codes(CUtensorMap *map, const int8_t *p, uint64_t width, uint64_t ro
 
 constexpr uint32_t kMmSmem = 227 * 1024 - 4096;  // dynamic, beside the static part
 
-// dynamic shared memory above 48 KB is opted into per kernel and device, when a handle is made there
+// dynamic shared memory above 48 KB is opted into per kernel and device
 template <typename K>
 cudaError_t allow_all_smem(K kernel) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmSmem);
@@ -592,28 +590,45 @@ cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, 
                            extra + (size_t)stages * stage, s, mm.wmap, xmap, a, p.nt, p.splits, stages, columns);
 }
 
-// prepares the kernels on the current device; how many clusters of each size it
-// runs at once with one CTA per SM
-bool count_clusters(MatmulQ8 *mm) {
-    if (allow_all_smem<float>() != cudaSuccess || allow_all_smem<__half>() != cudaSuccess ||
-        allow_all_smem<__nv_bfloat16>() != cudaSuccess)
-        return false;
-    for (uint32_t c = 1; c <= kMaxSplit; c++) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(c);
-        cfg.blockDim = dim3(kMmThreads);
-        cfg.dynamicSmemBytes = kMmSmem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = c;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, matmul_q8_split_kernel<float>, &cfg) != cudaSuccess) return false;
-        mm->clusters[c] = (uint32_t)n;
+// Prepares the kernels on a device (the current one), once, and tells how many
+// clusters of each size it runs at once with one CTA per SM.
+cudaError_t prepare_device(MatmulQ8 *mm) {
+    struct Device {
+        bool ready = false;
+        int sms = 0;
+        uint32_t clusters[kMaxSplit + 1] = {};
+    };
+    static std::mutex mu;
+    static Device devices[64];
+    if (mm->device < 0 || mm->device >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    Device &d = devices[mm->device];
+    if (!d.ready) {
+        cudaError_t e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, mm->device);
+        if (e == cudaSuccess) e = allow_all_smem<float>();
+        if (e == cudaSuccess) e = allow_all_smem<__half>();
+        if (e == cudaSuccess) e = allow_all_smem<__nv_bfloat16>();
+        for (uint32_t c = 1; c <= kMaxSplit && e == cudaSuccess; c++) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(c);
+            cfg.blockDim = dim3(kMmThreads);
+            cfg.dynamicSmemBytes = kMmSmem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = c;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, matmul_q8_split_kernel<float>, &cfg);
+            d.clusters[c] = (uint32_t)n;
+        }
+        if (e != cudaSuccess) return e;
+        d.ready = true;
     }
-    return true;
+    mm->sms = d.sms;
+    std::copy(d.clusters, d.clusters + kMaxSplit + 1, mm->clusters);
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -641,26 +656,30 @@ QWN_CUDA_ABI_API int qwn_matmul_q8_create(const QwnMatmulQ8Options *o, QwnMatmul
     m->n = o->out_features;
     m->k = o->in_features;
     m->kblocks = (o->in_features + kMmK - 1) / kMmK;
-    cudaDeviceGetAttribute(&m->sms, cudaDevAttrMultiProcessorCount, m->device);
     cudaStream_t s = static_cast<cudaStream_t>(o->stream);
-    const size_t wb = (size_t)m->kblocks * m->n * kMmK, fb = (size_t)m->n * sizeof(float);
-    if (!count_clusters(m)) {
-        set_cuda_error("qwn_matmul_q8_create", cudaGetLastError());
+    cudaError_t e = prepare_device(m);
+    if (e != cudaSuccess) {
+        set_cuda_error("qwn_matmul_q8_create", e);
         matmul_release(m);
         return QWN_CUDA_STATUS_RUNTIME_ERROR;
     }
-    if (cudaMalloc(&m->w, wb) != cudaSuccess || cudaMalloc(&m->scales, fb) != cudaSuccess ||
-        (o->bias_dev && cudaMalloc(&m->bias, fb) != cudaSuccess) ||
-        cudaMalloc(&m->status, sizeof(uint32_t)) != cudaSuccess) {
+    // one allocation: the weights, then scales, bias and the status word
+    const size_t wb = (size_t)m->kblocks * m->n * kMmK, fb = (size_t)m->n * sizeof(float);
+    if (cudaMalloc(&m->w, wb + 2 * fb + sizeof(uint32_t)) != cudaSuccess) {
         set_cuda_error("qwn_matmul_q8_create: allocation", cudaGetLastError());
         matmul_release(m);
         return QWN_CUDA_STATUS_OUT_OF_MEMORY;
     }
+    m->scales = reinterpret_cast<float *>(m->w + wb);
+    m->bias = o->bias_dev ? m->scales + m->n : nullptr;
+    m->status = reinterpret_cast<uint32_t *>(m->scales + 2 * (size_t)m->n);
     const uint64_t chunks = wb / 16;
-    pack_weight_kernel<<<(unsigned)std::min<uint64_t>((chunks + 255) / 256, (uint64_t)m->sms * 16), 256, 0, s>>>(
-        o->weight_dev, stride, m->n, m->k, chunks, m->w);
-    count_launch();
-    cudaError_t e = cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<uint64_t>((chunks + 255) / 256, (uint64_t)m->sms * 16));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    e = cudaLaunchKernelEx(&cfg, pack_weight_kernel, o->weight_dev, stride, m->n, m->k, chunks, m->w);
+    if (e == cudaSuccess) count_launch();
     if (e == cudaSuccess) e = cudaMemcpyAsync(m->scales, o->scales_dev, fb, cudaMemcpyDeviceToDevice, s);
     if (e == cudaSuccess && m->bias) e = cudaMemcpyAsync(m->bias, o->bias_dev, fb, cudaMemcpyDeviceToDevice, s);
     if (e == cudaSuccess) e = cudaMemsetAsync(m->status, 0, sizeof(uint32_t), s);
