@@ -15,6 +15,8 @@
 // rows_out takes 69 us, 6.5 TB/s (131 us with divisions and loads as they are
 // needed).  Rows over 8192 wide leave two CTAs' registers per SM and reach 4.1
 // TB/s.
+// Rows that are not whole 16-byte chunks, or start off them, are read value by
+// value (8192 x 4095 bf16: 86 us, 4096 wide 49; fp32 89).
 #include <type_traits>
 
 #include "kv_internal.cuh"
@@ -29,13 +31,15 @@ struct NormArgs {
     int8_t *codes;
     float *scales;
     uint64_t x_stride, residual_stride, residual_out_stride, codes_stride, rows_stride;
-    uint32_t width, rows_dtype;
+    uint32_t rows, width, rows_dtype;
     float eps;
     bool norm;
 };
 
-// the V values from `at` on, 16 bytes; beyond the row's end any values of it.
-// No branch: the loads of all chunks are in flight together.
+// V values, the first at `at`: 16 bytes that follow one another (STEP 1), or every
+// STEP-th value for a CTA of that many threads, so that a warp's accesses are
+// consecutive whatever the alignment.  Beyond the row's end any numbers.  No
+// branch: the loads of all chunks are in flight together.
 template <typename T>
 struct Chunk {
     uint32_t w[4];
@@ -48,17 +52,18 @@ struct Chunk {
 __device__ __forceinline__ uint32_t raw_bits(float x) { return __float_as_uint(x); }
 __device__ __forceinline__ uint32_t raw_bits(__half x) { return __half_as_ushort(x); }
 __device__ __forceinline__ uint32_t raw_bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
-template <bool VEC, typename T>
+template <int STEP, typename T>
 __device__ __forceinline__ Chunk<T> load_chunk(const T *p, int at, int width) {
     Chunk<T> c;
-    if constexpr (VEC) {
+    if constexpr (STEP == 1) {
         const uint4 v = *reinterpret_cast<const uint4 *>(p + (at < width ? at : 0));
         c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
     } else {
         constexpr int V = 16 / (int)sizeof(T), per = V / 4;
+        const T *q = p + at;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const uint32_t b = raw_bits(p[min(at + i, width - 1)]);
+            const uint32_t b = at + i * STEP < width ? raw_bits(q[i * STEP]) : 0u;
             if (i % per == 0) c.w[i / per] = b;
             else c.w[i / per] |= b << 16;
         }
@@ -71,29 +76,29 @@ __device__ __forceinline__ uint32_t pack2(const __nv_bfloat16 *, float a, float 
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-// the first n of V values, all in 16-byte (or one 8-byte) accesses where VEC
-template <bool VEC, int V, typename T>
-__device__ __forceinline__ void store_chunk(T *p, const float (&v)[V], int n) {
+// the same values back, those before the row's end
+template <int STEP, int V, typename T>
+__device__ __forceinline__ void store_chunk(T *p, int at, const float (&v)[V], int width) {
     constexpr int per = 4 / (int)sizeof(T), W = V / per;
     uint32_t w[W];
 #pragma unroll
     for (int i = 0; i < W; i++) w[i] = pack2(p, v[per * i], v[per * i + per - 1]);
-    if (VEC) {
-        if (n > 0) {
+    if (STEP == 1) {
+        if (at < width) {
             if constexpr (W % 4 == 0) {
 #pragma unroll
                 for (int i = 0; i < W; i += 4)
-                    *reinterpret_cast<uint4 *>(p + per * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+                    *reinterpret_cast<uint4 *>(p + at + per * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
             } else {
-                *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+                *reinterpret_cast<uint2 *>(p + at) = make_uint2(w[0], w[1]);
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            if (i >= n) break;
-            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
-            else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+            if (at + i * STEP >= width) continue;
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p + at)[i * STEP] = w[i];
+            else reinterpret_cast<uint16_t *>(p + at)[i * STEP] = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
         }
     }
 }
@@ -119,15 +124,19 @@ __device__ __forceinline__ float block_reduce(float v, float *sm) {
     return v;
 }
 
-// CH chunks of 16 bytes per thread hold the row; VEC: rows are whole chunks, and
-// every row and the weight start on 16 bytes (codes and rows_out on a chunk's part)
-template <typename T, int CH, bool VEC>
+// CH chunks of 16 bytes per thread hold the row.  STEP 1: rows are whole chunks,
+// and every row and the weight start on 16 bytes (codes and rows_out on a chunk's
+// part); otherwise STEP is the CTA's threads.
+template <typename T, int CH, int STEP>
 __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     __shared__ float sm[2][32];
     const int width = (int)a.width;
-    const size_t row = blockIdx.x;
-    auto at = [](int c) { return ((int)threadIdx.x + c * (int)blockDim.x) * V; };
+    const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (row >= a.rows) return;  // only with one warp per row, which waits for no other
+    auto at = [](int c) {
+        return STEP == 1 ? ((int)threadIdx.x + c * (int)blockDim.x) * V : (int)threadIdx.x + c * V * STEP;
+    };
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
     const T *w = static_cast<const T *>(a.weight);
@@ -139,14 +148,14 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
     {
         Chunk<T> xc[CH], rc[CH];
 #pragma unroll
-        for (int c = 0; c < CH; c++) xc[c] = load_chunk<VEC>(x, at(c), width);
+        for (int c = 0; c < CH; c++) xc[c] = load_chunk<STEP>(x, at(c), width);
         if (r) {
 #pragma unroll
-            for (int c = 0; c < CH; c++) rc[c] = load_chunk<VEC>(r, at(c), width);
+            for (int c = 0; c < CH; c++) rc[c] = load_chunk<STEP>(r, at(c), width);
         }
         if (w) {
 #pragma unroll
-            for (int c = 0; c < CH; c++) wc[c] = load_chunk<VEC>(w, at(c), width);
+            for (int c = 0; c < CH; c++) wc[c] = load_chunk<STEP>(w, at(c), width);
         }
 #pragma unroll
         for (int c = 0; c < CH; c++)
@@ -154,7 +163,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
             for (int i = 0; i < V; i++) {
                 float v = xc[c].get(i);
                 if (r) v += rc[c].get(i);
-                h[c][i] = at(c) + (VEC ? 0 : i) < width ? v : 0.f;
+                h[c][i] = at(c) + (STEP == 1 ? 0 : i * STEP) < width ? v : 0.f;
                 ss = fmaf(h[c][i], h[c][i], ss);
             }
     }
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
         T *out = static_cast<T *>(a.residual_out) + row * a.residual_out_stride;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            store_chunk<VEC>(out + at(c), h[c], width - at(c));
+            store_chunk<STEP>(out, at(c), h[c], width);
         }
     }
     float inv = 1.f;
@@ -190,7 +199,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
     const float magic = 12582912.f;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-        const int first = at(c), n = width - first;
+        const int first = at(c);
         uint32_t q[V / 4];
         float back[V];
 #pragma unroll
@@ -204,25 +213,35 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
             }
             q[i / 4] = prmt(prmt(bits[0], bits[1], 0x0040u), prmt(bits[2], bits[3], 0x0040u), 0x5410u);
         }
-        if (VEC && n > 0) {
-            if constexpr (V == 8) *reinterpret_cast<uint2 *>(codes + first) = make_uint2(q[0], q[1]);
-            else *reinterpret_cast<uint32_t *>(codes + first) = q[0];
-        } else if (!VEC) {
+        if (STEP == 1) {
+            if (first < width) {
+                if constexpr (V == 8) *reinterpret_cast<uint2 *>(codes + first) = make_uint2(q[0], q[1]);
+                else *reinterpret_cast<uint32_t *>(codes + first) = q[0];
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (i < n) codes[first + i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
+                if (first + i * STEP < width) (codes + first)[i * STEP] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
         }
         if (a.rows_out) {
-            const size_t o = row * a.rows_stride + first;
-            if (a.rows_dtype == QWN_DTYPE_F32) store_chunk<VEC>(static_cast<float *>(a.rows_out) + o, back, n);
-            else if (a.rows_dtype == QWN_DTYPE_F16) store_chunk<VEC>(static_cast<__half *>(a.rows_out) + o, back, n);
-            else store_chunk<VEC>(static_cast<__nv_bfloat16 *>(a.rows_out) + o, back, n);
+            const size_t o = row * a.rows_stride;
+            if (a.rows_dtype == QWN_DTYPE_F32) store_chunk<STEP>(static_cast<float *>(a.rows_out) + o, first, back, width);
+            else if (a.rows_dtype == QWN_DTYPE_F16) store_chunk<STEP>(static_cast<__half *>(a.rows_out) + o, first, back, width);
+            else store_chunk<STEP>(static_cast<__nv_bfloat16 *>(a.rows_out) + o, first, back, width);
         }
     }
 }
 
-template <typename T, bool VEC>
-cudaError_t launch_norm(const NormArgs &a, uint32_t rows, cudaStream_t s) {
+template <typename T, int STEP>
+cudaError_t launch_narrow(const NormArgs &a, uint32_t rows, uint32_t chunks, cudaStream_t s) {
+    const dim3 grid((rows + 7) / 8), block(32, 8);
+    if (chunks <= 32) return launch_next(rmsnorm_q8_kernel<T, 1, STEP>, grid, block, s, a);
+    if (chunks <= 64) return launch_next(rmsnorm_q8_kernel<T, 2, STEP>, grid, block, s, a);
+    return launch_next(rmsnorm_q8_kernel<T, 4, STEP>, grid, block, s, a);
+}
+
+template <typename T>
+cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
     const uint32_t chunks = (a.width + V - 1) / V;
     auto threads = [&](uint32_t ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
@@ -230,18 +249,42 @@ cudaError_t launch_norm(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     // one chunk per thread, 2.3 with four).  More: small CTAs with several
     // chunks each keep more loads in flight per SM (8191 x 6144 fp16: 69 us with
     // four chunks, 94 with one; 4096 x 1536 bf16: 10.2 with two, 11.2 with one).
+    // Many narrow rows go eight to a CTA, a warp each (8192 x 256 bf16: 4.4 us, 9.0
+    // with a CTA each; 8192 x 640: 10.2 and 11.8; 1000 x 1000: 4.5 and 4.1).
     const bool few = rows <= 296;
-    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, VEC>, dim3(rows), threads(1), s, a);
+    if (rows >= 2048 && chunks <= 96) return launch_narrow<T, 1>(a, rows, chunks, s);
+    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, 1>, dim3(rows), threads(1), s, a);
     if (threads(2) <= (few ? 1024u : 256u))
-        return launch_next(rmsnorm_q8_kernel<T, 2, VEC>, dim3(rows), threads(2), s, a);
-    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, VEC>, dim3(rows), threads(4), s, a);
-    if (V == 8 || threads(8) <= 512) return launch_next(rmsnorm_q8_kernel<T, 8, VEC>, dim3(rows), threads(8), s, a);
-    return launch_next(rmsnorm_q8_kernel<T, 64 / V, VEC>, dim3(rows), threads(64 / V), s, a);
+        return launch_next(rmsnorm_q8_kernel<T, 2, 1>, dim3(rows), threads(2), s, a);
+    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, 1>, dim3(rows), threads(4), s, a);
+    if (V == 8 || threads(8) <= 512) return launch_next(rmsnorm_q8_kernel<T, 8, 1>, dim3(rows), threads(8), s, a);
+    return launch_next(rmsnorm_q8_kernel<T, 64 / V, 1>, dim3(rows), threads(64 / V), s, a);
+}
+
+// rows off the 16-byte grid: CTAs of 128, 256 or 512 threads
+template <typename T, int CH>
+cudaError_t launch_values_ch(const NormArgs &a, uint32_t rows, uint32_t threads, cudaStream_t s) {
+    if (threads == 128) return launch_next(rmsnorm_q8_kernel<T, CH, 128>, dim3(rows), dim3(128), s, a);
+    if (threads == 256) return launch_next(rmsnorm_q8_kernel<T, CH, 256>, dim3(rows), dim3(256), s, a);
+    return launch_next(rmsnorm_q8_kernel<T, CH, 512>, dim3(rows), dim3(512), s, a);
+}
+template <typename T>
+cudaError_t launch_values(const NormArgs &a, uint32_t rows, cudaStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const uint32_t chunks = (a.width + V - 1) / V;
+    if (rows >= 2048 && chunks <= 96) return launch_narrow<T, 32>(a, rows, chunks, s);
+    uint32_t threads = rows <= 296 ? 512 : chunks <= 256 ? 128 : 256;
+    if (chunks > threads * (64 / V)) threads = 512;
+    if (chunks <= threads) return launch_values_ch<T, 1>(a, rows, threads, s);
+    if (chunks <= threads * 2) return launch_values_ch<T, 2>(a, rows, threads, s);
+    if (chunks <= threads * 4) return launch_values_ch<T, 4>(a, rows, threads, s);
+    if (V == 8 || chunks <= threads * 8) return launch_values_ch<T, 8>(a, rows, threads, s);
+    return launch_values_ch<T, 64 / V>(a, rows, threads, s);
 }
 
 template <typename T>
 cudaError_t launch_norm_type(const NormArgs &a, uint32_t rows, bool vec, cudaStream_t s) {
-    return vec ? launch_norm<T, true>(a, rows, s) : launch_norm<T, false>(a, rows, s);
+    return vec ? launch_chunks<T>(a, rows, s) : launch_values<T>(a, rows, s);
 }
 
 }  // namespace
@@ -270,6 +313,7 @@ QWN_CUDA_ABI_API int qwn_rmsnorm_q8(const QwnRmsNormQ8Request *r) {
     a.rows_out = r->rows_out_dev, a.rows_stride = stride(r->rows_stride);
     a.weight = r->weight_dev;
     a.scales = r->scales_dev;
+    a.rows = r->rows;
     a.width = r->width;
     a.rows_dtype = r->rows_dtype;
     a.eps = r->eps;

@@ -32,10 +32,10 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
 // launch a kernel that may start while the stream's previous one still runs (it
 // waits for it itself) and lets the next one start
 template <typename... Params, typename... Args>
-cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, uint32_t threads, cudaStream_t s, Args &&...args) {
+cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args &&...args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = block;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

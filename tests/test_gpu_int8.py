@@ -58,7 +58,9 @@ def _check_norm(torch, x, residual, weight, eps, norm, codes, scales, out_rows, 
 @pytest.mark.parametrize("rows,width,pad,offset", [(1, 1, 0, 0), (3, 7, 0, 0), (2, 64, 64, 0), (5, 100, 4, 0),
                                                    (4, 127, 0, 1), (33, 1536, 0, 0), (3, 2049, 7, 3), (2, 4096, 16, 0),
                                                    (2, 6144, 0, 8), (1, 12288, 0, 0), (2, 20011, 5, 1),
-                                                   (2, 32768, 0, 0)])
+                                                   (2, 32768, 0, 0), (2, 32767, 0, 0), (300, 4099, 0, 0), (301, 9000, 0, 1),
+                                                   (300, 1000, 24, 0), (2049, 257, 0, 0), (2051, 640, 0, 0),
+                                                   (2048, 64, 0, 1), (3000, 1, 0, 0), (2500, 380, 4, 4)])
 @pytest.mark.parametrize("residual,weighted,norm", [(True, True, True), (False, True, True), (True, False, False)])
 def test_rmsnorm(cuda, kind, rows, width, pad, offset, residual, weighted, norm):
     import qwanto_b200 as qb
