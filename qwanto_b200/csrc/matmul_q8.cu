@@ -530,9 +530,9 @@ struct MmPlan {
 //    2.6 us.
 // A few tokens thus go to the split kernel with as many shares as run at once
 // (1 x 1536 x 2048: 2.6 us in 4 shares, 4.3 in one; 32 x 4096 x 6144: 6.6 us
-// in 2 shares, 7.3 in one), more to pairs with the
-// widest tile that still reaches all of them (257 x 4099 x 4095: 10.7 us with
-// 96 tokens a tile, 14.1 with 256; 8192 x 6144 x 8192: 253 us with 256, 278
+// in 2 shares, 7.3 in one), more to pairs with the widest tile that still
+// reaches all of them (257 x 4099 x 4095: 10.7 us with 96 tokens a tile, 14.1
+// with 256; 8192 x 6144 x 8192 before its walk in groups: 253 us with 256, 278
 // with 192).
 MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
     MmPlan best{};

@@ -10,13 +10,17 @@
 // output is written once; bound by HBM, or by the launch for a few rows.
 // Codes come from y x (127 / max|y|) by adding 1.5 x 2^23: the sum's low byte
 // is the rounded code, and the sum less that number the code in fp32, with no
-// division or conversion per value.  All loads of a row, the weight's among
-// them, are issued before the first is used: 8191 x 6144 fp16 with residual and
-// rows_out takes 69 us, 6.5 TB/s (131 us with divisions and loads as they are
-// needed).  Rows over 8192 wide leave two CTAs' registers per SM and reach 4.1
-// TB/s.
+// division or conversion per value.  What can be done on two values in one
+// instruction is, and values that are no numbers are looked for once per thread
+// (a maximum that keeps NaN), so that 16-bit rows are not bound by instruction
+// issue (4096 x 12288 bf16: 71 us; 103 one by one).  All loads of a row are
+// issued before the first is used: 8191 x 6144 fp16 with residual and rows_out
+// takes 69 us, 6.5 TB/s (131 us with divisions and loads as they are needed).
+// Without a residual a row has fewer bytes in flight between its reductions
+// (8192 x 4096 bf16: 38 us, 4.4 TB/s, 47 and 6.4 with one); rows over 16384 wide
+// leave one CTA's registers per SM (2048 x 32768 bf16: 115 us, 5.3 TB/s).
 // Rows that are not whole 16-byte chunks, or start off them, are read value by
-// value (8192 x 4095 bf16: 86 us, 4096 wide 49; fp32 89).
+// value (8192 x 4095 bf16: 79 us, 4096 wide 47; fp32 87).
 #include <type_traits>
 
 #include "kv_internal.cuh"
@@ -48,7 +52,13 @@ struct Chunk {
         else if constexpr (std::is_same_v<T, __half>) return h2f((uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]));
         else return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
     }
+    __device__ __forceinline__ uint64_t two(int i) const { return pair(get(2 * i), get(2 * i + 1)); }
 };
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t raw_bits(float x) { return __float_as_uint(x); }
 __device__ __forceinline__ uint32_t raw_bits(__half x) { return __half_as_ushort(x); }
 __device__ __forceinline__ uint32_t raw_bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
@@ -77,9 +87,12 @@ __device__ __forceinline__ uint32_t pack2(const __nv_bfloat16 *, float a, float 
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 // the same values back, those before the row's end
-template <int STEP, int V, typename T>
-__device__ __forceinline__ void store_chunk(T *p, int at, const float (&v)[V], int width) {
-    constexpr int per = 4 / (int)sizeof(T), W = V / per;
+template <int STEP, int PAIRS, typename T>
+__device__ __forceinline__ void store_chunk(T *p, int at, const uint64_t (&pairs)[PAIRS], int width) {
+    constexpr int V = 2 * PAIRS, per = 4 / (int)sizeof(T), W = V / per;
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < PAIRS; i++) unpair(pairs[i], v[2 * i], v[2 * i + 1]);
     uint32_t w[W];
 #pragma unroll
     for (int i = 0; i < W; i++) w[i] = pack2(p, v[per * i], v[per * i + per - 1]);
@@ -126,10 +139,14 @@ __device__ __forceinline__ float block_reduce(float v, float *sm) {
 
 // CH chunks of 16 bytes per thread hold the row.  STEP 1: rows are whole chunks,
 // and every row and the weight start on 16 bytes (codes and rows_out on a chunk's
-// part); otherwise STEP is the CTA's threads.
-template <typename T, int CH, int STEP>
-__global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormArgs a) {
+// part); otherwise STEP is the CTA's threads.  CTAS: how many the compiler fits
+// the registers of an SM for.
+template <typename T, int CH, int STEP, int CTAS = 0>
+__global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
+    // the weight's chunks are held from the start, or come from L1 or L2 between the reductions where
+    // their registers would cost a CTA per SM (4096 x 14336 bf16 without residual: 61 us, 96)
+    constexpr bool kLateWeight = CH == (V == 8 ? 4 : 16);
     __shared__ float sm[2][32];
     const int width = (int)a.width;
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -140,9 +157,11 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
     const T *w = static_cast<const T *>(a.weight);
-    float h[CH][V];
+    uint64_t h[CH][V / 2];  // pairs of values
     Chunk<T> wc[CH];
-    float ss = 0.f;
+    // values past the row's end: any numbers in whole chunks, zeros otherwise
+    auto live = [&](int c) { return STEP != 1 || at(c) < width; };
+    uint64_t ss = 0;
     launch_dependents();
     wait_previous();
     {
@@ -153,46 +172,72 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
 #pragma unroll
             for (int c = 0; c < CH; c++) rc[c] = load_chunk<STEP>(r, at(c), width);
         }
-        if (w) {
+        if (w && !kLateWeight) {
 #pragma unroll
             for (int c = 0; c < CH; c++) wc[c] = load_chunk<STEP>(w, at(c), width);
         }
 #pragma unroll
-        for (int c = 0; c < CH; c++)
+        for (int c = 0; c < CH; c++) {
+            uint64_t sum = ss;
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                float v = xc[c].get(i);
-                if (r) v += rc[c].get(i);
-                h[c][i] = at(c) + (STEP == 1 ? 0 : i * STEP) < width ? v : 0.f;
-                ss = fmaf(h[c][i], h[c][i], ss);
+            for (int i = 0; i < V / 2; i++) {
+                h[c][i] = xc[c].two(i);
+                if (r) h[c][i] = add2(h[c][i], rc[c].two(i));
+                sum = fma2(h[c][i], h[c][i], sum);
             }
+            ss = live(c) ? sum : ss;
+        }
     }
     if (a.residual_out) {
         T *out = static_cast<T *>(a.residual_out) + row * a.residual_out_stride;
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            store_chunk<STEP>(out, at(c), h[c], width);
-        }
+        for (int c = 0; c < CH; c++) store_chunk<STEP>(out, at(c), h[c], width);
     }
     float inv = 1.f;
-    if (a.norm) inv = __frsqrt_rn(__fdiv_rn(block_reduce<false>(ss, sm[0]), (float)width) + a.eps);
-    float top = 0.f;
+    if (a.norm) {
+        float even, odd;
+        unpair(ss, even, odd);
+        inv = __frsqrt_rn(__fdiv_rn(block_reduce<false>(even + odd, sm[0]), (float)width) + a.eps);
+    }
+    float top = 0.f;  // NaN once a value is
 #pragma unroll
     for (int c = 0; c < CH; c++) {
+        if (w && kLateWeight) wc[c] = load_chunk<STEP>(w, at(c), width);
+        float most = top;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            float y = h[c][i] * inv;
-            if (w) y *= wc[c].get(i);
-            y = fabsf(y) < INFINITY ? y : 0.f;  // what is no number has code 0
-            top = fmaxf(top, fabsf(y));
-            h[c][i] = y;
+        for (int i = 0; i < V / 2; i++) {
+            h[c][i] = mul2(h[c][i], pair(inv, inv));
+            if (w) h[c][i] = mul2(h[c][i], wc[c].two(i));
+            float even, odd;
+            unpair(h[c][i], even, odd);
+            most = max_or_nan(max_or_nan(most, fabsf(even)), fabsf(odd));
         }
+        top = live(c) ? most : top;
+    }
+    if (!(top < INFINITY)) {  // what is no number has code 0
+        top = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) {
+                float even, odd;
+                unpair(h[c][i], even, odd);
+                even = fabsf(even) < INFINITY ? even : 0.f, odd = fabsf(odd) < INFINITY ? odd : 0.f;
+                h[c][i] = pair(even, odd);
+                if (live(c)) top = fmaxf(top, fmaxf(fabsf(even), fabsf(odd)));
+            }
     }
     top = block_reduce<true>(top, sm[1]);
     float scale = __fdiv_rn(top, 127.f);
-    // 127 / top as two factors, so that a row of values near the smallest ones does not overflow it
+    // 127 / top overflows in a row of values near the smallest ones: those are scaled up
     const float lift = top < 0x1p-100f ? 0x1p60f : 1.f;
     const float per = scale > 0.f ? __fdiv_rn(127.f, top * lift) : 0.f;
+    if (lift != 1.f) {
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) h[c][i] = mul2(h[c][i], pair(lift, lift));
+    }
     if (scale == 0.f) scale = 1.f;
     if (threadIdx.x == 0) a.scales[row] = scale;
     int8_t *codes = a.codes + row * a.codes_stride;
@@ -201,17 +246,19 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
     for (int c = 0; c < CH; c++) {
         const int first = at(c);
         uint32_t q[V / 4];
-        float back[V];
+        uint64_t back[V / 2];
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
+        for (int i = 0; i < V / 2; i += 2) {
             uint32_t bits[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float t = __fadd_rn(__fmul_rn(h[c][i + j] * lift, per), magic);
-                bits[j] = __float_as_uint(t);
-                back[i + j] = (t - magic) * scale;
+            for (int j = 0; j < 2; j++) {
+                float even, odd;
+                unpair(mul2(h[c][i + j], pair(per, per)), even, odd);
+                even = __fadd_rn(even, magic), odd = __fadd_rn(odd, magic);
+                bits[2 * j] = __float_as_uint(even), bits[2 * j + 1] = __float_as_uint(odd);
+                back[i + j] = mul2(add2(pair(even, odd), pair(-magic, -magic)), pair(scale, scale));
             }
-            q[i / 4] = prmt(prmt(bits[0], bits[1], 0x0040u), prmt(bits[2], bits[3], 0x0040u), 0x5410u);
+            q[i / 2] = prmt(prmt(bits[0], bits[1], 0x0040u), prmt(bits[2], bits[3], 0x0040u), 0x5410u);
         }
         if (STEP == 1) {
             if (first < width) {
@@ -232,11 +279,17 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512) rmsnorm_q8_kernel(NormAr
     }
 }
 
+// CTAS steers the compiler's use of registers: "at least one" gives 16-bit rows 44
+// instead of 48 (4096 x 1536 bf16: 9.3 us, 9.9; 8192 x 4095: 79, 82), and is worse
+// for fp32 rows value by value (8192 x 4095: 102 us, 87)
+template <typename T>
+constexpr int kCtas = sizeof(T) == 2 ? 1 : 0;
+
 template <typename T, int STEP>
 cudaError_t launch_narrow(const NormArgs &a, uint32_t rows, uint32_t chunks, cudaStream_t s) {
     const dim3 grid((rows + 7) / 8), block(32, 8);
-    if (chunks <= 32) return launch_next(rmsnorm_q8_kernel<T, 1, STEP>, grid, block, s, a);
-    if (chunks <= 64) return launch_next(rmsnorm_q8_kernel<T, 2, STEP>, grid, block, s, a);
+    if (chunks <= 32) return launch_next(rmsnorm_q8_kernel<T, 1, STEP, kCtas<T>>, grid, block, s, a);
+    if (chunks <= 64) return launch_next(rmsnorm_q8_kernel<T, 2, STEP, kCtas<T>>, grid, block, s, a);
     return launch_next(rmsnorm_q8_kernel<T, 4, STEP>, grid, block, s, a);
 }
 
@@ -248,15 +301,18 @@ cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     // Up to two rows per SM: wide CTAs answer sooner (1 x 1536 fp32: 1.9 us with
     // one chunk per thread, 2.3 with four).  More: small CTAs with several
     // chunks each keep more loads in flight per SM (8191 x 6144 fp16: 69 us with
-    // four chunks, 94 with one; 4096 x 1536 bf16: 10.2 with two, 11.2 with one).
-    // Many narrow rows go eight to a CTA, a warp each (8192 x 256 bf16: 4.4 us, 9.0
+    // four chunks, 94 with one; 4096 x 1536 bf16: 9.3 with two, 11.2 with one).
+    // Many narrow rows go eight to a CTA, a warp each (8192 x 256 bf16: 4.2 us, 9.0
     // with a CTA each; 8192 x 640: 10.2 and 11.8; 1000 x 1000: 4.5 and 4.1).
     const bool few = rows <= 296;
     if (rows >= 2048 && chunks <= 96) return launch_narrow<T, 1>(a, rows, chunks, s);
-    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, 1>, dim3(rows), threads(1), s, a);
+    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, 1, kCtas<T>>, dim3(rows), threads(1), s, a);
     if (threads(2) <= (few ? 1024u : 256u))
-        return launch_next(rmsnorm_q8_kernel<T, 2, 1>, dim3(rows), threads(2), s, a);
-    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, 1>, dim3(rows), threads(4), s, a);
+        return launch_next(rmsnorm_q8_kernel<T, 2, 1, kCtas<T>>, dim3(rows), threads(2), s, a);
+    // past 448 threads 72 registers leave one CTA per SM, 64 two (4096 x 16384 bf16: 119 us, 99)
+    if (V == 4 && threads(4) <= 512 || threads(4) <= 448)
+        return launch_next(rmsnorm_q8_kernel<T, 4, 1>, dim3(rows), threads(4), s, a);
+    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, 1, 2>, dim3(rows), threads(4), s, a);
     if (V == 8 || threads(8) <= 512) return launch_next(rmsnorm_q8_kernel<T, 8, 1>, dim3(rows), threads(8), s, a);
     return launch_next(rmsnorm_q8_kernel<T, 64 / V, 1>, dim3(rows), threads(64 / V), s, a);
 }
@@ -264,9 +320,10 @@ cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
 // rows off the 16-byte grid: CTAs of 128, 256 or 512 threads
 template <typename T, int CH>
 cudaError_t launch_values_ch(const NormArgs &a, uint32_t rows, uint32_t threads, cudaStream_t s) {
-    if (threads == 128) return launch_next(rmsnorm_q8_kernel<T, CH, 128>, dim3(rows), dim3(128), s, a);
-    if (threads == 256) return launch_next(rmsnorm_q8_kernel<T, CH, 256>, dim3(rows), dim3(256), s, a);
-    return launch_next(rmsnorm_q8_kernel<T, CH, 512>, dim3(rows), dim3(512), s, a);
+    constexpr int ctas = CH <= 2 ? kCtas<T> : 0;
+    if (threads == 128) return launch_next(rmsnorm_q8_kernel<T, CH, 128, ctas>, dim3(rows), dim3(128), s, a);
+    if (threads == 256) return launch_next(rmsnorm_q8_kernel<T, CH, 256, ctas>, dim3(rows), dim3(256), s, a);
+    return launch_next(rmsnorm_q8_kernel<T, CH, 512, ctas>, dim3(rows), dim3(512), s, a);
 }
 template <typename T>
 cudaError_t launch_values(const NormArgs &a, uint32_t rows, cudaStream_t s) {

@@ -141,6 +141,40 @@ def test_rmsnorm_rows_of_zeros_and_beyond_numbers(cuda):
         assert (codes[4] == 127).all()
 
 
+@pytest.mark.parametrize("kind", sorted(DTYPES))
+@pytest.mark.parametrize("width", [8, 257, 4096, 16384])
+def test_rows_beyond_numbers_of_every_type_and_width(cuda, kind, width):
+    import qwanto_b200 as qb
+    torch = cuda
+    dt, inf, nan = _type(torch, kind), float("inf"), float("nan")
+    x = torch.randn((6, width), device="cuda", generator=torch.Generator("cuda").manual_seed(width)).to(dt)
+    x[0] = 0.0
+    x[1, 0], x[1, width - 1] = nan, inf
+    x[2] = -inf
+    x[3] = float(torch.finfo(dt).tiny)  # its scale's inverse overflows in fp32
+    x[3, 1] = 0.0
+    codes = torch.full((6, width), 9, dtype=torch.int8, device="cuda")
+    scales = torch.full((6,), nan, device="cuda")
+    rows = torch.full((6, width), nan, device="cuda")
+    qb.rmsnorm_q8(x, 6, width, DTYPES[kind], codes, scales, norm=False, rows_out=rows, rows_dtype=1)
+    torch.cuda.synchronize()
+    assert rows.isfinite().all()
+    for i in (0, 2):
+        assert scales[i] == 1.0 and not codes[i].any() and not rows[i].any()
+    assert codes[3, 1] == 0 and (codes[3].abs().sum() == 127 * (width - 1))
+    for i in (1, 4, 5):
+        fine = x[i].isfinite()
+        top = float(x[i][fine].abs().max())
+        assert abs(float(scales[i]) - top / 127) <= 2 * U * top and not codes[i][~fine].any()
+        assert ((codes[i].double() - x[i].double() / (top / 127)).abs()[fine] <= 0.5 + 1e-4).all()
+    # rows of zeros have no root without eps; a value that is none spoils its row's mean alone
+    qb.rmsnorm_q8(x, 6, width, DTYPES[kind], codes, scales, eps=0.0)
+    torch.cuda.synchronize()
+    for i in (0, 1, 2):
+        assert scales[i] == 1.0 and not codes[i].any()
+    assert scales[4:].isfinite().all() and (codes[4:].abs().amax(1) == 127).all()
+
+
 # ---- products -------------------------------------------------------------------
 
 def _codes(torch, g, rows, k, low=-127):
