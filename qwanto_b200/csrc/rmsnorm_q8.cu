@@ -13,14 +13,17 @@
 // division or conversion per value.  What can be done on two values in one
 // instruction is, and values that are no numbers are looked for once per thread
 // (a maximum that keeps NaN), so that 16-bit rows are not bound by instruction
-// issue (4096 x 12288 bf16: 71 us; 103 one by one).  All loads of a row are
+// issue (4096 x 12288 bf16: 71 us; 103 one by one).  All loads of x and r are
 // issued before the first is used: 8191 x 6144 fp16 with residual and rows_out
 // takes 69 us, 6.5 TB/s (131 us with divisions and loads as they are needed).
-// Without a residual a row has fewer bytes in flight between its reductions
-// (8192 x 4096 bf16: 38 us, 4.4 TB/s, 47 and 6.4 with one); rows over 16384 wide
-// leave one CTA's registers per SM (2048 x 32768 bf16: 115 us, 5.3 TB/s).
+// What is not given is added as -0 or multiplied as 1, which changes no value:
+// conditions per value had cost as much (1000 x 6144 bf16: 9.5 us, 10.3).  Rows
+// without a residual have kernels of their own; they are bound by instruction issue
+// and by fewer bytes in flight between a row's reductions (8192 x 4096 bf16: 30
+// us, 5.6 TB/s; 46 and 6.5 with a residual).  Rows over 16384 wide leave one CTA's
+// registers per SM (2048 x 32768 bf16: 113 us, 5.3 TB/s).
 // Rows that are not whole 16-byte chunks, or start off them, are read value by
-// value (8192 x 4095 bf16: 79 us, 4096 wide 47; fp32 87).
+// value (8192 x 4095 bf16: 77 us, 4096 wide 46; fp32 87).
 #include <type_traits>
 
 #include "kv_internal.cuh"
@@ -54,6 +57,17 @@ struct Chunk {
     }
     __device__ __forceinline__ uint64_t two(int i) const { return pair(get(2 * i), get(2 * i + 1)); }
 };
+// what leaves every value as it is when added, or multiplied with
+template <typename T>
+__device__ __forceinline__ Chunk<T> minus_zeros() {
+    constexpr uint32_t b = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    return {{b, b, b, b}};
+}
+template <typename T>
+__device__ __forceinline__ Chunk<T> ones() {
+    constexpr uint32_t b = sizeof(T) == 4 ? 0x3F800000u : std::is_same_v<T, __half> ? 0x3C003C00u : 0x3F803F80u;
+    return {{b, b, b, b}};
+}
 __device__ __forceinline__ float max_or_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -140,13 +154,14 @@ __device__ __forceinline__ float block_reduce(float v, float *sm) {
 // CH chunks of 16 bytes per thread hold the row.  STEP 1: rows are whole chunks,
 // and every row and the weight start on 16 bytes (codes and rows_out on a chunk's
 // part); otherwise STEP is the CTA's threads.  CTAS: how many the compiler fits
-// the registers of an SM for.
-template <typename T, int CH, int STEP, int CTAS = 0>
+// the registers of an SM for.  RES: there may be a residual.
+template <typename T, int CH, int STEP, int CTAS = 0, bool RES = true>
 __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     // the weight's chunks are held from the start, or come from L1 or L2 between the reductions where
-    // their registers would cost a CTA per SM (4096 x 14336 bf16 without residual: 61 us, 96)
-    constexpr bool kLateWeight = CH == (V == 8 ? 4 : 16);
+    // their registers would cost a CTA per SM (4096 x 14336 bf16 without residual: 61 us, 96; 2048 x
+    // 10240 fp32: 50, 76); 16-bit rows over 16384 wide have one CTA either way (2048 x 32768: 113, 116)
+    constexpr bool kLateWeight = CH * V >= 32 && !(V == 8 && CH == 8);
     __shared__ float sm[2][32];
     const int width = (int)a.width;
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -155,7 +170,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(
         return STEP == 1 ? ((int)threadIdx.x + c * (int)blockDim.x) * V : (int)threadIdx.x + c * V * STEP;
     };
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+    const T *r = RES && a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
     const T *w = static_cast<const T *>(a.weight);
     uint64_t h[CH][V / 2];  // pairs of values
     Chunk<T> wc[CH];
@@ -168,10 +183,14 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(
         Chunk<T> xc[CH], rc[CH];
 #pragma unroll
         for (int c = 0; c < CH; c++) xc[c] = load_chunk<STEP>(x, at(c), width);
+#pragma unroll
+        for (int c = 0; c < CH; c++) rc[c] = minus_zeros<T>();
         if (r) {
 #pragma unroll
             for (int c = 0; c < CH; c++) rc[c] = load_chunk<STEP>(r, at(c), width);
         }
+#pragma unroll
+        for (int c = 0; c < CH; c++) wc[c] = ones<T>();
         if (w && !kLateWeight) {
 #pragma unroll
             for (int c = 0; c < CH; c++) wc[c] = load_chunk<STEP>(w, at(c), width);
@@ -182,7 +201,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(
 #pragma unroll
             for (int i = 0; i < V / 2; i++) {
                 h[c][i] = xc[c].two(i);
-                if (r) h[c][i] = add2(h[c][i], rc[c].two(i));
+                if (RES) h[c][i] = add2(h[c][i], rc[c].two(i));
                 sum = fma2(h[c][i], h[c][i], sum);
             }
             ss = live(c) ? sum : ss;
@@ -206,8 +225,7 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(
         float most = top;
 #pragma unroll
         for (int i = 0; i < V / 2; i++) {
-            h[c][i] = mul2(h[c][i], pair(inv, inv));
-            if (w) h[c][i] = mul2(h[c][i], wc[c].two(i));
+            h[c][i] = mul2(mul2(h[c][i], pair(inv, inv)), wc[c].two(i));
             float even, odd;
             unpair(h[c][i], even, odd);
             most = max_or_nan(max_or_nan(most, fabsf(even)), fabsf(odd));
@@ -280,8 +298,8 @@ __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(
 }
 
 // CTAS steers the compiler's use of registers: "at least one" gives 16-bit rows 44
-// instead of 48 (4096 x 1536 bf16: 9.3 us, 9.9; 8192 x 4095: 79, 82), and is worse
-// for fp32 rows value by value (8192 x 4095: 102 us, 87)
+// instead of 48 (4096 x 1536 bf16: 9.3 us, 9.9), and is worse for fp32 rows value by
+// value (8192 x 4095: 102 us, 87)
 template <typename T>
 constexpr int kCtas = sizeof(T) == 2 ? 1 : 0;
 
@@ -293,6 +311,11 @@ cudaError_t launch_narrow(const NormArgs &a, uint32_t rows, uint32_t chunks, cud
     return launch_next(rmsnorm_q8_kernel<T, 4, STEP>, grid, block, s, a);
 }
 
+template <typename T, int CH, int CTAS>
+cudaError_t launch_row(const NormArgs &a, uint32_t rows, uint32_t threads, cudaStream_t s) {
+    if (a.residual) return launch_next(rmsnorm_q8_kernel<T, CH, 1, CTAS>, dim3(rows), threads, s, a);
+    return launch_next(rmsnorm_q8_kernel<T, CH, 1, CTAS, false>, dim3(rows), threads, s, a);
+}
 template <typename T>
 cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
@@ -301,20 +324,24 @@ cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     // Up to two rows per SM: wide CTAs answer sooner (1 x 1536 fp32: 1.9 us with
     // one chunk per thread, 2.3 with four).  More: small CTAs with several
     // chunks each keep more loads in flight per SM (8191 x 6144 fp16: 69 us with
-    // four chunks, 94 with one; 4096 x 1536 bf16: 9.3 with two, 11.2 with one).
+    // four chunks, 94 with one; 4096 x 1536 bf16: 9.0 with two, 11.2 with one).
+    // Without a residual a row is less to load and instructions count more, of
+    // which four chunks need fewer each (8192 x 4096 bf16: 30 us, 37 with two).
     // Many narrow rows go eight to a CTA, a warp each (8192 x 256 bf16: 4.2 us, 9.0
     // with a CTA each; 8192 x 640: 10.2 and 11.8; 1000 x 1000: 4.5 and 4.1).
     const bool few = rows <= 296;
     if (rows >= 2048 && chunks <= 96) return launch_narrow<T, 1>(a, rows, chunks, s);
-    if (few && threads(1) <= 1024) return launch_next(rmsnorm_q8_kernel<T, 1, 1, kCtas<T>>, dim3(rows), threads(1), s, a);
-    if (threads(2) <= (few ? 1024u : 256u))
-        return launch_next(rmsnorm_q8_kernel<T, 2, 1, kCtas<T>>, dim3(rows), threads(2), s, a);
-    // past 448 threads 72 registers leave one CTA per SM, 64 two (4096 x 16384 bf16: 119 us, 99)
+    if (few && threads(1) <= 1024) return launch_row<T, 1, kCtas<T>>(a, rows, threads(1), s);
+    if (threads(2) <= (few ? 1024u : a.residual ? 256u : 96u))
+        return launch_row<T, 2, kCtas<T>>(a, rows, threads(2), s);
+    // past 448 threads 72 registers leave one CTA per SM, 64 two (4096 x 16384 bf16: 119 us, 91)
     if (V == 4 && threads(4) <= 512 || threads(4) <= 448)
-        return launch_next(rmsnorm_q8_kernel<T, 4, 1>, dim3(rows), threads(4), s, a);
-    if (threads(4) <= 512) return launch_next(rmsnorm_q8_kernel<T, 4, 1, 2>, dim3(rows), threads(4), s, a);
-    if (V == 8 || threads(8) <= 512) return launch_next(rmsnorm_q8_kernel<T, 8, 1>, dim3(rows), threads(8), s, a);
-    return launch_next(rmsnorm_q8_kernel<T, 64 / V, 1>, dim3(rows), threads(64 / V), s, a);
+        return launch_row<T, 4, 0>(a, rows, threads(4), s);
+    if (threads(4) <= 512) return launch_row<T, 4, 2>(a, rows, threads(4), s);
+    if (V == 4 && threads(8) > 448 && threads(8) <= 512 && !a.residual)  // 2048 x 16384 fp32: 53 us, 75
+        return launch_row<T, 8, 2>(a, rows, threads(8), s);
+    if (V == 8 || threads(8) <= 512) return launch_row<T, 8, 0>(a, rows, threads(8), s);
+    return launch_row<T, 64 / V, 0>(a, rows, threads(64 / V), s);
 }
 
 // rows off the 16-byte grid: CTAs of 128, 256 or 512 threads
