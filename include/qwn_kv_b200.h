@@ -470,9 +470,9 @@ QWN_CUDA_ABI_API int qwn_kv_load_tokens(QwnKvPoolHandle *pool, const QwnKvLoadTo
  *     h = x + residual                              (fp32)
  *     y = h / sqrt(mean(h^2) + eps) * weight        (QWN_NORM_RMS; QWN_NORM_NONE: y = h * weight)
  *     scale = max|y| / 127 over the finite y, 1 if that is 0
- *     code = y / scale rounded to nearest even, 0 where y is not finite
+ *     code = y / scale (in fp32) rounded to nearest even, within +-127; 0 where y is not finite
  * the rules of the pool's Q8 codecs (c/qwanto_turboquant.c:555-586) over a
- * whole row.  residual_out receives h in the rows' type; y comes from h before
+ * whole row, ties included.  residual_out receives h in the rows' type; y comes from h before
  * that rounding.  A mean of squares beyond fp32 is not finite: such a row's codes
  * are 0.  rows_out, where given, receives code x scale: what a product
  * that stays in 16 bits must see to agree with the int8 ones. */
