@@ -18,6 +18,12 @@
 // Both kernels start while the stream's previous kernel still runs
 // (programmatic launch), fetch weights, and wait for it before they read codes
 // or scales or write anything.
+//
+// Tensor memory is taken so that no allocation waits for a CTA that waits for
+// it.  A kernel lets the next one start only when all its CTAs hold theirs; at
+// most four CTAs of the split kernel fit an SM, by their shared memory, with a
+// quarter of its columns each; a CTA of the pair kernel, which takes all
+// columns, shares an SM with no other CTA of either kernel.
 #include <algorithm>
 #include <cstring>
 #include <mutex>
@@ -39,6 +45,14 @@ constexpr uint32_t kMaxStages = 12;
 constexpr uint32_t kOutWarps = 8;    // read TMEM and write: two for each quarter of its lanes
 constexpr uint32_t kMmThreads = 64 + 32 * kOutWarps; // TMA warp, MMA warp, those
 constexpr uint32_t kMaxSplit = 8;    // CTAs of a cluster that share an output tile
+constexpr uint32_t kColumns = 512;   // of an SM's tensor memory
+constexpr uint32_t kSplitColumns = 128, kSplitTokens = 128;
+// shared memory: of an SM, what a CTA takes beside its own, dynamic at most (beside the static part) and at least
+constexpr uint32_t kSmSmem = 228 * 1024, kCtaSmem = 1024, kMmSmem = 227 * 1024 - 4096;
+constexpr uint32_t kSplitSmem = 46 * 1024, kPairSmem = 182 * 1024;
+static_assert(kSplitTokens <= kSplitColumns, "a column per token");
+static_assert((kColumns / kSplitColumns + 1) * (kSplitSmem + kCtaSmem) > kSmSmem, "an SM has columns for all its split CTAs");
+static_assert(kPairSmem + kSplitSmem + 2 * kCtaSmem > kSmSmem && kPairSmem <= kMmSmem, "a pair's CTA is alone");
 
 struct MatmulQ8 {
     int device = 0, sms = 148;
@@ -117,7 +131,7 @@ template <typename T>
 __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __grid_constant__ CUtensorMap wmap,
                                                                         const __grid_constant__ CUtensorMap xmap,
                                                                         MmArgs a, uint32_t nt, uint32_t splits,
-                                                                        uint32_t stages, uint32_t columns) {
+                                                                        uint32_t stages) {
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_at;
@@ -130,7 +144,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     const uint32_t kb1 = (uint32_t)((uint64_t)a.kblocks * (rank + 1) / splits);
     const uint32_t stage_bytes = 2 * (kWBytes + nt * kMmK), count = kb1 - kb0;
     const uint32_t valid = min(nt, a.m - m0);  // tokens of this tile that exist
-    launch_dependents();
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < stages; i++) {
             mbar_init(&full[i], 1);
@@ -139,9 +152,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
         mbar_init(&done, 1);
         fence_barrier_init();
     }
-    if (warp == 1) tmem_alloc<1>(&tmem_at, columns);
+    if (warp == 1) tmem_alloc<1>(&tmem_at, kSplitColumns);
     tc_fence_before();
     __syncthreads();
+    launch_dependents();  // not before: what starts may want tensor memory too
     if (splits > 1) cluster_arrive();  // this CTA runs: the others may write to it from their wait on
     tc_fence_after();
     const uint32_t tmem = tmem_at;
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_free<1>(tmem, columns);
+        tmem_free<1>(tmem, kSplitColumns);
     }
 }
 
@@ -312,7 +326,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     const uint32_t rank = cluster_rank(), pairs = gridDim.x >> 1, n_tiles = tiles / m_tiles;
     const uint32_t half = nt / 2, stage_bytes = kWBytes + half * kMmK;
-    launch_dependents();
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kPairStages; i++) {
             mbar_init(&full[i], 1);
@@ -324,9 +337,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
         }
         fence_barrier_init();
     }
-    if (warp == 1) tmem_alloc<2>(&tmem_at, 512);
+    if (warp == 1) tmem_alloc<2>(&tmem_at, kColumns);
     tc_fence_before();
     __syncthreads();
+    launch_dependents();
     cluster_sync();  // both CTAs' barriers exist
     tc_fence_after();
     const uint32_t tmem = tmem_at;
@@ -439,7 +453,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
     cluster_sync();  // neither CTA's memory or barriers go while the other may still use them
     if (warp == 1) {
         tc_fence_after();
-        tmem_free<2>(tmem, 512);
+        tmem_free<2>(tmem, kColumns);
     }
 }
 
@@ -471,8 +485,6 @@ bool encode_codes(CUtensorMap *map, const int8_t *p, uint64_t width, uint64_t ro
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-constexpr uint32_t kMmSmem = 227 * 1024 - 4096;  // dynamic, beside the static part
 
 // dynamic shared memory above 48 KB is opted into per kernel and device
 template <typename K>
@@ -550,7 +562,7 @@ MmPlan plan_matmul(const MatmulQ8 &mm, uint32_t m) {
         }
     }
     if (m > 1024) return best;
-    for (uint32_t m_tiles = (m + 127) / 128; m_tiles <= 8 && (m_tiles - 1) * 16 < m; m_tiles++) {
+    for (uint32_t m_tiles = (m + kSplitTokens - 1) / kSplitTokens; m_tiles <= 8 && (m_tiles - 1) * 16 < m; m_tiles++) {
         const uint32_t nt = ((m + m_tiles - 1) / m_tiles + 15) / 16 * 16, count = (m + nt - 1) / nt;
         const uint64_t tiles = (uint64_t)n_tiles * count;
         const float tokens = (float)std::min(m, nt);
@@ -579,15 +591,13 @@ cudaError_t launch_matmul(const MatmulQ8 &mm, const MmArgs &a, const int8_t *x, 
     if (!encode_codes(&xmap, x, mm.k, a.m, x_stride, p.pair ? p.nt / 2 : p.nt)) return cudaErrorInvalidValue;
     if (p.pair) {
         const uint32_t tiles = (n_tiles + 1) / 2 * m_tiles, pairs = std::min(tiles, (uint32_t)mm.sms / 2);
-        const size_t smem = 1024 + (size_t)kPairStages * (kWBytes + p.nt / 2 * kMmK);
+        const uint32_t smem = std::max(kPairSmem, 1024 + kPairStages * (kWBytes + p.nt / 2 * kMmK));
         return launch_clusters(matmul_q8_pair_kernel<T>, dim3(2 * pairs), 2, smem, s, mm.wmap, xmap, a, p.nt, m_tiles, tiles);
     }
-    uint32_t columns = 32;
-    while (columns < p.nt) columns *= 2;
     const uint32_t stage = 2 * (kWBytes + p.nt * kMmK), extra = 1024 + share_bytes(p.nt, p.splits);
     const uint32_t stages = std::min({kMaxStages, (kMmSmem - extra) / stage, (mm.kblocks + 2 * p.splits - 1) / (2 * p.splits)});
     return launch_clusters(matmul_q8_split_kernel<T>, dim3(n_tiles * p.splits, m_tiles), p.splits,
-                           extra + (size_t)stages * stage, s, mm.wmap, xmap, a, p.nt, p.splits, stages, columns);
+                           std::max(kSplitSmem, extra + stages * stage), s, mm.wmap, xmap, a, p.nt, p.splits, stages);
 }
 
 // Prepares the kernels on a device (the current one), once, and tells how many

@@ -91,26 +91,29 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *m
 }
 
 // ---- TMEM and the MMA -----------------------------------------------------------
+// A CTA allocates once and gives up its permit at once: held to its end, the
+// permit keeps the SM's other CTAs waiting in their allocation, and clusters that
+// got to two SMs in different orders would wait for each other.
 template <int CTAS>
 __device__ __forceinline__ void tmem_alloc(uint32_t *where, uint32_t columns) {
-    if constexpr (CTAS == 1)
+    if constexpr (CTAS == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)),
                      "r"(columns)
                      : "memory");
-    else
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)),
                      "r"(columns)
                      : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
 }
 template <int CTAS>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
-    if constexpr (CTAS == 1) {
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CTAS == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
-    } else {
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    else
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
-    }
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

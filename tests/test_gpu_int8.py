@@ -343,3 +343,35 @@ def test_matmul_refusals(cuda):
         qb.MatmulQ8(w, 8, 131072, sx)
     assert mm.check() == 0
     mm.close()
+
+
+def test_products_of_both_kinds_one_behind_the_other(cuda):
+    """Every launch starts while the one before it runs, each with tensor memory
+    of its own: few tokens, a cluster per tile, pairs with narrow and wide tiles,
+    on one stream and on three at once."""
+    import qwanto_b200 as qb
+    torch = cuda
+    g = torch.Generator("cuda").manual_seed(21)
+    products = []
+    for n, k in ((2048, 128), (4096, 1536), (1000, 4096), (20000, 256)):
+        w = torch.randint(-127, 128, (n, k), device="cuda", generator=g).to(torch.int8)
+        sw = torch.rand(n, device="cuda", generator=g) * 0.01
+        products.append((qb.MatmulQ8(w, n, k, sw), w, sw))
+    jobs = []
+    for m in (1, 600, 33, 2, 257, 128, 64, 1500, 16):
+        for mm, w, sw in products:
+            x, stride = _codes(torch, g, m, mm.in_features)
+            jobs.append((mm, w, sw, x, stride, torch.rand(m, device="cuda", generator=g), m))
+    torch.cuda.synchronize()
+    for streams in ([None], [torch.cuda.Stream() for _ in range(3)]):
+        outs = [torch.full((j[6], j[0].out_features), float("nan"), device="cuda") for j in jobs]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for i, (mm, _, _, x, stride, sx, m) in enumerate(jobs):
+                mm(x, sx, m, outs[i], 1, codes_stride=stride, stream=streams[i % len(streams)])
+        torch.cuda.synchronize()
+        for (mm, w, sw, x, _, sx, m), out in zip(jobs, outs):
+            assert mm.check() == 0
+            _check_matmul(torch, x[:, :mm.in_features], w, sx, sw, None, "f32", out)
+    for mm, _, _ in products:
+        mm.close()

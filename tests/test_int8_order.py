@@ -1,0 +1,44 @@
+"""The product kernels' hand-overs, as their source states them: what must come
+before what for a launch never to wait for a later one.  A run could only show the
+opposite by hanging, so these are read, not run."""
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+KERNELS = ["matmul_q8_split_kernel", "matmul_q8_pair_kernel"]
+
+
+def _source(name):
+    text = open(os.path.join(ROOT, "qwanto_b200", "csrc", name)).read()
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def _body(text, name):
+    """The function's text from its first brace to the matching one."""
+    at = text.index("{", re.search(rf"\b{name}\s*\(", text).end())
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[at:i + 1]
+    raise AssertionError(name)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_the_next_launch_starts_after_tensor_memory_is_held(kernel):
+    """A CTA of the next launch that held columns while this one's allocation waits
+    for them would wait for this launch's end: both for good."""
+    body = _body(_source("matmul_q8.cu"), kernel)
+    starts = [m.start() for m in re.finditer(r"\blaunch_dependents\(\)", body)]
+    assert len(starts) == 1
+    assert body.index("tmem_alloc<") < body.index("__syncthreads()") < starts[0]
+
+
+def test_the_permit_to_allocate_is_given_up_at_once():
+    text = _source("tcgen05.cuh")
+    alloc, free = _body(text, "tmem_alloc"), _body(text, "tmem_free")
+    for group in ("cta_group::1", "cta_group::2"):
+        assert alloc.index(f"tcgen05.alloc.{group}") < alloc.index(f"tcgen05.relinquish_alloc_permit.{group}")
+    assert "relinquish" not in free
