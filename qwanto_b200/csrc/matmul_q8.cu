@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
         const uint32_t desc = i8_desc(kMmRows, nt);
         const uint64_t first = smem_desc(base);
         Ring r;
+        wait_previous();  // the tokens come after it: its time does not count as waiting for them
         for (uint32_t i = 0; i < steps; i++) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[r.stage], r.parity));
             if (!ok) break;
@@ -386,6 +387,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
         const uint64_t first = smem_desc(base);
         Ring r;
         uint32_t n = 0;
+        wait_previous();  // the tokens come after it: its time does not count as waiting for them
         for (uint32_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs, n++) {
             const uint32_t buf = n & 1, d = tmem + buf * kPairTokens;
             if (n >= 2) {

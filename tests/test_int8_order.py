@@ -42,3 +42,25 @@ def test_the_permit_to_allocate_is_given_up_at_once():
     for group in ("cta_group::1", "cta_group::2"):
         assert alloc.index(f"tcgen05.alloc.{group}") < alloc.index(f"tcgen05.relinquish_alloc_permit.{group}")
     assert "relinquish" not in free
+
+
+def _branch(body, start):
+    """The block behind a condition."""
+    at = body.index("{", body.index(start))
+    depth = 0
+    for i in range(at, len(body)):
+        depth += {"{": 1, "}": -1}.get(body[i], 0)
+        if depth == 0:
+            return body[at:i + 1]
+    raise AssertionError(start)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_no_bounded_wait_counts_the_previous_launch(kernel):
+    """Every role that polls a barrier which depends on the previous launch waits for
+    that launch first: its running time must not use up the limit."""
+    body = _body(_source("matmul_q8.cu"), kernel)
+    for role in ("if (warp == 0)", "if (warp == 1", "if (warp >= 2)"):
+        block = _branch(body[body.index("launch_dependents()"):], role)
+        assert "mbar_wait" in block, role
+        assert block.index("wait_previous()") < block.index("mbar_wait"), role
