@@ -195,8 +195,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
             }
             r.next(stages);
         }
-        if (!ok && one)  // the copies in flight land before the memory goes
-            for (uint32_t j = i - stages; j < i; j++) mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
+        // the copies in flight land before the memory goes, whichever warp gave up
+        if (one)
+            for (uint32_t j = i - min(i, stages); j < i; j++) ok &= mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
     } else if (warp == 1) {
         const bool one = elect_one();
         const uint32_t desc = i8_desc(kMmRows, nt);
@@ -217,6 +218,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_split_kernel(const __
             r.next(stages);
         }
         if (one) mma_commit(&done);
+        __syncwarp();
+        ok &= mbar_wait_bounded(&done, 0);  // no product in flight when the memory goes
     }
     const uint32_t quarter = warp & 3, feature = quarter * 32 + lane;  // TMEM lanes this warp may read
     const uint32_t lanes = tmem + (quarter << 21);
@@ -378,9 +381,20 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
                 r.next(kPairStages);
             }
         }
-        if (!ok && one && rank == 0)  // the copies in flight land before the memory goes
-            for (uint32_t j = i - kPairStages; j < i; j++)
-                mbar_wait_cluster(&full[j % kPairStages], (j / kPairStages) & 1);
+        // the copies in flight land before the memory goes, whichever warp gave up; where it was this one,
+        // the other CTA may be up to a ring of stages ahead (it fills them in order: the first half that
+        // does not come is the last)
+        if (one && rank == 0) {
+            const uint32_t walk = (tiles - (blockIdx.x >> 1) + pairs - 1) / pairs * a.kblocks;
+            const uint32_t ahead_of = ok ? i : min(i + kPairStages, walk);
+            for (uint32_t j = i - min(i, kPairStages); j < ahead_of; j++) {
+                if (j >= i) mbar_expect_tx(&full[j % kPairStages], stage_bytes);
+                if (!mbar_wait_cluster(&full[j % kPairStages], (j / kPairStages) & 1)) {
+                    ok = false;
+                    break;
+                }
+            }
+        }
     } else if (warp == 1 && rank == 0) {
         const bool one = elect_one();
         const uint32_t desc = i8_desc(2 * kMmRows, nt);
@@ -408,6 +422,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
             }
             if (one) mma_commit_pair(&acc_full[buf]);
         }
+        __syncwarp();
+        if (n > 0) ok &= mbar_wait_cluster(&acc_full[(n - 1) & 1], ((n - 1) / 2) & 1);  // none in flight when the memory goes
     } else if (warp >= 2) {
         const uint32_t quarter = warp & 3, second = (uint32_t)(warp - 2) >> 2;
         uint32_t n = 0;

@@ -64,3 +64,22 @@ def test_no_bounded_wait_counts_the_previous_launch(kernel):
         block = _branch(body[body.index("launch_dependents()"):], role)
         assert "mbar_wait" in block, role
         assert block.index("wait_previous()") < block.index("mbar_wait"), role
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_copies_land_whichever_role_gives_up(kernel):
+    """The loading warp waits for its last copies whether or not it was the one that gave up."""
+    block = _branch(_body(_source("matmul_q8.cu"), kernel), "if (warp == 0)")
+    drain = block[block.rindex("wait_previous()"):]
+    waits = [m.start() for m in re.finditer(r"mbar_wait_\w+\(&full\[", drain)]
+    assert waits
+    condition = re.findall(r"if \((?:[^()]|\([^()]*\))*\bone\b(?:[^()]|\([^()]*\))*\)", drain[:waits[0]])[-1]
+    assert "ok" not in condition, condition
+
+
+@pytest.mark.parametrize("kernel,last", [("matmul_q8_split_kernel", "mbar_wait_bounded(&done"),
+                                         ("matmul_q8_pair_kernel", "mbar_wait_cluster(&acc_full[")])
+def test_products_end_before_their_tensor_memory_goes(kernel, last):
+    """The warp that issues the products waits for the last of them, also when the warps that read them gave up."""
+    block = _branch(_body(_source("matmul_q8.cu"), kernel), "if (warp == 1 &&" if "pair" in kernel else "else if (warp == 1)")
+    assert last in block[block.rindex("mma_commit"):]
