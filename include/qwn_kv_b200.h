@@ -491,7 +491,8 @@ typedef struct {
     const void *x_dev;              /* [rows][width] */
     const void *residual_dev;       /* optional */
     const void *weight_dev;         /* optional [width] */
-    void *residual_out_dev;         /* optional; may be residual_dev or x_dev (with their stride) */
+    void *residual_out_dev;         /* optional; may be residual_dev or x_dev with their stride, and overlaps an
+                                       input in no other way (INVALID_ARGUMENT); the other outputs overlap none */
     int8_t *codes_dev;              /* [rows][width] */
     float *scales_dev;              /* [rows] */
     void *rows_out_dev;             /* optional */

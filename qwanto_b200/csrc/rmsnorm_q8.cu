@@ -424,6 +424,16 @@ QWN_CUDA_ABI_API int qwn_rmsnorm_q8(const QwnRmsNormQ8Request *r) {
         (uintptr_t)r->residual_out_dev % es || (uintptr_t)r->scales_dev % 4 ||
         (r->rows_out_dev && (uintptr_t)r->rows_out_dev % re))
         return invalid("qwn_rmsnorm_q8: a pointer is not aligned to its type");
+    if (r->residual_out_dev) {
+        const RowSpan out = {(uintptr_t)r->residual_out_dev, a.residual_out_stride * es, r->width * es, r->rows};
+        auto met = [&](const void *p, uint64_t stride, uint64_t rows) {  // in place is none: a row's CTA reads it first
+            const RowSpan in = {(uintptr_t)p, stride * es, out.bytes, rows};
+            return p && !(in.at == out.at && (in.stride == out.stride || r->rows == 1)) && rows_meet(in, out);
+        };
+        if (met(r->x_dev, a.x_stride, r->rows) || met(r->residual_dev, a.residual_stride, r->rows) ||
+            (r->weight_dev && rows_meet({(uintptr_t)r->weight_dev, out.bytes, out.bytes, 1}, out)))
+            return invalid("qwn_rmsnorm_q8: residual_out overlaps an input that it does not equal, row for row");
+    }
     auto on = [](const void *p, uint64_t s, uint64_t bytes) {  // rows of s bytes start on multiples of `bytes`
         return !p || ((uintptr_t)p % bytes == 0 && s % bytes == 0);
     };

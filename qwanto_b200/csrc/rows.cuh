@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 
 #include "kv_internal.cuh"
+#include "row_span.h"
 
 namespace qkv {
 namespace {

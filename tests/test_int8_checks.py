@@ -101,3 +101,51 @@ def test_calls_without_a_handle():
     assert L.qwn_matmul_q8_check(C.byref(h), C.byref(bits)) == INVALID
     assert L.qwn_kv_append_rotary(C.byref(h), C.byref(_lib.init(_lib.AppendRotaryRequest()))) == INVALID
     assert L.qwn_kv_load_tokens(C.byref(h), C.byref(_lib.init(_lib.LoadTokensRequest()))) == INVALID
+
+
+@pytest.mark.parametrize("over", [{"residual_out_dev": 4096, "residual_out_stride": 128},
+                                  {"residual_dev": 65536, "residual_out_dev": 65536, "residual_stride": 96},
+                                  {"residual_dev": 65536, "residual_out_dev": 65536 + 256},
+                                  {"residual_out_dev": 4096 + 4}, {"residual_out_dev": 4096 - 252},
+                                  {"x_stride": 100, "residual_out_dev": 4096 + 256, "residual_out_stride": 100},
+                                  {"weight_dev": 65536, "residual_out_dev": 65536 + 128}])
+def test_rmsnorm_refuses_a_residual_over_rows_still_read(over):
+    """In place is the same rows; any other overlap is a row that another row's output may have replaced."""
+    from qwanto_b200 import _lib
+    assert _lib.lib().qwn_rmsnorm_q8(C.byref(_norm(**over))) == INVALID
+    assert "overlaps" in _lib.last_error()
+
+
+def test_rows_meet_where_they_share_a_byte():
+    """The library's test of overlap against sets of bytes."""
+    import random
+    rng = random.Random(5)
+    cases = []
+    for i in range(4000):
+        spans = []
+        same = rng.randrange(1, 30)
+        for _ in range(2):
+            size = rng.randrange(1, 12)
+            stride = max(size, same) if i % 2 else size + rng.randrange(0, 20)
+            spans.append((rng.randrange(100, 220), stride, size, rng.randrange(1, 7)))
+        cases.append(spans)
+    lines = "\n".join(" ".join(str(v) for s in c for v in s) for c in cases)
+    code = """#include <cstdio>
+#include "row_span.h"
+int main() {
+    qkv::RowSpan s[2];
+    unsigned long v[8];
+    while (scanf("%lu %lu %lu %lu %lu %lu %lu %lu", v, v + 1, v + 2, v + 3, v + 4, v + 5, v + 6, v + 7) == 8) {
+        for (int i = 0; i < 2; i++) s[i] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        putchar('0' + qkv::rows_meet(s[0], s[1]));
+    }
+}
+"""
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "p.cpp"), os.path.join(d, "p")
+        open(src, "w").write(code)
+        subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "qwanto_b200", "csrc"), src, "-o", exe], check=True)
+        got = subprocess.run([exe], check=True, input=lines, capture_output=True, text=True).stdout
+    held = lambda s: {s[0] + r * s[1] + b for r in range(s[3]) for b in range(s[2])}  # noqa: E731
+    want = "".join(str(int(bool(held(a) & held(b)))) for a, b in cases)
+    assert got == want and "0" in got and "1" in got
