@@ -440,7 +440,9 @@ typedef struct {
     const void *query_dev;          /* [num_rows][query_heads][128] */
     const void *key_dev;            /* [num_rows][kv_heads][128] */
     const void *value_dev;
-    void *query_out_dev;            /* [num_rows][query_heads][128], contiguous; may be query_dev */
+    void *query_out_dev;            /* [num_rows][query_heads][128], contiguous; may be query_dev where that is
+                                       contiguous too (or one row) and the types have one size; overlaps query, key
+                                       and value in no other way (INVALID_ARGUMENT) */
     void *stream;
 } QwnKvAppendRotaryRequest;
 QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *pool, const QwnKvAppendRotaryRequest *request);

@@ -1011,6 +1011,17 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
         (r->query_heads && (!rows_aligned(r->query_dev, qs, r->dtype) ||
                             !rows_aligned(r->query_out_dev, q_width, r->query_out_dtype))))
         return invalid("qwn_kv_append_rotary: rows must start on four values (pointers and strides)");
+    if (r->query_heads) {
+        const uint64_t in = value_bytes(r->dtype), ob = value_bytes(r->query_out_dtype);
+        const RowSpan out = {(uintptr_t)r->query_out_dev, q_width * ob, q_width * ob, r->num_rows};
+        auto met = [&](const void *p, uint64_t stride, uint64_t width) {
+            return rows_meet({(uintptr_t)p, stride * in, width * in, r->num_rows}, out);
+        };
+        // in place a row's output lies on its own input, which the writing threads have read
+        const bool in_place = r->query_out_dev == r->query_dev && in == ob && (qs == q_width || r->num_rows == 1);
+        if ((!in_place && met(r->query_dev, qs, q_width)) || met(r->key_dev, ks, kv_width) || met(r->value_dev, vs, kv_width))
+            return invalid("qwn_kv_append_rotary: query_out overlaps rows that are still read");
+    }
     cudaSetDevice(p->device);
     RotaryArgs a{};
     a.rows = {r->seq_ids_dev, r->row_begin_dev, r->first_pos_dev, r->num_seqs, r->num_rows};
