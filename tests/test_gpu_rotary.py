@@ -492,3 +492,63 @@ def test_refusals(cuda):
         assert b.pool.check() == 0
     finally:
         b.close()
+
+
+@pytest.mark.parametrize("lead", [4, 8])
+@pytest.mark.parametrize("codec", CODECS)
+def test_rows_that_cannot_be_stored_leave_the_pages_alone(cuda, codec, lead):
+    """Of a call with bad rows, the pages hold the good rows and nothing else: every
+    byte of every page equals a pool's that only got the good ones."""
+    torch = cuda
+    counts, starts = [40, 33, 20], [0, 5, 12]
+    b = Batch(torch, codec, "f32", counts, starts, seed=codec, lead=lead)
+    try:
+        g = torch.Generator("cuda").manual_seed(40)
+        table = _table(torch, 64, 128)
+        out = torch.empty((b.rows, b.hq, 128), device="cuda")
+        held = sorted({int(p) for p in b.pool.page_table().ravel() if p >= 0})
+        total = b.pool.total_pages
+
+        def ints(*x):
+            return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+        far = torch.arange(b.rows, device="cuda", dtype=torch.int32) % 60
+        far[50], far[51] = 64, -1  # angles outside the table
+        # what is wrong, the status, the rows stored: (row, sequence, position)
+        normal = [(r, i, s + j) for i, (c, s, at) in enumerate(zip(counts, starts, (0, 40, 73)))
+                  for j, r in enumerate(range(at, at + c))]
+        cases = [
+            ({"seq_ids": ints(0, -1, 3)}, BAD_SEQUENCE, [x for x in normal if x[1] == 0]),
+            ({"seq_ids": ints(-2 ** 31, 1, 2 ** 31 - 1)}, BAD_SEQUENCE, [x for x in normal if x[1] == 1]),
+            ({"first_pos": ints(-3, 5, 12)}, BAD_LENGTH,
+             [(r, i, p - 3 if i == 0 else p) for r, i, p in normal if i or p >= 3]),
+            ({"first_pos": ints(0, 5, 20)}, BAD_LENGTH,
+             [(r, i, p + 8 if i == 2 else p) for r, i, p in normal if i < 2 or p + 8 < 32]),
+            ({"first_pos": ints(2 ** 31 - 5, 5, 12)}, BAD_LENGTH, [x for x in normal if x[1]]),
+            ({"first_pos": ints(-2 ** 31, 5, 12)}, BAD_LENGTH, [x for x in normal if x[1]]),
+            ({"row_begin": ints(7, 40, 73, 80), "first_pos": ints(7, 5, 12)}, BAD_LENGTH,
+             [x for x in normal if 7 <= x[0] < 80]),
+            ({"rotary_pos": far}, BAD_LENGTH, [x for x in normal if x[0] not in (50, 51)]),
+        ]
+        for over, bits, good in cases:
+            n = int(b.lens.max())
+            old = torch.randn((n, b.kv, 128), device="cuda", generator=g)
+            for p in (b.pool, b.twin):
+                for layer in range(2):
+                    for i, m in enumerate(b.lens.tolist()):
+                        p.store_tokens(i, layer, 0, m, old[:m], old[-m:].contiguous())
+            before = [b.pool.page(p).copy() for p in range(total)]
+            b.append(1, 128, False, table, out, "f32", **over)
+            assert b.pool.check() == bits, over
+            angle = far.long() if "rotary_pos" in over else None
+            rows = torch.tensor([r for r, _, _ in good], device="cuda")
+            where = angle[rows] if angle is not None else torch.tensor([p for _, _, p in good], device="cuda")
+            k32 = _rotated(torch, b.k[rows], table[where], 128, False)
+            for at, (r, i, p) in enumerate(good):
+                b.twin.store_tokens(i, 1, p, 1, k32[at:at + 1].contiguous(), b.v[r:r + 1].contiguous())
+            torch.cuda.synchronize()
+            for p in range(total):
+                want = b.twin.page(p) if p in held else before[p]
+                assert np.array_equal(b.pool.page(p), want), (over, p)
+    finally:
+        b.close()
