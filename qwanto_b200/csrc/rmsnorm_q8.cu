@@ -347,12 +347,13 @@ cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
     if (few && threads(1) <= 1024) return launch_row<T, 1, kCtas<T>>(a, rows, threads(1), s);
     if (threads(2) <= (few ? 1024u : a.residual ? 256u : 96u))
         return launch_row<T, 2, kCtas<T>>(a, rows, threads(2), s);
-    // past 448 threads 72 registers leave one CTA per SM, 64 two (4096 x 16384 bf16: 119 us, 91)
-    if (V == 4 && threads(4) <= 512 || threads(4) <= 448)
-        return launch_row<T, 4, 0>(a, rows, threads(4), s);
-    if (threads(4) <= 512) return launch_row<T, 4, 2>(a, rows, threads(4), s);
-    if (V == 4 && threads(8) > 448 && threads(8) <= 512 && !a.residual)  // 2048 x 16384 fp32: 56 us, 75
-        return launch_row<T, 8, 2>(a, rows, threads(8), s);
+    if (threads(4) <= (V == 4 ? 512u : 448u)) return launch_row<T, 4, 0>(a, rows, threads(4), s);
+    // 16-bit rows past 448 threads: 72 registers leave one CTA per SM, 64 two (4096 x 16384 bf16: 119 us, 91)
+    if constexpr (V == 8)
+        if (threads(4) <= 512) return launch_row<T, 4, 2>(a, rows, threads(4), s);
+    if constexpr (V == 4)  // 2048 x 16384 fp32: 56 us, 75
+        if (threads(8) > 448 && threads(8) <= 512 && !a.residual)
+            return launch_next(rmsnorm_q8_kernel<T, 8, 1, 2, false>, dim3(rows), threads(8), s, a);
     if (V == 8 || threads(8) <= 512) return launch_row<T, 8, 0>(a, rows, threads(8), s);
     return launch_row<T, 64 / V, 0>(a, rows, threads(64 / V), s);
 }
@@ -361,8 +362,10 @@ cudaError_t launch_chunks(const NormArgs &a, uint32_t rows, cudaStream_t s) {
 template <typename T, int CH>
 cudaError_t launch_values_ch(const NormArgs &a, uint32_t rows, uint32_t threads, cudaStream_t s) {
     constexpr int ctas = CH <= 2 ? kCtas<T> : 0;
-    if (threads == 128) return launch_next(rmsnorm_q8_kernel<T, CH, 128, ctas>, dim3(rows), dim3(128), s, a);
-    if (threads == 256) return launch_next(rmsnorm_q8_kernel<T, CH, 256, ctas>, dim3(rows), dim3(256), s, a);
+    if constexpr (CH <= 2)  // launch_values gives 128 threads up to two chunks each, 256 two at least
+        if (threads == 128) return launch_next(rmsnorm_q8_kernel<T, CH, 128, ctas>, dim3(rows), dim3(128), s, a);
+    if constexpr (CH >= 2)
+        if (threads == 256) return launch_next(rmsnorm_q8_kernel<T, CH, 256, ctas>, dim3(rows), dim3(256), s, a);
     return launch_next(rmsnorm_q8_kernel<T, CH, 512, ctas>, dim3(rows), dim3(512), s, a);
 }
 template <typename T>
