@@ -222,15 +222,16 @@ struct Turn16 {
     const float *row;
     __device__ __forceinline__ void load(const float *r, int j, int rot) {
         row = r;
-        if (MODE == kTurnPart) return;
+        if constexpr (MODE != kTurnPart) {
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-            if (MODE == kTurnNeighbours && 64 * q + 8 * j >= rot) continue;
-            const float *at = MODE == kTurnWhole ? r + 8 * j + 4 * q : r + 32 * q + 4 * j;
-            const float4 x = *reinterpret_cast<const float4 *>(at);
-            const float4 y = *reinterpret_cast<const float4 *>(at + (rot >> 1));
-            c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
-            s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
+            for (int q = 0; q < 2; q++) {
+                if (MODE == kTurnNeighbours && 64 * q + 8 * j >= rot) continue;
+                const float *at = MODE == kTurnWhole ? r + 8 * j + 4 * q : r + 32 * q + 4 * j;
+                const float4 x = *reinterpret_cast<const float4 *>(at);
+                const float4 y = *reinterpret_cast<const float4 *>(at + (rot >> 1));
+                c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
+                s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
+            }
         }
     }
     template <typename T>
