@@ -22,10 +22,12 @@
 //    halves meets in one lane and a maximum over a head takes 3 shuffles for 4
 //    rows (with 4 dims per lane, 4 + 5 per row); the tile is put together in
 //    shared memory and leaves in 16-byte stores.
-// 16384 rows of 32 + 2 x 8 bf16 heads with their rotation into 4-bit pages: 71 us
-// (4.9 TB/s; all rows by the first way 290), into int8 78; 131072 cached int8
-// rows of 8 heads back to bf16: 131 us (6.2 TB/s).  One row of 12 + 2 x 2 heads:
-// 3.1 us, back 2.2.  Six CTAs per SM (80 registers): 72 us, four 78.
+// 16384 rows of 32 + 2 x 8 bf16 heads with their rotation into 4-bit pages: 69 us
+// (5.1 TB/s; all rows by the first way 289), into int8 75; fp32 rows 128 and 133
+// (5.4 and 5.3 TB/s); 131072 cached int8 rows of 8 heads back to bf16: 132 us (6.1
+// TB/s).  One row of 12 + 2 x 2 heads: 2.9 us, back 1.9.  Six CTAs per SM: 72 us,
+// four 78, measured for bf16 into 4-bit pages; under that bound (80 registers)
+// every type spills, 16-bit rows 64 to 80 bytes per thread, fp32 rows up to 192.
 #include <algorithm>
 #include <type_traits>
 
@@ -1040,7 +1042,7 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
     const StoreGeo g = store_geo(p);
     cudaStream_t s = stream_of(p, r->stream);
     // runs of rows go by tiles; one row per sequence, or rows off the 16-byte grid, one by one
-    // (16384 rows of 32 + 2 x 8 bf16 heads into 4-bit pages: 71 us by tiles, 290 one by one)
+    // (16384 rows of 32 + 2 x 8 bf16 heads into 4-bit pages: 69 us by tiles, 289 one by one)
     const bool tiles = r->row_begin_dev && rows_wide(r->key_dev, ks, r->dtype) && rows_wide(r->value_dev, vs, r->dtype) &&
                        (!r->query_heads || (rows_wide(r->query_dev, qs, r->dtype) &&
                                             rows_wide(r->query_out_dev, q_width, r->query_out_dtype)));

@@ -552,14 +552,16 @@ struct MmPlan {
 //  - the split kernel spends 0.12 us on 128 codes of a CTA's share of k (four
 //    narrow MMAs), 0.18 when the CTAs fill the GPU, starts and ends in 2.2 us,
 //    writes a token in 20 ns, and joins a cluster's sums in 0.1 us and 25 ns per
-//    token.  Shares only as long as all clusters run at once (74 of two CTAs,
-//    45 of three, 33 of four, 15 of eight): beyond, a share costs a whole CTA's
-//    time (48 clusters of three took 1.5 times what 48 of two took);
+//    token.  Shares only as long as all clusters run at once with the largest
+//    shared memory that a CTA may ask for (74 of two CTAs, 45 of three, 33 of
+//    four, 15 of eight): beyond, a share costs a whole CTA's time (48 clusters of
+//    three took 1.5 times what 48 of two took).  With shorter rings more would
+//    run (93 of three at 100 KB), which the plan does not weigh;
 //  - a pair spends 0.13 us + 1.05 ns per token of its tile on 128 codes, at
 //    least 10.5 ns per token on a tile (its output), and starts and ends in
 //    2.6 us.
 // A few tokens thus go to the split kernel with as many shares as run at once
-// (1 x 1536 x 2048: 2.6 us in 4 shares, 4.3 in one; 32 x 4096 x 6144: 6.6 us
+// (1 x 1536 x 2048: 2.8 us in 4 shares, 4.3 in one; 32 x 4096 x 6144: 6.3 us
 // in 2 shares, 7.3 in one), more to pairs with the widest tile that still
 // reaches all of them (257 x 4099 x 4095: 10.7 us with 96 tokens a tile, 14.1
 // with 256; 8192 x 6144 x 8192 before its walk in groups: 253 us with 256, 278

@@ -25,10 +25,11 @@
 // conditions per value had cost as much (1000 x 6144 bf16: 9.5 us, 10.3).  Rows
 // without a residual have kernels of their own; they are bound by instruction issue
 // and by fewer bytes in flight between a row's reductions (8192 x 4096 bf16: 30
-// us, 5.6 TB/s; 46 and 6.5 with a residual).  Rows over 16384 wide leave one CTA's
-// registers per SM (2048 x 32768 bf16: 113 us, 5.3 TB/s).
+// us, 5.5 TB/s; 46 and 6.5 with a residual; 4.5 to 4.6 TB/s at 2560, 8960 and 12288
+// wide).  Rows over 16384 wide leave one CTA's registers per SM (bf16: 2048 x 32768
+// with a residual 114 us, 5.3 TB/s; 2048 x 28672 without 83 us, 3.5 TB/s).
 // Rows that are not whole 16-byte chunks, or start off them, are read value by
-// value (8192 x 4095 bf16: 77 us, 4096 wide 46; fp32 87).
+// value (8192 x 4095 bf16: 75 us, 4096 wide 46; fp32 85).
 #include <type_traits>
 
 #include "kv_internal.cuh"
@@ -168,7 +169,7 @@ template <typename T, int CH, int STEP, int CTAS = 0, bool RES = true>
 __global__ void __launch_bounds__(CH <= 2 ? 1024 : 512, CTAS) rmsnorm_q8_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     // the weight's chunks are held from the start, or come from L1 or L2 between the reductions where
-    // their registers would cost a CTA per SM (4096 x 14336 bf16 without residual: 61 us, 96; 2048 x
+    // their registers would cost a CTA per SM (4096 x 14336 bf16 without residual: 59 us, 96; 2048 x
     // 10240 fp32: 50, 76); 16-bit rows over 16384 wide have one CTA either way (2048 x 32768: 113, 116)
     constexpr bool kLateWeight = CH * V >= 32 && !(V == 8 && CH == 8);
     __shared__ float sm[2][32];
