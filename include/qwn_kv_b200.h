@@ -48,7 +48,8 @@ enum {
     QWN_CUDA_CAP_PAGE_EVICTION = 1ull << 10,  /* page scores, eviction, compaction */
     QWN_CUDA_CAP_LINEAR_ATTENTION = 1ull << 11, /* qwn_linear_attention_* */
     QWN_CUDA_CAP_ROTARY_KV = 1ull << 12,      /* qwn_kv_append_rotary, qwn_kv_load_tokens */
-    QWN_CUDA_CAP_INT8_LINEAR = 1ull << 13     /* qwn_rmsnorm_q8, qwn_matmul_q8_* */
+    QWN_CUDA_CAP_INT8_LINEAR = 1ull << 13,    /* qwn_rmsnorm_q8, qwn_matmul_q8_* */
+    QWN_CUDA_CAP_PROMPT_ATTENTION = 1ull << 14 /* qwn_kv_chunk_attention, qwn_prompt_attention */
 };
 
 /* types of rows in device memory */
@@ -465,6 +466,70 @@ typedef struct {
     void *stream;
 } QwnKvLoadTokensRequest;
 QWN_CUDA_ABI_API int qwn_kv_load_tokens(QwnKvPoolHandle *pool, const QwnKvLoadTokensRequest *request);
+
+/* ---- attention of prompts ---------------------------------------------------
+ * The reference attends token by token (c/qwn_paged_kv.c:225-382).  These calls
+ * take many query rows at once.  Row by row, with query head h reading kv head
+ * h / (query_heads / kv_heads) and p the row's position:
+ *     out = sum_t softmax_t(scale q.k_t) v_t   over the tokens t <= p,
+ * and t > p - window where a window is given.  A row that sees no token is zero.
+ * Tokens that a row does not see do not matter to it, whatever they hold.
+ * 16-bit rows: products of 16-bit operands with fp32 sums, probabilities rounded
+ * once to 16 bits; fp32 rows: operands in three bf16 parts, fp32 accuracy.
+ * Rows start on 16 bytes (pointers and strides; INVALID_ARGUMENT otherwise).
+ * Rows before the first sequence's and after the last one's stay as they are. */
+
+/* Queries of new tokens over the cached tokens of their sequences, themselves
+ * included: the rows' tokens must have been stored (qwn_kv_append_rotary,
+ * qwn_kv_store_tokens).  A row outside its sequence latches BAD_LENGTH, an
+ * unknown sequence BAD_SEQUENCE, and is zero; a bad page latches BAD_PAGE. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t layer, num_seqs;
+    const int32_t *seq_ids_dev;     /* [num_seqs] or NULL = 0..num_seqs-1 */
+    const int32_t *row_begin_dev;   /* as in QwnKvAppendRotaryRequest */
+    const int32_t *first_pos_dev;
+    uint32_t num_rows;
+    uint32_t dtype;                 /* QwnDType of query and output */
+    uint32_t query_heads;           /* multiple of kv_heads, within the pool's max_query_heads */
+    float scale;                    /* softmax scale; 0 = 1/sqrt(128) */
+    uint32_t window;                /* tokens that a row sees, itself included; 0: all before it */
+    uint32_t reserved;
+    uint64_t query_stride, output_stride; /* values between rows; 0: query_heads x 128 */
+    const void *query_dev;          /* [num_rows][query_heads][128] */
+    void *output_dev;               /* as query_dev, which it may not overlap */
+    void *workspace_dev;            /* optional, qwn_kv_chunk_workspace bytes, 16-byte aligned: lets a few rows over many
+                                       tokens use the whole GPU.  One call at a time uses it; nothing in it is kept */
+    uint64_t workspace_bytes;
+    void *stream;
+} QwnKvChunkAttentionRequest;
+QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *pool, const QwnKvChunkAttentionRequest *request);
+/* workspace of a call with these sizes, whatever its types and lengths; may be 0 */
+QWN_CUDA_ABI_API int qwn_kv_chunk_workspace(const QwnKvPoolHandle *pool, uint32_t num_seqs, uint32_t num_rows,
+                                            uint32_t query_heads, uint64_t *bytes);
+
+/* Prompts over their own rows, before or beside a cache: sequence i has the rows
+ * [begin[i], begin[i+1]), whose positions start at 0. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    int32_t device_id;
+    uint32_t num_seqs, num_rows;
+    uint32_t dtype;                 /* QwnDType of query, key, value and output */
+    uint32_t query_heads, kv_heads; /* query heads: a multiple of the kv heads */
+    float scale;                    /* 0 = 1/sqrt(128) */
+    uint32_t causal;                /* 0: every row sees its whole sequence */
+    uint32_t window;                /* causal only; 0: none */
+    uint32_t reserved;
+    const int32_t *row_begin_dev;   /* [num_seqs+1] ascending; NULL: one sequence of all rows */
+    uint64_t query_stride, key_stride, value_stride, output_stride; /* values between rows; 0: heads x 128 */
+    const void *query_dev;          /* [num_rows][query_heads][128] */
+    const void *key_dev;            /* [num_rows][kv_heads][128] */
+    const void *value_dev;
+    void *output_dev;               /* [num_rows][query_heads][128]; overlaps no input */
+    uint32_t *status_dev;           /* optional QWN_KV_STATUS_* bits: WAIT_TIMEOUT */
+    void *stream;
+} QwnPromptAttentionRequest;
+QWN_CUDA_ABI_API int qwn_prompt_attention(const QwnPromptAttentionRequest *request);
 
 /* ---- int8 activations and products -----------------------------------------
  * qwn_rmsnorm_q8 turns a layer's input rows into the int8 rows that

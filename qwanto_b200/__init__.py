@@ -27,7 +27,7 @@ from ._lib import (CODEC_F16, CODEC_Q4_G32, CODEC_Q8_B64_F32, CODEC_Q8_HEAD_F16,
 
 __all__ = ["CudaContext", "KvPool", "lib", "QwnCudaError", "generate_rows", "merge_partials",
            "CODEC_Q8_B64_F32", "CODEC_Q8_HEAD_F16", "CODEC_TQ35_G64", "CODEC_Q4_G32", "CODEC_F16", "launch_count", "merge_partials_packed",
-           "MatmulQ8", "rmsnorm_q8", "DTYPE_F32", "DTYPE_F16", "DTYPE_BF16"]
+           "MatmulQ8", "rmsnorm_q8", "prompt_attention", "DTYPE_F32", "DTYPE_F16", "DTYPE_BF16"]
 
 TILE_BYTES = {CODEC_Q8_B64_F32: 4352, CODEC_Q8_HEAD_F16: 4160, CODEC_TQ35_G64: 2048, CODEC_Q4_G32: 2560,
               CODEC_F16: 8192}
@@ -61,6 +61,8 @@ def _addr(x) -> int:
 
 _pack_append_rotary = _lib.packer(_lib.AppendRotaryRequest)
 _pack_load_tokens = _lib.packer(_lib.LoadTokensRequest)
+_pack_chunk_attention = _lib.packer(_lib.ChunkAttentionRequest)
+_pack_prompt_attention = _lib.packer(_lib.PromptAttentionRequest)
 _pack_rmsnorm_q8 = _lib.packer(_lib.RmsNormQ8Request)
 _pack_matmul_q8 = _lib.packer(_lib.MatmulQ8Request)
 
@@ -233,6 +235,27 @@ class KvPool:
             value_stride, _addr(key_out), _addr(value_out), _stream(stream) or 0))
         check("qwn_kv_load_tokens", rc)
 
+    def chunk_attention(self, layer: int, num_seqs: int, num_rows: int, dtype: int, query_heads: int, query, output,
+                        row_begin=None, first_pos=None, seq_ids=None, scale: float = 0.0, window: int = 0,
+                        query_stride: int = 0, output_stride: int = 0, workspace=None, workspace_bytes: int = 0,
+                        stream=None) -> None:
+        """Attention of new tokens' queries over their sequences' cached tokens,
+        themselves included (qwn_kv_chunk_attention): one row per sequence, or
+        with row_begin [num_seqs + 1] ragged runs of rows.  A workspace of
+        chunk_workspace() bytes lets a few rows use the whole GPU."""
+        rc = lib().qwn_kv_chunk_attention(self._href, _pack_chunk_attention(
+            layer, num_seqs, _addr(seq_ids), _addr(row_begin), _addr(first_pos), num_rows, dtype, query_heads, scale,
+            window, 0, query_stride, output_stride, _addr(query), _addr(output), _addr(workspace), workspace_bytes,
+            _stream(stream) or 0))
+        check("qwn_kv_chunk_attention", rc)
+
+    def chunk_workspace(self, num_seqs: int, num_rows: int, query_heads: int) -> int:
+        """Bytes of workspace for chunk_attention calls of these sizes."""
+        n = C.c_uint64(0)
+        check("qwn_kv_chunk_workspace", lib().qwn_kv_chunk_workspace(self._href, num_seqs, num_rows, query_heads,
+                                                                      C.byref(n)))
+        return int(n.value)
+
     def prefill_synthetic(self, seq_ids, lens, seed: int, outlier_mask: np.ndarray | None = None,
                           stream=None) -> None:
         ids = np.ascontiguousarray(seq_ids, dtype=np.int32)
@@ -256,6 +279,20 @@ class KvPool:
         r.host_output = _ptr(host_output)
         tel = telemetry if telemetry is not None else init(_lib.Telemetry())
         check("qwn_kv_decode_step_host", lib().qwn_kv_decode_step_host(C.byref(self.h), C.byref(r), C.byref(tel)))
+
+
+def prompt_attention(query, key, value, output, num_rows: int, dtype: int, query_heads: int, kv_heads: int,
+                     num_seqs: int = 1, row_begin=None, scale: float = 0.0, causal: bool = True, window: int = 0,
+                     query_stride: int = 0, key_stride: int = 0, value_stride: int = 0, output_stride: int = 0,
+                     status=None, device: int = 0, stream=None) -> None:
+    """Attention of packed prompts over their own rows (qwn_prompt_attention):
+    sequence i has the rows row_begin[i] .. row_begin[i + 1]; without row_begin
+    all rows are one sequence.  Strides are in values between rows (0: contiguous)."""
+    rc = lib().qwn_prompt_attention(_pack_prompt_attention(
+        device, num_seqs, num_rows, dtype, query_heads, kv_heads, scale, causal, window, 0, _addr(row_begin),
+        query_stride, key_stride, value_stride, output_stride, _addr(query), _addr(key), _addr(value), _addr(output),
+        _addr(status), _stream(stream) or 0))
+    check("qwn_prompt_attention", rc)
 
 
 def rmsnorm_q8(x, rows: int, width: int, dtype: int, codes, scales, weight=None, eps: float = 1e-6, residual=None,

@@ -34,6 +34,7 @@ CAP_PAGE_EVICTION = 1 << 10
 CAP_LINEAR_ATTENTION = 1 << 11
 CAP_ROTARY_KV = 1 << 12
 CAP_INT8_LINEAR = 1 << 13
+CAP_PROMPT_ATTENTION = 1 << 14
 
 DTYPE_F32 = 1
 DTYPE_F16 = 2
@@ -216,6 +217,25 @@ class LoadTokensRequest(C.Structure):
                 ("key_out_dev", C.c_void_p), ("value_out_dev", C.c_void_p), ("stream", C.c_void_p)]
 
 
+class ChunkAttentionRequest(C.Structure):
+    _fields_ = [("header", Header), ("layer", C.c_uint32), ("num_seqs", C.c_uint32), ("seq_ids_dev", C.c_void_p),
+                ("row_begin_dev", C.c_void_p), ("first_pos_dev", C.c_void_p), ("num_rows", C.c_uint32),
+                ("dtype", C.c_uint32), ("query_heads", C.c_uint32), ("scale", C.c_float), ("window", C.c_uint32),
+                ("reserved", C.c_uint32), ("query_stride", C.c_uint64), ("output_stride", C.c_uint64),
+                ("query_dev", C.c_void_p), ("output_dev", C.c_void_p), ("workspace_dev", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("stream", C.c_void_p)]
+
+
+class PromptAttentionRequest(C.Structure):
+    _fields_ = [("header", Header), ("device_id", C.c_int32), ("num_seqs", C.c_uint32), ("num_rows", C.c_uint32),
+                ("dtype", C.c_uint32), ("query_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("scale", C.c_float),
+                ("causal", C.c_uint32), ("window", C.c_uint32), ("reserved", C.c_uint32), ("row_begin_dev", C.c_void_p),
+                ("query_stride", C.c_uint64), ("key_stride", C.c_uint64), ("value_stride", C.c_uint64),
+                ("output_stride", C.c_uint64), ("query_dev", C.c_void_p), ("key_dev", C.c_void_p),
+                ("value_dev", C.c_void_p), ("output_dev", C.c_void_p), ("status_dev", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
 class RmsNormQ8Request(C.Structure):
     _fields_ = [("header", Header), ("device_id", C.c_int32), ("rows", C.c_uint32), ("width", C.c_uint32),
                 ("dtype", C.c_uint32), ("mode", C.c_uint32), ("eps", C.c_float), ("rows_dtype", C.c_uint32),
@@ -294,6 +314,9 @@ _SIGS = {
     # requests as bytes: see packer()
     "qwn_kv_append_rotary": (C.c_int, [_P(Handle), C.c_void_p]),
     "qwn_kv_load_tokens": (C.c_int, [_P(Handle), C.c_void_p]),
+    "qwn_kv_chunk_attention": (C.c_int, [_P(Handle), C.c_void_p]),
+    "qwn_kv_chunk_workspace": (C.c_int, [_P(Handle), C.c_uint32, C.c_uint32, C.c_uint32, _P(C.c_uint64)]),
+    "qwn_prompt_attention": (C.c_int, [C.c_void_p]),
     "qwn_rmsnorm_q8": (C.c_int, [C.c_void_p]),
     "qwn_matmul_q8_create": (C.c_int, [_P(MatmulQ8Options), _P(Handle)]),
     "qwn_matmul_q8_destroy": (C.c_int, [_P(Handle)]),

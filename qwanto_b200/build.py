@@ -19,8 +19,8 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "qwn_cuda.so")
 
 SOURCES = ["kv_pool.cu", "kv_attention.cu", "kv_evict.cu", "abi_v1.cu", "linear_attention.cu", "ref_api.cu",
-           "kv_rotary.cu", "rmsnorm_q8.cu", "matmul_q8.cu"]
-HEADERS = [os.path.join(CSRC, "kv_internal.cuh"), os.path.join(CSRC, "kv_store.cuh"), os.path.join(CSRC, "rows.cuh"), os.path.join(CSRC, "row_span.h"),
+           "kv_rotary.cu", "rmsnorm_q8.cu", "matmul_q8.cu", "chunk_attention.cu", "prompt_attention.cu"]
+HEADERS = [os.path.join(CSRC, "kv_internal.cuh"), os.path.join(CSRC, "kv_store.cuh"), os.path.join(CSRC, "rows.cuh"), os.path.join(CSRC, "row_span.h"), os.path.join(CSRC, "tile_rows.cuh"), os.path.join(CSRC, "prompt_tile.cuh"),
            os.path.join(CSRC, "tcgen05.cuh")] + [
     os.path.join(INCLUDE, h) for h in ("qwn_cuda_abi.h", "qwn_kv_b200.h", "qwn_paged_kv.h", "qwanto_turboquant.h",
                                        "qwanto_attention.h", "qwanto_pagedeviction.h")]

@@ -74,7 +74,7 @@ __host__ __device__ constexpr size_t tile_bytes_of(uint32_t codec) {
 // the pool (device state behind QwnKvPoolHandle)
 // ----------------------------------------------------------------------------
 struct Pool {
-    int device = 0;
+    int device = 0, sms = 148;
     uint32_t codec = 0, layers = 0, kv_heads = 0, page_tokens = 0, tiles_per_page = 0;
     uint32_t total_pages = 0, max_seqs = 0, max_pages_per_seq = 0, max_query_heads = 0;
     uint64_t perm_seed = 0;

@@ -403,6 +403,7 @@ QWN_CUDA_ABI_API int qwn_kv_pool_create(const QwnKvPoolOptions *o, QwnKvPoolHand
     // (one or two head groups of four query heads)
     int sms = 0;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device);
+    if (sms > 0) p->sms = sms;
     uint32_t ctas[2] = {0, 0};
     for (int hg = 1; hg <= 2; hg++) {
         int per_sm = 0;

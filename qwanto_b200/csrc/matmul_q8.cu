@@ -477,22 +477,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_q8_pair_kernel(const __g
 
 // ---- host ---------------------------------------------------------------------
 
-// the driver's encoder, found once (the library does not link libcuda)
-using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encoder() {
-    static const EncodeFn fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
-                cudaSuccess || found != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
 // codes [rows][width], `stride` bytes apart, in tiles of box x 128
 bool encode_codes(CUtensorMap *map, const int8_t *p, uint64_t width, uint64_t rows, uint64_t stride, uint32_t box) {
     const EncodeFn fn = encoder();

@@ -1,0 +1,1304 @@
+// Causal attention of many query rows on the tensor core: the kernel behind
+// qwn_kv_chunk_attention (keys and values in the paged cache) and
+// qwn_prompt_attention (keys and values as rows).
+//
+// Per query row q at position p, over the tokens t that it sees (t <= p, and
+// t > p - window where there is one):
+//     s_t = scale q.k_t,   out = sum_t 2^(c s_t - M) v_t / sum_t 2^(c s_t - M)
+// with c = log2 e and M near the largest c s_t so far.  M moves, and with it the
+// sums, only when a row's largest score has outgrown it by kSlack (as factors of
+// two): then the sums of the 128 rows are read from tensor memory, scaled and put
+// back; otherwise they stay where the MMAs add to them.
+//
+// The rows of one kv head's query heads are one matrix: row r of a sequence is
+// token r / group, head r % group, so that a tile of 128 rows reads each key and
+// value once for all heads that share it.  Both products run on tcgen05 (M = 128
+// rows): S = Q K^T from shared memory, then O += P V with P as the A operand out
+// of tensor memory, where it lies over the S that it came from.
+//
+// A CTA has 16 warps:
+//   0-3, 4-7   softmax, one thread per row: S out of tensor memory, P back into it
+//   8-11       Q into shared memory; cached tiles into operand tiles; whatever a
+//              sequence's ends ask for
+//   12         MMAs      13  loads      14  the list of work
+// The two softmax groups take turns with the tensor core.  TILES = 2: each has 128
+// of the CTA's 256 rows and both read the same keys.  TILES = 1: both work on the
+// same 128 rows, one on the even blocks of tokens and one on the odd ones, and
+// join at the end; for few rows, where the keys are what costs.
+//
+// PARTS = 1: 16-bit operands.  PARTS = 3: fp32 values as three bf16 parts (8 bits
+// each, exact) whose products down to 2^-16 of the largest are all taken: six
+// MMAs instead of one, fp32 accuracy.
+#pragma once
+
+#include <mutex>
+
+#include "kv_internal.cuh"
+#include "kv_store.cuh"
+#include "rows.cuh"
+#include "tcgen05.cuh"
+#include "tile_rows.cuh"
+
+namespace qkv {
+namespace {
+
+constexpr int kAtThreads = 512;
+constexpr int kAtRows = 128;  // rows of a tile: the lanes of tensor memory
+// registers per thread after the split: 2 x softmax + helpers + the rest = 4 x 128 at launch
+constexpr int kSoftmaxRegs = 184, kHelperRegs = 96, kOtherRegs = 48;
+static_assert(2 * kSoftmaxRegs + kHelperRegs + kOtherRegs <= 4 * 128, "no more registers than the block starts with");
+
+// one CTA's piece of work: rows of one sequence and kv head, and the blocks of tokens that it takes
+struct AtSegment {
+    int32_t valid;             // 0: no more work
+    int32_t rows;              // of the CTA's tiles
+    uint32_t row0;             // the first, among the sequence's rows (token x group + head)
+    uint32_t token_row;        // the sequence's first token among the call's rows
+    int32_t seq, head;         // sequence slot (-1: unknown), kv head
+    int32_t len;               // tokens that exist
+    int64_t pos0;              // position of the sequence's first row
+    int32_t block0, blocks;    // blocks of tokens
+    int32_t whole_lo, whole_hi;// blocks in [whole_lo, whole_hi) are seen whole by every row
+    int32_t slot;              // of the workspace, -1: the rows are finished here
+};
+
+struct AtArgs {
+    RowMap rows;
+    uint32_t group, kv_heads, query_heads, window, causal, layer;
+    uint32_t dtype;            // of query and output
+    float scale2;              // scale x log2 e
+    uint64_t query_stride, key_stride, value_stride, out_stride;  // values
+    const void *query, *key, *value;
+    void *out;
+    StoreGeo geo;              // paged
+    uint32_t *status;
+    uint32_t units;            // one segment per CTA: (row tiles, kv heads)
+    uint64_t *prefix;          // split: blocks before each sequence, then
+    float *slots;              // the partial results
+};
+// a partial result: o[rows][128], then M[rows], l[rows]
+__host__ __device__ constexpr uint32_t at_slot_floats(uint32_t tiles) { return tiles * kAtRows * (kHeadDim + 2); }
+
+template <int SRC, int PARTS, int TILES>
+struct AtShape {
+    static constexpr bool kPaged = SRC != 0;
+    static constexpr bool kTma = !kPaged && PARTS == 1;            // operand tiles straight from the rows
+    static constexpr bool kRaw = kPaged && SRC != QWN_KV_CODEC_F16;// cached tiles by way of shared memory
+    static constexpr int kBlock = PARTS == 1 ? 128 : 64;           // tokens
+    static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
+    static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
+    static constexpr uint32_t kKvBytes = kKvPart * PARTS;
+    static constexpr int kStagesK = PARTS == 1 ? 2 : 1;
+    static constexpr int kStagesV = PARTS == 1 && !(kPaged && TILES == 2) ? 2 : 1;
+    static constexpr uint32_t kOperands = TILES * kQBytes + (kStagesK + kStagesV) * kKvBytes;
+    static constexpr uint32_t kSmem = 227 * 1024 - 12 * 1024;      // the rest is static
+    static constexpr uint32_t kTileBytes = (uint32_t)tile_bytes_of(SRC);
+    static constexpr uint32_t kRawAll = kRaw ? (kSmem - 1024 - kOperands) / (kRaw ? kTileBytes : 1) : 0;
+    static constexpr uint32_t kRawTiles = kRawAll > 32 ? 32 : kRawAll;
+    static_assert(kOperands + 1024 <= kSmem, "operands fit");
+    // K of a block is converted before its V, so all its tiles are there at once
+    static_assert(!kRaw || kRawTiles >= (uint32_t)kTiles, "a block's cached tiles fit");
+    // tensor memory: S and P share columns; P has 16-bit pairs, PARTS of them
+    static constexpr uint32_t kSColumns = PARTS == 1 ? 128 : 96, kOColumn = 2 * kSColumns;
+    static_assert(kOColumn + 2 * 128 <= 512, "tensor memory");
+};
+
+struct AtShared {
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2];
+    uint64_t vpart[2], vfixed[2];  // TMA: values of a block seen in part have landed, are ready
+    uint64_t qfull, qempty, sfull[2], pready[2], ofull[2], oempty[2], joined, helped, drained;
+    uint64_t segfull[2], segempty[2], rawfull[32], rawempty[32];
+    AtSegment seg[2];
+    alignas(16) float kscale[4][128];      // of a block's tokens; read four at a time
+    alignas(16) float vscale[4][128];
+    alignas(16) float vtop[4][8];                      // log2 of a bound on a cached tile's value scales
+    float ml[2][2][kAtRows][2];            // TILES 1: M and l of both groups' rows, by segment parity
+    float qscale[2][2 * kAtRows];          // what a row of Q was divided by, by segment parity
+    uint32_t odd_v[4][2][16];              // tokens with values that are not finite, in blocks seen in part
+    uint32_t tmem;
+    int give_up;
+};
+
+// bounded waits that also end when another role of the CTA has given up
+__device__ __forceinline__ bool at_wait(AtShared &sh, uint64_t *bar, uint32_t parity) {
+    for (uint32_t it = 0; it < kWaitLimit; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63) == 63 && *(volatile int *)&sh.give_up) return false;
+    }
+    *(volatile int *)&sh.give_up = 1;
+    return false;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// all lanes' work is done: one arrival for the warp
+__device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
+// ---- tensor memory and MMAs of 16-bit operands ------------------------------
+__host__ __device__ constexpr uint32_t f16_desc(bool bf16, uint32_t n, bool b_by_rows) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_by_rows ? 1u : 0u) << 16) | ((n >> 3) << 17) |
+           ((128u >> 4) << 24);
+}
+// D += A B^T, both from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+        : "memory");
+}
+// the same with A in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+        : "memory");
+}
+// B by rows of K (values: a token's dims side by side), 64-wide columns of 128-byte
+// rows: the columns' distance, and 8 rows to the next 8
+__device__ __forceinline__ uint64_t rows_desc(uint32_t addr, uint32_t column_bytes) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(column_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+#define QKV_R8(r, b) "=r"(r[b]), "=r"(r[b + 1]), "=r"(r[b + 2]), "=r"(r[b + 3]), "=r"(r[b + 4]), "=r"(r[b + 5]), "=r"(r[b + 6]), "=r"(r[b + 7])
+#define QKV_R64(r, b) QKV_R8(r, b), QKV_R8(r, b + 8), QKV_R8(r, b + 16), QKV_R8(r, b + 24), QKV_R8(r, b + 32), QKV_R8(r, b + 40), QKV_R8(r, b + 48), QKV_R8(r, b + 56)
+// 64 columns of the warp's 32 lanes, complete on return
+__device__ __forceinline__ void tmem_load64(uint32_t *r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : QKV_R64(r, 0)
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ---- the work ----------------------------------------------------------------
+
+// sequence i of the batch
+struct AtSequence {
+    int64_t begin, rows;   // its tokens' rows
+    int32_t seq, len;
+    int64_t pos0;
+};
+__device__ __forceinline__ AtSequence at_sequence(const AtArgs &a, bool paged, uint32_t i) {
+    AtSequence s;
+    int64_t b = i, e = (int64_t)i + 1;
+    if (a.rows.row_begin) {
+        b = a.rows.row_begin[i];
+        e = a.rows.row_begin[i + 1];
+    } else if (!paged) {
+        b = 0;
+        e = a.rows.num_rows;
+    }
+    s.begin = max(b, (int64_t)0);
+    s.rows = max(min(e, (int64_t)a.rows.num_rows) - s.begin, (int64_t)0);
+    if (paged) {
+        const int32_t id = a.rows.seq_ids ? a.rows.seq_ids[i] : (int32_t)i;
+        const bool known = id >= 0 && (uint32_t)id < a.geo.max_seqs;
+        s.seq = known ? id : -1;
+        s.len = known ? min((int64_t)max(a.geo.seq_lens[id], 0), (int64_t)a.geo.mp * a.geo.page_tokens) : 0;
+        s.pos0 = (a.rows.first_pos ? (int64_t)a.rows.first_pos[i] : known ? (int64_t)a.geo.seq_lens[id] - (e - b) : 0) +
+                 (s.begin - b);
+    } else {
+        s.seq = (int32_t)i;
+        s.len = (int32_t)s.rows;
+        s.pos0 = 0;
+    }
+    return s;
+}
+// the tokens [lo, hi) that a row at a position sees; none where the position does not exist
+struct Seen {
+    int32_t lo, hi;
+};
+__device__ __forceinline__ Seen at_seen(const AtArgs &a, int64_t pos, int32_t len) {
+    Seen s = {0, 0};
+    if (pos < 0 || pos >= len) return s;
+    s.hi = a.causal ? (int32_t)pos + 1 : len;
+    if (a.window && pos + 1 > (int64_t)a.window) s.lo = (int32_t)(pos + 1 - a.window);
+    return s;
+}
+// the blocks that rows at positions p0 .. p1 see some of
+__device__ __forceinline__ void at_blocks(const AtArgs &a, int64_t p0, int64_t p1, int32_t len, int block, int32_t &b0,
+                                          int32_t &b1) {
+    p0 = max(p0, (int64_t)0);
+    p1 = min(p1, (int64_t)len - 1);
+    b0 = b1 = 0;
+    if (p0 > p1) return;
+    b0 = at_seen(a, p0, len).lo / block;
+    b1 = (at_seen(a, p1, len).hi + block - 1) / block;
+}
+// the tile of `rows` rows that starts at row0 of a sequence, its blocks first .. first + count - 1 (count < 0: all)
+__device__ __forceinline__ AtSegment at_segment(const AtArgs &a, const AtSequence &s, uint32_t row0, uint32_t most,
+                                                int32_t head, int block) {
+    AtSegment t;
+    t.valid = 1;
+    t.row0 = row0;
+    t.rows = (int32_t)min((uint64_t)most, (uint64_t)s.rows * a.group - row0);
+    t.token_row = (uint32_t)s.begin;
+    t.seq = s.seq;
+    t.head = head;
+    t.len = s.len;
+    t.pos0 = s.pos0;
+    const int64_t p0 = s.pos0 + row0 / a.group, p1 = s.pos0 + (row0 + t.rows - 1) / a.group;
+    int32_t b1;
+    at_blocks(a, p0, p1, s.len, block, t.block0, b1);
+    t.blocks = b1 - t.block0;
+    // rows that do not exist count for nothing
+    const Seen first = at_seen(a, max(p0, (int64_t)0), s.len), last = at_seen(a, min(p1, (int64_t)s.len - 1), s.len);
+    t.whole_lo = (last.lo + block - 1) / block;
+    t.whole_hi = first.hi / block;
+    t.slot = -1;
+    return t;
+}
+__device__ __forceinline__ uint64_t at_row_tiles(const AtArgs &a, const AtSequence &s, uint32_t tile_rows) {
+    return ((uint64_t)s.rows * a.group + tile_rows - 1) / tile_rows;
+}
+// blocks of a sequence's last tile up to its first tile's begin: what each of its tiles counts as
+__device__ __forceinline__ uint32_t at_span(const AtArgs &a, const AtSequence &s, int block, int32_t &first) {
+    int32_t b1;
+    at_blocks(a, s.pos0, s.pos0 + s.rows - 1, s.len, block, first, b1);
+    return (uint32_t)max(b1 - first, 1);  // a tile without tokens still writes its rows
+}
+
+// The CTA's segments, one after another, by one whole warp.
+//
+// Without a split a CTA has one: row tile u of (sequence, tile) pairs counted by
+// base_i = begin_i group / R + i, which covers any ragged batch without a table.
+// The last tiles see the most tokens and go first.
+//
+// With one, the blocks of all tiles in a row (sequence, tile, head, block) are cut
+// into as many equal runs as there are CTAs; a tile that a cut goes through is
+// finished by the join kernel.
+template <int SRC, int PARTS, int TILES>
+struct AtWork {
+    using S = AtShape<SRC, PARTS, TILES>;
+    static constexpr uint32_t kRows = TILES * kAtRows;
+    const AtArgs &a;
+    uint64_t at, end;      // run of blocks
+    uint64_t left;         // of it, in this sequence
+    uint32_t i, span, n;   // sequence, its blocks per tile, segments so far
+    int32_t first;
+    uint64_t within;       // blocks into the sequence
+    AtSequence s;
+
+    __device__ __forceinline__ explicit AtWork(const AtArgs &args) : a(args) {
+        at = end = left = 0;
+        i = span = n = 0;
+        first = 0;
+        within = 0;
+        if (!a.slots) return;
+        const uint32_t lane = threadIdx.x & 31;
+        // the blocks of all sequences, 32 sequences at a time
+        uint64_t total = 0;
+        for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) total += warp_sum(weight(k + lane));
+        const uint64_t ctas = min((uint64_t)gridDim.x, total);  // each has a block at least
+        if (blockIdx.x >= ctas) return;
+        at = blockIdx.x * total / ctas;
+        end = (blockIdx.x + 1) * total / ctas;
+        uint64_t before = 0;
+        bool found = false;
+        for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) {
+            const uint64_t w = weight(k + lane);
+            uint64_t upto = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += y;
+            }
+            if (blockIdx.x == 0 && k + lane < a.rows.num_seqs) a.prefix[k + lane] = before + upto - w;
+            if (blockIdx.x == 0 && lane == 0) a.prefix[a.rows.num_seqs] = total;
+            const uint32_t has = __ballot_sync(0xffffffffu, before + upto > at);
+            if (has && !found) {
+                const int l = __ffs(has) - 1;
+                i = k + l;
+                within = at - (before + __shfl_sync(0xffffffffu, upto - w, l));
+                found = true;
+                if (blockIdx.x != 0) break;  // the first CTA also writes the table
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (at < end) open();
+    }
+    __device__ __forceinline__ static uint64_t warp_sum(uint64_t v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    __device__ __forceinline__ uint64_t weight(uint32_t k) const {
+        if (k >= a.rows.num_seqs) return 0;
+        const AtSequence q = at_sequence(a, S::kPaged, k);
+        int32_t f;
+        return at_row_tiles(a, q, kRows) * a.kv_heads * at_span(a, q, S::kBlock, f);
+    }
+    __device__ __forceinline__ void open() {
+        s = at_sequence(a, S::kPaged, i);
+        span = at_span(a, s, S::kBlock, first);
+    }
+    __device__ __forceinline__ AtSegment next() {
+        AtSegment t{};
+        if (!a.slots) {
+            if (n++) return t;
+            return single();
+        }
+        while (at < end) {
+            const uint64_t item = within / span, tiles = at_row_tiles(a, s, kRows);
+            if (item >= tiles * a.kv_heads) {  // the next sequence
+                if (++i >= a.rows.num_seqs) return t;
+                within = 0;
+                open();
+                continue;
+            }
+            const uint32_t from = (uint32_t)(within % span);
+            const uint32_t count = (uint32_t)min((uint64_t)(span - from), end - at);
+            t = at_segment(a, s, (uint32_t)(item / a.kv_heads) * kRows, kRows, (int32_t)(item % a.kv_heads), S::kBlock);
+            // of the tile's own blocks those in the run
+            const int32_t b0 = max(t.block0, first + (int32_t)from), b1 = min(t.block0 + t.blocks, first + (int32_t)(from + count));
+            if (count != span) t.slot = (int32_t)(2 * blockIdx.x + (n ? 1 : 0));
+            t.block0 = b0;
+            t.blocks = max(b1 - b0, 0);
+            within += count;
+            at += count;
+            n++;
+            return t;
+        }
+        return t;
+    }
+    __device__ __forceinline__ AtSegment single() const {
+        AtSegment t{};
+        const uint32_t u = a.units - 1 - blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
+        const uint32_t lane = threadIdx.x & 31;
+        uint32_t lo = 0, count = a.rows.num_seqs;  // the last sequence whose base is not beyond u
+        while (count > 1 && a.rows.row_begin) {
+            const uint32_t step = (count + 31) / 32, k = lo + lane * step;
+            const bool below = lane * step < count && base(k) <= u;
+            const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+            count = min(step, count - last * step);
+            lo += last * step;
+        }
+        if (!a.rows.row_begin && S::kPaged) lo = u / max(base(1), 1u);  // as many rows each
+        if (lo >= a.rows.num_seqs) return t;
+        const AtSequence q = at_sequence(a, S::kPaged, lo);
+        const uint64_t first_unit = base(lo);
+        if (u < first_unit || u - first_unit >= at_row_tiles(a, q, kRows)) return t;
+        return at_segment(a, q, (uint32_t)(u - first_unit) * kRows, kRows, (int32_t)head, S::kBlock);
+    }
+    // the first unit of a sequence
+    __device__ __forceinline__ uint32_t base(uint32_t k) const {
+        if (a.rows.row_begin) return (uint32_t)((uint64_t)max(a.rows.row_begin[k], 0) * a.group / kRows) + k;
+        return k * ((a.group + kRows - 1) / kRows);
+    }
+};
+
+// ---- Q ------------------------------------------------------------------------
+
+// three bf16 parts of eight fp32 values, exact: each takes the next 8 bits
+__device__ __forceinline__ void split3(const float *v, uint4 (&part)[3]) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t u = __float_as_uint(v[i]);
+        const bool fine = (u & 0x7F800000u) != 0x7F800000u;
+        // what is not finite stays whole in the first part (a NaN keeps a bit set)
+        const uint32_t h0 = fine ? u >> 16 : (u >> 16) | ((u & 0xFFFFu) ? 1u : 0u);
+        const float r1 = fine ? v[i] - __uint_as_float(u & 0xFFFF0000u) : 0.f;
+        const uint32_t u1 = __float_as_uint(r1);
+        const float r2 = r1 - __uint_as_float(u1 & 0xFFFF0000u);
+        const uint32_t p[3] = {h0, u1 >> 16, __float_as_uint(r2) >> 16};
+#pragma unroll
+        for (int k = 0; k < 3; k++) w[k][i >> 1] = i & 1 ? w[k][i >> 1] | (p[k] << 16) : p[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) part[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// 16-byte chunk c (of 16) of row r in an operand tile of `rows` rows: two columns of 128-byte rows, swizzled
+__device__ __forceinline__ uint32_t chunk_at(uint32_t base, uint32_t rows, uint32_t r, uint32_t c) {
+    return base + (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+// Row r of the segment by one thread.  For a cache, whose codes are f16 operands,
+// a row of bf16 is brought into f16's range by a power of two.
+template <int SRC, int PARTS>
+__device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint32_t r, uint32_t tile, float &unit) {
+    const uint32_t row = t.row0 + r, token = row / a.group, h = t.head * a.group + row % a.group;
+    const uint64_t at = (uint64_t)(t.token_row + token) * a.query_stride + h * kHeadDim;
+    const uint32_t lane_row = r % kAtRows;
+    unit = 1.f;
+    if constexpr (PARTS == 3) {
+        const float *q = static_cast<const float *>(a.query) + at;
+#pragma unroll 4
+        for (uint32_t c = 0; c < 16; c++) {
+            float v[8];
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(q + 8 * c);
+            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(q + 8 * c + 4);
+            uint4 p[3];
+            split3(v, p);
+#pragma unroll
+            for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(tile + k * kAtRows * 256, kAtRows, lane_row, c), p[k]);
+        }
+    } else {
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.query) + at);
+        uint4 w[16];
+#pragma unroll
+        for (uint32_t c = 0; c < 16; c++) w[c] = q[c];
+        if (SRC != 0 && a.dtype == QWN_DTYPE_BF16) {
+            uint32_t top = 0;  // largest exponent of a finite value
+#pragma unroll
+            for (uint32_t c = 0; c < 16; c++) {
+                const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t e0 = u[k] & 0x7F80u, e1 = (u[k] >> 16) & 0x7F80u;
+                    top = max(top, max(e0 == 0x7F80u ? 0u : e0, e1 == 0x7F80u ? 0u : e1));
+                }
+            }
+            // the largest value to 2^8 .. 2^9: what is below 2^-22 of it loses bits
+            const int e = max(-100, min((int)(top >> 7) - 127 - 8, 119));
+            unit = __uint_as_float((uint32_t)(e + 127) << 23);
+            const float per = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+            for (uint32_t c = 0; c < 16; c++) {
+                uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    u[k] = pack_h2(__uint_as_float(u[k] << 16) * per, __uint_as_float(u[k] & 0xFFFF0000u) * per);
+                w[c] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < 16; c++) st_shared16(chunk_at(tile, kAtRows, lane_row, c), w[c]);
+    }
+}
+
+// ---- keys and values ------------------------------------------------------------
+
+// a cached tile's address for a token that exists; a bad page latches and reads page 0
+__device__ __forceinline__ const uint8_t *at_tile(const AtArgs &a, int32_t seq, int32_t head, int32_t token) {
+    const StoreGeo &g = a.geo;
+    int32_t pg = g.page_table[(size_t)seq * g.mp + (uint32_t)token / g.page_tokens];
+    if (pg < 0 || (uint32_t)pg >= g.total_pages) {
+        latch(a.status, QWN_KV_STATUS_BAD_PAGE);
+        pg = 0;
+    }
+    return g.pages + (size_t)pg * g.page_bytes +
+           ((size_t)(a.layer * g.kv_heads + head) * g.tpp + (uint32_t)token % g.page_tokens / kTileTokens) * g.tile_bytes;
+}
+
+// What the operands hold of a cached value, so that f16 holds it without loss of range: int8 codes by
+// themselves (per 64 channels: times the half's share of the token's larger scale), with the token's scale
+// applied to its score and its probability; 4- and 3.5-bit values halved (at most 65504 + 65504); fp16 as it is.
+template <int SRC>
+struct AtScale {
+    static constexpr bool kTokens = SRC == QWN_KV_CODEC_Q8_B64_F32 || SRC == QWN_KV_CODEC_Q8_HEAD_F16;
+    static constexpr float kFixed = SRC == QWN_KV_CODEC_TQ35_G64 || SRC == QWN_KV_CODEC_Q4_G32 ? 2.f : 1.f;
+};
+// the scale of K (which 0) or V of token t
+template <int SRC>
+__device__ __forceinline__ float token_scale(const uint8_t *tile, int t, int which) {
+    if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16) {
+        return h2f(*reinterpret_cast<const uint16_t *>(tile + (which ? 4128 : 4096) + s16_off(t)));
+    } else {
+        const uint8_t *s = tile + (which ? 4224 : 4096);
+        return fmaxf(*reinterpret_cast<const float *>(s + s32_off(t, 0)), *reinterpret_cast<const float *>(s + s32_off(t, 1)));
+    }
+}
+template <int SRC, int PARTS>
+__device__ __forceinline__ Row16 operand_row(const uint8_t *tile, int t, int which, int j) {
+    if constexpr (PARTS == 3) {
+        return take_row<SRC>(tile, t, which, j);
+    } else if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16) {
+        return take_q8(tile, t, which, j, 1.f, 1.f);
+    } else if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+        const uint8_t *s = tile + (which ? 4224 : 4096);
+        const float s0 = *reinterpret_cast<const float *>(s + s32_off(t, 0)), s1 = *reinterpret_cast<const float *>(s + s32_off(t, 1));
+        const float top = fmaxf(s0, s1);
+        return take_q8(tile, t, which, j, s0 / top, s1 / top);
+    } else {
+        Row16 x = take_row<SRC>(tile, t, which, j);
+        if (AtScale<SRC>::kFixed != 1.f)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x.v[i] *= 1.f / AtScale<SRC>::kFixed;
+        return x;
+    }
+}
+// a row's 16 values of this lane into an operand tile, as f16 or as three bf16 parts
+template <int PARTS>
+__device__ __forceinline__ void put_operand(uint32_t base, uint32_t rows, uint32_t part, uint32_t r, int j, const Row16 &x) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float *v = x.v + 8 * h;
+        if constexpr (PARTS == 1) {
+            st_shared16(chunk_at(base, rows, r, 8 * h + j),
+                        make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]), pack_h2(v[4], v[5]), pack_h2(v[6], v[7])));
+        } else {
+            uint4 p[3];
+            split3(v, p);
+#pragma unroll
+            for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
+        }
+    }
+}
+// K or V of a cached tile, which is tile ti of its block, by one warp; tokens from `len` on are zero
+template <int SRC, int PARTS, int BLOCK>
+__device__ __forceinline__ void put_tile(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
+    const int lane = threadIdx.x & 31, j = lane & 7;
+#pragma unroll
+    for (int pass = 0; pass < 4; pass++) {
+        const int t = 4 * pass + (lane >> 3);
+        Row16 x = operand_row<SRC, PARTS>(tile, t, which, j);
+        if (token0 + t >= len) x = Row16{};
+        put_operand<PARTS>(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
+    }
+}
+
+// ---- values that a sequence's ends ask for ---------------------------------------
+//
+// A masked token must not matter, but 0 x inf is NaN in an MMA.  In blocks that
+// some rows see only in part, values that are not finite are therefore taken out of
+// the operand tile (tokens past the end altogether) and noted; the rows that do see
+// them get them added at the end (add_odd).  A CTA's rows span 256 tokens at most,
+// so that such blocks span 512 from the first block on and 512 from `zone` on.
+__device__ __forceinline__ int32_t odd_zone(const AtSegment &t, int block) {
+    return max(t.whole_hi, max(t.whole_lo, t.block0)) * block;
+}
+__device__ __forceinline__ bool odd_word(uint32_t w, bool bf16, uint32_t &out) {
+    const uint32_t e = bf16 ? 0x7F80u : 0x7C00u;
+    const bool lo = (w & e) == e, hi = ((w >> 16) & e) == e;
+    out = (lo ? 0u : w & 0xFFFFu) | (hi ? 0u : w & 0xFFFF0000u);
+    return lo || hi;
+}
+template <int PARTS, int BLOCK>
+__device__ void clear_odd(AtShared &sh, const AtSegment &seg, int32_t token0, uint32_t base, bool bf16, uint32_t which) {
+    const uint32_t tid = threadIdx.x & 127, r = tid % BLOCK, c0 = tid / BLOCK * (BLOCK / 8);
+    const int32_t token = token0 + (int32_t)r;
+    const bool past = token >= seg.len;
+    bool odd = false;
+#pragma unroll 4
+    for (uint32_t c = c0; c < c0 + BLOCK / 8; c++) {
+        const uint32_t at = chunk_at(base, BLOCK, r, c);
+        if (past) {
+#pragma unroll
+            for (uint32_t k = 0; k < PARTS; k++) st_shared16(at + k * BLOCK * 256, make_uint4(0, 0, 0, 0));
+            continue;
+        }
+        const uint4 w = ld_shared16(at);
+        uint4 y;
+        const bool o = odd_word(w.x, bf16, y.x) | odd_word(w.y, bf16, y.y) | odd_word(w.z, bf16, y.z) | odd_word(w.w, bf16, y.w);
+        if (o) st_shared16(at, y);
+        odd |= o;
+    }
+    if (odd) {
+        const int32_t z = odd_zone(seg, BLOCK);
+        const uint32_t i = (uint32_t)(token < z ? token - seg.block0 * BLOCK : token - z);
+        if (i < 512) atomicOr(&sh.odd_v[which][token < z ? 0 : 1][i >> 5], 1u << (i & 31));
+    }
+}
+// value d of a token
+template <int SRC, int PARTS>
+__device__ float at_value(const AtArgs &a, const AtSegment &seg, int32_t token, int d) {
+    if constexpr (SRC != 0) {
+        const float4 v = load_token<SRC>(at_tile(a, seg.seq, seg.head, token), token & 15, 1, d >> 2);
+        return (d & 2) ? ((d & 1) ? v.w : v.z) : ((d & 1) ? v.y : v.x);
+    } else {
+        const uint64_t at = (uint64_t)(seg.token_row + token) * a.value_stride + seg.head * kHeadDim + d;
+        if constexpr (PARTS == 3) return static_cast<const float *>(a.value)[at];
+        if (a.dtype == QWN_DTYPE_F16) return __half2float(static_cast<const __half *>(a.value)[at]);
+        return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.value)[at]);
+    }
+}
+template <int SRC, int PARTS, int BLOCK, int N>
+__device__ __noinline__ void add_odd(const AtArgs &a, const AtShared &sh, const AtSegment &seg, uint32_t which, Seen seen,
+                                     int col, float *o) {
+    for (int z = 0; z < 2; z++) {
+        const int32_t from = z ? odd_zone(seg, BLOCK) : seg.block0 * BLOCK;
+        for (int w = 0; w < 16; w++)
+            for (uint32_t bits = sh.odd_v[which][z][w]; bits; bits &= bits - 1) {
+                const int32_t token = from + 32 * w + __ffs(bits) - 1;
+                if (token < seen.lo || token >= seen.hi) continue;
+                for (int k = 0; k < N; k++) {
+                    const float v = at_value<SRC, PARTS>(a, seg, token, col + k);
+                    if (!isfinite(v)) o[k] += v;
+                }
+            }
+    }
+}
+
+// ---- softmax -------------------------------------------------------------------
+
+// P is 2^kBias near the largest score and grows by 2^kSlack at most before M moves:
+// f16 holds 2^14 down to 2^-24, so that a probability is lost below 2^-32 of the
+// largest; bf16 and fp32 have room.
+template <bool BF16>
+struct AtRange {
+    static constexpr float kBias = BF16 ? 0.f : 8.f, kSlack = BF16 ? 8.f : 6.f;
+};
+
+// `n` values of a row: 32-byte stores where the type fills them
+template <int N>
+__device__ __forceinline__ void store_values(void *out, uint64_t at, uint32_t dtype, const float *v) {
+    if (dtype == QWN_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) store4(static_cast<float *>(out) + at + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (dtype == QWN_DTYPE_F16) {
+                w[k] = pack_h2(v[i + 2 * k], v[i + 2 * k + 1]);
+            } else {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
+                w[k] = *reinterpret_cast<const uint32_t *>(&b);
+            }
+        }
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int SRC, int PARTS, int TILES, bool BF16>
+struct AtRoles {
+    using S = AtShape<SRC, PARTS, TILES>;
+    using Scale = AtScale<SRC>;
+    static constexpr bool kTokenScales = PARTS == 1 && Scale::kTokens;
+    // the operands' own scaling: of scores and of outputs
+    static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
+    const AtArgs &a;
+    AtShared &sh;
+    uint32_t q_at, k_at, v_at, raw_at;  // shared memory
+    int warp, lane;
+
+    // the next segment, for a warp that works on all of them
+    struct Feed {
+        uint32_t n = 0;
+    };
+    __device__ __forceinline__ bool take(Feed &f, AtSegment &seg) {
+        const uint32_t s = f.n & 1;
+        if (!at_wait(sh, &sh.segfull[s], (f.n >> 1) & 1)) return false;
+        seg = sh.seg[s];
+        warp_arrive(&sh.segempty[s], lane);
+        f.n++;
+        return seg.valid != 0;
+    }
+
+    __device__ __forceinline__ void plan() {
+        AtWork<SRC, PARTS, TILES> work(a);
+        for (uint32_t n = 0;; n++) {
+            const uint32_t s = n & 1;
+            const AtSegment seg = work.next();
+            if (!at_wait(sh, &sh.segempty[s], ((n >> 1) & 1) ^ 1)) return;
+            if (lane == 0) sh.seg[s] = seg;
+            warp_arrive(&sh.segfull[s], lane);
+            if (!seg.valid) return;
+        }
+    }
+
+    __device__ __forceinline__ void load(const CUtensorMap *kmap, const CUtensorMap *vmap) {
+        Feed f;
+        AtSegment seg;
+        uint32_t done = 0;  // blocks, or cached tiles
+        uint32_t v_uses[2][2] = {};
+        bool ok = true;
+        while (ok && take(f, seg)) {
+            if constexpr (S::kTma) {
+                for (int b = 0; b < seg.blocks && ok; b++, done++) {
+                    const int y = (int)seg.token_row + (seg.block0 + b) * S::kBlock, x = seg.head * kHeadDim;
+                    auto fetch = [&](uint64_t *full, uint64_t *empty, uint32_t use, uint32_t at, const CUtensorMap *map) {
+                        if (!at_wait(sh, empty, (use & 1) ^ 1)) return false;
+                        if (lane == 0) {
+                            mbar_expect_tx(full, S::kKvBytes);
+                            tma_load(at, map, x, y, smem_u32(full));
+                            tma_load(at + S::kBlock * 128, map, x + 64, y, smem_u32(full));
+                        }
+                        __syncwarp();
+                        return true;
+                    };
+                    const uint32_t ks = done % S::kStagesK, vs = done % S::kStagesV;
+                    const bool part = !whole(seg, seg.block0 + b);
+                    ok = fetch(&sh.kfull[ks], &sh.kempty[ks], done / S::kStagesK, k_at + ks * S::kKvBytes, kmap) &&
+                         fetch(part ? &sh.vpart[vs] : &sh.vfull[vs], &sh.vempty[vs], done / S::kStagesV, v_at + vs * S::kKvBytes, vmap);
+                    v_uses[part ? 1 : 0][vs] += ok;
+                }
+            } else if constexpr (S::kRaw) {
+                auto address = [&](int b) -> const uint8_t * {
+                    const int32_t token = (seg.block0 + b) * S::kBlock + lane * kTileTokens;
+                    return b < seg.blocks && lane < S::kTiles && token < seg.len ? at_tile(a, seg.seq, seg.head, token) : nullptr;
+                };
+                const uint8_t *ahead = address(0);
+                for (int b = 0; b < seg.blocks && ok; b++) {
+                    const uint8_t *from = ahead;
+                    ahead = address(b + 1);  // the next block's pages are looked up while this one's tiles go out
+                    for (int t = 0; t < S::kTiles && ok; t++, done++) {
+                        const uint32_t s = done % S::kRawTiles;
+                        ok = at_wait(sh, &sh.rawempty[s], ((done / S::kRawTiles) & 1) ^ 1);
+                        if (ok && lane == t) {
+                            if (from) {
+                                mbar_expect_tx(&sh.rawfull[s], S::kTileBytes);
+                                asm volatile(
+                                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+                                        "r"(raw_at + s * S::kTileBytes),
+                                    "l"(from), "r"(S::kTileBytes), "r"(smem_u32(&sh.rawfull[s]))
+                                    : "memory");
+                            } else {
+                                mbar_arrive(&sh.rawfull[s]);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        // copies in flight end before the CTA's memory goes, whoever gave up
+        if constexpr (S::kTma) {
+            for (uint32_t d = done > S::kStagesK ? done - S::kStagesK : 0; d < done; d++)
+                mbar_wait_bounded(&sh.kfull[d % S::kStagesK], (d / S::kStagesK) & 1);
+            for (uint32_t v = 0; v < 2; v++) {
+                if (v_uses[0][v]) mbar_wait_bounded(&sh.vfull[v], (v_uses[0][v] - 1) & 1);
+                if (v_uses[1][v]) mbar_wait_bounded(&sh.vpart[v], (v_uses[1][v] - 1) & 1);
+            }
+        } else if constexpr (S::kRaw) {
+            for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++)
+                mbar_wait_bounded(&sh.rawfull[d % S::kRawTiles], (d / S::kRawTiles) & 1);
+        }
+    }
+
+    __device__ __forceinline__ static bool whole(const AtSegment &seg, int blk) { return blk >= seg.whole_lo && blk < seg.whole_hi; }
+
+    // the helpers' four warps meet; a wait like the others, so that it ends when one of them has given up
+    __device__ __forceinline__ bool helpers_sync(uint32_t &syncs) {
+        warp_arrive(&sh.helped, lane);
+        return at_wait(sh, &sh.helped, syncs++ & 1);
+    }
+    // K and V of a block out of cached tiles or fp32 rows
+    __device__ __forceinline__ bool convert(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
+        const int w = warp & 3;
+        const int32_t token0 = blk * S::kBlock;
+        const uint32_t ks = done % S::kStagesK, vs = done % S::kStagesV, slot = done & 3;
+        const uint32_t kd = k_at + ks * S::kKvBytes, vd = v_at + vs * S::kKvBytes;
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            const uint32_t stages = which ? S::kStagesV : S::kStagesK, s = which ? vs : ks, dst = which ? vd : kd;
+            if (!at_wait(sh, which ? &sh.vempty[s] : &sh.kempty[s], ((done / stages) & 1) ^ 1)) return false;
+            for (int ti = w; ti < S::kTiles; ti += 4) {
+                const int32_t at = token0 + ti * kTileTokens;
+                if constexpr (S::kPaged) {
+                    const uint8_t *tile = nullptr;
+                    if constexpr (S::kRaw) {
+                        const uint32_t g = done * S::kTiles + ti, r = g % S::kRawTiles;
+                        if (!which && !at_wait(sh, &sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
+                        extern __shared__ uint8_t dynamic[];
+                        tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
+                    } else if (at < seg.len) {
+                        tile = at_tile(a, seg.seq, seg.head, at);
+                    }
+                    if (kTokenScales && !which) {  // both scales, read when the block's scores are there
+                        const int t = lane & 15, v = lane >> 4;
+                        const float sc = at + t < seg.len ? token_scale<SRC>(tile, t, v) : 0.f;
+                        (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + t] = sc;
+                        const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
+                        if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
+                    }
+                    if (tile) {
+                        put_tile<SRC, PARTS, S::kBlock>(tile, which, ti, at, seg.len, dst);
+                    } else {
+                        for (int pass = 0; pass < 4; pass++)
+                            put_operand<PARTS>(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + 4 * pass + (lane >> 3)),
+                                               lane & 7, Row16{});
+                    }
+                    if constexpr (S::kRaw)
+                        if (which) warp_arrive(&sh.rawempty[(done * S::kTiles + ti) % S::kRawTiles], lane);
+                } else {
+                    const float *rows = static_cast<const float *>(which ? a.value : a.key) + (size_t)seg.head * kHeadDim;
+                    const uint64_t stride = which ? a.value_stride : a.key_stride;
+#pragma unroll
+                    for (int pass = 0; pass < 4; pass++) {
+                        const int t = 4 * pass + (lane >> 3);
+                        Row16 x = {};
+                        if (at + t < seg.len) {
+                            Raw16<float> raw;
+                            raw.load(rows + (uint64_t)(seg.token_row + at + t) * stride, lane & 7);
+                            x = raw.row();
+                        }
+                        put_operand<PARTS>(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + t), lane & 7, x);
+                    }
+                }
+            }
+            if (which && !whole(seg, blk)) {
+                if (!helpers_sync(syncs)) return false;
+                clear_odd<PARTS, S::kBlock>(sh, seg, token0, dst, PARTS == 3, segment & 3);
+            }
+            fence_proxy_async_shared();
+            warp_arrive(which ? &sh.vfull[s] : &sh.kfull[s], lane);
+        }
+        return true;
+    }
+
+    __device__ __forceinline__ void help() {
+        Feed f;
+        AtSegment seg;
+        uint32_t done = 0, used = 0, syncs = 0;  // blocks, segments with any
+        uint32_t parts[2] = {};
+        const uint32_t tid = threadIdx.x & 127;
+        while (take(f, seg)) {
+            if (seg.blocks == 0) continue;
+            if (!at_wait(sh, &sh.qempty, (used & 1) ^ 1)) return;
+            if (tid < 32) sh.odd_v[used & 3][tid >> 4][tid & 15] = 0;
+#pragma unroll
+            for (int t = 0; t < TILES; t++) {
+                const uint32_t r = t * kAtRows + tid;
+                if ((int32_t)r < seg.rows) {
+                    float unit;
+                    put_q<SRC, PARTS>(a, seg, r, q_at + t * S::kQBytes, unit);
+                    sh.qscale[used & 1][r] = unit;
+                }
+            }
+            fence_proxy_async_shared();
+            if (!helpers_sync(syncs)) return;  // odd_v is empty before any warp notes a token
+            warp_arrive(&sh.qfull, lane);
+            for (int b = 0; b < seg.blocks; b++, done++) {
+                const int blk = seg.block0 + b;
+                if constexpr (!S::kTma) {
+                    if (!convert(seg, blk, done, used, syncs)) return;
+                } else if (!whole(seg, blk)) {
+                    const uint32_t s = done % S::kStagesV;
+                    if (!at_wait(sh, &sh.vpart[s], parts[s]++ & 1)) return;
+                    clear_odd<PARTS, S::kBlock>(sh, seg, blk * S::kBlock, v_at + s * S::kKvBytes, BF16, used & 3);
+                    fence_proxy_async_shared();
+                    warp_arrive(&sh.vfixed[s], lane);
+                }
+            }
+            used++;
+        }
+    }
+
+    // one warp; its elected lane issues
+    __device__ __forceinline__ void multiply() {
+        Feed f;
+        AtSegment seg;
+        const uint32_t tmem = sh.tmem;
+        const bool leader = elect_one();
+        uint32_t done = 0, used = 0, o_uses[2] = {0, 0}, p_uses[2] = {0, 0}, fixes[2] = {0, 0}, wholes[2] = {0, 0};
+        constexpr uint32_t kQk = f16_desc(BF16 || PARTS == 3, S::kBlock, false), kPv = f16_desc(BF16 || PARTS == 3, 128, true);
+        // the products of parts that count, the small ones first
+        constexpr int kPairs = PARTS == 1 ? 1 : 6;
+        constexpr int kFirst[6] = {PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
+        auto scores = [&](int t, uint32_t stage) {  // S_t = Q K^T
+            const uint32_t q = q_at + (TILES == 2 ? t * S::kQBytes : 0), k = k_at + stage * S::kKvBytes;
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) {
+                const uint64_t qd = smem_desc(q + kFirst[p] * kAtRows * 256), kd = smem_desc(k + kSecond[p] * S::kKvPart);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (leader)
+                        mma_ss(tmem + t * S::kSColumns, qd + (c >> 2) * (kAtRows * 128 / 16) + (c & 3) * 2,
+                               kd + (c >> 2) * (S::kBlock * 128 / 16) + (c & 3) * 2, kQk, p + c > 0);
+            }
+        };
+        auto values = [&](int t, uint32_t stage, bool add) {  // O_t += P_t V
+            const uint32_t v = v_at + stage * S::kKvBytes;
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) {
+                const uint64_t vd = rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
+#pragma unroll
+                for (int c = 0; c < S::kBlock / 16; c++)
+                    if (leader)
+                        mma_ts(tmem + S::kOColumn + t * 128, tmem + t * S::kSColumns + kFirst[p] * (S::kBlock / 2) + c * 8,
+                               vd + c * (2048 / 16), kPv, add || p + c > 0);
+            }
+        };
+        auto commit = [&](uint64_t *bar) {
+            if (leader) mma_commit(bar);
+        };
+        auto wait_k = [&](uint32_t d) { return at_wait(sh, &sh.kfull[d % S::kStagesK], (d / S::kStagesK) & 1); };
+        bool ok = true;
+        while (ok && take(f, seg)) {
+            const int nb = seg.blocks;
+            if (nb == 0) continue;
+            ok = at_wait(sh, &sh.qfull, used & 1);
+            // block b's scores for group t, and what becomes free behind them
+            auto do_scores = [&](int b, int t) {
+                if (TILES == 1 || t == 0) ok = ok && wait_k(done + b);
+                if (!ok) return;
+                tc_fence_after();
+                scores(t, (done + b) % S::kStagesK);
+                commit(&sh.sfull[t]);
+                if (TILES == 1 || t == 1) {
+                    commit(&sh.kempty[(done + b) % S::kStagesK]);
+                    if (b == nb - 1) commit(&sh.qempty);
+                }
+            };
+            for (int t = 0; t < 2; t++)
+                if (TILES == 2) do_scores(0, t);
+                else if (t < nb) do_scores(t, t);
+            for (int b = 0; b < nb && ok; b++) {
+                const uint32_t vs = (done + b) % S::kStagesV;
+                if (!S::kTma) ok = at_wait(sh, &sh.vfull[vs], ((done + b) / S::kStagesV) & 1);
+                else if (whole(seg, seg.block0 + b)) ok = at_wait(sh, &sh.vfull[vs], wholes[vs]++ & 1);
+                else ok = at_wait(sh, &sh.vfixed[vs], fixes[vs]++ & 1);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    if (TILES == 1 && t != (b & 1)) continue;
+                    ok = ok && at_wait(sh, &sh.pready[t], p_uses[t]++ & 1);
+                    const bool first = TILES == 2 ? b == 0 : b < 2;
+                    if (first) ok = ok && at_wait(sh, &sh.oempty[t], (o_uses[t]++ & 1) ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(t, vs, !first);
+                    if (TILES == 1 || t == 1) commit(&sh.vempty[vs]);
+                    const int nextb = b + (TILES == 2 ? 1 : 2);
+                    if (nextb < nb) do_scores(nextb, t);
+                    else commit(&sh.ofull[t]);
+                }
+            }
+            done += nb;
+            used++;
+        }
+        if (*(volatile int *)&sh.give_up) {  // products in flight end before the CTA's memory goes
+            commit(&sh.drained);
+            mbar_wait_bounded(&sh.drained, 0);
+        }
+    }
+
+    __device__ __forceinline__ void soften() {
+        Feed f;
+        AtSegment seg;
+        const int g = warp >> 2, w = warp & 3;
+        const uint32_t lanes = sh.tmem + ((uint32_t)(w * 32) << 16);
+        const uint32_t s_col = lanes + g * S::kSColumns, o_col = lanes + S::kOColumn + g * 128;
+        uint32_t done = 0, used = 0, s_uses = 0, o_uses[2] = {0, 0}, joins = 0;
+        const uint32_t r = (TILES == 2 ? g * kAtRows : 0) + w * 32 + lane;
+        while (take(f, seg)) {
+            const bool have = (int32_t)r < seg.rows, any = (int32_t)(r - lane) < seg.rows;
+            const int64_t pos = seg.pos0 + (have ? (seg.row0 + r) / a.group : 0);
+            const Seen seen = have ? at_seen(a, pos, seg.len) : Seen{0, 0};
+            if (have && S::kPaged && (pos < 0 || pos >= seg.len))
+                latch(a.status, seg.seq < 0 ? QWN_KV_STATUS_BAD_SEQUENCE : QWN_KV_STATUS_BAD_LENGTH);
+            float M = -INFINITY, l = 0.f, c = 0.f;
+            for (int b = TILES == 2 ? 0 : g; b < seg.blocks; b += TILES == 2 ? 1 : 2) {
+                if (!at_wait(sh, &sh.sfull[g], s_uses++ & 1)) return;
+                tc_fence_after();
+                if (any) {
+                    const bool first = b < (TILES == 2 ? 1 : 2);
+                    if (first) c = a.scale2 * kUnit * (SRC != 0 && PARTS == 1 && have ? sh.qscale[used & 1][r] : 1.f);
+                    block(seg, seg.block0 + b, (done + b) & 3, first, have, seen, c, s_col, o_col, M, l);
+                }
+                tc_fence_before();
+                warp_arrive(&sh.pready[g], lane);
+            }
+            if (seen.lo >= seen.hi) {  // a row that does not exist: blocks seen whole by the others are no business of its
+                M = -INFINITY;
+                l = 0.f;
+            }
+            if (!finish(seg, used, have, any, r, seen, g, lanes, M, l, o_uses, joins)) return;
+            done += seg.blocks;
+            if (seg.blocks) used++;
+        }
+    }
+
+    // a block's scores to probabilities; M, l and, where M moves, the sums so far
+    __device__ __forceinline__ void block(const AtSegment &seg, int blk, uint32_t slot, bool first, bool have, const Seen &seen,
+                                          float c, uint32_t s_col, uint32_t o_col, float &M, float &l) {
+        constexpr int N = S::kBlock;
+        using Range = AtRange<BF16 || PARTS == 3>;
+        uint32_t u[N];
+        float *x = reinterpret_cast<float *>(u);
+        tmem_load64(u, s_col);
+        if constexpr (N == 128) tmem_load64(u + 64, s_col + 64);
+        float vtop = 0.f;
+        if constexpr (kTokenScales) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const float4 k = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i]);
+                x[i] *= k.x, x[i + 1] *= k.y, x[i + 2] *= k.z, x[i + 3] *= k.w;
+            }
+            const float4 v0 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][0]), v1 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][4]);
+            vtop = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)), fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
+        }
+        if (!whole(seg, blk)) {
+            const int lo = seen.lo - blk * N, hi = seen.hi - blk * N;
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i < lo || i >= hi) x[i] = -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+        const float reach = top * c + vtop;
+        const bool grows = have && reach > M + Range::kSlack;  // true for the first that is not -inf
+        if (__any_sync(0xffffffffu, grows)) {
+            const float factor = grows && M != -INFINITY ? ex2(M - reach) : 1.f;
+            if (grows) {
+                l *= factor;
+                M = reach;
+            }
+            if (!first) {
+#pragma unroll 1
+                for (int i = 0; i < 128; i += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o, o_col + i);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                    tmem_store16(o_col + i, o);
+                }
+            }
+        }
+        const float off = Range::kBias - (M == -INFINITY ? 0.f : M);
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i += 32) {
+            uint32_t p[PARTS][16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+                const float e0 = ex2(fmaf(x[i + k], c, off)), e1 = ex2(fmaf(x[i + k + 1], c, off));
+                l0 += e0;
+                l1 += e1;
+                if constexpr (PARTS == 3) {
+                    const uint32_t a0 = __float_as_uint(e0), a1 = __float_as_uint(e1);
+                    const float f0 = e0 - __uint_as_float(a0 & 0xFFFF0000u), f1 = e1 - __uint_as_float(a1 & 0xFFFF0000u);
+                    const uint32_t b0 = __float_as_uint(f0), b1 = __float_as_uint(f1);
+                    const float g0 = f0 - __uint_as_float(b0 & 0xFFFF0000u), g1 = f1 - __uint_as_float(b1 & 0xFFFF0000u);
+                    p[0][k >> 1] = prmt(a0, a1, 0x7632u);
+                    p[1][k >> 1] = prmt(b0, b1, 0x7632u);
+                    p[2][k >> 1] = prmt(__float_as_uint(g0), __float_as_uint(g1), 0x7632u);
+                } else if constexpr (BF16) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(e0, e1);
+                    p[0][k >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+                } else if constexpr (kTokenScales) {
+                    const float2 v = *reinterpret_cast<const float2 *>(&sh.vscale[slot][i + k]);
+                    p[0][k >> 1] = pack_h2(e0 * v.x, e1 * v.y);
+                } else {
+                    p[0][k >> 1] = pack_h2(e0, e1);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (N / 2) + i / 2, p[k]);
+        }
+        l += l0 + l1;
+        tmem_store_wait();
+    }
+
+    // the rows of a segment: to the output, or to the workspace where other CTAs have a share of them
+    __device__ __forceinline__ bool finish(const AtSegment &seg, uint32_t used, bool have, bool any, uint32_t r, const Seen &seen,
+                                           int g, uint32_t lanes, float M, float l, uint32_t (&o_uses)[2], uint32_t &joins) {
+        constexpr int kWide = 32;  // columns at a time
+        const uint32_t o_at = lanes + S::kOColumn;
+        float w0 = 1.f, w1 = 0.f;
+        const bool two = TILES == 1 && seg.blocks > 1;
+        if (TILES == 1) {  // both groups' rows are the same ones: each group finishes half of the columns
+            const uint32_t row = r, turn = joins & 1;
+            sh.ml[turn][g][row][0] = M;
+            sh.ml[turn][g][row][1] = l;
+            warp_arrive(&sh.joined, lane);
+            if (!at_wait(sh, &sh.joined, joins & 1)) return false;
+            joins++;
+            const float M0 = sh.ml[turn][0][row][0], M1 = sh.ml[turn][1][row][0];
+            M = fmaxf(M0, M1);
+            w0 = M0 == -INFINITY ? 0.f : ex2(M0 - M);
+            w1 = M1 == -INFINITY ? 0.f : ex2(M1 - M);
+            l = w0 * sh.ml[turn][0][row][1] + w1 * sh.ml[turn][1][row][1];
+        }
+        if (seg.blocks) {
+            if (TILES == 2) {
+                if (!at_wait(sh, &sh.ofull[g], o_uses[0]++ & 1)) return false;
+            } else {
+                if (!at_wait(sh, &sh.ofull[0], o_uses[0]++ & 1)) return false;
+                if (two && !at_wait(sh, &sh.ofull[1], o_uses[1]++ & 1)) return false;
+            }
+            tc_fence_after();
+        }
+        if (any) {
+            uint32_t odd = 0;
+            if (seg.blocks) {
+                for (int z = 0; z < 2; z++) odd |= sh.odd_v[used & 3][z][lane & 15];
+                odd = __any_sync(0xffffffffu, odd != 0);
+            }
+            const uint32_t row = seg.row0 + (have ? r : 0), token = row / a.group, h = seg.head * a.group + row % a.group;
+            const uint64_t at = (uint64_t)(seg.token_row + token) * a.out_stride + h * kHeadDim;
+            float *slot = seg.slot < 0 ? nullptr : a.slots + (size_t)seg.slot * at_slot_floats(TILES);
+            const float per = l > 0.f || l != l ? kUnit / l : 0.f;
+            const int from = TILES == 1 ? g * 64 : 0, to = TILES == 1 ? from + 64 : 128;
+#pragma unroll 1
+            for (int col = from; col < to; col += kWide) {
+                float o[kWide];
+                uint32_t u[kWide];
+                if (seg.blocks) {
+                    tmem_load32(u, o_at + (TILES == 2 ? g * 128 : 0) + col);
+#pragma unroll
+                    for (int k = 0; k < kWide; k++) o[k] = w0 == 1.f ? __uint_as_float(u[k]) : w0 == 0.f ? 0.f : __uint_as_float(u[k]) * w0;
+                    if (two) {
+                        tmem_load32(u, o_at + 128 + col);
+#pragma unroll
+                        for (int k = 0; k < kWide; k++)
+                            if (w1 != 0.f) o[k] = fmaf(__uint_as_float(u[k]), w1, o[k]);
+                    }
+                    if (odd && have) add_odd<SRC, PARTS, S::kBlock, kWide>(a, sh, seg, used & 3, seen, col, o);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kWide; k++) o[k] = 0.f;
+                }
+                if (!have) continue;
+                if (slot) {
+#pragma unroll
+                    for (int k = 0; k < kWide; k += 4)
+                        store4(slot + (size_t)r * kHeadDim + col + k, make_float4(o[k] * kUnit, o[k + 1] * kUnit, o[k + 2] * kUnit, o[k + 3] * kUnit));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
+                    store_values<kWide>(a.out, at + col, a.dtype, o);
+                }
+            }
+            if (slot && have && (TILES == 2 || g == 0)) {
+                slot[TILES * kAtRows * kHeadDim + r] = M;
+                slot[TILES * kAtRows * (kHeadDim + 1) + r] = l;
+            }
+        }
+        if (seg.blocks) {
+            tc_fence_before();
+            if (TILES == 2) {
+                warp_arrive(&sh.oempty[g], lane);
+            } else {
+                warp_arrive(&sh.oempty[0], lane);
+                if (two) warp_arrive(&sh.oempty[1], lane);
+            }
+        }
+        return true;
+    }
+};
+
+template <int SRC, int PARTS, int TILES, bool BF16>
+__global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                    const __grid_constant__ CUtensorMap vmap,
+                                                                    const __grid_constant__ AtArgs a) {
+    using S = AtShape<SRC, PARTS, TILES>;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ __align__(16) AtShared sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
+    AtRoles<SRC, PARTS, TILES, BF16> roles = {a, sh, base, base + TILES * S::kQBytes,
+                                              base + TILES * S::kQBytes + S::kStagesK * S::kKvBytes, base + S::kOperands, warp, lane};
+    if (threadIdx.x == 0) {
+        const uint32_t helpers = S::kTma ? 1 : 4, finishers = TILES == 2 ? 4 : 8;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.kfull[i], helpers);
+            mbar_init(&sh.vfull[i], helpers);
+            mbar_init(&sh.kempty[i], 1);
+            mbar_init(&sh.vempty[i], 1);
+            mbar_init(&sh.vpart[i], 1);
+            mbar_init(&sh.vfixed[i], 4);
+            mbar_init(&sh.sfull[i], 1);
+            mbar_init(&sh.pready[i], 4);
+            mbar_init(&sh.ofull[i], 1);
+            mbar_init(&sh.oempty[i], finishers);
+            mbar_init(&sh.segfull[i], 1);
+            mbar_init(&sh.segempty[i], 14);
+        }
+        mbar_init(&sh.qfull, 4);
+        mbar_init(&sh.qempty, 1);
+        mbar_init(&sh.joined, 8);
+        mbar_init(&sh.helped, 4);
+        mbar_init(&sh.drained, 1);
+        for (int i = 0; i < 32; i++) {
+            mbar_init(&sh.rawfull[i], 1);
+            mbar_init(&sh.rawempty[i], 1);
+        }
+        sh.give_up = 0;
+        fence_barrier_init();
+    }
+    if (warp == 12) tmem_alloc<1>(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    launch_dependents();
+    wait_previous();
+    if (warp < 8) {
+        take_registers<kSoftmaxRegs>();
+        roles.soften();
+    } else if (warp < 12) {
+        give_registers<kHelperRegs>();
+        roles.help();
+    } else {
+        give_registers<kOtherRegs>();
+        if (warp == 12) roles.multiply();
+        else if (warp == 13) roles.load(&kmap, &vmap);
+        else if (warp == 14) roles.plan();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && sh.give_up) latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_free<1>(sh.tmem, 512);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+// Prepares a kernel on the current device, once.  Refuses one whose block does not
+// start with the registers that its warps share out: it would wait for them for good.
+template <int SRC, int PARTS, int TILES, bool BF16>
+cudaError_t prepare_tile_kernel(int device) {
+    static std::mutex mu;
+    static bool ready[64];
+    if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    if (ready[device]) return cudaSuccess;
+    const auto kernel = prompt_tile_kernel<SRC, PARTS, TILES, BF16>;
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, kernel);
+    if (e == cudaSuccess && at.numRegs * 4 < 2 * kSoftmaxRegs + kHelperRegs + kOtherRegs) return cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AtShape<SRC, PARTS, TILES>::kSmem);
+    ready[device] = e == cudaSuccess;
+    return e;
+}
+template <int SRC, int PARTS, int TILES, bool BF16>
+cudaError_t launch_tile_kernel(int device, uint32_t ctas, cudaStream_t s, const CUtensorMap &kmap, const CUtensorMap &vmap,
+                               const AtArgs &a) {
+    cudaError_t e = prepare_tile_kernel<SRC, PARTS, TILES, BF16>(device);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kAtThreads);
+    cfg.dynamicSmemBytes = AtShape<SRC, PARTS, TILES>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    note_early_trigger();
+    e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<SRC, PARTS, TILES, BF16>, kmap, vmap, a);
+    if (e == cudaSuccess) count_launch();
+    else cudaGetLastError();  // reported here, not by a later launch
+    return e;
+}
+
+}  // namespace
+}  // namespace qkv

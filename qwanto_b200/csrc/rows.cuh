@@ -85,6 +85,15 @@ cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, dim3 block, cudaSt
 }
 
 inline bool dtype_ok(uint32_t d) { return d == QWN_DTYPE_F32 || d == QWN_DTYPE_F16 || d == QWN_DTYPE_BF16; }
+inline uint64_t value_bytes(uint32_t dtype) { return dtype == QWN_DTYPE_F32 ? 4 : 2; }
+// rows start on `values` values
+inline bool rows_aligned(const void *p, uint64_t stride, uint32_t dtype, uint64_t values = 4) {
+    return (uintptr_t)p % (value_bytes(dtype) * values) == 0 && stride % values == 0;
+}
+// 16-byte accesses
+inline bool rows_wide(const void *p, uint64_t stride, uint32_t dtype) {
+    return rows_aligned(p, stride, dtype, 16 / value_bytes(dtype));
+}
 inline int invalid(const char *msg) {
     set_error(msg);
     return QWN_CUDA_STATUS_INVALID_ARGUMENT;

@@ -1,6 +1,6 @@
-// The 5th-generation tensor core's instructions as the int8 product uses
-// them: TMA tile loads, TMEM, tcgen05.mma with kind::i8, and the cluster
-// operations around them.
+// The 5th-generation tensor core's instructions as the products and the tile
+// attention use them: TMA tile loads, TMEM, tcgen05.mma with kind::i8, and the
+// cluster operations around them.
 #pragma once
 
 #include <cuda.h>
@@ -88,6 +88,22 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *m
         "[%1, {%2, %3}], [%4];" ::"r"(dst),
         "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
+}
+
+// the driver's encoder, found once (the library does not link libcuda)
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess || found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
 }
 
 // ---- TMEM and the MMA -----------------------------------------------------------
