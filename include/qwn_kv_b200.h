@@ -418,6 +418,10 @@ QWN_CUDA_ABI_API int qwn_linear_attention_prefill_host(QwnLinearAttentionState *
  * Rows start on four values: 16 bytes for fp32, 8 for the 16-bit types, row
  * strides multiples of 4 (INVALID_ARGUMENT otherwise). */
 enum { QWN_ROTARY_HALVES = 0, QWN_ROTARY_NEIGHBOURS = 1 };
+/* The first t of the rotary_dim/2 pairs turn by the row's position on the first axis, the next h by that on the
+ * second, the last w by that on the third; multiples of 4 pairs.  A row with a position outside the table on an
+ * axis that has pairs is as one whose angle is outside it. */
+#define QWN_ROTARY_SECTIONS(t, h, w) ((uint32_t)(t) | (uint32_t)(h) << 8 | (uint32_t)(w) << 16)
 typedef struct {
     QwnCudaAbiHeader header;
     uint32_t layer, num_seqs;
@@ -427,7 +431,8 @@ typedef struct {
     const int32_t *first_pos_dev;   /* [num_seqs] cache position of each sequence's first row;
                                        NULL: the rows are the sequence's newest tokens */
     const int32_t *rotary_pos_dev;  /* [num_rows] table row of each row's angles, where it is not the
-                                       cache position (after an eviction); NULL: the cache position */
+                                       cache position (after an eviction); NULL: the cache position.
+                                       With rotary_sections [3][num_rows], one axis after another */
     uint32_t num_rows;
     uint32_t dtype;                 /* QwnDType of query, key and value */
     uint32_t query_heads;           /* multiple of kv_heads; 0: no query rows */
@@ -435,7 +440,8 @@ typedef struct {
     uint32_t rotary_dim;            /* multiple of 8 up to 128; 0: no rotation */
     uint32_t rotary_style;          /* QWN_ROTARY_* */
     uint32_t max_position;          /* rows of the table */
-    uint32_t reserved;
+    uint32_t rotary_sections;       /* QWN_ROTARY_SECTIONS, for positions on three axes (time, height, width of an image
+                                       or a video); 0: one axis */
     const float *rotations_dev;     /* [max_position][rotary_dim]: cosines of the rotary_dim/2 angles, then sines */
     uint64_t query_stride, key_stride, value_stride; /* values between rows; 0: heads x 128 */
     const void *query_dev;          /* [num_rows][query_heads][128] */

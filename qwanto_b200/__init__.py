@@ -67,6 +67,16 @@ _pack_rmsnorm_q8 = _lib.packer(_lib.RmsNormQ8Request)
 _pack_matmul_q8 = _lib.packer(_lib.MatmulQ8Request)
 
 
+def _sections(s) -> int:
+    """Pairs on three axes as a request has them; more than a byte each is refused there."""
+    if s is None:
+        return 0
+    t, h, w = s
+    if min(t, h, w) < 0 or max(t, h, w) > 255:
+        raise ValueError("rotary_sections are numbers of pairs")
+    return t | h << 8 | w << 16
+
+
 def _stream(s) -> int | None:
     if s is None:
         return None
@@ -215,14 +225,16 @@ class KvPool:
                       query_heads: int = 0, query_out=None, query_out_dtype: int = DTYPE_F32, rotations=None,
                       rotary_dim: int = 0, max_position: int = 0, neighbours: bool = False, row_begin=None,
                       first_pos=None, rotary_pos=None, seq_ids=None, query_stride: int = 0, key_stride: int = 0,
-                      value_stride: int = 0, stream=None) -> None:
+                      value_stride: int = 0, rotary_sections=None, stream=None) -> None:
         """Rotate the projection's rows by their positions, store K and V in
         their pages and Q in query_out (qwn_kv_append_rotary): one row per
         sequence, or with row_begin [num_seqs + 1] ragged runs of rows.
+        rotary_sections (t, h, w): so many pairs turn by the positions on each
+        of three axes, rotary_pos [3][num_rows].
         Strides are in values between rows (0: contiguous)."""
         rc = lib().qwn_kv_append_rotary(self._href, _pack_append_rotary(
             layer, num_seqs, _addr(seq_ids), _addr(row_begin), _addr(first_pos), _addr(rotary_pos), num_rows, dtype,
-            query_heads, query_out_dtype, rotary_dim, neighbours, max_position, 0, _addr(rotations), query_stride,
+            query_heads, query_out_dtype, rotary_dim, neighbours, max_position, _sections(rotary_sections), _addr(rotations), query_stride,
             key_stride, value_stride, _addr(query), _addr(key), _addr(value), _addr(query_out), _stream(stream) or 0))
         check("qwn_kv_append_rotary", rc)
 

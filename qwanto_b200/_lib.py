@@ -204,7 +204,7 @@ class AppendRotaryRequest(C.Structure):
                 ("row_begin_dev", C.c_void_p), ("first_pos_dev", C.c_void_p), ("rotary_pos_dev", C.c_void_p),
                 ("num_rows", C.c_uint32), ("dtype", C.c_uint32), ("query_heads", C.c_uint32),
                 ("query_out_dtype", C.c_uint32), ("rotary_dim", C.c_uint32), ("rotary_style", C.c_uint32),
-                ("max_position", C.c_uint32), ("reserved", C.c_uint32), ("rotations_dev", C.c_void_p),
+                ("max_position", C.c_uint32), ("rotary_sections", C.c_uint32), ("rotations_dev", C.c_void_p),
                 ("query_stride", C.c_uint64), ("key_stride", C.c_uint64), ("value_stride", C.c_uint64),
                 ("query_dev", C.c_void_p), ("key_dev", C.c_void_p), ("value_dev", C.c_void_p),
                 ("query_out_dev", C.c_void_p), ("stream", C.c_void_p)]

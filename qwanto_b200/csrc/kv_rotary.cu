@@ -10,6 +10,7 @@
 // sines s from a table row [c(0..r/2-1), s(0..r/2-1)], over the pairs (i, j) =
 // (p, p + r/2), or (2p, 2p + 1):
 //     x'[i] = x[i] c[p] - x[j] s[p],   x'[j] = x[j] c[p] + x[i] s[p]
+// (each pair from the table row of its axis' position, where there are three)
 // in fp32 with every product and sum rounded by itself, so that K's codes do
 // not depend on how the compiler contracts.
 //
@@ -167,6 +168,31 @@ __device__ __forceinline__ void store16(__nv_bfloat16 *row, int j, const Row16 &
                        pack_b2(r.v[8 * q + 4], r.v[8 * q + 5]), pack_b2(r.v[8 * q + 6], r.v[8 * q + 7]));
 }
 
+struct RotaryArgs {
+    RowMap rows;
+    const int32_t *rotary_pos;
+    const float *table;
+    uint32_t layer, query_heads, rot, max_position, query_out_dtype;
+    uint32_t sections;  // pairs on each of three axes, a byte each; 0: one axis
+    bool neighbours;
+    uint64_t query_stride, key_stride, value_stride;
+};
+
+// the axis of a pair
+__device__ __forceinline__ uint32_t axis_of(uint32_t sections, uint32_t p) {
+    const uint32_t first = sections & 255u, second = first + ((sections >> 8) & 255u);
+    return (p >= first) + (p >= second);
+}
+// a row's position on an axis
+__device__ __forceinline__ int32_t axis_pos(const RotaryArgs &a, uint32_t row, uint32_t axis) {
+    return a.rotary_pos[(size_t)axis * a.rows.num_rows + row];
+}
+// the table row that holds the angles of a row's pair p and the three beside it: sections are of 4 pairs,
+// so that 16 bytes of the table are on one axis
+__device__ __forceinline__ const float *table_row(const RotaryArgs &a, uint32_t row, int32_t angle, uint32_t p) {
+    if (a.sections) angle = axis_pos(a, row, axis_of(a.sections, p));
+    return a.table + (size_t)angle * a.rot;
+}
 // A row's rotation for this lane.  All 128 dims as halves: the pairs are (v[i],
 // v[i + 8]).  Neighbours: (v[2i], v[2i + 1]), where the eight dims are below
 // rotary_dim.  Both keep their angles for all heads of the row; halves of fewer
@@ -176,22 +202,25 @@ template <int MODE>
 struct Turn16 {
     float c[8], s[8];
     const float *row;
-    __device__ __forceinline__ void load(const float *r, int j, int rot) {
-        row = r;
+    // `at(p)`: the table row of pair p
+    template <class F>
+    __device__ __forceinline__ void load(F &&at, int j, int rot) {
+        row = at(0);
         if constexpr (MODE != kTurnPart) {
 #pragma unroll
             for (int q = 0; q < 2; q++) {
                 if (MODE == kTurnNeighbours && 64 * q + 8 * j >= rot) continue;
-                const float *at = MODE == kTurnWhole ? r + 8 * j + 4 * q : r + 32 * q + 4 * j;
-                const float4 x = *reinterpret_cast<const float4 *>(at);
-                const float4 y = *reinterpret_cast<const float4 *>(at + (rot >> 1));
+                const int p = MODE == kTurnWhole ? 8 * j + 4 * q : 32 * q + 4 * j;
+                const float *from = at(p) + p;
+                const float4 x = *reinterpret_cast<const float4 *>(from);
+                const float4 y = *reinterpret_cast<const float4 *>(from + (rot >> 1));
                 c[4 * q] = x.x, c[4 * q + 1] = x.y, c[4 * q + 2] = x.z, c[4 * q + 3] = x.w;
                 s[4 * q] = y.x, s[4 * q + 1] = y.y, s[4 * q + 2] = y.z, s[4 * q + 3] = y.w;
             }
         }
     }
     template <typename T>
-    __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot) const {
+    __device__ __forceinline__ void apply(Row16 &x, const T *from, int j, int rot, const RotaryArgs &a, uint32_t r) const {
         if (MODE == kTurnWhole) {  // turn_first and turn_second, the products two at a time
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
@@ -234,8 +263,9 @@ struct Turn16 {
             if (d >= rot) continue;
             const bool second = d >= half;
             const int p = second ? d - half : d;
-            const float4 cc = *reinterpret_cast<const float4 *>(row + p);
-            const float4 ss = *reinterpret_cast<const float4 *>(row + half + p);
+            const float *at = a.sections ? table_row(a, r, 0, p) : row;
+            const float4 cc = *reinterpret_cast<const float4 *>(at + p);
+            const float4 ss = *reinterpret_cast<const float4 *>(at + half + p);
             const float4 o = load4(from + (second ? p : d + half));
             const float cs[4] = {cc.x, cc.y, cc.z, cc.w}, sn[4] = {ss.x, ss.y, ss.z, ss.w}, y[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
@@ -471,19 +501,17 @@ __device__ __forceinline__ bool put_row<QWN_KV_CODEC_TQ35_G64>(uint8_t *tile, in
     return ok;
 }
 
-struct RotaryArgs {
-    RowMap rows;
-    const int32_t *rotary_pos;
-    const float *table;
-    uint32_t layer, query_heads, rot, max_position, query_out_dtype;
-    bool neighbours;
-    uint64_t query_stride, key_stride, value_stride;
-};
-
-// whether a row's angles are in the table
+// whether a row's angles are in the table, on all axes that have pairs
 __device__ __forceinline__ bool angle_ok(const StoreGeo &g, const RotaryArgs &a, int64_t pos, uint32_t row,
                                          int32_t &angle, bool tell) {
     if (!a.rot) return true;
+    if (a.sections) {
+        bool ok = true;
+#pragma unroll
+        for (uint32_t x = 0; x < 3; x++) ok &= !((a.sections >> (8 * x)) & 255u) || (uint32_t)axis_pos(a, row, x) < a.max_position;
+        if (!ok && tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
+        return ok;
+    }
     angle = a.rotary_pos ? a.rotary_pos[row] : (int32_t)pos;
     if (angle >= 0 && (uint32_t)angle < a.max_position) return true;
     if (tell) latch(g.status, QWN_KV_STATUS_BAD_LENGTH);
@@ -502,7 +530,8 @@ __device__ __forceinline__ void append_row(const StoreGeo &g, const RotaryArgs &
                                            int32_t angle, uint32_t row, uint32_t slot, float4 x, float4 v,
                                            void *query_out, int lane) {
     if (ok && a.rot) {
-        const Turn t = load_turn(a.table + (size_t)angle * a.rot, (int)a.rot, a.neighbours, lane);
+        const uint32_t half = a.rot >> 1, d = 4 * (uint32_t)lane, p = a.neighbours ? 2 * lane : d < half ? d : d - half;
+        const Turn t = load_turn(table_row(a, row, angle, p < half ? p : 0), (int)a.rot, a.neighbours, lane);
         x = rotate(x, t, a.neighbours);
     }
     if (slot < g.kv_heads) {
@@ -649,7 +678,7 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
     const bool ok = have && unit_row_ok(g, u.seq, u.len, u.pos + r, tell) && angle_ok(g, a, u.pos + r, row, angle, tell);
     const bool turns = ok && (MODE != kTurnPart || a.rot);
     Turn16<MODE> turn;
-    if (turns) turn.load(a.table + (size_t)angle * a.rot, j, (int)a.rot);
+    if (turns) turn.load([&](uint32_t p) { return table_row(a, row, angle, p); }, j, (int)a.rot);
     for (uint32_t q0 = 0; q0 < group; q0 += kAhead) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; i++) {
@@ -657,7 +686,7 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
             if (q >= group) break;
             if (ok) {
                 Row16 x = qw[i].row();
-                if (MODE != kTurnPart || a.rot) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot);
+                if (MODE != kTurnPart || a.rot) turn.apply(x, qr + q * kHeadDim, j, (int)a.rot, a, row);
                 // query_out may be query: the row's lanes have read their partners' values
                 if (MODE == kTurnPart) __syncwarp(0xFFu << (8 * (lane >> 3)));
                 put_query(row, q, x);
@@ -669,7 +698,7 @@ __global__ void __launch_bounds__(kTileThreads, 6) append_tiles_kernel(StoreGeo 
     }
     Row16 k = kw.row();
     const Row16 v = vw.row();
-    if (turns) turn.apply(k, kr, j, (int)a.rot);
+    if (turns) turn.apply(k, kr, j, (int)a.rot, a, row);
     if (CODEC == QWN_KV_CODEC_TQ35_G64)
         for (int i = threadIdx.x; i < kImage / 16; i += kTileThreads)
             reinterpret_cast<uint4 *>(buf)[i] = make_uint4(0, 0, 0, 0);
@@ -831,6 +860,12 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
     if (r->rotary_dim % 8 || r->rotary_dim > (uint32_t)kHeadDim || r->rotary_style > QWN_ROTARY_NEIGHBOURS ||
         (r->rotary_dim && (!r->rotations_dev || r->max_position == 0 || (uintptr_t)r->rotations_dev % 16)))
         return invalid("qwn_kv_append_rotary: rotary_dim must be a multiple of 8 up to 128 with a 16-byte aligned table");
+    if (r->rotary_sections) {
+        const uint32_t n[4] = {r->rotary_sections & 255u, (r->rotary_sections >> 8) & 255u, (r->rotary_sections >> 16) & 255u,
+                               r->rotary_sections >> 24};
+        if (n[3] || (n[0] | n[1] | n[2]) % 4 || 2 * (n[0] + n[1] + n[2]) != r->rotary_dim || !r->rotary_pos_dev)
+            return invalid("qwn_kv_append_rotary: sections are multiples of 4 pairs, rotary_dim / 2 in all, with rotary_pos_dev");
+    }
     if (r->query_heads && (r->query_heads % p->kv_heads || r->query_heads > p->max_query_heads || !r->query_dev ||
                            !r->query_out_dev || !dtype_ok(r->query_out_dtype)))
         return invalid("qwn_kv_append_rotary: query heads need query_dev, query_out_dev and the pool's limits");
@@ -864,6 +899,7 @@ QWN_CUDA_ABI_API int qwn_kv_append_rotary(QwnKvPoolHandle *h, const QwnKvAppendR
     a.rot = r->rotary_dim;
     a.max_position = r->max_position;
     a.query_out_dtype = r->query_out_dtype;
+    a.sections = r->rotary_sections;
     a.neighbours = r->rotary_style == QWN_ROTARY_NEIGHBOURS;
     a.query_stride = qs;
     a.key_stride = ks;
