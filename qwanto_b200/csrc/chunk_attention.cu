@@ -97,7 +97,7 @@ ChunkPlan plan_chunk(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32
 
 template <int SRC>
 cudaError_t launch_chunk(const Pool *p, const ChunkPlan &c, AtArgs &a, cudaStream_t s) {
-    const uint32_t ctas = a.slots ? (uint32_t)p->sms : (uint32_t)(c.units * p->kv_heads);
+    const uint32_t ctas = a.slots ? (uint32_t)p->sms : (uint32_t)std::min<uint64_t>(c.units * p->kv_heads, (uint64_t)p->sms);
     const CUtensorMap none{};
     auto run = [&](auto parts, auto tiles) {
         constexpr int P = decltype(parts)::value, T = decltype(tiles)::value;

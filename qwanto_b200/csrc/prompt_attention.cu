@@ -1,6 +1,8 @@
 // Attention of packed prompts over their own rows (qwn_prompt_attention), by the
 // tile kernel of prompt_tile.cuh.  16-bit keys and values go from the rows into
 // operand tiles by TMA; fp32 ones are cut into three bf16 parts on the way.
+#include <algorithm>
+
 #include "prompt_tile.cuh"
 
 namespace qkv {
@@ -63,6 +65,7 @@ QWN_CUDA_ABI_API int qwn_prompt_attention(const QwnPromptAttentionRequest *r) {
     DeviceScope scope(r->device_id);
     if (!scope.ok) return scope.fail("qwn_prompt_attention");
     const int sms = device_sms(r->device_id);
+    if (sms <= 0) return scope.fail("qwn_prompt_attention");
     AtArgs a{};
     a.rows = {nullptr, r->row_begin_dev, nullptr, r->num_seqs, r->num_rows};
     a.group = r->query_heads / r->kv_heads;
@@ -92,7 +95,7 @@ QWN_CUDA_ABI_API int qwn_prompt_attention(const QwnPromptAttentionRequest *r) {
     }
     cudaStream_t s = static_cast<cudaStream_t>(r->stream);
     const int d = r->device_id;
-    const uint32_t n = (uint32_t)ctas;
+    const uint32_t n = (uint32_t)std::min<uint64_t>(ctas, (uint64_t)sms);
     cudaError_t e;
     if (r->dtype == QWN_DTYPE_F32) e = launch_tile_kernel<0, 3, 1, true>(d, n, s, kmap, vmap, a);
     else if (r->dtype == QWN_DTYPE_BF16)

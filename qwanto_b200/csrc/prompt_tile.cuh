@@ -72,7 +72,7 @@ struct AtArgs {
     void *out;
     StoreGeo geo;              // paged
     uint32_t *status;
-    uint32_t units;            // one segment per CTA: (row tiles, kv heads)
+    uint32_t units;            // row tiles, without a split
     uint64_t *prefix;          // split: blocks before each sequence, then
     float *slots;              // the partial results
 };
@@ -119,14 +119,19 @@ struct AtShared {
     int give_up;
 };
 
-// bounded waits that also end when another role of the CTA has given up
+// Bounded waits that also end when another role of the CTA has given up.  The
+// answer is the whole warp's, so that its loops stay uniform: the roles that issue
+// copies and MMAs then have counters and descriptors in uniform registers (8192
+// rows of 32/8 heads: 570 us otherwise, of which the issue took most).
 __device__ __forceinline__ bool at_wait(AtShared &sh, uint64_t *bar, uint32_t parity) {
+    bool ok = false;
     for (uint32_t it = 0; it < kWaitLimit; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63) == 63 && *(volatile int *)&sh.give_up) return false;
+        ok = mbar_try_wait(bar, parity);
+        if (ok || ((it & 63) == 63 && *(volatile int *)&sh.give_up)) break;
     }
-    *(volatile int *)&sh.give_up = 1;
-    return false;
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) *(volatile int *)&sh.give_up = 1;
+    return ok;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -176,6 +181,24 @@ __device__ __forceinline__ void tmem_load64(uint32_t *r, uint32_t addr) {
         "tcgen05.wait::ld.sync.aligned;"
         : QKV_R64(r, 0)
         : "r"(addr)
+        : "memory");
+}
+// the same for 128 columns, in two loads behind one wait
+__device__ __forceinline__ void tmem_load128(uint32_t *r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63" "}, [%128];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127" "}, [%129];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : QKV_R64(r, 0), QKV_R64(r, 64)
+        : "r"(addr), "r"(addr + 64)
         : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *r) {
@@ -282,9 +305,10 @@ __device__ __forceinline__ uint32_t at_span(const AtArgs &a, const AtSequence &s
 
 // The CTA's segments, one after another, by one whole warp.
 //
-// Without a split a CTA has one: row tile u of (sequence, tile) pairs counted by
-// base_i = begin_i group / R + i, which covers any ragged batch without a table.
-// The last tiles see the most tokens and go first.
+// Without a split the CTAs take row tiles in turn, forth and back: tile u of
+// (sequence, tile) pairs counted by base_i = begin_i group / R + i, which covers
+// any ragged batch without a table.  A sequence's last tiles see the most tokens
+// and go first.
 //
 // With one, the blocks of all tiles in a row (sequence, tile, head, block) are cut
 // into as many equal runs as there are CTAs; a tile that a cut goes through is
@@ -357,8 +381,14 @@ struct AtWork {
     __device__ __forceinline__ AtSegment next() {
         AtSegment t{};
         if (!a.slots) {
-            if (n++) return t;
-            return single();
+            const uint64_t all = (uint64_t)a.units * a.kv_heads;
+            for (;;) {
+                const uint64_t k = (uint64_t)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                if ((uint64_t)n * gridDim.x >= all) return t;
+                n++;
+                if (k < all) t = single(a.units - 1 - (uint32_t)(k / a.kv_heads), (uint32_t)(k % a.kv_heads));
+                if (t.valid) return t;
+            }
         }
         while (at < end) {
             const uint64_t item = within / span, tiles = at_row_tiles(a, s, kRows);
@@ -383,9 +413,8 @@ struct AtWork {
         }
         return t;
     }
-    __device__ __forceinline__ AtSegment single() const {
+    __device__ __forceinline__ AtSegment single(uint32_t u, uint32_t head) const {
         AtSegment t{};
-        const uint32_t u = a.units - 1 - blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
         const uint32_t lane = threadIdx.x & 31;
         uint32_t lo = 0, count = a.rows.num_seqs;  // the last sequence whose base is not beyond u
         while (count > 1 && a.rows.row_begin) {
@@ -582,7 +611,7 @@ __device__ __forceinline__ void put_tile(const uint8_t *tile, int which, int ti,
 // A masked token must not matter, but 0 x inf is NaN in an MMA.  In blocks that
 // some rows see only in part, values that are not finite are therefore taken out of
 // the operand tile (tokens past the end altogether) and noted; the rows that do see
-// them get them added at the end (add_odd).  A CTA's rows span 256 tokens at most,
+// them get them added at the end (odd_sum).  A CTA's rows span 256 tokens at most,
 // so that such blocks span 512 from the first block on and 512 from `zone` on.
 __device__ __forceinline__ int32_t odd_zone(const AtSegment &t, int block) {
     return max(t.whole_hi, max(t.whole_lo, t.block0)) * block;
@@ -632,21 +661,23 @@ __device__ float at_value(const AtArgs &a, const AtSegment &seg, int32_t token, 
         return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.value)[at]);
     }
 }
-template <int SRC, int PARTS, int BLOCK, int N>
-__device__ __noinline__ void add_odd(const AtArgs &a, const AtShared &sh, const AtSegment &seg, uint32_t which, Seen seen,
-                                     int col, float *o) {
+// what the noted tokens that a row sees add to its sum in column d
+template <int SRC, int PARTS, int BLOCK>
+__device__ __noinline__ float odd_sum(const AtArgs &a, const AtShared &sh, const AtSegment &seg, uint32_t which, Seen seen, int d) {
+    float sum = 0.f;
+#pragma unroll 1
     for (int z = 0; z < 2; z++) {
         const int32_t from = z ? odd_zone(seg, BLOCK) : seg.block0 * BLOCK;
+#pragma unroll 1
         for (int w = 0; w < 16; w++)
             for (uint32_t bits = sh.odd_v[which][z][w]; bits; bits &= bits - 1) {
                 const int32_t token = from + 32 * w + __ffs(bits) - 1;
                 if (token < seen.lo || token >= seen.hi) continue;
-                for (int k = 0; k < N; k++) {
-                    const float v = at_value<SRC, PARTS>(a, seg, token, col + k);
-                    if (!isfinite(v)) o[k] += v;
-                }
+                const float v = at_value<SRC, PARTS>(a, seg, token, d);
+                if (!isfinite(v)) sum += v;
             }
     }
+    return sum;
 }
 
 // ---- softmax -------------------------------------------------------------------
@@ -658,6 +689,41 @@ template <bool BF16>
 struct AtRange {
     static constexpr float kBias = BF16 ? 0.f : 8.f, kSlack = BF16 ? 8.f : 6.f;
 };
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 2^t of two values without the special function unit, which does 16 a cycle and
+// SM: a block of 256 x 128 scores keeps it as busy as the tensor core.  t = n + f
+// with n whole and |f| <= 1/2; 2^f by the polynomial of least relative error on
+// that interval (found by exchange; degree 3: 7.5e-5, below bf16's half step of
+// 3.9e-3; degree 4: 2.6e-6, below fp16's 4.9e-4), times 2^n put together from its
+// exponent, which is zero at -127 and below.
+template <bool BF16>
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
+    float a, b;
+    unpair(t, a, b);
+    t = pair(max_nan(a, -127.f), max_nan(b, -127.f));
+    constexpr float kWhole = 12582912.f + 127.f;  // 1.5 x 2^23: the sum's low bits are n + 127
+    const uint64_t w = add2(t, pair(kWhole, kWhole));
+    const uint64_t f = add2(t, mul2(add2(w, pair(-kWhole, -kWhole)), pair(-1.f, -1.f)));
+    uint64_t y;
+    if constexpr (BF16) {
+        y = fma2(f, pair(0.05517166853f, 0.05517166853f), pair(0.2426111251f, 0.2426111251f));
+        y = fma2(y, f, pair(0.6932609677f, 0.6932609677f));
+        y = fma2(y, f, pair(0.9999280572f, 0.9999280572f));
+    } else {
+        y = fma2(f, pair(0.009570102207f, 0.009570102207f), pair(0.05591785908f, 0.05591785908f));
+        y = fma2(y, f, pair(0.2402474433f, 0.2402474433f));
+        y = fma2(y, f, pair(0.6931217909f, 0.6931217909f));
+        y = fma2(y, f, pair(0.9999992847f, 0.9999992847f));
+    }
+    uint32_t n0, n1;
+    unpair(w, n0, n1);
+    return mul2(y, pair(__uint_as_float(n0 << 23), __uint_as_float(n1 << 23)));
+}
 
 // `n` values of a row: 32-byte stores where the type fills them
 template <int N>
@@ -690,6 +756,7 @@ struct AtRoles {
     static constexpr bool kTokenScales = PARTS == 1 && Scale::kTokens;
     // the operands' own scaling: of scores and of outputs
     static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
+    static constexpr uint32_t kFmaPairs = 0x10;  // of eight pairs of powers, those that FMAs compute
     const AtArgs &a;
     AtShared &sh;
     uint32_t q_at, k_at, v_at, raw_at;  // shared memory
@@ -705,6 +772,10 @@ struct AtRoles {
         seg = sh.seg[s];
         warp_arrive(&sh.segempty[s], lane);
         f.n++;
+        // the same in all lanes, as the compiler can tell from this
+        auto one = [](int32_t &v) { v = __shfl_sync(0xffffffffu, v, 0); };
+        one(seg.valid), one(seg.rows), one(seg.seq), one(seg.head), one(seg.len), one(seg.block0), one(seg.blocks);
+        one(seg.whole_lo), one(seg.whole_hi), one(seg.slot);
         return seg.valid != 0;
     }
 
@@ -902,7 +973,7 @@ struct AtRoles {
     __device__ __forceinline__ void multiply() {
         Feed f;
         AtSegment seg;
-        const uint32_t tmem = sh.tmem;
+        const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
         const bool leader = elect_one();
         uint32_t done = 0, used = 0, o_uses[2] = {0, 0}, p_uses[2] = {0, 0}, fixes[2] = {0, 0}, wholes[2] = {0, 0};
         constexpr uint32_t kQk = f16_desc(BF16 || PARTS == 3, S::kBlock, false), kPv = f16_desc(BF16 || PARTS == 3, 128, true);
@@ -914,9 +985,9 @@ struct AtRoles {
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
                 const uint64_t qd = smem_desc(q + kFirst[p] * kAtRows * 256), kd = smem_desc(k + kSecond[p] * S::kKvPart);
+                if (leader)
 #pragma unroll
-                for (int c = 0; c < 8; c++)
-                    if (leader)
+                    for (int c = 0; c < 8; c++)
                         mma_ss(tmem + t * S::kSColumns, qd + (c >> 2) * (kAtRows * 128 / 16) + (c & 3) * 2,
                                kd + (c >> 2) * (S::kBlock * 128 / 16) + (c & 3) * 2, kQk, p + c > 0);
             }
@@ -926,9 +997,9 @@ struct AtRoles {
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
                 const uint64_t vd = rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
+                if (leader)
 #pragma unroll
-                for (int c = 0; c < S::kBlock / 16; c++)
-                    if (leader)
+                    for (int c = 0; c < S::kBlock / 16; c++)
                         mma_ts(tmem + S::kOColumn + t * 128, tmem + t * S::kSColumns + kFirst[p] * (S::kBlock / 2) + c * 8,
                                vd + c * (2048 / 16), kPv, add || p + c > 0);
             }
@@ -1029,27 +1100,34 @@ struct AtRoles {
         using Range = AtRange<BF16 || PARTS == 3>;
         uint32_t u[N];
         float *x = reinterpret_cast<float *>(u);
-        tmem_load64(u, s_col);
-        if constexpr (N == 128) tmem_load64(u + 64, s_col + 64);
+        if constexpr (N == 128) tmem_load128(u, s_col);
+        else tmem_load64(u, s_col);
         float vtop = 0.f;
         if constexpr (kTokenScales) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
                 const float4 k = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i]);
-                x[i] *= k.x, x[i + 1] *= k.y, x[i + 2] *= k.z, x[i + 3] *= k.w;
+                unpair(mul2(pair(x[i], x[i + 1]), pair(k.x, k.y)), x[i], x[i + 1]);
+                unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k.z, k.w)), x[i + 2], x[i + 3]);
             }
             const float4 v0 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][0]), v1 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][4]);
             vtop = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)), fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
         }
-        if (!whole(seg, blk)) {
+        const bool full = whole(seg, blk);
+        if (!full) {
             const int lo = seen.lo - blk * N, hi = seen.hi - blk * N;
 #pragma unroll
             for (int i = 0; i < N; i++)
                 if (i < lo || i >= hi) x[i] = -INFINITY;
         }
-        float top = x[0];
+        float t[8];
 #pragma unroll
-        for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+        for (int i = 0; i < 8; i++) t[i] = x[i];
+#pragma unroll
+        for (int i = 8; i < N; i += 8)
+#pragma unroll
+            for (int k = 0; k < 8; k++) t[k] = fmaxf(t[k], x[i + k]);
+        const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
         const float reach = top * c + vtop;
         const bool grows = have && reach > M + Range::kSlack;  // true for the first that is not -inf
         if (__any_sync(0xffffffffu, grows)) {
@@ -1070,15 +1148,40 @@ struct AtRoles {
             }
         }
         const float off = Range::kBias - (M == -INFINITY ? 0.f : M);
-        float l0 = 0.f, l1 = 0.f;
+        // masked scores are -inf, whose power is exactly zero in the special function unit only
+        if (PARTS == 1 && full) l += powers<true>(x, slot, c, off, s_col);
+        else l += powers<false>(x, slot, c, off, s_col);
+        tmem_store_wait();
+    }
+
+    // P = 2^(c x + off) into tensor memory; returns their sum.  With MIXED some pairs of eight are computed
+    // by FMAs.
+    template <bool MIXED>
+    __device__ __forceinline__ float powers(const float *x, uint32_t slot, float c, float off, uint32_t s_col) {
+        constexpr int N = S::kBlock;
+        const uint64_t cc = pair(c, c), oo = pair(off, off);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < N; i += 32) {
             uint32_t p[PARTS][16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-                const float e0 = ex2(fmaf(x[i + k], c, off)), e1 = ex2(fmaf(x[i + k + 1], c, off));
-                l0 += e0;
-                l1 += e1;
+                const uint64_t t = fma2(pair(x[i + k], x[i + k + 1]), cc, oo);
+                uint64_t e;
+                if (MIXED && (kFmaPairs >> ((k >> 1) & 7) & 1)) {
+                    e = exp2_pair<BF16>(t);
+                } else {
+                    float t0, t1;
+                    unpair(t, t0, t1);
+                    e = pair(ex2(t0), ex2(t1));
+                }
+                sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
+                float e0, e1;
+                if constexpr (kTokenScales) {
+                    const float2 v = *reinterpret_cast<const float2 *>(&sh.vscale[slot][i + k]);
+                    e = mul2(e, pair(v.x, v.y));
+                }
+                unpair(e, e0, e1);
                 if constexpr (PARTS == 3) {
                     const uint32_t a0 = __float_as_uint(e0), a1 = __float_as_uint(e1);
                     const float f0 = e0 - __uint_as_float(a0 & 0xFFFF0000u), f1 = e1 - __uint_as_float(a1 & 0xFFFF0000u);
@@ -1090,9 +1193,6 @@ struct AtRoles {
                 } else if constexpr (BF16) {
                     const __nv_bfloat162 v = __floats2bfloat162_rn(e0, e1);
                     p[0][k >> 1] = *reinterpret_cast<const uint32_t *>(&v);
-                } else if constexpr (kTokenScales) {
-                    const float2 v = *reinterpret_cast<const float2 *>(&sh.vscale[slot][i + k]);
-                    p[0][k >> 1] = pack_h2(e0 * v.x, e1 * v.y);
                 } else {
                     p[0][k >> 1] = pack_h2(e0, e1);
                 }
@@ -1100,14 +1200,16 @@ struct AtRoles {
 #pragma unroll
             for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (N / 2) + i / 2, p[k]);
         }
-        l += l0 + l1;
-        tmem_store_wait();
+        float l[4];
+        unpair(sum[0], l[0], l[1]);
+        unpair(sum[1], l[2], l[3]);
+        return (l[0] + l[1]) + (l[2] + l[3]);
     }
 
     // the rows of a segment: to the output, or to the workspace where other CTAs have a share of them
     __device__ __forceinline__ bool finish(const AtSegment &seg, uint32_t used, bool have, bool any, uint32_t r, const Seen &seen,
                                            int g, uint32_t lanes, float M, float l, uint32_t (&o_uses)[2], uint32_t &joins) {
-        constexpr int kWide = 32;  // columns at a time
+        constexpr int kWide = 16;  // columns at a time
         const uint32_t o_at = lanes + S::kOColumn;
         float w0 = 1.f, w1 = 0.f;
         const bool two = TILES == 1 && seg.blocks > 1;
@@ -1142,35 +1244,38 @@ struct AtRoles {
             const uint32_t row = seg.row0 + (have ? r : 0), token = row / a.group, h = seg.head * a.group + row % a.group;
             const uint64_t at = (uint64_t)(seg.token_row + token) * a.out_stride + h * kHeadDim;
             float *slot = seg.slot < 0 ? nullptr : a.slots + (size_t)seg.slot * at_slot_floats(TILES);
-            const float per = l > 0.f || l != l ? kUnit / l : 0.f;
+            const float per = slot ? kUnit : l > 0.f || l != l ? kUnit / l : 0.f;
             const int from = TILES == 1 ? g * 64 : 0, to = TILES == 1 ? from + 64 : 128;
+            // a short loop: this code runs once a segment, and a long one waits for its instructions
 #pragma unroll 1
             for (int col = from; col < to; col += kWide) {
                 float o[kWide];
-                uint32_t u[kWide];
                 if (seg.blocks) {
-                    tmem_load32(u, o_at + (TILES == 2 ? g * 128 : 0) + col);
+                    uint32_t u[kWide];
+                    tmem_load16(u, o_at + (TILES == 2 ? g * 128 : 0) + col);
 #pragma unroll
-                    for (int k = 0; k < kWide; k++) o[k] = w0 == 1.f ? __uint_as_float(u[k]) : w0 == 0.f ? 0.f : __uint_as_float(u[k]) * w0;
+                    for (int k = 0; k < kWide; k++) o[k] = TILES == 2 ? __uint_as_float(u[k]) : w0 == 0.f ? 0.f : __uint_as_float(u[k]) * w0;
                     if (two) {
-                        tmem_load32(u, o_at + 128 + col);
+                        tmem_load16(u, o_at + 128 + col);
 #pragma unroll
                         for (int k = 0; k < kWide; k++)
                             if (w1 != 0.f) o[k] = fmaf(__uint_as_float(u[k]), w1, o[k]);
                     }
-                    if (odd && have) add_odd<SRC, PARTS, S::kBlock, kWide>(a, sh, seg, used & 3, seen, col, o);
+                    if (odd)
+#pragma unroll
+                        for (int k = 0; k < kWide; k++) o[k] += odd_sum<SRC, PARTS, S::kBlock>(a, sh, seg, used & 3, seen, col + k);
                 } else {
 #pragma unroll
                     for (int k = 0; k < kWide; k++) o[k] = 0.f;
                 }
                 if (!have) continue;
+#pragma unroll
+                for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
                 if (slot) {
 #pragma unroll
                     for (int k = 0; k < kWide; k += 4)
-                        store4(slot + (size_t)r * kHeadDim + col + k, make_float4(o[k] * kUnit, o[k + 1] * kUnit, o[k + 2] * kUnit, o[k + 3] * kUnit));
+                        store4(slot + (size_t)r * kHeadDim + col + k, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
                 } else {
-#pragma unroll
-                    for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
                     store_values<kWide>(a.out, at + col, a.dtype, o);
                 }
             }
