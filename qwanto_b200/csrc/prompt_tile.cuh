@@ -88,14 +88,25 @@ struct AtShape {
     static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
     static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
     static constexpr uint32_t kKvBytes = kKvPart * PARTS;
-    static constexpr int kStagesK = PARTS == 1 ? 2 : 1;
-    static constexpr int kStagesV = PARTS == 1 && !(kPaged && TILES == 2) ? 2 : 1;
-    static constexpr uint32_t kOperands = TILES * kQBytes + (kStagesK + kStagesV) * kKvBytes;
-    static constexpr uint32_t kSmem = 227 * 1024 - 12 * 1024;      // the rest is static
+    // Stages of K and V: loaded ones are a ring that both go through in turn, K0 V0 K1 V1 ..; converted ones
+    // are apart, so that K of the next block does not wait behind V of this one.
+    static constexpr uint32_t kRing = kTma ? 5 : 0;
+    static constexpr uint32_t kStagesK = PARTS == 1 ? 2 : 1;
+    static constexpr uint32_t kStagesV = PARTS == 1 && !(kPaged && TILES == 2) ? 2 : 1;
+    static constexpr uint32_t kStages = kRing ? kRing : kStagesK + kStagesV;
+    static constexpr uint32_t kOperands = TILES * kQBytes + kStages * kKvBytes;
+    static constexpr uint32_t kSmem = (227 - (!kTma ? 12 : TILES == 2 ? 2 : 8)) * 1024;  // the rest is static
+    // where K and V of the d-th block go, and for which time
+    __device__ static constexpr uint32_t k_slot(uint32_t d) { return kRing ? 2 * d % (kRing ? kRing : 1) : d % kStagesK; }
+    __device__ static constexpr uint32_t k_turn(uint32_t d) { return kRing ? 2 * d / (kRing ? kRing : 1) : d / kStagesK; }
+    __device__ static constexpr uint32_t v_slot(uint32_t d) {
+        return kRing ? (2 * d + 1) % (kRing ? kRing : 1) : kStagesK + d % kStagesV;
+    }
+    __device__ static constexpr uint32_t v_turn(uint32_t d) { return kRing ? (2 * d + 1) / (kRing ? kRing : 1) : d / kStagesV; }
     static constexpr uint32_t kTileBytes = (uint32_t)tile_bytes_of(SRC);
     static constexpr uint32_t kRawAll = kRaw ? (kSmem - 1024 - kOperands) / (kRaw ? kTileBytes : 1) : 0;
     static constexpr uint32_t kRawTiles = kRawAll > 32 ? 32 : kRawAll;
-    static_assert(kOperands + 1024 <= kSmem, "operands fit");
+    static_assert(kOperands + (kTma ? 0 : 1024) <= kSmem, "operands fit");
     // K of a block is converted before its V, so all its tiles are there at once
     static_assert(!kRaw || kRawTiles >= (uint32_t)kTiles, "a block's cached tiles fit");
     // tensor memory: S and P share columns; P has 16-bit pairs, PARTS of them
@@ -103,18 +114,22 @@ struct AtShape {
     static_assert(kOColumn + 2 * 128 <= 512, "tensor memory");
 };
 
+constexpr uint32_t kAtStages = 5;
+template <int SRC, int PARTS, int TILES>
 struct AtShared {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2];
-    uint64_t vpart[2], vfixed[2];  // TMA: values of a block seen in part have landed, are ready
-    uint64_t qfull, qempty, sfull[2], pready[2], ofull[2], oempty[2], joined, helped, drained;
-    uint64_t segfull[2], segempty[2], rawfull[32], rawempty[32];
+    static constexpr bool kTokens = PARTS == 1 && (SRC == QWN_KV_CODEC_Q8_B64_F32 || SRC == QWN_KV_CODEC_Q8_HEAD_F16);
+    static constexpr int kRaw = SRC == 0 ? 1 : 32;
+    // operands of K and V have landed, are free again; V of a block seen in part (loaded ones only): has landed, is ready
+    uint64_t full[kAtStages], empty[kAtStages], part[kAtStages], fixed[kAtStages];
+    uint64_t qfull, qempty, sfull[2], pready[2][2], ofull[2], oempty[2], joined, helped, drained;
+    uint64_t segfull[2], segempty[2], rawfull[kRaw], rawempty[kRaw];
     AtSegment seg[2];
-    alignas(16) float kscale[4][128];      // of a block's tokens; read four at a time
-    alignas(16) float vscale[4][128];
-    alignas(16) float vtop[4][8];                      // log2 of a bound on a cached tile's value scales
-    float ml[2][2][kAtRows][2];            // TILES 1: M and l of both groups' rows, by segment parity
-    float qscale[2][2 * kAtRows];          // what a row of Q was divided by, by segment parity
-    uint32_t odd_v[4][2][16];              // tokens with values that are not finite, in blocks seen in part
+    alignas(16) float kscale[kTokens ? 4 : 1][kTokens ? 128 : 4];  // of a block's tokens; read four at a time
+    alignas(16) float vscale[kTokens ? 4 : 1][kTokens ? 128 : 4];
+    alignas(16) float vtop[4][8];                  // log2 of a bound on a cached tile's value scales
+    float ml[2][2][TILES == 1 ? kAtRows : 1][2];   // M and l of both groups' rows, by segment parity
+    float qscale[2][SRC && PARTS == 1 ? TILES * kAtRows : 1];  // what a row of Q was divided by, by segment parity
+    uint32_t odd_v[4][2][16];                      // tokens with values that are not finite, in blocks seen in part
     uint32_t tmem;
     int give_up;
 };
@@ -123,14 +138,14 @@ struct AtShared {
 // answer is the whole warp's, so that its loops stay uniform: the roles that issue
 // copies and MMAs then have counters and descriptors in uniform registers (8192
 // rows of 32/8 heads: 570 us otherwise, of which the issue took most).
-__device__ __forceinline__ bool at_wait(AtShared &sh, uint64_t *bar, uint32_t parity) {
+__device__ __forceinline__ bool at_wait(volatile int &give_up, uint64_t *bar, uint32_t parity) {
     bool ok = false;
     for (uint32_t it = 0; it < kWaitLimit; ++it) {
         ok = mbar_try_wait(bar, parity);
-        if (ok || ((it & 63) == 63 && *(volatile int *)&sh.give_up)) break;
+        if (ok || ((it & 63) == 63 && give_up)) break;
     }
     ok = __all_sync(0xffffffffu, ok);
-    if (!ok) *(volatile int *)&sh.give_up = 1;
+    if (!ok) give_up = 1;
     return ok;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
@@ -623,7 +638,7 @@ __device__ __forceinline__ bool odd_word(uint32_t w, bool bf16, uint32_t &out) {
     return lo || hi;
 }
 template <int PARTS, int BLOCK>
-__device__ void clear_odd(AtShared &sh, const AtSegment &seg, int32_t token0, uint32_t base, bool bf16, uint32_t which) {
+__device__ void clear_odd(uint32_t (&noted)[2][16], const AtSegment &seg, int32_t token0, uint32_t base, bool bf16) {
     const uint32_t tid = threadIdx.x & 127, r = tid % BLOCK, c0 = tid / BLOCK * (BLOCK / 8);
     const int32_t token = token0 + (int32_t)r;
     const bool past = token >= seg.len;
@@ -645,7 +660,7 @@ __device__ void clear_odd(AtShared &sh, const AtSegment &seg, int32_t token0, ui
     if (odd) {
         const int32_t z = odd_zone(seg, BLOCK);
         const uint32_t i = (uint32_t)(token < z ? token - seg.block0 * BLOCK : token - z);
-        if (i < 512) atomicOr(&sh.odd_v[which][token < z ? 0 : 1][i >> 5], 1u << (i & 31));
+        if (i < 512) atomicOr(&noted[token < z ? 0 : 1][i >> 5], 1u << (i & 31));
     }
 }
 // value d of a token
@@ -663,14 +678,14 @@ __device__ float at_value(const AtArgs &a, const AtSegment &seg, int32_t token, 
 }
 // what the noted tokens that a row sees add to its sum in column d
 template <int SRC, int PARTS, int BLOCK>
-__device__ __noinline__ float odd_sum(const AtArgs &a, const AtShared &sh, const AtSegment &seg, uint32_t which, Seen seen, int d) {
+__device__ __noinline__ float odd_sum(const AtArgs &a, const uint32_t (&noted)[2][16], const AtSegment &seg, Seen seen, int d) {
     float sum = 0.f;
 #pragma unroll 1
     for (int z = 0; z < 2; z++) {
         const int32_t from = z ? odd_zone(seg, BLOCK) : seg.block0 * BLOCK;
 #pragma unroll 1
         for (int w = 0; w < 16; w++)
-            for (uint32_t bits = sh.odd_v[which][z][w]; bits; bits &= bits - 1) {
+            for (uint32_t bits = noted[z][w]; bits; bits &= bits - 1) {
                 const int32_t token = from + 32 * w + __ffs(bits) - 1;
                 if (token < seen.lo || token >= seen.hi) continue;
                 const float v = at_value<SRC, PARTS>(a, seg, token, d);
@@ -758,9 +773,14 @@ struct AtRoles {
     static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
     static constexpr uint32_t kFmaPairs = 0x10;  // of eight pairs of powers, those that FMAs compute
     const AtArgs &a;
-    AtShared &sh;
-    uint32_t q_at, k_at, v_at, raw_at;  // shared memory
+    AtShared<SRC, PARTS, TILES> &sh;
+    uint32_t q_at, kv_at, raw_at;  // shared memory
     int warp, lane;
+
+    __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) const {
+        return at_wait(*(volatile int *)&sh.give_up, bar, parity);
+    }
+    __device__ __forceinline__ uint32_t slot_at(uint32_t slot) const { return kv_at + slot * S::kKvBytes; }
 
     // the next segment, for a warp that works on all of them
     struct Feed {
@@ -768,7 +788,7 @@ struct AtRoles {
     };
     __device__ __forceinline__ bool take(Feed &f, AtSegment &seg) {
         const uint32_t s = f.n & 1;
-        if (!at_wait(sh, &sh.segfull[s], (f.n >> 1) & 1)) return false;
+        if (!wait(&sh.segfull[s], (f.n >> 1) & 1)) return false;
         seg = sh.seg[s];
         warp_arrive(&sh.segempty[s], lane);
         f.n++;
@@ -784,7 +804,7 @@ struct AtRoles {
         for (uint32_t n = 0;; n++) {
             const uint32_t s = n & 1;
             const AtSegment seg = work.next();
-            if (!at_wait(sh, &sh.segempty[s], ((n >> 1) & 1) ^ 1)) return;
+            if (!wait(&sh.segempty[s], ((n >> 1) & 1) ^ 1)) return;
             if (lane == 0) sh.seg[s] = seg;
             warp_arrive(&sh.segfull[s], lane);
             if (!seg.valid) return;
@@ -795,27 +815,27 @@ struct AtRoles {
         Feed f;
         AtSegment seg;
         uint32_t done = 0;  // blocks, or cached tiles
-        uint32_t v_uses[2][2] = {};
+        uint32_t phase[2] = {}, issued[2] = {};  // a bit per slot: of full and part, the phase that the next copy fills
         bool ok = true;
         while (ok && take(f, seg)) {
             if constexpr (S::kTma) {
                 for (int b = 0; b < seg.blocks && ok; b++, done++) {
                     const int y = (int)seg.token_row + (seg.block0 + b) * S::kBlock, x = seg.head * kHeadDim;
-                    auto fetch = [&](uint64_t *full, uint64_t *empty, uint32_t use, uint32_t at, const CUtensorMap *map) {
-                        if (!at_wait(sh, empty, (use & 1) ^ 1)) return false;
+                    auto fetch = [&](uint64_t *full, uint32_t slot, uint32_t turn, const CUtensorMap *map) {
+                        if (!wait(&sh.empty[slot], (turn & 1) ^ 1)) return false;
                         if (lane == 0) {
-                            mbar_expect_tx(full, S::kKvBytes);
-                            tma_load(at, map, x, y, smem_u32(full));
-                            tma_load(at + S::kBlock * 128, map, x + 64, y, smem_u32(full));
+                            mbar_expect_tx(&full[slot], S::kKvBytes);
+                            tma_load(slot_at(slot), map, x, y, smem_u32(&full[slot]));
+                            tma_load(slot_at(slot) + S::kBlock * 128, map, x + 64, y, smem_u32(&full[slot]));
                         }
                         __syncwarp();
+                        const uint32_t kind = full == sh.part;
+                        phase[kind] ^= 1u << slot;
+                        issued[kind] |= 1u << slot;
                         return true;
                     };
-                    const uint32_t ks = done % S::kStagesK, vs = done % S::kStagesV;
-                    const bool part = !whole(seg, seg.block0 + b);
-                    ok = fetch(&sh.kfull[ks], &sh.kempty[ks], done / S::kStagesK, k_at + ks * S::kKvBytes, kmap) &&
-                         fetch(part ? &sh.vpart[vs] : &sh.vfull[vs], &sh.vempty[vs], done / S::kStagesV, v_at + vs * S::kKvBytes, vmap);
-                    v_uses[part ? 1 : 0][vs] += ok;
+                    ok = fetch(sh.full, S::k_slot(done), S::k_turn(done), kmap) &&
+                         fetch(whole(seg, seg.block0 + b) ? sh.full : sh.part, S::v_slot(done), S::v_turn(done), vmap);
                 }
             } else if constexpr (S::kRaw) {
                 auto address = [&](int b) -> const uint8_t * {
@@ -828,7 +848,7 @@ struct AtRoles {
                     ahead = address(b + 1);  // the next block's pages are looked up while this one's tiles go out
                     for (int t = 0; t < S::kTiles && ok; t++, done++) {
                         const uint32_t s = done % S::kRawTiles;
-                        ok = at_wait(sh, &sh.rawempty[s], ((done / S::kRawTiles) & 1) ^ 1);
+                        ok = wait(&sh.rawempty[s], ((done / S::kRawTiles) & 1) ^ 1);
                         if (ok && lane == t) {
                             if (from) {
                                 mbar_expect_tx(&sh.rawfull[s], S::kTileBytes);
@@ -848,11 +868,9 @@ struct AtRoles {
         }
         // copies in flight end before the CTA's memory goes, whoever gave up
         if constexpr (S::kTma) {
-            for (uint32_t d = done > S::kStagesK ? done - S::kStagesK : 0; d < done; d++)
-                mbar_wait_bounded(&sh.kfull[d % S::kStagesK], (d / S::kStagesK) & 1);
-            for (uint32_t v = 0; v < 2; v++) {
-                if (v_uses[0][v]) mbar_wait_bounded(&sh.vfull[v], (v_uses[0][v] - 1) & 1);
-                if (v_uses[1][v]) mbar_wait_bounded(&sh.vpart[v], (v_uses[1][v] - 1) & 1);
+            for (uint32_t v = 0; v < S::kRing; v++) {
+                if (issued[0] >> v & 1) mbar_wait_bounded(&sh.full[v], (phase[0] >> v & 1) ^ 1);
+                if (issued[1] >> v & 1) mbar_wait_bounded(&sh.part[v], (phase[1] >> v & 1) ^ 1);
             }
         } else if constexpr (S::kRaw) {
             for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++)
@@ -865,25 +883,24 @@ struct AtRoles {
     // the helpers' four warps meet; a wait like the others, so that it ends when one of them has given up
     __device__ __forceinline__ bool helpers_sync(uint32_t &syncs) {
         warp_arrive(&sh.helped, lane);
-        return at_wait(sh, &sh.helped, syncs++ & 1);
+        return wait(&sh.helped, syncs++ & 1);
     }
     // K and V of a block out of cached tiles or fp32 rows
     __device__ __forceinline__ bool convert(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
         const int w = warp & 3;
         const int32_t token0 = blk * S::kBlock;
-        const uint32_t ks = done % S::kStagesK, vs = done % S::kStagesV, slot = done & 3;
-        const uint32_t kd = k_at + ks * S::kKvBytes, vd = v_at + vs * S::kKvBytes;
+        const uint32_t slot = done & 3;
 #pragma unroll
         for (int which = 0; which < 2; which++) {
-            const uint32_t stages = which ? S::kStagesV : S::kStagesK, s = which ? vs : ks, dst = which ? vd : kd;
-            if (!at_wait(sh, which ? &sh.vempty[s] : &sh.kempty[s], ((done / stages) & 1) ^ 1)) return false;
+            const uint32_t s = which ? S::v_slot(done) : S::k_slot(done), dst = slot_at(s);
+            if (!wait(&sh.empty[s], ((which ? S::v_turn(done) : S::k_turn(done)) & 1) ^ 1)) return false;
             for (int ti = w; ti < S::kTiles; ti += 4) {
                 const int32_t at = token0 + ti * kTileTokens;
                 if constexpr (S::kPaged) {
                     const uint8_t *tile = nullptr;
                     if constexpr (S::kRaw) {
                         const uint32_t g = done * S::kTiles + ti, r = g % S::kRawTiles;
-                        if (!which && !at_wait(sh, &sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
+                        if (!which && !wait(&sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
                         extern __shared__ uint8_t dynamic[];
                         tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
                     } else if (at < seg.len) {
@@ -923,10 +940,10 @@ struct AtRoles {
             }
             if (which && !whole(seg, blk)) {
                 if (!helpers_sync(syncs)) return false;
-                clear_odd<PARTS, S::kBlock>(sh, seg, token0, dst, PARTS == 3, segment & 3);
+                clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
             }
             fence_proxy_async_shared();
-            warp_arrive(which ? &sh.vfull[s] : &sh.kfull[s], lane);
+            warp_arrive(&sh.full[s], lane);
         }
         return true;
     }
@@ -935,11 +952,11 @@ struct AtRoles {
         Feed f;
         AtSegment seg;
         uint32_t done = 0, used = 0, syncs = 0;  // blocks, segments with any
-        uint32_t parts[2] = {};
+        uint32_t phase = 0;  // of part, a bit per slot
         const uint32_t tid = threadIdx.x & 127;
         while (take(f, seg)) {
             if (seg.blocks == 0) continue;
-            if (!at_wait(sh, &sh.qempty, (used & 1) ^ 1)) return;
+            if (!wait(&sh.qempty, (used & 1) ^ 1)) return;
             if (tid < 32) sh.odd_v[used & 3][tid >> 4][tid & 15] = 0;
 #pragma unroll
             for (int t = 0; t < TILES; t++) {
@@ -947,7 +964,7 @@ struct AtRoles {
                 if ((int32_t)r < seg.rows) {
                     float unit;
                     put_q<SRC, PARTS>(a, seg, r, q_at + t * S::kQBytes, unit);
-                    sh.qscale[used & 1][r] = unit;
+                    if (SRC && PARTS == 1) sh.qscale[used & 1][r] = unit;
                 }
             }
             fence_proxy_async_shared();
@@ -958,11 +975,12 @@ struct AtRoles {
                 if constexpr (!S::kTma) {
                     if (!convert(seg, blk, done, used, syncs)) return;
                 } else if (!whole(seg, blk)) {
-                    const uint32_t s = done % S::kStagesV;
-                    if (!at_wait(sh, &sh.vpart[s], parts[s]++ & 1)) return;
-                    clear_odd<PARTS, S::kBlock>(sh, seg, blk * S::kBlock, v_at + s * S::kKvBytes, BF16, used & 3);
+                    const uint32_t s = S::v_slot(done);
+                    if (!wait(&sh.part[s], phase >> s & 1)) return;
+                    phase ^= 1u << s;
+                    clear_odd<PARTS, S::kBlock>(sh.odd_v[used & 3], seg, blk * S::kBlock, slot_at(s), BF16);
                     fence_proxy_async_shared();
-                    warp_arrive(&sh.vfixed[s], lane);
+                    warp_arrive(&sh.fixed[s], lane);
                 }
             }
             used++;
@@ -975,13 +993,14 @@ struct AtRoles {
         AtSegment seg;
         const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
         const bool leader = elect_one();
-        uint32_t done = 0, used = 0, o_uses[2] = {0, 0}, p_uses[2] = {0, 0}, fixes[2] = {0, 0}, wholes[2] = {0, 0};
+        uint32_t done = 0, used = 0, o_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+        uint32_t phase[2] = {};  // loaded operands: of full and fixed, a bit per slot
         constexpr uint32_t kQk = f16_desc(BF16 || PARTS == 3, S::kBlock, false), kPv = f16_desc(BF16 || PARTS == 3, 128, true);
         // the products of parts that count, the small ones first
         constexpr int kPairs = PARTS == 1 ? 1 : 6;
         constexpr int kFirst[6] = {PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
-        auto scores = [&](int t, uint32_t stage) {  // S_t = Q K^T
-            const uint32_t q = q_at + (TILES == 2 ? t * S::kQBytes : 0), k = k_at + stage * S::kKvBytes;
+        auto scores = [&](int t, uint32_t slot) {  // S_t = Q K^T
+            const uint32_t q = q_at + (TILES == 2 ? t * S::kQBytes : 0), k = slot_at(slot);
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
                 const uint64_t qd = smem_desc(q + kFirst[p] * kAtRows * 256), kd = smem_desc(k + kSecond[p] * S::kKvPart);
@@ -992,14 +1011,17 @@ struct AtRoles {
                                kd + (c >> 2) * (S::kBlock * 128 / 16) + (c & 3) * 2, kQk, p + c > 0);
             }
         };
-        auto values = [&](int t, uint32_t stage, bool add) {  // O_t += P_t V
-            const uint32_t v = v_at + stage * S::kKvBytes;
+        // O_t += P_t V for half the tokens (16-bit operands, so that the products start while the other half's
+        // powers are computed) or all
+        constexpr int kHalves = PARTS == 1 ? 2 : 1, kSteps = S::kBlock / 16 / kHalves;
+        auto values = [&](int t, uint32_t slot, bool add, int half) {
+            const uint32_t v = slot_at(slot);
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
                 const uint64_t vd = rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
                 if (leader)
 #pragma unroll
-                    for (int c = 0; c < S::kBlock / 16; c++)
+                    for (int c = half * kSteps; c < (half + 1) * kSteps; c++)
                         mma_ts(tmem + S::kOColumn + t * 128, tmem + t * S::kSColumns + kFirst[p] * (S::kBlock / 2) + c * 8,
                                vd + c * (2048 / 16), kPv, add || p + c > 0);
             }
@@ -1007,21 +1029,38 @@ struct AtRoles {
         auto commit = [&](uint64_t *bar) {
             if (leader) mma_commit(bar);
         };
-        auto wait_k = [&](uint32_t d) { return at_wait(sh, &sh.kfull[d % S::kStagesK], (d / S::kStagesK) & 1); };
+        auto wait_k = [&](uint32_t d) {
+            const uint32_t s = S::k_slot(d);
+            if constexpr (S::kTma) {
+                const bool ok = wait(&sh.full[s], phase[0] >> s & 1);
+                phase[0] ^= 1u << s;
+                return ok;
+            }
+            return wait(&sh.full[s], S::k_turn(d) & 1);
+        };
+        auto wait_v = [&](uint32_t d, bool all) {
+            const uint32_t s = S::v_slot(d);
+            if constexpr (S::kTma) {
+                const bool ok = wait(all ? &sh.full[s] : &sh.fixed[s], phase[all ? 0 : 1] >> s & 1);
+                phase[all ? 0 : 1] ^= 1u << s;
+                return ok;
+            }
+            return wait(&sh.full[s], S::v_turn(d) & 1);
+        };
         bool ok = true;
         while (ok && take(f, seg)) {
             const int nb = seg.blocks;
             if (nb == 0) continue;
-            ok = at_wait(sh, &sh.qfull, used & 1);
+            ok = wait(&sh.qfull, used & 1);
             // block b's scores for group t, and what becomes free behind them
             auto do_scores = [&](int b, int t) {
                 if (TILES == 1 || t == 0) ok = ok && wait_k(done + b);
                 if (!ok) return;
                 tc_fence_after();
-                scores(t, (done + b) % S::kStagesK);
+                scores(t, S::k_slot(done + b));
                 commit(&sh.sfull[t]);
                 if (TILES == 1 || t == 1) {
-                    commit(&sh.kempty[(done + b) % S::kStagesK]);
+                    commit(&sh.empty[S::k_slot(done + b)]);
                     if (b == nb - 1) commit(&sh.qempty);
                 }
             };
@@ -1029,20 +1068,23 @@ struct AtRoles {
                 if (TILES == 2) do_scores(0, t);
                 else if (t < nb) do_scores(t, t);
             for (int b = 0; b < nb && ok; b++) {
-                const uint32_t vs = (done + b) % S::kStagesV;
-                if (!S::kTma) ok = at_wait(sh, &sh.vfull[vs], ((done + b) / S::kStagesV) & 1);
-                else if (whole(seg, seg.block0 + b)) ok = at_wait(sh, &sh.vfull[vs], wholes[vs]++ & 1);
-                else ok = at_wait(sh, &sh.vfixed[vs], fixes[vs]++ & 1);
+                const uint32_t vs = S::v_slot(done + b);
+                ok = wait_v(done + b, whole(seg, seg.block0 + b));
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     if (TILES == 1 && t != (b & 1)) continue;
-                    ok = ok && at_wait(sh, &sh.pready[t], p_uses[t]++ & 1);
                     const bool first = TILES == 2 ? b == 0 : b < 2;
-                    if (first) ok = ok && at_wait(sh, &sh.oempty[t], (o_uses[t]++ & 1) ^ 1);
+                    if (first) ok = ok && wait(&sh.oempty[t], (o_uses[t]++ & 1) ^ 1);
+#pragma unroll
+                    for (int half = 0; half < kHalves; half++) {
+                        ok = ok && wait(&sh.pready[t][half], p_uses[t] & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        values(t, vs, !first, half);
+                    }
+                    p_uses[t]++;
                     if (!ok) break;
-                    tc_fence_after();
-                    values(t, vs, !first);
-                    if (TILES == 1 || t == 1) commit(&sh.vempty[vs]);
+                    if (TILES == 1 || t == 1) commit(&sh.empty[vs]);
                     const int nextb = b + (TILES == 2 ? 1 : 2);
                     if (nextb < nb) do_scores(nextb, t);
                     else commit(&sh.ofull[t]);
@@ -1073,15 +1115,17 @@ struct AtRoles {
                 latch(a.status, seg.seq < 0 ? QWN_KV_STATUS_BAD_SEQUENCE : QWN_KV_STATUS_BAD_LENGTH);
             float M = -INFINITY, l = 0.f, c = 0.f;
             for (int b = TILES == 2 ? 0 : g; b < seg.blocks; b += TILES == 2 ? 1 : 2) {
-                if (!at_wait(sh, &sh.sfull[g], s_uses++ & 1)) return;
+                if (!wait(&sh.sfull[g], s_uses++ & 1)) return;
                 tc_fence_after();
-                if (any) {
+                if (!any) {
+                    if (PARTS == 1) warp_arrive(&sh.pready[g][0], lane);
+                } else {
                     const bool first = b < (TILES == 2 ? 1 : 2);
                     if (first) c = a.scale2 * kUnit * (SRC != 0 && PARTS == 1 && have ? sh.qscale[used & 1][r] : 1.f);
                     block(seg, seg.block0 + b, (done + b) & 3, first, have, seen, c, s_col, o_col, M, l);
                 }
                 tc_fence_before();
-                warp_arrive(&sh.pready[g], lane);
+                warp_arrive(&sh.pready[g][PARTS == 1 ? 1 : 0], lane);
             }
             if (seen.lo >= seen.hi) {  // a row that does not exist: blocks seen whole by the others are no business of its
                 M = -INFINITY;
@@ -1199,6 +1243,11 @@ struct AtRoles {
             }
 #pragma unroll
             for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (N / 2) + i / 2, p[k]);
+            if (PARTS == 1 && i == N / 2 - 32) {
+                tmem_store_wait();
+                tc_fence_before();
+                warp_arrive(&sh.pready[warp >> 2][0], lane);
+            }
         }
         float l[4];
         unpair(sum[0], l[0], l[1]);
@@ -1218,7 +1267,7 @@ struct AtRoles {
             sh.ml[turn][g][row][0] = M;
             sh.ml[turn][g][row][1] = l;
             warp_arrive(&sh.joined, lane);
-            if (!at_wait(sh, &sh.joined, joins & 1)) return false;
+            if (!wait(&sh.joined, joins & 1)) return false;
             joins++;
             const float M0 = sh.ml[turn][0][row][0], M1 = sh.ml[turn][1][row][0];
             M = fmaxf(M0, M1);
@@ -1228,10 +1277,10 @@ struct AtRoles {
         }
         if (seg.blocks) {
             if (TILES == 2) {
-                if (!at_wait(sh, &sh.ofull[g], o_uses[0]++ & 1)) return false;
+                if (!wait(&sh.ofull[g], o_uses[0]++ & 1)) return false;
             } else {
-                if (!at_wait(sh, &sh.ofull[0], o_uses[0]++ & 1)) return false;
-                if (two && !at_wait(sh, &sh.ofull[1], o_uses[1]++ & 1)) return false;
+                if (!wait(&sh.ofull[0], o_uses[0]++ & 1)) return false;
+                if (two && !wait(&sh.ofull[1], o_uses[1]++ & 1)) return false;
             }
             tc_fence_after();
         }
@@ -1263,7 +1312,7 @@ struct AtRoles {
                     }
                     if (odd)
 #pragma unroll
-                        for (int k = 0; k < kWide; k++) o[k] += odd_sum<SRC, PARTS, S::kBlock>(a, sh, seg, used & 3, seen, col + k);
+                        for (int k = 0; k < kWide; k++) o[k] += odd_sum<SRC, PARTS, S::kBlock>(a, sh.odd_v[used & 3], seg, seen, col + k);
                 } else {
 #pragma unroll
                     for (int k = 0; k < kWide; k++) o[k] = 0.f;
@@ -1303,22 +1352,26 @@ __global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid
                                                                     const __grid_constant__ AtArgs a) {
     using S = AtShape<SRC, PARTS, TILES>;
     extern __shared__ uint8_t dynamic[];
-    __shared__ __align__(16) AtShared sh;
+    __shared__ __align__(16) AtShared<SRC, PARTS, TILES> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
-    AtRoles<SRC, PARTS, TILES, BF16> roles = {a, sh, base, base + TILES * S::kQBytes,
-                                              base + TILES * S::kQBytes + S::kStagesK * S::kKvBytes, base + S::kOperands, warp, lane};
+    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;  // the host has seen that this leaves room
+    if (base + S::kOperands + S::kRawTiles * S::kTileBytes > smem_u32(dynamic) + S::kSmem) {  // cannot be
+        latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
+        return;
+    }
+    AtRoles<SRC, PARTS, TILES, BF16> roles = {a, sh, base, base + TILES * S::kQBytes, base + S::kOperands, warp, lane};
     if (threadIdx.x == 0) {
         const uint32_t helpers = S::kTma ? 1 : 4, finishers = TILES == 2 ? 4 : 8;
+        for (uint32_t i = 0; i < kAtStages; i++) {
+            mbar_init(&sh.full[i], helpers);
+            mbar_init(&sh.empty[i], 1);
+            mbar_init(&sh.part[i], 1);
+            mbar_init(&sh.fixed[i], 4);
+        }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.kfull[i], helpers);
-            mbar_init(&sh.vfull[i], helpers);
-            mbar_init(&sh.kempty[i], 1);
-            mbar_init(&sh.vempty[i], 1);
-            mbar_init(&sh.vpart[i], 1);
-            mbar_init(&sh.vfixed[i], 4);
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pready[i], 4);
+            mbar_init(&sh.pready[i][0], 4);
+            mbar_init(&sh.pready[i][1], 4);
             mbar_init(&sh.ofull[i], 1);
             mbar_init(&sh.oempty[i], finishers);
             mbar_init(&sh.segfull[i], 1);
@@ -1329,7 +1382,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid
         mbar_init(&sh.joined, 8);
         mbar_init(&sh.helped, 4);
         mbar_init(&sh.drained, 1);
-        for (int i = 0; i < 32; i++) {
+        for (int i = 0; i < AtShared<SRC, PARTS, TILES>::kRaw; i++) {
             mbar_init(&sh.rawfull[i], 1);
             mbar_init(&sh.rawempty[i], 1);
         }
@@ -1378,6 +1431,10 @@ cudaError_t prepare_tile_kernel(int device) {
     cudaFuncAttributes at;
     cudaError_t e = cudaFuncGetAttributes(&at, kernel);
     if (e == cudaSuccess && at.numRegs * 4 < 2 * kSoftmaxRegs + kHelperRegs + kOtherRegs) return cudaErrorInvalidConfiguration;
+    // operands start on 1024 bytes behind the static part; the window itself does
+    using S = AtShape<SRC, PARTS, TILES>;
+    if (e == cudaSuccess && (1024 - at.sharedSizeBytes % 1024) % 1024 + S::kOperands + S::kRawTiles * S::kTileBytes > S::kSmem)
+        return cudaErrorInvalidConfiguration;
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AtShape<SRC, PARTS, TILES>::kSmem);
     ready[device] = e == cudaSuccess;
