@@ -84,6 +84,9 @@ struct AtShape {
     static constexpr bool kPaged = SRC != 0;
     static constexpr bool kTma = !kPaged && PARTS == 1;            // operand tiles straight from the rows
     static constexpr bool kRaw = kPaged && SRC != QWN_KV_CODEC_F16;// cached tiles by way of shared memory
+    // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
+    // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
+    static constexpr bool kByDims = PARTS == 1 && kRaw;
     static constexpr int kBlock = PARTS == 1 ? 128 : 64;           // tokens
     static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
     static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
@@ -535,6 +538,23 @@ __device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint3
                 w[c] = make_uint4(u[0], u[1], u[2], u[3]);
             }
         }
+        // dims in the order that K's words give them
+        if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+#pragma unroll
+            for (uint32_t c = 0; c < 16; c++)
+                w[c] = make_uint4(prmt(w[c].x, w[c].y, 0x5410u), prmt(w[c].z, w[c].w, 0x5410u), prmt(w[c].x, w[c].y, 0x7632u),
+                                  prmt(w[c].z, w[c].w, 0x7632u));
+        } else if constexpr (SRC == QWN_KV_CODEC_TQ35_G64) {
+#pragma unroll
+            for (uint32_t c = 0; c < 16; c += 2) {
+                const uint4 a = w[c], b = w[c + 1];
+                auto order = [&](uint32_t sel) {
+                    return make_uint4(prmt(a.x, a.z, sel), prmt(b.x, b.z, sel), prmt(a.y, a.w, sel), prmt(b.y, b.w, sel));
+                };
+                w[c] = order(0x5410u);
+                w[c + 1] = order(0x7632u);
+            }
+        }
 #pragma unroll
         for (uint32_t c = 0; c < 16; c++) st_shared16(chunk_at(tile, kAtRows, lane_row, c), w[c]);
     }
@@ -542,6 +562,12 @@ __device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint3
 
 // ---- keys and values ------------------------------------------------------------
 
+// Where token t of a cached tile goes among its 16 operand columns, and back: the four tokens that a lane's words
+// of V hold (2a, 2a + 1, 2a + 8, 2a + 9) are neighbours.  Scores and probabilities are in this order.
+__host__ __device__ constexpr int cached_order(int t) { return 4 * ((t & 7) >> 1) + (t & 1) + 2 * (t >> 3); }
+__host__ __device__ constexpr int cached_token(int column) {
+    return (column & ~15) + 2 * ((column & 15) >> 2) + (column & 1) + 8 * ((column >> 1) & 1);
+}
 // a cached tile's address for a token that exists; a bad page latches and reads page 0
 __device__ __forceinline__ const uint8_t *at_tile(const AtArgs &a, int32_t seq, int32_t head, int32_t token) {
     const StoreGeo &g = a.geo;
@@ -572,52 +598,221 @@ __device__ __forceinline__ float token_scale(const uint8_t *tile, int t, int whi
         return fmaxf(*reinterpret_cast<const float *>(s + s32_off(t, 0)), *reinterpret_cast<const float *>(s + s32_off(t, 1)));
     }
 }
-template <int SRC, int PARTS>
-__device__ __forceinline__ Row16 operand_row(const uint8_t *tile, int t, int which, int j) {
-    if constexpr (PARTS == 3) {
-        return take_row<SRC>(tile, t, which, j);
-    } else if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16) {
-        return take_q8(tile, t, which, j, 1.f, 1.f);
-    } else if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
-        const uint8_t *s = tile + (which ? 4224 : 4096);
-        const float s0 = *reinterpret_cast<const float *>(s + s32_off(t, 0)), s1 = *reinterpret_cast<const float *>(s + s32_off(t, 1));
-        const float top = fmaxf(s0, s1);
-        return take_q8(tile, t, which, j, s0 / top, s1 / top);
-    } else {
-        Row16 x = take_row<SRC>(tile, t, which, j);
-        if (AtScale<SRC>::kFixed != 1.f)
-#pragma unroll
-            for (int i = 0; i < 16; i++) x.v[i] *= 1.f / AtScale<SRC>::kFixed;
-        return x;
-    }
-}
-// a row's 16 values of this lane into an operand tile, as f16 or as three bf16 parts
-template <int PARTS>
+// a row's 16 values of this lane into an operand tile, as three bf16 parts
 __device__ __forceinline__ void put_operand(uint32_t base, uint32_t rows, uint32_t part, uint32_t r, int j, const Row16 &x) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const float *v = x.v + 8 * h;
-        if constexpr (PARTS == 1) {
-            st_shared16(chunk_at(base, rows, r, 8 * h + j),
-                        make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]), pack_h2(v[4], v[5]), pack_h2(v[6], v[7])));
-        } else {
-            uint4 p[3];
-            split3(v, p);
+        uint4 p[3];
+        split3(x.v + 8 * h, p);
 #pragma unroll
-            for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
-        }
+        for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
     }
 }
-// K or V of a cached tile, which is tile ti of its block, by one warp; tokens from `len` on are zero
-template <int SRC, int PARTS, int BLOCK>
-__device__ __forceinline__ void put_tile(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
+// K or V of a cached tile, which is tile ti of its block, as fp32 in parts, by one warp; tokens from `len` on are zero
+template <int SRC, int BLOCK>
+__device__ __forceinline__ void put_parts(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
     const int lane = threadIdx.x & 31, j = lane & 7;
 #pragma unroll
     for (int pass = 0; pass < 4; pass++) {
         const int t = 4 * pass + (lane >> 3);
-        Row16 x = operand_row<SRC, PARTS>(tile, t, which, j);
-        if (token0 + t >= len) x = Row16{};
-        put_operand<PARTS>(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
+        Row16 x = {};
+        if (token0 + t < len) x = take_row<SRC>(tile, t, which, j);
+        put_operand(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
+    }
+}
+
+// Cached tiles as f16 operands, by one warp: codes to f16 by exponent tricks (exact), then one rounded step for
+// what is not exact.
+__device__ __forceinline__ void st_shared8(uint32_t addr, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+// a pair of ranges over 2 LEVELS, rounded once: f16's nearest to the factor, and what that lacks
+template <int LEVELS>
+__device__ __forceinline__ uint32_t half_steps(uint32_t ranges) {
+    constexpr float f = 0.5f / LEVELS, near = LEVELS == 15 ? 1092.f / 32768.f : 1170.f / 16384.f;
+    return hfma2(ranges, pack_h2(near, near), hmul2(ranges, pack_h2(f - near, f - near)));
+}
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 ld16(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
+// eight codes of 3.5-bit words: odd dims of half 1 have their lowest bit above half 0's and two in a plane
+__device__ __forceinline__ uint32_t odd_codes(uint32_t odd, uint32_t plane, int x) {
+    if (x == 0) return odd & 0x77777777u;
+    uint32_t p = (plane | (plane << 8)) & 0x00FF00FFu;
+    p = (p | (p << 4)) & 0x0F0F0F0Fu;
+    p = (p | (p << 2)) & 0x33333333u;
+    return ((odd >> 3) & 0x11111111u) | (p << 1);
+}
+// K of a tile: rows of 128 dims (in the order that put_q gives the queries)
+template <int SRC>
+__device__ __forceinline__ void put_keys(const uint8_t *tile, int ti, uint32_t base) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // 16 codes of a row
+            const int t = 4 * i + (lane >> 3), at = lane & 7, d16 = at ^ ((t & 1) << 2), half = d16 >> 2;
+            const uint4 w = ld16(tile + 128 * t + 16 * at);
+            uint32_t h[8];
+            u8x4_to_h2x2(w.x, h[0], h[1]);
+            u8x4_to_h2x2(w.y, h[2], h[3]);
+            u8x4_to_h2x2(w.z, h[4], h[5]);
+            u8x4_to_h2x2(w.w, h[6], h[7]);
+            if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+                const float s0 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 0));
+                const float s1 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 1));
+                const float share = __fdividef(half ? s1 : s0, fmaxf(s0, s1));
+                const uint32_t f = pack_h2(share, share);
+#pragma unroll
+                for (int k = 0; k < 8; k++) h[k] = hmul2(h[k], f);
+            }
+            const uint32_t r = ti * kTileTokens + cached_order(t);
+            // the halves' lanes write their two chunks in opposite order: eight lanes, eight banks of 16 bytes
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            st_shared16(chunk_at(base, 128, r, 2 * d16 + half), half ? hi : lo);
+            st_shared16(chunk_at(base, 128, r, 2 * d16 + (half ^ 1)), half ? lo : hi);
+        }
+    } else {
+#pragma unroll
+        for (int pass = 0; pass < 2; pass++) {
+            const int t = (lane >> 2) + 8 * pass, tig = lane & 3;
+            const uint32_t r = ti * kTileTokens + cached_order(t);
+            if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+                const uint4 w = ld16(tile + 64 * t + 16 * tig);
+                const uint4 p0 = ld16(tile + 2048 + 32 * (t & 7)), p1 = ld16(tile + 2048 + 32 * (t & 7) + 16);
+                const uint32_t par[4] = {pass ? p0.y : p0.x, pass ? p0.w : p0.z, pass ? p1.y : p1.x, pass ? p1.w : p1.z};
+                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                const bool odd = t & 1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {  // odd tokens in another order, for the banks
+                    const uint32_t c = odd ? k ^ 1 : k, p = odd ? par[k ^ 1] : par[k];
+                    const uint32_t step = half_steps<15>(prmt(p, p, 0x1010u)), low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+                    uint32_t v[4];
+                    nib8_to_h2x4(odd ? word[k ^ 1] : word[k], v);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
+                    st_shared16(chunk_at(base, 128, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
+                }
+            } else {
+                const uint2 e = *reinterpret_cast<const uint2 *>(tile + 32 * t + 8 * tig);
+                const uint32_t odd = *reinterpret_cast<const uint32_t *>(tile + 512 + 16 * t + 4 * tig);
+                const uint32_t plane = *reinterpret_cast<const uint16_t *>(tile + 768 + 8 * t + 2 * tig);
+                const uint4 par = ld16(tile + 896 + 16 * (t & 7));
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint32_t p = x ? (pass ? par.w : par.z) : (pass ? par.y : par.x), ranges = prmt(p, p, 0x1010u);
+                    const uint32_t low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+#pragma unroll
+                    for (int o = 0; o < 2; o++) {
+                        const uint32_t step = o ? half_steps<7>(ranges) : half_steps<15>(ranges);
+                        uint32_t v[4];
+                        nib8_to_h2x4(o ? odd_codes(odd, plane, x) : x ? e.y : e.x, v);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
+                        st_shared16(chunk_at(base, 128, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
+                    }
+                }
+            }
+        }
+    }
+}
+// V of a tile: of each dim the 16 tokens.  Lane 4 r + a has the tokens 2a, 2a + 1, 2a + 8, 2a + 9 of the dims with
+// index r (and r + 8) in its classes of 16.
+template <int SRC>
+__device__ __forceinline__ void put_values(const uint8_t *tile, int ti, uint32_t base) {
+    const int lane = threadIdx.x & 31, a = lane & 3, r = lane >> 2;
+    const uint32_t chunk = 2 * (ti & 3) + (a >> 1), to = base + (ti >> 2) * 16384 + 8 * (a & 1);
+    auto put = [&](uint32_t d, uint32_t first, uint32_t second) {
+        st_shared8(to + d * 128 + ((chunk ^ (d & 7)) << 4), first, second);
+    };
+    if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32) {
+        uint32_t share[2][2];  // of the dims' half, the tokens 2a, 2a + 1 and those plus 8
+        if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+            const float4 s = *reinterpret_cast<const float4 *>(tile + 4224 + 32 * a), n = *reinterpret_cast<const float4 *>(tile + 4224 + 32 * a + 16);
+            // (half 0 of t, of t + 8, half 1 of t, of t + 8) for t = 2a and 2a + 1
+            share[0][0] = pack_h2(__fdividef(s.x, fmaxf(s.x, s.z)), __fdividef(n.x, fmaxf(n.x, n.z)));
+            share[0][1] = pack_h2(__fdividef(s.y, fmaxf(s.y, s.w)), __fdividef(n.y, fmaxf(n.y, n.w)));
+            share[1][0] = pack_h2(__fdividef(s.z, fmaxf(s.x, s.z)), __fdividef(n.z, fmaxf(n.x, n.z)));
+            share[1][1] = pack_h2(__fdividef(s.w, fmaxf(s.y, s.w)), __fdividef(n.w, fmaxf(n.y, n.w)));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint4 w = ld16(tile + 2048 + 64 * lane + 16 * (q ^ ((lane >> 1) & 3)));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint32_t lo[2], hi[2];  // dims r and r + 8 of the class, tokens below and from 8
+                u8x4_to_h2x2(i ? w.z : w.x, lo[0], lo[1]);
+                u8x4_to_h2x2(i ? w.w : w.y, hi[0], hi[1]);
+                const uint32_t d = 32 * q + 16 * i + r;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+                        lo[k] = hmul2(lo[k], share[q >> 1][0]);
+                        hi[k] = hmul2(hi[k], share[q >> 1][1]);
+                    }
+                    put(d + 8 * k, lo[k], hi[k]);
+                }
+            }
+        }
+    } else if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+        uint4 w[2], p[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) w[i] = ld16(tile + 1024 + 32 * lane + 16 * (i ^ (r & 1)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = ld16(tile + 2304 + 64 * a + 16 * i);  // t = 2a: groups 0, 1; 2, 3; t = 2a + 1
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint4 s = p[c >> 1], n = p[2 + (c >> 1)];
+            const uint32_t s0 = c & 1 ? s.z : s.x, s8 = c & 1 ? s.w : s.y, n0 = c & 1 ? n.z : n.x, n8 = c & 1 ? n.w : n.y;
+            const uint32_t step0 = half_steps<15>(prmt(s0, n0, 0x5410u)), step8 = half_steps<15>(prmt(s8, n8, 0x5410u));
+            const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint4 y = w[c >> 1];
+                const int k = 2 * (c & 1) + i;
+                uint32_t v[4];
+                nib8_to_h2x4(k == 0 ? y.x : k == 1 ? y.y : k == 2 ? y.z : y.w, v);
+                const uint32_t d = 32 * c + 16 * i + r;
+                put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
+                put(d + 8, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
+            }
+        }
+    } else {
+        const uint8_t *half = tile + 1024;
+        const uint4 e = ld16(half + 16 * lane);
+        const uint2 o = *reinterpret_cast<const uint2 *>(half + 512 + 8 * lane);
+        const uint32_t plane = *reinterpret_cast<const uint32_t *>(half + 768 + 4 * lane);
+        const uint4 s = ld16(half + 896 + 32 * a), n = ld16(half + 896 + 32 * a + 16);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const uint32_t s0 = x ? s.z : s.x, s8 = x ? s.w : s.y, n0 = x ? n.z : n.x, n8 = x ? n.w : n.y;
+            const uint32_t r0 = prmt(s0, n0, 0x5410u), r8 = prmt(s8, n8, 0x5410u);
+            const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
+#pragma unroll
+            for (int odd = 0; odd < 2; odd++) {
+                const uint32_t step0 = odd ? half_steps<7>(r0) : half_steps<15>(r0), step8 = odd ? half_steps<7>(r8) : half_steps<15>(r8);
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const uint32_t codes = odd ? odd_codes(b ? o.y : o.x, (plane >> (16 * b)) & 0xFFFFu, x)
+                                               : x ? (b ? e.w : e.z) : (b ? e.y : e.x);
+                    uint32_t v[4];
+                    nib8_to_h2x4(codes, v);
+                    const uint32_t d = 64 * x + 32 * b + 2 * r + odd;
+                    put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
+                    put(d + 16, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
+                }
+            }
+        }
     }
 }
 
@@ -636,6 +831,36 @@ __device__ __forceinline__ bool odd_word(uint32_t w, bool bf16, uint32_t &out) {
     const bool lo = (w & e) == e, hi = ((w >> 16) & e) == e;
     out = (lo ? 0u : w & 0xFFFFu) | (hi ? 0u : w & 0xFFFF0000u);
     return lo || hi;
+}
+// the same where the values lie by dims: a thread has a dim
+__device__ __forceinline__ void note_odd(uint32_t (&noted)[2][16], const AtSegment &seg, int block, int32_t token) {
+    const int32_t z = odd_zone(seg, block);
+    const uint32_t i = (uint32_t)(token < z ? token - seg.block0 * block : token - z);
+    if (i < 512) atomicOr(&noted[token < z ? 0 : 1][i >> 5], 1u << (i & 31));
+}
+__device__ __noinline__ void clear_odd_by_dims(uint32_t (&noted)[2][16], const AtSegment &seg, int32_t token0, uint32_t base) {
+    const uint32_t d = threadIdx.x & 127;
+    const int32_t left = seg.len - token0;  // tokens of the block that exist
+#pragma unroll 1
+    for (uint32_t c = 0; c < 16; c++) {  // eight tokens each
+        const uint32_t at = base + (c >> 3) * 16384 + d * 128 + (((c & 7) ^ (d & 7)) << 4);
+        const uint4 w = ld_shared16(at);
+        uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        bool change = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int32_t t = cached_token((int)(8 * c) + 2 * k + h);
+                const bool odd = ((u[k] >> (16 * h)) & 0x7C00u) == 0x7C00u;
+                if (odd && t < left) note_odd(noted, seg, 128, token0 + t);
+                if (odd || t >= left) {
+                    u[k] &= h ? 0x0000FFFFu : 0xFFFF0000u;
+                    change = true;
+                }
+            }
+        if (change) st_shared16(at, make_uint4(u[0], u[1], u[2], u[3]));
+    }
 }
 template <int PARTS, int BLOCK>
 __device__ void clear_odd(uint32_t (&noted)[2][16], const AtSegment &seg, int32_t token0, uint32_t base, bool bf16) {
@@ -657,11 +882,7 @@ __device__ void clear_odd(uint32_t (&noted)[2][16], const AtSegment &seg, int32_
         if (o) st_shared16(at, y);
         odd |= o;
     }
-    if (odd) {
-        const int32_t z = odd_zone(seg, BLOCK);
-        const uint32_t i = (uint32_t)(token < z ? token - seg.block0 * BLOCK : token - z);
-        if (i < 512) atomicOr(&noted[token < z ? 0 : 1][i >> 5], 1u << (i & 31));
-    }
+    if (odd) note_odd(noted, seg, BLOCK, token);
 }
 // value d of a token
 template <int SRC, int PARTS>
@@ -906,19 +1127,29 @@ struct AtRoles {
                     } else if (at < seg.len) {
                         tile = at_tile(a, seg.seq, seg.head, at);
                     }
-                    if (kTokenScales && !which) {  // both scales, read when the block's scores are there
-                        const int t = lane & 15, v = lane >> 4;
-                        const float sc = at + t < seg.len ? token_scale<SRC>(tile, t, v) : 0.f;
-                        (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + t] = sc;
-                        const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
-                        if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
+                    if constexpr (kTokenScales) {
+                        if (!which) {  // both scales, read when the block's scores are there
+                            const int t = lane & 15, v = lane >> 4;
+                            const float sc = at + t < seg.len ? token_scale<SRC>(tile, t, v) : 0.f;
+                            (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + cached_order(t)] = sc;
+                            const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
+                            if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
+                        }
                     }
-                    if (tile) {
-                        put_tile<SRC, PARTS, S::kBlock>(tile, which, ti, at, seg.len, dst);
+                    if constexpr (S::kByDims) {
+                        if (which) put_values<SRC>(tile, ti, dst);
+                        else put_keys<SRC>(tile, ti, dst);
+                    } else if constexpr (PARTS == 1) {  // fp16 as it is: the tile's chunks are swizzled alike
+                        if (tile) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                const int i = 32 * k + lane, t = i >> 4, c = i & 15;
+                                cp_async16_at(dst + (c >> 3) * S::kBlock * 128 + (ti * kTileTokens + t) * 128 + (c & 7) * 16,
+                                              tile + which * 4096 + 16 * i);
+                            }
+                        }
                     } else {
-                        for (int pass = 0; pass < 4; pass++)
-                            put_operand<PARTS>(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + 4 * pass + (lane >> 3)),
-                                               lane & 7, Row16{});
+                        put_parts<SRC, S::kBlock>(tile, which, ti, at, seg.len, dst);
                     }
                     if constexpr (S::kRaw)
                         if (which) warp_arrive(&sh.rawempty[(done * S::kTiles + ti) % S::kRawTiles], lane);
@@ -934,13 +1165,15 @@ struct AtRoles {
                             raw.load(rows + (uint64_t)(seg.token_row + at + t) * stride, lane & 7);
                             x = raw.row();
                         }
-                        put_operand<PARTS>(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + t), lane & 7, x);
+                        put_operand(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + t), lane & 7, x);
                     }
                 }
             }
+            if constexpr (S::kPaged && PARTS == 1 && !S::kRaw) asm volatile("cp.async.wait_all;" ::: "memory");
             if (which && !whole(seg, blk)) {
                 if (!helpers_sync(syncs)) return false;
-                clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
+                if constexpr (S::kByDims) clear_odd_by_dims(sh.odd_v[segment & 3], seg, token0, dst);
+                else clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
             }
             fence_proxy_async_shared();
             warp_arrive(&sh.full[s], lane);
@@ -995,7 +1228,7 @@ struct AtRoles {
         const bool leader = elect_one();
         uint32_t done = 0, used = 0, o_uses[2] = {0, 0}, p_uses[2] = {0, 0};
         uint32_t phase[2] = {};  // loaded operands: of full and fixed, a bit per slot
-        constexpr uint32_t kQk = f16_desc(BF16 || PARTS == 3, S::kBlock, false), kPv = f16_desc(BF16 || PARTS == 3, 128, true);
+        constexpr uint32_t kQk = f16_desc(BF16 || PARTS == 3, S::kBlock, false), kPv = f16_desc(BF16 || PARTS == 3, 128, !S::kByDims);
         // the products of parts that count, the small ones first
         constexpr int kPairs = PARTS == 1 ? 1 : 6;
         constexpr int kFirst[6] = {PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, kSecond[6] = {0, 2, 1, 0, 1, 0};
@@ -1018,12 +1251,12 @@ struct AtRoles {
             const uint32_t v = slot_at(slot);
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
-                const uint64_t vd = rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
+                const uint64_t vd = S::kByDims ? smem_desc(v) : rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
                 if (leader)
 #pragma unroll
                     for (int c = half * kSteps; c < (half + 1) * kSteps; c++)
                         mma_ts(tmem + S::kOColumn + t * 128, tmem + t * S::kSColumns + kFirst[p] * (S::kBlock / 2) + c * 8,
-                               vd + c * (2048 / 16), kPv, add || p + c > 0);
+                               vd + (S::kByDims ? (c >> 2) * (16384 / 16) + (c & 3) * 2 : c * (2048 / 16)), kPv, add || p + c > 0);
             }
         };
         auto commit = [&](uint64_t *bar) {
@@ -1161,8 +1394,10 @@ struct AtRoles {
         if (!full) {
             const int lo = seen.lo - blk * N, hi = seen.hi - blk * N;
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (i < lo || i >= hi) x[i] = -INFINITY;
+            for (int i = 0; i < N; i++) {
+                const int t = S::kByDims ? cached_token(i) : i;
+                if (t < lo || t >= hi) x[i] = -INFINITY;
+            }
         }
         float t[8];
 #pragma unroll
