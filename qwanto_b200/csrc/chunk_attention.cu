@@ -173,6 +173,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     a.scale2 = (r->scale > 0.f ? r->scale : 0.08838834764831845f) * 1.4426950408889634f;
     a.query_stride = qs;
     a.out_stride = os;
+    a.wide_out = rows_aligned(r->output_dev, os, r->dtype, 32 / es);
     a.query = r->query_dev;
     a.out = r->output_dev;
     a.geo = store_geo(p);
@@ -181,6 +182,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     if (c.split && r->workspace_dev) {
         a.prefix = static_cast<uint64_t *>(r->workspace_dev);
         a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(r->workspace_dev) + c.prefix_bytes);
+        a.wide_slots = (uintptr_t)a.slots % 32 == 0;
     }
     cudaStream_t s = stream_of(p, r->stream);
     cudaError_t e;

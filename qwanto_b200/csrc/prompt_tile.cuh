@@ -75,6 +75,7 @@ struct AtArgs {
     uint32_t units;            // row tiles, without a split
     uint64_t *prefix;          // split: blocks before each sequence, then
     float *slots;              // the partial results
+    bool wide_out, wide_slots; // rows of the output and of the partial results start on 32 bytes
 };
 // a partial result: o[rows][128], then M[rows], l[rows]
 __host__ __device__ constexpr uint32_t at_slot_floats(uint32_t tiles) { return tiles * kAtRows * (kHeadDim + 2); }
@@ -654,167 +655,206 @@ __device__ __forceinline__ uint32_t odd_codes(uint32_t odd, uint32_t plane, int 
     p = (p | (p << 2)) & 0x33333333u;
     return ((odd >> 3) & 0x11111111u) | (p << 1);
 }
-// K of a tile: rows of 128 dims (in the order that put_q gives the queries)
+// K of a tile: rows of 128 dims (in the order that put_q gives the queries).  What
+// a lane converts is loaded before it stores anything, two tiles at a time: a lone
+// warp per scheduler waits for its loads otherwise (32 x 4 rows over 8192 int8
+// tokens: 248 us).
 template <int SRC>
-__device__ __forceinline__ void put_keys(const uint8_t *tile, int ti, uint32_t base) {
-    const int lane = threadIdx.x & 31;
-    if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32) {
+struct KeyWords {
+    static constexpr bool kInt8 = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32;
+    uint4 w[4];   // int8: 16 codes of rows t, t + 4, ..; 4-bit: words of t and t + 8, their parameters; 3.5-bit: likewise
+    __device__ __forceinline__ void load(const uint8_t *tile) {
+        const int lane = threadIdx.x & 31;
+        if constexpr (kInt8) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {  // 16 codes of a row
-            const int t = 4 * i + (lane >> 3), at = lane & 7, d16 = at ^ ((t & 1) << 2), half = d16 >> 2;
-            const uint4 w = ld16(tile + 128 * t + 16 * at);
-            uint32_t h[8];
-            u8x4_to_h2x2(w.x, h[0], h[1]);
-            u8x4_to_h2x2(w.y, h[2], h[3]);
-            u8x4_to_h2x2(w.z, h[4], h[5]);
-            u8x4_to_h2x2(w.w, h[6], h[7]);
-            if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
-                const float s0 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 0));
-                const float s1 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 1));
-                const float share = __fdividef(half ? s1 : s0, fmaxf(s0, s1));
-                const uint32_t f = pack_h2(share, share);
+            for (int i = 0; i < 4; i++) w[i] = ld16(tile + 512 * i + 16 * lane);
+        } else if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+            w[0] = ld16(tile + 16 * lane);
+            w[1] = ld16(tile + 512 + 16 * lane);
+            w[2] = ld16(tile + 2048 + 32 * (lane >> 2));
+            w[3] = ld16(tile + 2048 + 32 * (lane >> 2) + 16);
+        } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) h[k] = hmul2(h[k], f);
+            for (int i = 0; i < 2; i++) {
+                const uint2 e = *reinterpret_cast<const uint2 *>(tile + 256 * i + 8 * lane);
+                w[i] = make_uint4(e.x, e.y, *reinterpret_cast<const uint32_t *>(tile + 512 + 128 * i + 4 * lane),
+                                  *reinterpret_cast<const uint16_t *>(tile + 768 + 64 * i + 2 * lane));
             }
-            const uint32_t r = ti * kTileTokens + cached_order(t);
-            // the halves' lanes write their two chunks in opposite order: eight lanes, eight banks of 16 bytes
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            st_shared16(chunk_at(base, 128, r, 2 * d16 + half), half ? hi : lo);
-            st_shared16(chunk_at(base, 128, r, 2 * d16 + (half ^ 1)), half ? lo : hi);
+            w[2] = ld16(tile + 896 + 16 * (lane >> 2));
         }
-    } else {
+    }
+    // `tile` still holds the scales of int8 codes per 64 channels
+    __device__ __forceinline__ void store(const uint8_t *tile, int ti, uint32_t base) const {
+        const int lane = threadIdx.x & 31;
+        if constexpr (kInt8) {
+            const int at = lane & 7;
 #pragma unroll
-        for (int pass = 0; pass < 2; pass++) {
-            const int t = (lane >> 2) + 8 * pass, tig = lane & 3;
-            const uint32_t r = ti * kTileTokens + cached_order(t);
-            if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
-                const uint4 w = ld16(tile + 64 * t + 16 * tig);
-                const uint4 p0 = ld16(tile + 2048 + 32 * (t & 7)), p1 = ld16(tile + 2048 + 32 * (t & 7) + 16);
-                const uint32_t par[4] = {pass ? p0.y : p0.x, pass ? p0.w : p0.z, pass ? p1.y : p1.x, pass ? p1.w : p1.z};
-                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-                const bool odd = t & 1;
+            for (int i = 0; i < 4; i++) {
+                const int t = 4 * i + (lane >> 3), d16 = at ^ ((t & 1) << 2), half = d16 >> 2;
+                uint32_t h[8];
+                u8x4_to_h2x2(w[i].x, h[0], h[1]);
+                u8x4_to_h2x2(w[i].y, h[2], h[3]);
+                u8x4_to_h2x2(w[i].z, h[4], h[5]);
+                u8x4_to_h2x2(w[i].w, h[6], h[7]);
+                if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+                    const float s0 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 0));
+                    const float s1 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 1));
+                    const float share = __fdividef(half ? s1 : s0, fmaxf(s0, s1));
+                    const uint32_t f = pack_h2(share, share);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {  // odd tokens in another order, for the banks
-                    const uint32_t c = odd ? k ^ 1 : k, p = odd ? par[k ^ 1] : par[k];
-                    const uint32_t step = half_steps<15>(prmt(p, p, 0x1010u)), low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
-                    uint32_t v[4];
-                    nib8_to_h2x4(odd ? word[k ^ 1] : word[k], v);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
-                    st_shared16(chunk_at(base, 128, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
+                    for (int k = 0; k < 8; k++) h[k] = hmul2(h[k], f);
                 }
-            } else {
-                const uint2 e = *reinterpret_cast<const uint2 *>(tile + 32 * t + 8 * tig);
-                const uint32_t odd = *reinterpret_cast<const uint32_t *>(tile + 512 + 16 * t + 4 * tig);
-                const uint32_t plane = *reinterpret_cast<const uint16_t *>(tile + 768 + 8 * t + 2 * tig);
-                const uint4 par = ld16(tile + 896 + 16 * (t & 7));
+                const uint32_t r = ti * kTileTokens + cached_order(t);
+                // the halves' lanes write their two chunks in opposite order: eight lanes, eight banks of 16 bytes
+                const uint32_t first = chunk_at(base, 128, r, 2 * d16 + half);
+                const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+                st_shared16(first, half ? hi : lo);
+                st_shared16(first ^ 16, half ? lo : hi);
+            }
+        } else {
+            const int tig = lane & 3;
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint32_t p = x ? (pass ? par.w : par.z) : (pass ? par.y : par.x), ranges = prmt(p, p, 0x1010u);
-                    const uint32_t low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+            for (int pass = 0; pass < 2; pass++) {
+                const int t = (lane >> 2) + 8 * pass;
+                const uint32_t r = ti * kTileTokens + cached_order(t);
+                if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+                    const uint32_t par[4] = {pass ? w[2].y : w[2].x, pass ? w[2].w : w[2].z, pass ? w[3].y : w[3].x, pass ? w[3].w : w[3].z};
+                    const uint32_t word[4] = {w[pass].x, w[pass].y, w[pass].z, w[pass].w};
+                    const bool odd = t & 1;
 #pragma unroll
-                    for (int o = 0; o < 2; o++) {
-                        const uint32_t step = o ? half_steps<7>(ranges) : half_steps<15>(ranges);
+                    for (int k = 0; k < 4; k++) {  // odd tokens in another order, for the banks
+                        const uint32_t c = odd ? k ^ 1 : k, p = odd ? par[k ^ 1] : par[k];
+                        const uint32_t step = half_steps<15>(prmt(p, p, 0x1010u)), low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
                         uint32_t v[4];
-                        nib8_to_h2x4(o ? odd_codes(odd, plane, x) : x ? e.y : e.x, v);
+                        nib8_to_h2x4(odd ? word[k ^ 1] : word[k], v);
 #pragma unroll
                         for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
-                        st_shared16(chunk_at(base, 128, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
+                        st_shared16(chunk_at(base, 128, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const uint32_t p = x ? (pass ? w[2].w : w[2].z) : (pass ? w[2].y : w[2].x), ranges = prmt(p, p, 0x1010u);
+                        const uint32_t low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+#pragma unroll
+                        for (int o = 0; o < 2; o++) {
+                            const uint32_t step = o ? half_steps<7>(ranges) : half_steps<15>(ranges);
+                            uint32_t v[4];
+                            nib8_to_h2x4(o ? odd_codes(w[pass].z, w[pass].w, x) : x ? w[pass].y : w[pass].x, v);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
+                            st_shared16(chunk_at(base, 128, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
+                        }
                     }
                 }
             }
         }
     }
-}
+};
 // V of a tile: of each dim the 16 tokens.  Lane 4 r + a has the tokens 2a, 2a + 1, 2a + 8, 2a + 9 of the dims with
-// index r (and r + 8) in its classes of 16.
+// index r (and r + 8) in its classes of 16.  All is loaded before the tile's room is given back.
 template <int SRC>
-__device__ __forceinline__ void put_values(const uint8_t *tile, int ti, uint32_t base) {
-    const int lane = threadIdx.x & 31, a = lane & 3, r = lane >> 2;
-    const uint32_t chunk = 2 * (ti & 3) + (a >> 1), to = base + (ti >> 2) * 16384 + 8 * (a & 1);
-    auto put = [&](uint32_t d, uint32_t first, uint32_t second) {
-        st_shared8(to + d * 128 + ((chunk ^ (d & 7)) << 4), first, second);
-    };
-    if constexpr (SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32) {
-        uint32_t share[2][2];  // of the dims' half, the tokens 2a, 2a + 1 and those plus 8
-        if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
-            const float4 s = *reinterpret_cast<const float4 *>(tile + 4224 + 32 * a), n = *reinterpret_cast<const float4 *>(tile + 4224 + 32 * a + 16);
-            // (half 0 of t, of t + 8, half 1 of t, of t + 8) for t = 2a and 2a + 1
-            share[0][0] = pack_h2(__fdividef(s.x, fmaxf(s.x, s.z)), __fdividef(n.x, fmaxf(n.x, n.z)));
-            share[0][1] = pack_h2(__fdividef(s.y, fmaxf(s.y, s.w)), __fdividef(n.y, fmaxf(n.y, n.w)));
-            share[1][0] = pack_h2(__fdividef(s.z, fmaxf(s.x, s.z)), __fdividef(n.z, fmaxf(n.x, n.z)));
-            share[1][1] = pack_h2(__fdividef(s.w, fmaxf(s.y, s.w)), __fdividef(n.w, fmaxf(n.y, n.w)));
+struct ValueWords {
+    static constexpr bool kInt8 = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32;
+    static constexpr int kPar = SRC == QWN_KV_CODEC_Q8_HEAD_F16 ? 0 : SRC == QWN_KV_CODEC_Q4_G32 ? 4 : 2;
+    uint4 w[kInt8 ? 4 : 2], p[kPar ? kPar : 1];
+    __device__ __forceinline__ void load(const uint8_t *tile) {
+        const int lane = threadIdx.x & 31, a = lane & 3;
+        if constexpr (kInt8) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = ld16(tile + 2048 + 64 * lane + 16 * (q ^ ((lane >> 1) & 3)));
+#pragma unroll
+            for (int i = 0; i < kPar; i++) p[i] = ld16(tile + 4224 + 32 * a + 16 * i);
+        } else if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) w[i] = ld16(tile + 1024 + 32 * lane + 16 * (i ^ ((lane >> 2) & 1)));
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = ld16(tile + 2304 + 64 * a + 16 * i);  // t = 2a: groups 0, 1; 2, 3; t = 2a + 1
+        } else {
+            w[0] = ld16(tile + 1024 + 16 * lane);
+            const uint2 o = *reinterpret_cast<const uint2 *>(tile + 1536 + 8 * lane);
+            w[1] = make_uint4(o.x, o.y, *reinterpret_cast<const uint32_t *>(tile + 1792 + 4 * lane), 0);
+#pragma unroll
+            for (int i = 0; i < 2; i++) p[i] = ld16(tile + 1920 + 32 * a + 16 * i);
         }
+    }
+    __device__ __forceinline__ void store(int ti, uint32_t base) const {
+        const int lane = threadIdx.x & 31, a = lane & 3, r = lane >> 2;
+        const uint32_t chunk = 2 * (ti & 3) + (a >> 1), to = base + (ti >> 2) * 16384 + 8 * (a & 1);
+        auto put = [&](uint32_t d, uint32_t first, uint32_t second) {
+            st_shared8(to + d * 128 + ((chunk ^ (d & 7)) << 4), first, second);
+        };
+        if constexpr (kInt8) {
+            uint32_t share[2][2];  // of the dims' half, the tokens 2a, 2a + 1 and those plus 8
+            if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+                // (half 0 of t, of t + 8, half 1 of t, of t + 8) for t = 2a and 2a + 1
+                const float s[4] = {__uint_as_float(p[0].x), __uint_as_float(p[0].y), __uint_as_float(p[0].z), __uint_as_float(p[0].w)};
+                const float n[4] = {__uint_as_float(p[1].x), __uint_as_float(p[1].y), __uint_as_float(p[1].z), __uint_as_float(p[1].w)};
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint4 w = ld16(tile + 2048 + 64 * lane + 16 * (q ^ ((lane >> 1) & 3)));
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint32_t lo[2], hi[2];  // dims r and r + 8 of the class, tokens below and from 8
-                u8x4_to_h2x2(i ? w.z : w.x, lo[0], lo[1]);
-                u8x4_to_h2x2(i ? w.w : w.y, hi[0], hi[1]);
-                const uint32_t d = 32 * q + 16 * i + r;
+                    for (int e = 0; e < 2; e++)
+                        share[h][e] = pack_h2(__fdividef(s[2 * h + e], fmaxf(s[e], s[2 + e])), __fdividef(n[2 * h + e], fmaxf(n[e], n[2 + e])));
+            }
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
-                        lo[k] = hmul2(lo[k], share[q >> 1][0]);
-                        hi[k] = hmul2(hi[k], share[q >> 1][1]);
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t lo[2], hi[2];  // dims r and r + 8 of the class, tokens below and from 8
+                    u8x4_to_h2x2(i ? w[q].z : w[q].x, lo[0], lo[1]);
+                    u8x4_to_h2x2(i ? w[q].w : w[q].y, hi[0], hi[1]);
+                    const uint32_t d = 32 * q + 16 * i + r;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
+                            lo[k] = hmul2(lo[k], share[q >> 1][0]);
+                            hi[k] = hmul2(hi[k], share[q >> 1][1]);
+                        }
+                        put(d + 8 * k, lo[k], hi[k]);
                     }
-                    put(d + 8 * k, lo[k], hi[k]);
+                }
+        } else if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint4 s = p[c >> 1], n = p[2 + (c >> 1)];
+                const uint32_t s0 = c & 1 ? s.z : s.x, s8 = c & 1 ? s.w : s.y, n0 = c & 1 ? n.z : n.x, n8 = c & 1 ? n.w : n.y;
+                const uint32_t step0 = half_steps<15>(prmt(s0, n0, 0x5410u)), step8 = half_steps<15>(prmt(s8, n8, 0x5410u));
+                const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint4 y = w[c >> 1];
+                    const int k = 2 * (c & 1) + i;
+                    uint32_t v[4];
+                    nib8_to_h2x4(k == 0 ? y.x : k == 1 ? y.y : k == 2 ? y.z : y.w, v);
+                    const uint32_t d = 32 * c + 16 * i + r;
+                    put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
+                    put(d + 8, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
                 }
             }
-        }
-    } else if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
-        uint4 w[2], p[4];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) w[i] = ld16(tile + 1024 + 32 * lane + 16 * (i ^ (r & 1)));
+            for (int x = 0; x < 2; x++) {
+                const uint32_t s0 = x ? p[0].z : p[0].x, s8 = x ? p[0].w : p[0].y, n0 = x ? p[1].z : p[1].x, n8 = x ? p[1].w : p[1].y;
+                const uint32_t r0 = prmt(s0, n0, 0x5410u), r8 = prmt(s8, n8, 0x5410u);
+                const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = ld16(tile + 2304 + 64 * a + 16 * i);  // t = 2a: groups 0, 1; 2, 3; t = 2a + 1
+                for (int odd = 0; odd < 2; odd++) {
+                    const uint32_t step0 = odd ? half_steps<7>(r0) : half_steps<15>(r0), step8 = odd ? half_steps<7>(r8) : half_steps<15>(r8);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint4 s = p[c >> 1], n = p[2 + (c >> 1)];
-            const uint32_t s0 = c & 1 ? s.z : s.x, s8 = c & 1 ? s.w : s.y, n0 = c & 1 ? n.z : n.x, n8 = c & 1 ? n.w : n.y;
-            const uint32_t step0 = half_steps<15>(prmt(s0, n0, 0x5410u)), step8 = half_steps<15>(prmt(s8, n8, 0x5410u));
-            const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint4 y = w[c >> 1];
-                const int k = 2 * (c & 1) + i;
-                uint32_t v[4];
-                nib8_to_h2x4(k == 0 ? y.x : k == 1 ? y.y : k == 2 ? y.z : y.w, v);
-                const uint32_t d = 32 * c + 16 * i + r;
-                put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
-                put(d + 8, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
-            }
-        }
-    } else {
-        const uint8_t *half = tile + 1024;
-        const uint4 e = ld16(half + 16 * lane);
-        const uint2 o = *reinterpret_cast<const uint2 *>(half + 512 + 8 * lane);
-        const uint32_t plane = *reinterpret_cast<const uint32_t *>(half + 768 + 4 * lane);
-        const uint4 s = ld16(half + 896 + 32 * a), n = ld16(half + 896 + 32 * a + 16);
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const uint32_t s0 = x ? s.z : s.x, s8 = x ? s.w : s.y, n0 = x ? n.z : n.x, n8 = x ? n.w : n.y;
-            const uint32_t r0 = prmt(s0, n0, 0x5410u), r8 = prmt(s8, n8, 0x5410u);
-            const uint32_t low0 = hmul2(prmt(s0, n0, 0x7632u), 0x38003800u), low8 = hmul2(prmt(s8, n8, 0x7632u), 0x38003800u);
-#pragma unroll
-            for (int odd = 0; odd < 2; odd++) {
-                const uint32_t step0 = odd ? half_steps<7>(r0) : half_steps<15>(r0), step8 = odd ? half_steps<7>(r8) : half_steps<15>(r8);
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const uint32_t codes = odd ? odd_codes(b ? o.y : o.x, (plane >> (16 * b)) & 0xFFFFu, x)
-                                               : x ? (b ? e.w : e.z) : (b ? e.y : e.x);
-                    uint32_t v[4];
-                    nib8_to_h2x4(codes, v);
-                    const uint32_t d = 64 * x + 32 * b + 2 * r + odd;
-                    put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
-                    put(d + 16, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
+                    for (int b = 0; b < 2; b++) {
+                        const uint32_t codes = odd ? odd_codes(b ? w[1].y : w[1].x, (w[1].z >> (16 * b)) & 0xFFFFu, x)
+                                                   : x ? (b ? w[0].w : w[0].z) : (b ? w[0].y : w[0].x);
+                        uint32_t v[4];
+                        nib8_to_h2x4(codes, v);
+                        const uint32_t d = 64 * x + 32 * b + 2 * r + odd;
+                        put(d, hfma2(v[0], step0, low0), hfma2(v[2], step8, low8));
+                        put(d + 16, hfma2(v[1], step0, low0), hfma2(v[3], step8, low8));
+                    }
                 }
             }
         }
     }
-}
+};
 
 // ---- values that a sequence's ends ask for ---------------------------------------
 //
@@ -962,26 +1002,45 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
 }
 
 // `n` values of a row: 32-byte stores where the type fills them
+__device__ __forceinline__ void store32(void *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 template <int N>
-__device__ __forceinline__ void store_values(void *out, uint64_t at, uint32_t dtype, const float *v) {
-    if (dtype == QWN_DTYPE_F32) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) store4(static_cast<float *>(out) + at + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-        return;
-    }
+__device__ __forceinline__ void store_floats(float *p, const float *v, bool wide) {
 #pragma unroll
     for (int i = 0; i < N; i += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (dtype == QWN_DTYPE_F16) {
-                w[k] = pack_h2(v[i + 2 * k], v[i + 2 * k + 1]);
-            } else {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
-                w[k] = *reinterpret_cast<const uint32_t *>(&b);
-            }
+        if (wide) {
+            store32(p + i, reinterpret_cast<const uint32_t *>(v + i));
+        } else {
+            store4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+            store4(p + i + 4, make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]));
         }
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_values(void *out, uint64_t at, uint32_t dtype, const float *v, bool wide) {
+    if (dtype == QWN_DTYPE_F32) return store_floats<N>(static_cast<float *>(out) + at, v, wide);
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; k++) {
+        if (dtype == QWN_DTYPE_F16) {
+            w[k] = pack_h2(v[2 * k], v[2 * k + 1]);
+        } else {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t *>(&b);
+        }
+    }
+    uint16_t *p = static_cast<uint16_t *>(out) + at;
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 8) {
+        if (wide) {
+            store32(p + 2 * i, w + i);
+        } else {
+            *reinterpret_cast<uint4 *>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            *reinterpret_cast<uint4 *>(p + 2 * i + 8) = make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]);
+        }
     }
 }
 
@@ -1106,11 +1165,59 @@ struct AtRoles {
         warp_arrive(&sh.helped, lane);
         return wait(&sh.helped, syncs++ & 1);
     }
-    // K and V of a block out of cached tiles or fp32 rows
+    // K and V of a block out of cached codes: this warp's two tiles
+    __device__ __forceinline__ bool convert_codes(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
+        const int w = warp & 3;
+        const int32_t token0 = blk * S::kBlock;
+        const uint32_t slot = done & 3, ks = S::k_slot(done), vs = S::v_slot(done);
+        extern __shared__ uint8_t dynamic[];
+        uint32_t ring[2];
+        const uint8_t *tile[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t g = done * S::kTiles + w + 4 * i;
+            ring[i] = g % S::kRawTiles;
+            tile[i] = dynamic + (raw_at - smem_u32(dynamic)) + ring[i] * S::kTileBytes;
+            if (!wait(&sh.rawfull[ring[i]], (g / S::kRawTiles) & 1)) return false;
+        }
+        KeyWords<SRC> k[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) k[i].load(tile[i]);
+        if (!wait(&sh.empty[ks], (S::k_turn(done) & 1) ^ 1)) return false;
+        if constexpr (kTokenScales) {  // read when the block's scores are there
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int t = lane & 15, v = lane >> 4, ti = w + 4 * i;
+                const float sc = token0 + ti * kTileTokens + t < seg.len ? token_scale<SRC>(tile[i], t, v) : 0.f;
+                (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + cached_order(t)] = sc;
+                const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
+                if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) k[i].store(tile[i], w + 4 * i, slot_at(ks));
+        fence_proxy_async_shared();
+        warp_arrive(&sh.full[ks], lane);
+        ValueWords<SRC> v[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) v[i].load(tile[i]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) warp_arrive(&sh.rawempty[ring[i]], lane);
+        if (!wait(&sh.empty[vs], (S::v_turn(done) & 1) ^ 1)) return false;
+#pragma unroll
+        for (int i = 0; i < 2; i++) v[i].store(w + 4 * i, slot_at(vs));
+        if (!whole(seg, blk)) {
+            if (!helpers_sync(syncs)) return false;
+            clear_odd_by_dims(sh.odd_v[segment & 3], seg, token0, slot_at(vs));
+        }
+        fence_proxy_async_shared();
+        warp_arrive(&sh.full[vs], lane);
+        return true;
+    }
+    // the same out of fp16 pages, and of anything in parts
     __device__ __forceinline__ bool convert(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
         const int w = warp & 3;
         const int32_t token0 = blk * S::kBlock;
-        const uint32_t slot = done & 3;
 #pragma unroll
         for (int which = 0; which < 2; which++) {
             const uint32_t s = which ? S::v_slot(done) : S::k_slot(done), dst = slot_at(s);
@@ -1127,19 +1234,7 @@ struct AtRoles {
                     } else if (at < seg.len) {
                         tile = at_tile(a, seg.seq, seg.head, at);
                     }
-                    if constexpr (kTokenScales) {
-                        if (!which) {  // both scales, read when the block's scores are there
-                            const int t = lane & 15, v = lane >> 4;
-                            const float sc = at + t < seg.len ? token_scale<SRC>(tile, t, v) : 0.f;
-                            (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + cached_order(t)] = sc;
-                            const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
-                            if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
-                        }
-                    }
-                    if constexpr (S::kByDims) {
-                        if (which) put_values<SRC>(tile, ti, dst);
-                        else put_keys<SRC>(tile, ti, dst);
-                    } else if constexpr (PARTS == 1) {  // fp16 as it is: the tile's chunks are swizzled alike
+                    if constexpr (PARTS == 1) {  // fp16 as it is: the tile's chunks are swizzled alike
                         if (tile) {
 #pragma unroll
                             for (int k = 0; k < 8; k++) {
@@ -1172,8 +1267,7 @@ struct AtRoles {
             if constexpr (S::kPaged && PARTS == 1 && !S::kRaw) asm volatile("cp.async.wait_all;" ::: "memory");
             if (which && !whole(seg, blk)) {
                 if (!helpers_sync(syncs)) return false;
-                if constexpr (S::kByDims) clear_odd_by_dims(sh.odd_v[segment & 3], seg, token0, dst);
-                else clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
+                clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
             }
             fence_proxy_async_shared();
             warp_arrive(&sh.full[s], lane);
@@ -1206,7 +1300,10 @@ struct AtRoles {
             for (int b = 0; b < seg.blocks; b++, done++) {
                 const int blk = seg.block0 + b;
                 if constexpr (!S::kTma) {
-                    if (!convert(seg, blk, done, used, syncs)) return;
+                    bool ok;
+                    if constexpr (S::kByDims) ok = convert_codes(seg, blk, done, used, syncs);
+                    else ok = convert(seg, blk, done, used, syncs);
+                    if (!ok) return;
                 } else if (!whole(seg, blk)) {
                     const uint32_t s = S::v_slot(done);
                     if (!wait(&sh.part[s], phase >> s & 1)) return;
@@ -1556,11 +1653,9 @@ struct AtRoles {
 #pragma unroll
                 for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
                 if (slot) {
-#pragma unroll
-                    for (int k = 0; k < kWide; k += 4)
-                        store4(slot + (size_t)r * kHeadDim + col + k, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+                    store_floats<kWide>(slot + (size_t)r * kHeadDim + col, o, a.wide_slots);
                 } else {
-                    store_values<kWide>(a.out, at + col, a.dtype, o);
+                    store_values<kWide>(a.out, at + col, a.dtype, o, a.wide_out);
                 }
             }
             if (slot && have && (TILES == 2 || g == 0)) {
