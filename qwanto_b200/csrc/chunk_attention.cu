@@ -19,9 +19,8 @@ template <int SRC, int PARTS, int TILES>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArgs a, uint32_t grid) {
     using W = AtWork<SRC, PARTS, TILES>;
     constexpr uint32_t kRows = W::kRows;
-    const uint64_t warp = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t row = (uint32_t)(warp / a.query_heads), qh = (uint32_t)(warp % a.query_heads);
+    const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t row = warp / a.query_heads, qh = warp - row * a.query_heads;
     launch_dependents();
     wait_previous();
     if (row >= a.rows.num_rows) return;
@@ -39,15 +38,16 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
     if ((int64_t)row < s.begin || (int64_t)row >= s.begin + s.rows) return;  // of no sequence
     int32_t first;
     const uint32_t span = at_span(a, s, AtShape<SRC, PARTS, TILES>::kBlock, first);
-    const uint64_t total = a.prefix[a.rows.num_seqs], ctas = min((uint64_t)grid, total);
-    const uint64_t r = (uint64_t)(row - s.begin) * a.group + qh % a.group;
-    const uint64_t u0 = a.prefix[i] + (r / kRows * a.kv_heads + qh / a.group) * span, u1 = u0 + span;
-    // CTA b has blocks [b total / ctas, (b + 1) total / ctas)
-    const uint32_t b0 = (uint32_t)(((u0 + 1) * ctas - 1) / total), b1 = (uint32_t)((u1 * ctas - 1) / total);
+    const uint32_t total = a.prefix[a.rows.num_seqs];
+    const AtRuns runs(total, min(grid, total));
+    const uint32_t kv = qh / a.group, r = (row - (uint32_t)s.begin) * a.group + qh - kv * a.group;
+    const uint32_t u0 = a.prefix[i] + (r / kRows * a.kv_heads + kv) * span;
+    const uint32_t b0 = runs.owner(u0), b1 = runs.owner(u0 + span - 1);
     if (b0 == b1) return;  // finished by its CTA
-    const uint32_t at = (uint32_t)(r % kRows);
+    const uint32_t at = r % kRows;
+    const bool second = u0 > runs.begin(b0);
     auto slot = [&](uint32_t b) {  // a CTA's first segment, or its second slot
-        const bool later = b == b0 && u0 > (uint64_t)b * total / ctas;
+        const bool later = b == b0 && second;
         return a.slots + (size_t)(2 * b + (later ? 1 : 0)) * at_slot_floats(TILES);
     };
     float M = -INFINITY;
@@ -89,8 +89,10 @@ ChunkPlan plan_chunk(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32
     c.tiles = dtype != QWN_DTYPE_F32 && rows > 128ull * num_seqs ? 2 : 1;
     const uint64_t tile = 128ull * c.tiles;
     c.units = runs ? rows / tile + num_seqs : num_seqs * ((group + tile - 1) / tile);
-    c.prefix_bytes = ((uint64_t)num_seqs + 1) * 8 + 255 & ~255ull;
-    c.split = c.units * p->kv_heads < 8ull * p->sms;
+    c.prefix_bytes = ((uint64_t)num_seqs + 1) * 4 + 255 & ~255ull;
+    // blocks are counted in 32 bits
+    const uint64_t most = (uint64_t)p->max_pages_per_seq * p->page_tokens / 64 + 2;
+    c.split = c.units * p->kv_heads < 8ull * p->sms && c.units * p->kv_heads * most < 1ull << 31;
     c.workspace = c.split ? c.prefix_bytes + 2ull * p->sms * at_slot_floats(c.tiles) * sizeof(float) : 0;
     return c;
 }
@@ -156,7 +158,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     const ChunkPlan c = plan_chunk(p, r->num_seqs, r->num_rows, r->query_heads, r->dtype, r->row_begin_dev != nullptr);
     if (r->workspace_dev && ((uintptr_t)r->workspace_dev % 16 || r->workspace_bytes < c.workspace))
         return invalid("qwn_kv_chunk_attention: workspace must be 16-byte aligned and as large as qwn_kv_chunk_workspace tells");
-    if (c.units * p->kv_heads > 0x7FFFFFFFull || ((uint64_t)r->num_rows * r->query_heads + 3) / 4 > 0x7FFFFFFFull ||
+    if (c.units * p->kv_heads > 0x7FFFFFFFull || (uint64_t)r->num_rows * r->query_heads > 0x7FFFFFFFull ||
         (uint64_t)r->num_rows * (r->query_heads / p->kv_heads) > 0xFFFFFFFFull)
         return invalid("qwn_kv_chunk_attention: too many rows for one call");
     DeviceScope scope(p->device);
@@ -173,16 +175,14 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     a.scale2 = (r->scale > 0.f ? r->scale : 0.08838834764831845f) * 1.4426950408889634f;
     a.query_stride = qs;
     a.out_stride = os;
-    a.wide_out = rows_aligned(r->output_dev, os, r->dtype, 32 / es);
     a.query = r->query_dev;
     a.out = r->output_dev;
     a.geo = store_geo(p);
     a.status = p->status;
     a.units = (uint32_t)c.units;
     if (c.split && r->workspace_dev) {
-        a.prefix = static_cast<uint64_t *>(r->workspace_dev);
+        a.prefix = static_cast<uint32_t *>(r->workspace_dev);
         a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(r->workspace_dev) + c.prefix_bytes);
-        a.wide_slots = (uintptr_t)a.slots % 32 == 0;
     }
     cudaStream_t s = stream_of(p, r->stream);
     cudaError_t e;

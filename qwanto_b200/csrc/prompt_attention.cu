@@ -77,7 +77,6 @@ QWN_CUDA_ABI_API int qwn_prompt_attention(const QwnPromptAttentionRequest *r) {
     a.scale2 = (r->scale > 0.f ? r->scale : 0.08838834764831845f) * 1.4426950408889634f;
     a.query_stride = qs, a.key_stride = ks, a.value_stride = vs, a.out_stride = os;
     a.query = r->query_dev, a.key = r->key_dev, a.value = r->value_dev, a.out = r->output_dev;
-    a.wide_out = rows_aligned(r->output_dev, os, r->dtype, 32 / es);
     a.status = r->status_dev;
     const uint64_t rows = (uint64_t)r->num_rows * a.group;
     if (rows > 0xFFFFFFFFull) return invalid("qwn_prompt_attention: too many rows for one call");

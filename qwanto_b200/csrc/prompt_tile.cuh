@@ -16,11 +16,11 @@
 // rows): S = Q K^T from shared memory, then O += P V with P as the A operand out
 // of tensor memory, where it lies over the S that it came from.
 //
-// A CTA has 16 warps:
+// A CTA has 16 warps, or 20:
 //   0-3, 4-7   softmax, one thread per row: S out of tensor memory, P back into it
-//   8-11       Q into shared memory; cached tiles into operand tiles; whatever a
-//              sequence's ends ask for
-//   12         MMAs      13  loads      14  the list of work
+//   8-11       helpers: Q into shared memory; cached tiles into operand tiles;
+//              whatever a sequence's ends ask for.  8-15 where codes are converted
+//   then       MMAs, loads, the list of work
 // The two softmax groups take turns with the tensor core.  TILES = 2: each has 128
 // of the CTA's 256 rows and both read the same keys.  TILES = 1: both work on the
 // same 128 rows, one on the even blocks of tokens and one on the odd ones, and
@@ -42,12 +42,7 @@
 namespace qkv {
 namespace {
 
-constexpr int kAtThreads = 512;
 constexpr int kAtRows = 128;  // rows of a tile: the lanes of tensor memory
-// registers per thread after the split: 2 x softmax + helpers + the rest = 4 x 128 at launch
-constexpr int kSoftmaxRegs = 184, kHelperRegs = 96, kOtherRegs = 48;
-static_assert(2 * kSoftmaxRegs + kHelperRegs + kOtherRegs <= 4 * 128, "no more registers than the block starts with");
-
 // one CTA's piece of work: rows of one sequence and kv head, and the blocks of tokens that it takes
 struct AtSegment {
     int32_t valid;             // 0: no more work
@@ -73,9 +68,8 @@ struct AtArgs {
     StoreGeo geo;              // paged
     uint32_t *status;
     uint32_t units;            // row tiles, without a split
-    uint64_t *prefix;          // split: blocks before each sequence, then
+    uint32_t *prefix;          // split: blocks before each sequence and in all, then
     float *slots;              // the partial results
-    bool wide_out, wide_slots; // rows of the output and of the partial results start on 32 bytes
 };
 // a partial result: o[rows][128], then M[rows], l[rows]
 __host__ __device__ constexpr uint32_t at_slot_floats(uint32_t tiles) { return tiles * kAtRows * (kHeadDim + 2); }
@@ -85,6 +79,14 @@ struct AtShape {
     static constexpr bool kPaged = SRC != 0;
     static constexpr bool kTma = !kPaged && PARTS == 1;            // operand tiles straight from the rows
     static constexpr bool kRaw = kPaged && SRC != QWN_KV_CODEC_F16;// cached tiles by way of shared memory
+    // Registers per thread after the split, no more in all than the block starts with.  The softmax warps hold a
+    // row's 128 scores; what they lack goes to memory (16384 rows of 13 prompts: 334 us with 184, 299 with 200).
+    // Where codes are converted the scores are read twice out of tensor memory instead, and twice as many helpers
+    // have the registers.
+    static constexpr int kHelpers = PARTS == 1 && kRaw ? 8 : 4, kThreads = 384 + 32 * kHelpers;
+    static constexpr int kLaunchRegs = kHelpers == 8 ? 96 : 128, kSoftmaxRegs = kTma ? 200 : kHelpers == 8 ? 104 : 184;
+    static constexpr int kHelperRegs = kTma ? 64 : 96, kOtherRegs = kHelpers == 8 ? 80 : 48;
+    static_assert(2 * kSoftmaxRegs + kHelpers / 4 * kHelperRegs + kOtherRegs <= kThreads / 128 * kLaunchRegs, "registers");
     // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
     // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
     static constexpr bool kByDims = PARTS == 1 && kRaw;
@@ -96,7 +98,7 @@ struct AtShape {
     // are apart, so that K of the next block does not wait behind V of this one.
     static constexpr uint32_t kRing = kTma ? 5 : 0;
     static constexpr uint32_t kStagesK = PARTS == 1 ? 2 : 1;
-    static constexpr uint32_t kStagesV = PARTS == 1 && !(kPaged && TILES == 2) ? 2 : 1;
+    static constexpr uint32_t kStagesV = kTma ? 2 : 1;
     static constexpr uint32_t kStages = kRing ? kRing : kStagesK + kStagesV;
     static constexpr uint32_t kOperands = TILES * kQBytes + kStages * kKvBytes;
     static constexpr uint32_t kSmem = (227 - (!kTma ? 12 : TILES == 2 ? 2 : 8)) * 1024;  // the rest is static
@@ -120,7 +122,7 @@ struct AtShape {
 
 constexpr uint32_t kAtStages = 5;
 template <int SRC, int PARTS, int TILES>
-struct AtShared {
+struct alignas(1024) AtShared {  // the operands behind it start on 1024 bytes
     static constexpr bool kTokens = PARTS == 1 && (SRC == QWN_KV_CODEC_Q8_B64_F32 || SRC == QWN_KV_CODEC_Q8_HEAD_F16);
     static constexpr int kRaw = SRC == 0 ? 1 : 32;
     // operands of K and V have landed, are free again; V of a block seen in part (loaded ones only): has landed, is ready
@@ -190,16 +192,19 @@ __device__ __forceinline__ uint64_t rows_desc(uint32_t addr, uint32_t column_byt
 }
 #define QKV_R8(r, b) "=r"(r[b]), "=r"(r[b + 1]), "=r"(r[b + 2]), "=r"(r[b + 3]), "=r"(r[b + 4]), "=r"(r[b + 5]), "=r"(r[b + 6]), "=r"(r[b + 7])
 #define QKV_R64(r, b) QKV_R8(r, b), QKV_R8(r, b + 8), QKV_R8(r, b + 16), QKV_R8(r, b + 24), QKV_R8(r, b + 32), QKV_R8(r, b + 40), QKV_R8(r, b + 48), QKV_R8(r, b + 56)
-// 64 columns of the warp's 32 lanes, complete on return
+// 64 columns of the warp's 32 lanes, complete on return; in two loads, as one may
+// not take more registers than a thread has at launch
 __device__ __forceinline__ void tmem_load64(uint32_t *r, uint32_t addr) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31" "}, [%64];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
         "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63" "}, [%65];\n"
         "tcgen05.wait::ld.sync.aligned;"
         : QKV_R64(r, 0)
-        : "r"(addr)
+        : "r"(addr), "r"(addr + 32)
         : "memory");
 }
 // the same for 128 columns, in two loads behind one wait
@@ -301,7 +306,7 @@ __device__ __forceinline__ AtSegment at_segment(const AtArgs &a, const AtSequenc
     t.head = head;
     t.len = s.len;
     t.pos0 = s.pos0;
-    const int64_t p0 = s.pos0 + row0 / a.group, p1 = s.pos0 + (row0 + t.rows - 1) / a.group;
+    const int64_t p0 = s.pos0 + row0 / a.group, p1 = s.pos0 + (row0 + (uint32_t)t.rows - 1) / a.group;
     int32_t b1;
     at_blocks(a, p0, p1, s.len, block, t.block0, b1);
     t.blocks = b1 - t.block0;
@@ -332,66 +337,73 @@ __device__ __forceinline__ uint32_t at_span(const AtArgs &a, const AtSequence &s
 // With one, the blocks of all tiles in a row (sequence, tile, head, block) are cut
 // into as many equal runs as there are CTAs; a tile that a cut goes through is
 // finished by the join kernel.
+// The runs of `total` blocks over `ctas` CTAs: the first `more` of them have one block more than `each`.
+struct AtRuns {
+    uint32_t each, more;
+    __device__ __forceinline__ AtRuns(uint32_t total, uint32_t ctas) : each(total / ctas), more(total % ctas) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t cta) const { return cta * each + min(cta, more); }
+    __device__ __forceinline__ uint32_t owner(uint32_t block) const {
+        const uint32_t longer = more * (each + 1);
+        return block < longer ? block / (each + 1) : more + (block - longer) / each;
+    }
+};
 template <int SRC, int PARTS, int TILES>
 struct AtWork {
     using S = AtShape<SRC, PARTS, TILES>;
     static constexpr uint32_t kRows = TILES * kAtRows;
     const AtArgs &a;
-    uint64_t at, end;      // run of blocks
-    uint64_t left;         // of it, in this sequence
+    uint32_t at, end;      // run of blocks
     uint32_t i, span, n;   // sequence, its blocks per tile, segments so far
     int32_t first;
-    uint64_t within;       // blocks into the sequence
+    uint32_t item, from;   // (row tile, head) of the sequence, block of it
     AtSequence s;
 
     __device__ __forceinline__ explicit AtWork(const AtArgs &args) : a(args) {
-        at = end = left = 0;
-        i = span = n = 0;
+        at = end = i = span = n = item = from = 0;
         first = 0;
-        within = 0;
         if (!a.slots) return;
         const uint32_t lane = threadIdx.x & 31;
         // the blocks of all sequences, 32 sequences at a time
-        uint64_t total = 0;
-        for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) total += warp_sum(weight(k + lane));
-        const uint64_t ctas = min((uint64_t)gridDim.x, total);  // each has a block at least
-        if (blockIdx.x >= ctas) return;
-        at = blockIdx.x * total / ctas;
-        end = (blockIdx.x + 1) * total / ctas;
-        uint64_t before = 0;
+        uint32_t w = weight(lane), total = warp_sum(w);
+        for (uint32_t k = 32; k < a.rows.num_seqs; k += 32) total += warp_sum(weight(k + lane));
+        if (blockIdx.x >= min(gridDim.x, total)) return;  // each of the others has a block at least
+        const AtRuns runs(total, min(gridDim.x, total));
+        at = runs.begin(blockIdx.x);
+        end = runs.begin(blockIdx.x + 1);
+        uint32_t before = 0, within = 0;
         bool found = false;
         for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) {
-            const uint64_t w = weight(k + lane);
-            uint64_t upto = w;
+            if (k) w = weight(k + lane);
+            uint32_t upto = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= (uint32_t)o) upto += y;
             }
-            if (blockIdx.x == 0 && k + lane < a.rows.num_seqs) a.prefix[k + lane] = before + upto - w;
-            if (blockIdx.x == 0 && lane == 0) a.prefix[a.rows.num_seqs] = total;
+            if (blockIdx.x == 0) {  // the table for the join kernel
+                if (k + lane < a.rows.num_seqs) a.prefix[k + lane] = before + upto - w;
+                if (lane == 0) a.prefix[a.rows.num_seqs] = total;
+            }
             const uint32_t has = __ballot_sync(0xffffffffu, before + upto > at);
             if (has && !found) {
                 const int l = __ffs(has) - 1;
                 i = k + l;
                 within = at - (before + __shfl_sync(0xffffffffu, upto - w, l));
                 found = true;
-                if (blockIdx.x != 0) break;  // the first CTA also writes the table
+                if (blockIdx.x != 0) break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (at < end) open();
+        open();
+        item = within / span;
+        from = within % span;
     }
-    __device__ __forceinline__ static uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    }
-    __device__ __forceinline__ uint64_t weight(uint32_t k) const {
+    __device__ __forceinline__ static uint32_t warp_sum(uint32_t v) { return __reduce_add_sync(0xffffffffu, v); }
+    __device__ __forceinline__ uint32_t weight(uint32_t k) const {
         if (k >= a.rows.num_seqs) return 0;
         const AtSequence q = at_sequence(a, S::kPaged, k);
         int32_t f;
-        return at_row_tiles(a, q, kRows) * a.kv_heads * at_span(a, q, S::kBlock, f);
+        return (uint32_t)at_row_tiles(a, q, kRows) * a.kv_heads * at_span(a, q, S::kBlock, f);
     }
     __device__ __forceinline__ void open() {
         s = at_sequence(a, S::kPaged, i);
@@ -400,34 +412,33 @@ struct AtWork {
     __device__ __forceinline__ AtSegment next() {
         AtSegment t{};
         if (!a.slots) {
-            const uint64_t all = (uint64_t)a.units * a.kv_heads;
+            const uint32_t all = a.units * a.kv_heads;
             for (;;) {
-                const uint64_t k = (uint64_t)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                if ((uint64_t)n * gridDim.x >= all) return t;
+                if (n >= (all + gridDim.x - 1) / gridDim.x) return t;
+                const uint32_t k = n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 n++;
-                if (k < all) t = single(a.units - 1 - (uint32_t)(k / a.kv_heads), (uint32_t)(k % a.kv_heads));
+                if (k < all) t = single(a.units - 1 - k / a.kv_heads, k % a.kv_heads);
                 if (t.valid) return t;
             }
         }
         while (at < end) {
-            const uint64_t item = within / span, tiles = at_row_tiles(a, s, kRows);
-            if (item >= tiles * a.kv_heads) {  // the next sequence
+            if (item >= (uint32_t)at_row_tiles(a, s, kRows) * a.kv_heads) {  // the next sequence
                 if (++i >= a.rows.num_seqs) return t;
-                within = 0;
+                item = from = 0;
                 open();
                 continue;
             }
-            const uint32_t from = (uint32_t)(within % span);
-            const uint32_t count = (uint32_t)min((uint64_t)(span - from), end - at);
-            t = at_segment(a, s, (uint32_t)(item / a.kv_heads) * kRows, kRows, (int32_t)(item % a.kv_heads), S::kBlock);
+            const uint32_t count = min(span - from, end - at);
+            t = at_segment(a, s, item / a.kv_heads * kRows, kRows, (int32_t)(item % a.kv_heads), S::kBlock);
             // of the tile's own blocks those in the run
             const int32_t b0 = max(t.block0, first + (int32_t)from), b1 = min(t.block0 + t.blocks, first + (int32_t)(from + count));
             if (count != span) t.slot = (int32_t)(2 * blockIdx.x + (n ? 1 : 0));
             t.block0 = b0;
             t.blocks = max(b1 - b0, 0);
-            within += count;
             at += count;
             n++;
+            item++;  // the run ends here, or the tile does
+            from = 0;
             return t;
         }
         return t;
@@ -486,78 +497,107 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // 16-byte chunk c (of 16) of row r in an operand tile of `rows` rows: two columns of 128-byte rows, swizzled
 __device__ __forceinline__ uint32_t chunk_at(uint32_t base, uint32_t rows, uint32_t r, uint32_t c) {
     return base + (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
-// Row r of the segment by one thread.  For a cache, whose codes are f16 operands,
-// a row of bf16 is brought into f16's range by a power of two.
+// The 32 rows of a warp in a tile of Q, two at a time: 16 lanes read a row side by
+// side (a lane per row took 7 us for 256 rows, 32 lines to an instruction).  For a
+// cache, whose codes are f16 operands, a row of bf16 is brought into f16's range by
+// a power of two.
 template <int SRC, int PARTS>
-__device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint32_t r, uint32_t tile, float &unit) {
-    const uint32_t row = t.row0 + r, token = row / a.group, h = t.head * a.group + row % a.group;
-    const uint64_t at = (uint64_t)(t.token_row + token) * a.query_stride + h * kHeadDim;
-    const uint32_t lane_row = r % kAtRows;
-    unit = 1.f;
-    if constexpr (PARTS == 3) {
-        const float *q = static_cast<const float *>(a.query) + at;
-#pragma unroll 4
-        for (uint32_t c = 0; c < 16; c++) {
-            float v[8];
-            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(q + 8 * c);
-            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(q + 8 * c + 4);
-            uint4 p[3];
-            split3(v, p);
+__device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint32_t row0, uint32_t tile, float *unit) {
+    const uint32_t lane = threadIdx.x & 31, c = lane & 15, w0 = threadIdx.x & 96;  // the warp's first row
+    uint64_t mine = 0;  // where the lane's row starts
+    const bool have = (int32_t)(row0 + w0 + lane) < t.rows;
+    if (have) {
+        const uint32_t row = t.row0 + row0 + w0 + lane, token = row / a.group;
+        mine = (uint64_t)(t.token_row + token) * a.query_stride + (t.head * a.group + row - token * a.group) * kHeadDim;
+    }
+    const uint32_t rows = __ballot_sync(0xffffffffu, have);
+    if constexpr (SRC == 0 && PARTS == 1) {  // as it is
 #pragma unroll
-            for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(tile + k * kAtRows * 256, kAtRows, lane_row, c), p[k]);
+        for (uint32_t i = 0; i < 16; i++) {
+            const uint32_t r = 2 * i + (lane >> 4);
+            const uint64_t at = __shfl_sync(0xffffffffu, mine, r) + 8 * c;
+            if (rows >> r & 1) cp_async16_at(chunk_at(tile, kAtRows, w0 + r, c), static_cast<const uint16_t *>(a.query) + at);
         }
-    } else {
-        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.query) + at);
-        uint4 w[16];
+        return;
+    }
+    constexpr int kAhead = PARTS == 3 ? 4 : 16;  // loads in flight
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < 16; i0 += kAhead) {
+        if (!(rows >> (2 * i0))) break;
+        uint4 w[kAhead][PARTS == 3 ? 2 : 1];
 #pragma unroll
-        for (uint32_t c = 0; c < 16; c++) w[c] = q[c];
-        if (SRC != 0 && a.dtype == QWN_DTYPE_BF16) {
-            uint32_t top = 0;  // largest exponent of a finite value
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const uint32_t r = 2 * (i0 + i) + (lane >> 4);
+            const uint64_t at = __shfl_sync(0xffffffffu, mine, r) + 8 * c;
 #pragma unroll
-            for (uint32_t c = 0; c < 16; c++) {
-                const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint32_t e0 = u[k] & 0x7F80u, e1 = (u[k] >> 16) & 0x7F80u;
-                    top = max(top, max(e0 == 0x7F80u ? 0u : e0, e1 == 0x7F80u ? 0u : e1));
+            for (int k = 0; k < (PARTS == 3 ? 2 : 1); k++) w[i][k] = make_uint4(0, 0, 0, 0);
+            if (rows >> r & 1) {
+                if constexpr (PARTS == 3) {
+                    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.query) + at);
+                    w[i][0] = q[0];
+                    w[i][1] = q[1];
+                } else {
+                    w[i][0] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.query) + at);
                 }
             }
-            // the largest value to 2^8 .. 2^9: what is below 2^-22 of it loses bits
-            const int e = max(-100, min((int)(top >> 7) - 127 - 8, 119));
-            unit = __uint_as_float((uint32_t)(e + 127) << 23);
-            const float per = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-            for (uint32_t c = 0; c < 16; c++) {
-                uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    u[k] = pack_h2(__uint_as_float(u[k] << 16) * per, __uint_as_float(u[k] & 0xFFFF0000u) * per);
-                w[c] = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-        }
-        // dims in the order that K's words give them
-        if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
-#pragma unroll
-            for (uint32_t c = 0; c < 16; c++)
-                w[c] = make_uint4(prmt(w[c].x, w[c].y, 0x5410u), prmt(w[c].z, w[c].w, 0x5410u), prmt(w[c].x, w[c].y, 0x7632u),
-                                  prmt(w[c].z, w[c].w, 0x7632u));
-        } else if constexpr (SRC == QWN_KV_CODEC_TQ35_G64) {
-#pragma unroll
-            for (uint32_t c = 0; c < 16; c += 2) {
-                const uint4 a = w[c], b = w[c + 1];
-                auto order = [&](uint32_t sel) {
-                    return make_uint4(prmt(a.x, a.z, sel), prmt(b.x, b.z, sel), prmt(a.y, a.w, sel), prmt(b.y, b.w, sel));
-                };
-                w[c] = order(0x5410u);
-                w[c + 1] = order(0x7632u);
-            }
         }
 #pragma unroll
-        for (uint32_t c = 0; c < 16; c++) st_shared16(chunk_at(tile, kAtRows, lane_row, c), w[c]);
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const uint32_t r = w0 + 2 * (i0 + i) + (lane >> 4);
+            if constexpr (PARTS == 3) {
+                uint4 p[3];
+                split3(reinterpret_cast<const float *>(w[i]), p);
+#pragma unroll
+                for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(tile + k * kAtRows * 256, kAtRows, r, c), p[k]);
+            } else {
+                uint32_t u[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
+                if (SRC != 0) {
+                    float scale = 1.f;
+                    if (a.dtype == QWN_DTYPE_BF16) {
+                        uint32_t top = 0;  // largest exponent of a finite value
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t e0 = u[k] & 0x7F80u, e1 = (u[k] >> 16) & 0x7F80u;
+                            top = max(top, max(e0 == 0x7F80u ? 0u : e0, e1 == 0x7F80u ? 0u : e1));
+                        }
+#pragma unroll
+                        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        // the largest value to 2^8 .. 2^9: what is below 2^-22 of it loses bits
+                        const int e = max(-100, min((int)(top >> 7) - 127 - 8, 119));
+                        scale = __uint_as_float((uint32_t)(e + 127) << 23);
+                        const float per = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            u[k] = pack_h2(__uint_as_float(u[k] << 16) * per, __uint_as_float(u[k] & 0xFFFF0000u) * per);
+                    }
+                    if (c == 0) unit[row0 + r] = scale;
+                }
+                // dims in the order that K's words give them
+                if constexpr (SRC == QWN_KV_CODEC_Q4_G32) {
+                    const uint32_t v[4] = {u[0], u[1], u[2], u[3]};
+                    u[0] = prmt(v[0], v[1], 0x5410u), u[1] = prmt(v[2], v[3], 0x5410u);
+                    u[2] = prmt(v[0], v[1], 0x7632u), u[3] = prmt(v[2], v[3], 0x7632u);
+                } else if constexpr (SRC == QWN_KV_CODEC_TQ35_G64) {  // even dims of 16 to the first chunk, odd ones to the second
+                    uint32_t o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) o[k] = __shfl_xor_sync(0xffffffffu, u[k], 1);
+                    const bool odd = c & 1;
+                    const uint32_t sel = odd ? 0x7632u : 0x5410u;
+                    const uint32_t x[4] = {odd ? o[0] : u[0], odd ? o[1] : u[1], odd ? o[2] : u[2], odd ? o[3] : u[3]};
+                    const uint32_t y[4] = {odd ? u[0] : o[0], odd ? u[1] : o[1], odd ? u[2] : o[2], odd ? u[3] : o[3]};
+                    u[0] = prmt(x[0], x[2], sel), u[1] = prmt(y[0], y[2], sel);
+                    u[2] = prmt(x[1], x[3], sel), u[3] = prmt(y[1], y[3], sel);
+                }
+                st_shared16(chunk_at(tile, kAtRows, r, c), make_uint4(u[0], u[1], u[2], u[3]));
+            }
+        }
     }
 }
 
@@ -643,9 +683,6 @@ __device__ __forceinline__ uint32_t half_steps(uint32_t ranges) {
     constexpr float f = 0.5f / LEVELS, near = LEVELS == 15 ? 1092.f / 32768.f : 1170.f / 16384.f;
     return hfma2(ranges, pack_h2(near, near), hmul2(ranges, pack_h2(f - near, f - near)));
 }
-__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ uint4 ld16(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 // eight codes of 3.5-bit words: odd dims of half 1 have their lowest bit above half 0's and two in a plane
 __device__ __forceinline__ uint32_t odd_codes(uint32_t odd, uint32_t plane, int x) {
@@ -656,9 +693,7 @@ __device__ __forceinline__ uint32_t odd_codes(uint32_t odd, uint32_t plane, int 
     return ((odd >> 3) & 0x11111111u) | (p << 1);
 }
 // K of a tile: rows of 128 dims (in the order that put_q gives the queries).  What
-// a lane converts is loaded before it stores anything, two tiles at a time: a lone
-// warp per scheduler waits for its loads otherwise (32 x 4 rows over 8192 int8
-// tokens: 248 us).
+// a lane converts is loaded before it stores anything.
 template <int SRC>
 struct KeyWords {
     static constexpr bool kInt8 = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32;
@@ -879,10 +914,10 @@ __device__ __forceinline__ void note_odd(uint32_t (&noted)[2][16], const AtSegme
     if (i < 512) atomicOr(&noted[token < z ? 0 : 1][i >> 5], 1u << (i & 31));
 }
 __device__ __noinline__ void clear_odd_by_dims(uint32_t (&noted)[2][16], const AtSegment &seg, int32_t token0, uint32_t base) {
-    const uint32_t d = threadIdx.x & 127;
+    const uint32_t d = threadIdx.x & 127, c0 = threadIdx.x & 128 ? 8 : 0;  // two warpgroups: a half of the tokens each
     const int32_t left = seg.len - token0;  // tokens of the block that exist
 #pragma unroll 1
-    for (uint32_t c = 0; c < 16; c++) {  // eight tokens each
+    for (uint32_t c = c0; c < c0 + 8; c++) {  // eight tokens each
         const uint32_t at = base + (c >> 3) * 16384 + d * 128 + (((c & 7) ^ (d & 7)) << 4);
         const uint4 w = ld_shared16(at);
         uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -1001,47 +1036,48 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
     return mul2(y, pair(__uint_as_float(n0 << 23), __uint_as_float(n1 << 23)));
 }
 
-// `n` values of a row: 32-byte stores where the type fills them
-__device__ __forceinline__ void store32(void *p, const uint32_t *w) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-template <int N>
-__device__ __forceinline__ void store_floats(float *p, const float *v, bool wide) {
+// Four 16-byte pieces of each lane's row to memory: the four lanes of a group
+// exchange them, so that they write 64 bytes of a row side by side, eight rows to an
+// instruction (a lane per row: 32 rows, 7 us a tile).  `row` is where the lane's row
+// starts, `have` the lanes that have one.
+__device__ __forceinline__ void store_rows(uint8_t *row, uint32_t have, const uint4 (&piece)[4]) {
+    const uint32_t lane = threadIdx.x & 31, q = lane & 3;
+    uint32_t w[4][4];
 #pragma unroll
-    for (int i = 0; i < N; i += 8) {
-        if (wide) {
-            store32(p + i, reinterpret_cast<const uint32_t *>(v + i));
-        } else {
-            store4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-            store4(p + i + 4, make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]));
+    for (int k = 0; k < 4; k++) w[k][0] = piece[k].x, w[k][1] = piece[k].y, w[k][2] = piece[k].z, w[k][3] = piece[k].w;
+    // a 4 x 4 transposition: pieces (0, 1), (2, 3) with the neighbour, then (0, 2), (1, 3) with the lane two on
+#pragma unroll
+    for (int s = 1; s <= 2; s <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k & s) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t give = q & s ? w[k][e] : w[k | s][e], got = __shfl_xor_sync(0xffffffffu, give, s);
+                if (q & s) w[k][e] = got;
+                else w[k | s][e] = got;
+            }
         }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {  // piece q of the group's row k
+        const uint32_t from = (lane & ~3u) | k;
+        uint8_t *p = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), from));
+        if (have >> from & 1) *reinterpret_cast<uint4 *>(p + 16 * q) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
     }
 }
-template <int N>
-__device__ __forceinline__ void store_values(void *out, uint64_t at, uint32_t dtype, const float *v, bool wide) {
-    if (dtype == QWN_DTYPE_F32) return store_floats<N>(static_cast<float *>(out) + at, v, wide);
-    uint32_t w[N / 2];
+// 16 values of the lane's row as 16-bit pieces 0 and 1, or as fp32 pieces 0 to 3
+__device__ __forceinline__ uint4 pack8(const float *v, bool f16) {
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < N / 2; k++) {
-        if (dtype == QWN_DTYPE_F16) {
+    for (int k = 0; k < 4; k++) {
+        if (f16) {
             w[k] = pack_h2(v[2 * k], v[2 * k + 1]);
         } else {
             const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
             w[k] = *reinterpret_cast<const uint32_t *>(&b);
         }
     }
-    uint16_t *p = static_cast<uint16_t *>(out) + at;
-#pragma unroll
-    for (int i = 0; i < N / 2; i += 8) {
-        if (wide) {
-            store32(p + 2 * i, w + i);
-        } else {
-            *reinterpret_cast<uint4 *>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-            *reinterpret_cast<uint4 *>(p + 2 * i + 8) = make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]);
-        }
-    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int SRC, int PARTS, int TILES, bool BF16>
@@ -1051,6 +1087,7 @@ struct AtRoles {
     static constexpr bool kTokenScales = PARTS == 1 && Scale::kTokens;
     // the operands' own scaling: of scores and of outputs
     static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
+    static constexpr bool kHold = PARTS == 3 || S::kTma;  // a row's scores stay in registers
     static constexpr uint32_t kFmaPairs = 0x10;  // of eight pairs of powers, those that FMAs compute
     const AtArgs &a;
     AtShared<SRC, PARTS, TILES> &sh;
@@ -1165,29 +1202,30 @@ struct AtRoles {
         warp_arrive(&sh.helped, lane);
         return wait(&sh.helped, syncs++ & 1);
     }
-    // K and V of a block out of cached codes: this warp's two tiles
+    // K and V of a block out of cached codes: this warp's tiles
     __device__ __forceinline__ bool convert_codes(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
-        const int w = warp & 3;
+        constexpr int kMine = S::kTiles / S::kHelpers;
+        const int w = warp - 8;
         const int32_t token0 = blk * S::kBlock;
         const uint32_t slot = done & 3, ks = S::k_slot(done), vs = S::v_slot(done);
         extern __shared__ uint8_t dynamic[];
-        uint32_t ring[2];
-        const uint8_t *tile[2];
+        uint32_t ring[kMine];
+        const uint8_t *tile[kMine];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t g = done * S::kTiles + w + 4 * i;
+        for (int i = 0; i < kMine; i++) {
+            const uint32_t g = done * S::kTiles + w + S::kHelpers * i;
             ring[i] = g % S::kRawTiles;
             tile[i] = dynamic + (raw_at - smem_u32(dynamic)) + ring[i] * S::kTileBytes;
             if (!wait(&sh.rawfull[ring[i]], (g / S::kRawTiles) & 1)) return false;
         }
-        KeyWords<SRC> k[2];
+        KeyWords<SRC> k[kMine];
 #pragma unroll
-        for (int i = 0; i < 2; i++) k[i].load(tile[i]);
+        for (int i = 0; i < kMine; i++) k[i].load(tile[i]);
         if (!wait(&sh.empty[ks], (S::k_turn(done) & 1) ^ 1)) return false;
         if constexpr (kTokenScales) {  // read when the block's scores are there
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int t = lane & 15, v = lane >> 4, ti = w + 4 * i;
+            for (int i = 0; i < kMine; i++) {
+                const int t = lane & 15, v = lane >> 4, ti = w + S::kHelpers * i;
                 const float sc = token0 + ti * kTileTokens + t < seg.len ? token_scale<SRC>(tile[i], t, v) : 0.f;
                 (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + cached_order(t)] = sc;
                 const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
@@ -1195,17 +1233,17 @@ struct AtRoles {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++) k[i].store(tile[i], w + 4 * i, slot_at(ks));
+        for (int i = 0; i < kMine; i++) k[i].store(tile[i], w + S::kHelpers * i, slot_at(ks));
         fence_proxy_async_shared();
         warp_arrive(&sh.full[ks], lane);
-        ValueWords<SRC> v[2];
+        ValueWords<SRC> v[kMine];
 #pragma unroll
-        for (int i = 0; i < 2; i++) v[i].load(tile[i]);
+        for (int i = 0; i < kMine; i++) v[i].load(tile[i]);
 #pragma unroll
-        for (int i = 0; i < 2; i++) warp_arrive(&sh.rawempty[ring[i]], lane);
+        for (int i = 0; i < kMine; i++) warp_arrive(&sh.rawempty[ring[i]], lane);
         if (!wait(&sh.empty[vs], (S::v_turn(done) & 1) ^ 1)) return false;
 #pragma unroll
-        for (int i = 0; i < 2; i++) v[i].store(w + 4 * i, slot_at(vs));
+        for (int i = 0; i < kMine; i++) v[i].store(w + S::kHelpers * i, slot_at(vs));
         if (!whole(seg, blk)) {
             if (!helpers_sync(syncs)) return false;
             clear_odd_by_dims(sh.odd_v[segment & 3], seg, token0, slot_at(vs));
@@ -1280,20 +1318,14 @@ struct AtRoles {
         AtSegment seg;
         uint32_t done = 0, used = 0, syncs = 0;  // blocks, segments with any
         uint32_t phase = 0;  // of part, a bit per slot
-        const uint32_t tid = threadIdx.x & 127;
+        const uint32_t tid = threadIdx.x & 127, wg = (warp - 8) >> 2;
         while (take(f, seg)) {
             if (seg.blocks == 0) continue;
             if (!wait(&sh.qempty, (used & 1) ^ 1)) return;
-            if (tid < 32) sh.odd_v[used & 3][tid >> 4][tid & 15] = 0;
-#pragma unroll
-            for (int t = 0; t < TILES; t++) {
-                const uint32_t r = t * kAtRows + tid;
-                if ((int32_t)r < seg.rows) {
-                    float unit;
-                    put_q<SRC, PARTS>(a, seg, r, q_at + t * S::kQBytes, unit);
-                    if (SRC && PARTS == 1) sh.qscale[used & 1][r] = unit;
-                }
-            }
+            if (wg == 0 && tid < 32) sh.odd_v[used & 3][tid >> 4][tid & 15] = 0;
+#pragma unroll 1
+            for (int t = wg; t < TILES; t += S::kHelpers / 4) put_q<SRC, PARTS>(a, seg, t * kAtRows, q_at + t * S::kQBytes, sh.qscale[used & 1]);
+            if constexpr (S::kTma) asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async_shared();
             if (!helpers_sync(syncs)) return;  // odd_v is empty before any warp notes a token
             warp_arrive(&sh.qfull, lane);
@@ -1472,37 +1504,38 @@ struct AtRoles {
                                           float c, uint32_t s_col, uint32_t o_col, float &M, float &l) {
         constexpr int N = S::kBlock;
         using Range = AtRange<BF16 || PARTS == 3>;
-        uint32_t u[N];
-        float *x = reinterpret_cast<float *>(u);
-        if constexpr (N == 128) tmem_load128(u, s_col);
-        else tmem_load64(u, s_col);
+        const bool full = whole(seg, blk);
+        const int lo = seen.lo - blk * S::kBlock, hi = seen.hi - blk * S::kBlock;
         float vtop = 0.f;
         if constexpr (kTokenScales) {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const float4 k = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i]);
-                unpair(mul2(pair(x[i], x[i + 1]), pair(k.x, k.y)), x[i], x[i + 1]);
-                unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k.z, k.w)), x[i + 2], x[i + 3]);
-            }
             const float4 v0 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][0]), v1 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][4]);
             vtop = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)), fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
         }
-        const bool full = whole(seg, blk);
-        if (!full) {
-            const int lo = seen.lo - blk * N, hi = seen.hi - blk * N;
+        float t[8];
+        uint32_t held[kHold ? N : 1];
+        const float *x = reinterpret_cast<const float *>(held);
+        if constexpr (kHold) {
+            if constexpr (N == 128) tmem_load128(held, s_col);
+            else tmem_load64(held, s_col);
+            if (!full) hide(held, lo, hi);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int t = S::kByDims ? cached_token(i) : i;
-                if (t < lo || t >= hi) x[i] = -INFINITY;
+            for (int i = 0; i < 8; i++) t[i] = x[i];
+#pragma unroll
+            for (int i = 8; i < N; i += 8)
+#pragma unroll
+                for (int k = 0; k < 8; k++) t[k] = fmaxf(t[k], x[i + k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) t[k] = -INFINITY;
+#pragma unroll 1
+            for (int i = 0; i < N; i += 32) {
+                uint32_t u[32];
+                tmem_load32(u, s_col + i);
+                adjust(u, i, slot, full, lo, hi);
+#pragma unroll
+                for (int k = 0; k < 32; k++) t[k & 7] = fmaxf(t[k & 7], __uint_as_float(u[k]));
             }
         }
-        float t[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = x[i];
-#pragma unroll
-        for (int i = 8; i < N; i += 8)
-#pragma unroll
-            for (int k = 0; k < 8; k++) t[k] = fmaxf(t[k], x[i + k]);
         const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
         const float reach = top * c + vtop;
         const bool grows = have && reach > M + Range::kSlack;  // true for the first that is not -inf
@@ -1524,17 +1557,51 @@ struct AtRoles {
             }
         }
         const float off = Range::kBias - (M == -INFINITY ? 0.f : M);
-        // masked scores are -inf, whose power is exactly zero in the special function unit only
-        if (PARTS == 1 && full) l += powers<true>(x, slot, c, off, s_col);
-        else l += powers<false>(x, slot, c, off, s_col);
+        // P follows on S's columns, half as many (three parts: all of them).  Masked scores are -inf, whose power is
+        // exactly zero in the special function unit only.
+        if constexpr (kHold) {
+            if (PARTS == 1 && full) l += powers<true, N>(held, 0, slot, c, off, s_col);
+            else l += powers<false, N>(held, 0, slot, c, off, s_col);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < N; i += 32) {
+                uint32_t u[32];
+                tmem_load32(u, s_col + i);
+                adjust(u, i, slot, full, lo, hi);
+                if (full) l += powers<true, 32>(u, i, slot, c, off, s_col);
+                else l += powers<false, 32>(u, i, slot, c, off, s_col);
+            }
+        }
         tmem_store_wait();
     }
 
-    // P = 2^(c x + off) into tensor memory; returns their sum.  With MIXED some pairs of eight are computed
-    // by FMAs.
-    template <bool MIXED>
-    __device__ __forceinline__ float powers(const float *x, uint32_t slot, float c, float off, uint32_t s_col) {
-        constexpr int N = S::kBlock;
+    // -inf where a row does not see the token of a column
+    template <int N>
+    __device__ __forceinline__ void hide(uint32_t (&u)[N], int lo, int hi) const {
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int t = S::kByDims ? cached_token(k) : k;
+            if (t < lo || t >= hi) u[k] = 0xFF800000u;
+        }
+    }
+    // 32 columns of scores from column i on: times the tokens' scales, -inf where a row does not see the token
+    __device__ __forceinline__ void adjust(uint32_t (&u)[32], int i, uint32_t slot, bool full, int lo, int hi) {
+        float *x = reinterpret_cast<float *>(u);
+        if constexpr (kTokenScales) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i + k]);
+                unpair(mul2(pair(x[k], x[k + 1]), pair(f.x, f.y)), x[k], x[k + 1]);
+                unpair(mul2(pair(x[k + 2], x[k + 3]), pair(f.z, f.w)), x[k + 2], x[k + 3]);
+            }
+        }
+        if (!full) hide(u, lo - i, hi - i);
+    }
+    // P = 2^(c x + off) of N columns from column at0 on into tensor memory; returns their sum.  With MIXED some pairs
+    // of eight are computed by FMAs.
+    template <bool MIXED, int N>
+    __device__ __forceinline__ float powers(const uint32_t (&u)[N], int at0, uint32_t slot, float c, float off, uint32_t s_col) {
+        const float *x = reinterpret_cast<const float *>(u);
         const uint64_t cc = pair(c, c), oo = pair(off, off);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -1554,7 +1621,7 @@ struct AtRoles {
                 sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
                 float e0, e1;
                 if constexpr (kTokenScales) {
-                    const float2 v = *reinterpret_cast<const float2 *>(&sh.vscale[slot][i + k]);
+                    const float2 v = *reinterpret_cast<const float2 *>(&sh.vscale[slot][at0 + i + k]);
                     e = mul2(e, pair(v.x, v.y));
                 }
                 unpair(e, e0, e1);
@@ -1574,8 +1641,8 @@ struct AtRoles {
                 }
             }
 #pragma unroll
-            for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (N / 2) + i / 2, p[k]);
-            if (PARTS == 1 && i == N / 2 - 32) {
+            for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (S::kBlock / 2) + (at0 + i) / 2, p[k]);
+            if (PARTS == 1 && at0 + i == S::kBlock / 2 - 32) {  // the products of half the tokens may start
                 tmem_store_wait();
                 tc_fence_before();
                 warp_arrive(&sh.pready[warp >> 2][0], lane);
@@ -1622,14 +1689,20 @@ struct AtRoles {
                 for (int z = 0; z < 2; z++) odd |= sh.odd_v[used & 3][z][lane & 15];
                 odd = __any_sync(0xffffffffu, odd != 0);
             }
-            const uint32_t row = seg.row0 + (have ? r : 0), token = row / a.group, h = seg.head * a.group + row % a.group;
+            const uint32_t row = seg.row0 + (have ? r : 0), token = row / a.group, h = seg.head * a.group + row - token * a.group;
             const uint64_t at = (uint64_t)(seg.token_row + token) * a.out_stride + h * kHeadDim;
             float *slot = seg.slot < 0 ? nullptr : a.slots + (size_t)seg.slot * at_slot_floats(TILES);
+            const bool floats = slot || PARTS == 3;  // what a row's values are written as
+            uint8_t *to = slot ? reinterpret_cast<uint8_t *>(slot + (size_t)r * kHeadDim)
+                               : static_cast<uint8_t *>(a.out) + at * (PARTS == 3 ? 4 : 2);
+            const uint32_t rows = __ballot_sync(0xffffffffu, have);
             const float per = slot ? kUnit : l > 0.f || l != l ? kUnit / l : 0.f;
-            const int from = TILES == 1 ? g * 64 : 0, to = TILES == 1 ? from + 64 : 128;
+            const int part = TILES == 1 ? g : 0;
+            const int from = part * 64, to_col = TILES == 1 ? from + 64 : 128;
             // a short loop: this code runs once a segment, and a long one waits for its instructions
+            uint4 piece[4];
 #pragma unroll 1
-            for (int col = from; col < to; col += kWide) {
+            for (int col = from; col < to_col; col += kWide) {
                 float o[kWide];
                 if (seg.blocks) {
                     uint32_t u[kWide];
@@ -1649,16 +1722,27 @@ struct AtRoles {
 #pragma unroll
                     for (int k = 0; k < kWide; k++) o[k] = 0.f;
                 }
-                if (!have) continue;
 #pragma unroll
                 for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
-                if (slot) {
-                    store_floats<kWide>(slot + (size_t)r * kHeadDim + col, o, a.wide_slots);
-                } else {
-                    store_values<kWide>(a.out, at + col, a.dtype, o, a.wide_out);
+                if (floats) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        piece[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]),
+                                              __float_as_uint(o[4 * k + 3]));
+                    store_rows(to + 4 * col, rows, piece);
+                } else {  // two steps make 64 bytes
+                    const bool f16 = a.dtype == QWN_DTYPE_F16;
+                    if (col & kWide) {
+                        piece[2] = pack8(o, f16);
+                        piece[3] = pack8(o + 8, f16);
+                        store_rows(to + 2 * (col - kWide), rows, piece);
+                    } else {
+                        piece[0] = pack8(o, f16);
+                        piece[1] = pack8(o + 8, f16);
+                    }
                 }
             }
-            if (slot && have && (TILES == 2 || g == 0)) {
+            if (slot && have && part == 0) {
                 slot[TILES * kAtRows * kHeadDim + r] = M;
                 slot[TILES * kAtRows * (kHeadDim + 1) + r] = l;
             }
@@ -1677,12 +1761,13 @@ struct AtRoles {
 };
 
 template <int SRC, int PARTS, int TILES, bool BF16>
-__global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(AtShape<SRC, PARTS, TILES>::kThreads, 1) prompt_tile_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                     const __grid_constant__ CUtensorMap vmap,
                                                                     const __grid_constant__ AtArgs a) {
     using S = AtShape<SRC, PARTS, TILES>;
     extern __shared__ uint8_t dynamic[];
-    __shared__ __align__(16) AtShared<SRC, PARTS, TILES> sh;
+    __shared__ AtShared<SRC, PARTS, TILES> sh;
+    constexpr int kFirst = 8;  // the helpers' first warp
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;  // the host has seen that this leaves room
     if (base + S::kOperands + S::kRawTiles * S::kTileBytes > smem_u32(dynamic) + S::kSmem) {  // cannot be
@@ -1691,12 +1776,12 @@ __global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid
     }
     AtRoles<SRC, PARTS, TILES, BF16> roles = {a, sh, base, base + TILES * S::kQBytes, base + S::kOperands, warp, lane};
     if (threadIdx.x == 0) {
-        const uint32_t helpers = S::kTma ? 1 : 4, finishers = TILES == 2 ? 4 : 8;
+        const uint32_t helpers = S::kTma ? 1 : S::kHelpers, finishers = TILES == 2 ? 4 : 8;
         for (uint32_t i = 0; i < kAtStages; i++) {
             mbar_init(&sh.full[i], helpers);
             mbar_init(&sh.empty[i], 1);
             mbar_init(&sh.part[i], 1);
-            mbar_init(&sh.fixed[i], 4);
+            mbar_init(&sh.fixed[i], S::kHelpers);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.sfull[i], 1);
@@ -1705,12 +1790,12 @@ __global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid
             mbar_init(&sh.ofull[i], 1);
             mbar_init(&sh.oempty[i], finishers);
             mbar_init(&sh.segfull[i], 1);
-            mbar_init(&sh.segempty[i], 14);
+            mbar_init(&sh.segempty[i], kFirst + S::kHelpers + 2);
         }
-        mbar_init(&sh.qfull, 4);
+        mbar_init(&sh.qfull, S::kHelpers);
         mbar_init(&sh.qempty, 1);
         mbar_init(&sh.joined, 8);
-        mbar_init(&sh.helped, 4);
+        mbar_init(&sh.helped, S::kHelpers);
         mbar_init(&sh.drained, 1);
         for (int i = 0; i < AtShared<SRC, PARTS, TILES>::kRaw; i++) {
             mbar_init(&sh.rawfull[i], 1);
@@ -1719,28 +1804,28 @@ __global__ void __launch_bounds__(kAtThreads, 1) prompt_tile_kernel(const __grid
         sh.give_up = 0;
         fence_barrier_init();
     }
-    if (warp == 12) tmem_alloc<1>(&sh.tmem, 512);
+    if (warp == kFirst + S::kHelpers) tmem_alloc<1>(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     launch_dependents();
     wait_previous();
-    if (warp < 8) {
-        take_registers<kSoftmaxRegs>();
+    if (warp < kFirst) {
+        take_registers<S::kSoftmaxRegs>();
         roles.soften();
-    } else if (warp < 12) {
-        give_registers<kHelperRegs>();
+    } else if (warp < kFirst + S::kHelpers) {
+        if (S::kHelperRegs < S::kLaunchRegs) give_registers<S::kHelperRegs>();
         roles.help();
     } else {
-        give_registers<kOtherRegs>();
-        if (warp == 12) roles.multiply();
-        else if (warp == 13) roles.load(&kmap, &vmap);
-        else if (warp == 14) roles.plan();
+        give_registers<S::kOtherRegs>();
+        if (warp == kFirst + S::kHelpers) roles.multiply();
+        else if (warp == kFirst + S::kHelpers + 1) roles.load(&kmap, &vmap);
+        else if (warp == kFirst + S::kHelpers + 2) roles.plan();
     }
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && sh.give_up) latch(a.status, QWN_KV_STATUS_WAIT_TIMEOUT);
-    if (warp == 12) {
+    if (warp == kFirst + S::kHelpers) {
         tc_fence_after();
         tmem_free<1>(sh.tmem, 512);
     }
@@ -1760,7 +1845,7 @@ cudaError_t prepare_tile_kernel(int device) {
     const auto kernel = prompt_tile_kernel<SRC, PARTS, TILES, BF16>;
     cudaFuncAttributes at;
     cudaError_t e = cudaFuncGetAttributes(&at, kernel);
-    if (e == cudaSuccess && at.numRegs * 4 < 2 * kSoftmaxRegs + kHelperRegs + kOtherRegs) return cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess && at.numRegs < AtShape<SRC, PARTS, TILES>::kLaunchRegs) return cudaErrorInvalidConfiguration;
     // operands start on 1024 bytes behind the static part; the window itself does
     using S = AtShape<SRC, PARTS, TILES>;
     if (e == cudaSuccess && (1024 - at.sharedSizeBytes % 1024) % 1024 + S::kOperands + S::kRawTiles * S::kTileBytes > S::kSmem)
@@ -1777,7 +1862,7 @@ cudaError_t launch_tile_kernel(int device, uint32_t ctas, cudaStream_t s, const 
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kAtThreads);
+    cfg.blockDim = dim3(AtShape<SRC, PARTS, TILES>::kThreads);
     cfg.dynamicSmemBytes = AtShape<SRC, PARTS, TILES>::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
