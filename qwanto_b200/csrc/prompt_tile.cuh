@@ -83,9 +83,9 @@ struct AtShape {
     // row's 128 scores; what they lack goes to memory (16384 rows of 13 prompts: 334 us with 184, 299 with 200).
     // Where codes are converted the scores are read twice out of tensor memory instead, and twice as many helpers
     // have the registers.
-    static constexpr int kHelpers = PARTS == 1 && kRaw ? 8 : 4, kThreads = 384 + 32 * kHelpers;
-    static constexpr int kLaunchRegs = kHelpers == 8 ? 96 : 128, kSoftmaxRegs = kTma ? 200 : kHelpers == 8 ? 104 : 184;
-    static constexpr int kHelperRegs = kTma ? 64 : 96, kOtherRegs = kHelpers == 8 ? 80 : 48;
+    static constexpr int kHelpers = kTma ? 4 : 8, kThreads = 384 + 32 * kHelpers;
+    static constexpr int kLaunchRegs = kHelpers == 8 ? 96 : 128, kSoftmaxRegs = kTma ? 200 : 112;
+    static constexpr int kHelperRegs = kTma ? 64 : 96, kOtherRegs = kHelpers == 8 ? 64 : 48;
     static_assert(2 * kSoftmaxRegs + kHelpers / 4 * kHelperRegs + kOtherRegs <= kThreads / 128 * kLaunchRegs, "registers");
     // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
     // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
@@ -98,7 +98,7 @@ struct AtShape {
     // are apart, so that K of the next block does not wait behind V of this one.
     static constexpr uint32_t kRing = kTma ? 5 : 0;
     static constexpr uint32_t kStagesK = PARTS == 1 ? 2 : 1;
-    static constexpr uint32_t kStagesV = kTma ? 2 : 1;
+    static constexpr uint32_t kStagesV = kTma || (PARTS == 1 && !kRaw) ? 2 : 1;
     static constexpr uint32_t kStages = kRing ? kRing : kStagesK + kStagesV;
     static constexpr uint32_t kOperands = TILES * kQBytes + kStages * kKvBytes;
     static constexpr uint32_t kSmem = (227 - (!kTma ? 12 : TILES == 2 ? 2 : 8)) * 1024;  // the rest is static
@@ -111,7 +111,9 @@ struct AtShape {
     __device__ static constexpr uint32_t v_turn(uint32_t d) { return kRing ? (2 * d + 1) / (kRing ? kRing : 1) : d / kStagesV; }
     static constexpr uint32_t kTileBytes = (uint32_t)tile_bytes_of(SRC);
     static constexpr uint32_t kRawAll = kRaw ? (kSmem - 1024 - kOperands) / (kRaw ? kTileBytes : 1) : 0;
-    static constexpr uint32_t kRawTiles = kRawAll > 32 ? 32 : kRawAll;
+    // (by four, so that a slot's tiles are always the same warps': one that had not seen each turn of a barrier
+    // could take the last turn but one for the last)
+    static constexpr uint32_t kRawTiles = (kRawAll > 32 ? 32 : kRawAll) & ~3u;
     static_assert(kOperands + (kTma ? 0 : 1024) <= kSmem, "operands fit");
     // K of a block is converted before its V, so all its tiles are there at once
     static_assert(!kRaw || kRawTiles >= (uint32_t)kTiles, "a block's cached tiles fit");
@@ -127,7 +129,7 @@ struct alignas(1024) AtShared {  // the operands behind it start on 1024 bytes
     static constexpr int kRaw = SRC == 0 ? 1 : 32;
     // operands of K and V have landed, are free again; V of a block seen in part (loaded ones only): has landed, is ready
     uint64_t full[kAtStages], empty[kAtStages], part[kAtStages], fixed[kAtStages];
-    uint64_t qfull, qempty, sfull[2], pready[2][2], ofull[2], oempty[2], joined, helped, drained;
+    uint64_t qfull, qempty, sfull[2], pready[2][2], ofull[2], oempty[2], joined, helped, cleared, drained;
     uint64_t segfull[2], segempty[2], rawfull[kRaw], rawempty[kRaw];
     AtSegment seg[2];
     alignas(16) float kscale[kTokens ? 4 : 1][kTokens ? 128 : 4];  // of a block's tokens; read four at a time
@@ -914,10 +916,10 @@ __device__ __forceinline__ void note_odd(uint32_t (&noted)[2][16], const AtSegme
     if (i < 512) atomicOr(&noted[token < z ? 0 : 1][i >> 5], 1u << (i & 31));
 }
 __device__ __noinline__ void clear_odd_by_dims(uint32_t (&noted)[2][16], const AtSegment &seg, int32_t token0, uint32_t base) {
-    const uint32_t d = threadIdx.x & 127, c0 = threadIdx.x & 128 ? 8 : 0;  // two warpgroups: a half of the tokens each
+    const uint32_t d = threadIdx.x & 127;
     const int32_t left = seg.len - token0;  // tokens of the block that exist
 #pragma unroll 1
-    for (uint32_t c = c0; c < c0 + 8; c++) {  // eight tokens each
+    for (uint32_t c = 0; c < 16; c++) {  // eight tokens each
         const uint32_t at = base + (c >> 3) * 16384 + d * 128 + (((c & 7) ^ (d & 7)) << 4);
         const uint4 w = ld_shared16(at);
         uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -1202,122 +1204,154 @@ struct AtRoles {
         warp_arrive(&sh.helped, lane);
         return wait(&sh.helped, syncs++ & 1);
     }
-    // K and V of a block out of cached codes: this warp's tiles
-    __device__ __forceinline__ bool convert_codes(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
-        constexpr int kMine = S::kTiles / S::kHelpers;
-        const int w = warp - 8;
-        const int32_t token0 = blk * S::kBlock;
-        const uint32_t slot = done & 3, ks = S::k_slot(done), vs = S::v_slot(done);
-        extern __shared__ uint8_t dynamic[];
-        uint32_t ring[kMine];
-        const uint8_t *tile[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; i++) {
-            const uint32_t g = done * S::kTiles + w + S::kHelpers * i;
-            ring[i] = g % S::kRawTiles;
-            tile[i] = dynamic + (raw_at - smem_u32(dynamic)) + ring[i] * S::kTileBytes;
-            if (!wait(&sh.rawfull[ring[i]], (g / S::kRawTiles) & 1)) return false;
-        }
-        KeyWords<SRC> k[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; i++) k[i].load(tile[i]);
-        if (!wait(&sh.empty[ks], (S::k_turn(done) & 1) ^ 1)) return false;
-        if constexpr (kTokenScales) {  // read when the block's scores are there
-#pragma unroll
-            for (int i = 0; i < kMine; i++) {
-                const int t = lane & 15, v = lane >> 4, ti = w + S::kHelpers * i;
-                const float sc = token0 + ti * kTileTokens + t < seg.len ? token_scale<SRC>(tile[i], t, v) : 0.f;
-                (v ? sh.vscale : sh.kscale)[slot][ti * kTileTokens + cached_order(t)] = sc;
-                const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
-                if (lane == 0) sh.vtop[slot][ti] = (float)((int)(top >> 23) - 126);
+    // Operands out of cached tiles, and out of fp32 rows: four warps make K, four make V, so that the next blocks'
+    // scores do not wait for the room of this one's values.  A tile of codes is in its warp's registers before its
+    // room is given back.  fp16 tiles go as they are, in asynchronous copies of 16 bytes (their chunks are swizzled as the operands'
+    // are); a block's are on their way while the next block's start.
+    __device__ __forceinline__ bool convert_side(const AtSegment &seg, uint32_t done, uint32_t segment, uint32_t &meetings) {
+        const int which = (warp - 8) >> 2, w = warp & 3;
+        auto slot_of = [&](uint32_t d) { return which ? S::v_slot(d) : S::k_slot(d); };
+        auto free_slot = [&](uint32_t d) { return wait(&sh.empty[slot_of(d)], ((which ? S::v_turn(d) : S::k_turn(d)) & 1) ^ 1); };
+        auto ready = [&](uint32_t d, int blk) {  // the block's operands are written
+            if (which && !whole(seg, blk)) {
+                warp_arrive(&sh.cleared, lane);
+                if (!wait(&sh.cleared, meetings++ & 1)) return false;
+                if constexpr (S::kByDims) clear_odd_by_dims(sh.odd_v[segment & 3], seg, blk * S::kBlock, slot_at(slot_of(d)));
+                else clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, blk * S::kBlock, slot_at(slot_of(d)), PARTS == 3);
             }
-        }
+            fence_proxy_async_shared();
+            warp_arrive(&sh.full[slot_of(d)], lane);
+            return true;
+        };
+        // Cached tiles' room for the next copies.  They write through the async proxy: without the fence they were
+        // seen to overtake loads whose warp had arrived.
+        auto give_back = [&](const auto &ring) {
+            fence_proxy_async_shared();
+            for (const uint32_t r : ring) warp_arrive(&sh.rawempty[r], lane);
+        };
+        if constexpr (S::kByDims) {
+            extern __shared__ uint8_t dynamic[];
+            for (int b = 0; b < seg.blocks; b++) {
+                const uint32_t d = done + b, dst = slot_at(slot_of(d));
+                const int32_t token0 = (seg.block0 + b) * S::kBlock;
+                uint32_t ring[2];
+                const uint8_t *tile[2];
 #pragma unroll
-        for (int i = 0; i < kMine; i++) k[i].store(tile[i], w + S::kHelpers * i, slot_at(ks));
-        fence_proxy_async_shared();
-        warp_arrive(&sh.full[ks], lane);
-        ValueWords<SRC> v[kMine];
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t g = d * S::kTiles + w + 4 * i;
+                    ring[i] = g % S::kRawTiles;
+                    tile[i] = dynamic + (raw_at - smem_u32(dynamic)) + ring[i] * S::kTileBytes;
+                    if (!wait(&sh.rawfull[ring[i]], (g / S::kRawTiles) & 1)) return false;
+                }
+                if (which) {
+                    ValueWords<SRC> v[2];
 #pragma unroll
-        for (int i = 0; i < kMine; i++) v[i].load(tile[i]);
+                    for (int i = 0; i < 2; i++) v[i].load(tile[i]);
+                    give_back(ring);
+                    if (!free_slot(d)) return false;
 #pragma unroll
-        for (int i = 0; i < kMine; i++) warp_arrive(&sh.rawempty[ring[i]], lane);
-        if (!wait(&sh.empty[vs], (S::v_turn(done) & 1) ^ 1)) return false;
+                    for (int i = 0; i < 2; i++) v[i].store(w + 4 * i, dst);
+                } else {
+                    KeyWords<SRC> k[2];
 #pragma unroll
-        for (int i = 0; i < kMine; i++) v[i].store(w + S::kHelpers * i, slot_at(vs));
-        if (!whole(seg, blk)) {
-            if (!helpers_sync(syncs)) return false;
-            clear_odd_by_dims(sh.odd_v[segment & 3], seg, token0, slot_at(vs));
-        }
-        fence_proxy_async_shared();
-        warp_arrive(&sh.full[vs], lane);
-        return true;
-    }
-    // the same out of fp16 pages, and of anything in parts
-    __device__ __forceinline__ bool convert(const AtSegment &seg, int blk, uint32_t done, uint32_t segment, uint32_t &syncs) {
-        const int w = warp & 3;
-        const int32_t token0 = blk * S::kBlock;
+                    for (int i = 0; i < 2; i++) k[i].load(tile[i]);
+                    if (!free_slot(d)) return false;
+                    if constexpr (kTokenScales) {  // read when the block's scores are there
 #pragma unroll
-        for (int which = 0; which < 2; which++) {
-            const uint32_t s = which ? S::v_slot(done) : S::k_slot(done), dst = slot_at(s);
-            if (!wait(&sh.empty[s], ((which ? S::v_turn(done) : S::k_turn(done)) & 1) ^ 1)) return false;
-            for (int ti = w; ti < S::kTiles; ti += 4) {
-                const int32_t at = token0 + ti * kTileTokens;
-                if constexpr (S::kPaged) {
-                    const uint8_t *tile = nullptr;
-                    if constexpr (S::kRaw) {
-                        const uint32_t g = done * S::kTiles + ti, r = g % S::kRawTiles;
-                        if (!which && !wait(&sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
-                        extern __shared__ uint8_t dynamic[];
-                        tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
-                    } else if (at < seg.len) {
-                        tile = at_tile(a, seg.seq, seg.head, at);
-                    }
-                    if constexpr (PARTS == 1) {  // fp16 as it is: the tile's chunks are swizzled alike
-                        if (tile) {
-#pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                const int i = 32 * k + lane, t = i >> 4, c = i & 15;
-                                cp_async16_at(dst + (c >> 3) * S::kBlock * 128 + (ti * kTileTokens + t) * 128 + (c & 7) * 16,
-                                              tile + which * 4096 + 16 * i);
-                            }
+                        for (int i = 0; i < 2; i++) {
+                            const int t = lane & 15, v = lane >> 4, ti = w + 4 * i;
+                            const float sc = token0 + ti * kTileTokens + t < seg.len ? token_scale<SRC>(tile[i], t, v) : 0.f;
+                            (v ? sh.vscale : sh.kscale)[d & 3][ti * kTileTokens + cached_order(t)] = sc;
+                            const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
+                            if (lane == 0) sh.vtop[d & 3][ti] = (float)((int)(top >> 23) - 126);
                         }
-                    } else {
-                        put_parts<SRC, S::kBlock>(tile, which, ti, at, seg.len, dst);
                     }
-                    if constexpr (S::kRaw)
-                        if (which) warp_arrive(&sh.rawempty[(done * S::kTiles + ti) % S::kRawTiles], lane);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) k[i].store(tile[i], w + 4 * i, dst);
+                    give_back(ring);
+                }
+                if (!ready(d, seg.block0 + b)) return false;
+            }
+            return true;
+        } else if constexpr (PARTS == 1) {
+            auto address = [&](int b, int ti) -> const uint8_t * {
+                const int32_t token = (seg.block0 + b) * S::kBlock + ti * kTileTokens;
+                return b < seg.blocks && token < seg.len ? at_tile(a, seg.seq, seg.head, token) : nullptr;
+            };
+            const uint8_t *ahead[2] = {address(0, w), address(0, w + 4)};
+            for (int b = 0; b < seg.blocks; b++) {
+                if (!free_slot(done + b)) return false;
+                const uint32_t dst = slot_at(slot_of(done + b));
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint8_t *tile = ahead[i];
+                    ahead[i] = address(b + 1, w + 4 * i);
+                    if (tile) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int n = 32 * k + lane, t = n >> 4, c = n & 15;
+                            cp_async16_at(dst + (c >> 3) * S::kBlock * 128 + ((w + 4 * i) * kTileTokens + t) * 128 + (c & 7) * 16,
+                                          tile + which * 4096 + 16 * n);
+                        }
+                    }
+                }
+                cp_async_commit();
+                if (b) {
+                    cp_async_wait1();
+                    if (!ready(done + b - 1, seg.block0 + b - 1)) return false;
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            return ready(done + seg.blocks - 1, seg.block0 + seg.blocks - 1);
+        } else {
+            for (int b = 0; b < seg.blocks; b++) {
+                const int32_t at = (seg.block0 + b) * S::kBlock + w * kTileTokens;  // a warp's tile
+                const uint8_t *tile = nullptr;
+                const uint32_t g = (done + b) * S::kTiles + w, r = g % (S::kRaw ? S::kRawTiles : 1);
+                if constexpr (S::kRaw) {
+                    extern __shared__ uint8_t dynamic[];
+                    tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
+                    if (!wait(&sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
+                } else if (S::kPaged && at < seg.len) {
+                    tile = at_tile(a, seg.seq, seg.head, at);
+                }
+                if (!free_slot(done + b)) return false;
+                const uint32_t dst = slot_at(slot_of(done + b));
+                if constexpr (S::kPaged) {
+                    put_parts<SRC, S::kBlock>(tile, which, w, at, seg.len, dst);
+                    if constexpr (S::kRaw) {
+                        const uint32_t ring[1] = {r};
+                        give_back(ring);
+                    }
                 } else {
                     const float *rows = static_cast<const float *>(which ? a.value : a.key) + (size_t)seg.head * kHeadDim;
                     const uint64_t stride = which ? a.value_stride : a.key_stride;
+#pragma unroll 1
+                    for (int pass = 0; pass < 4; pass += 2) {
+                        Raw16<float> raw[2];
 #pragma unroll
-                    for (int pass = 0; pass < 4; pass++) {
-                        const int t = 4 * pass + (lane >> 3);
-                        Row16 x = {};
-                        if (at + t < seg.len) {
-                            Raw16<float> raw;
-                            raw.load(rows + (uint64_t)(seg.token_row + at + t) * stride, lane & 7);
-                            x = raw.row();
+                        for (int i = 0; i < 2; i++) {
+                            const int t = 4 * (pass + i) + (lane >> 3);
+                            raw[i] = Raw16<float>{};
+                            if (at + t < seg.len) raw[i].load(rows + (uint64_t)(seg.token_row + at + t) * stride, lane & 7);
                         }
-                        put_operand(dst, S::kBlock, S::kKvPart, (uint32_t)(ti * kTileTokens + t), lane & 7, x);
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+                            put_operand(dst, S::kBlock, S::kKvPart, (uint32_t)(w * kTileTokens + 4 * (pass + i) + (lane >> 3)), lane & 7,
+                                        raw[i].row());
                     }
                 }
+                if (!ready(done + b, seg.block0 + b)) return false;
             }
-            if constexpr (S::kPaged && PARTS == 1 && !S::kRaw) asm volatile("cp.async.wait_all;" ::: "memory");
-            if (which && !whole(seg, blk)) {
-                if (!helpers_sync(syncs)) return false;
-                clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, token0, dst, PARTS == 3);
-            }
-            fence_proxy_async_shared();
-            warp_arrive(&sh.full[s], lane);
+            return true;
         }
-        return true;
     }
 
     __device__ __forceinline__ void help() {
         Feed f;
         AtSegment seg;
         uint32_t done = 0, used = 0, syncs = 0;  // blocks, segments with any
-        uint32_t phase = 0;  // of part, a bit per slot
+        uint32_t phase = 0, meetings = 0;  // of part, a bit per slot; of the warps that make V
         const uint32_t tid = threadIdx.x & 127, wg = (warp - 8) >> 2;
         while (take(f, seg)) {
             if (seg.blocks == 0) continue;
@@ -1329,15 +1363,13 @@ struct AtRoles {
             fence_proxy_async_shared();
             if (!helpers_sync(syncs)) return;  // odd_v is empty before any warp notes a token
             warp_arrive(&sh.qfull, lane);
-            for (int b = 0; b < seg.blocks; b++, done++) {
-                const int blk = seg.block0 + b;
-                if constexpr (!S::kTma) {
-                    bool ok;
-                    if constexpr (S::kByDims) ok = convert_codes(seg, blk, done, used, syncs);
-                    else ok = convert(seg, blk, done, used, syncs);
-                    if (!ok) return;
-                } else if (!whole(seg, blk)) {
-                    const uint32_t s = S::v_slot(done);
+            if constexpr (!S::kTma) {
+                if (!convert_side(seg, done, used, meetings)) return;
+            } else {
+                for (int b = 0; b < seg.blocks; b++) {
+                    const int blk = seg.block0 + b;
+                    if (whole(seg, blk)) continue;
+                    const uint32_t s = S::v_slot(done + b);
                     if (!wait(&sh.part[s], phase >> s & 1)) return;
                     phase ^= 1u << s;
                     clear_odd<PARTS, S::kBlock>(sh.odd_v[used & 3], seg, blk * S::kBlock, slot_at(s), BF16);
@@ -1345,6 +1377,7 @@ struct AtRoles {
                     warp_arrive(&sh.fixed[s], lane);
                 }
             }
+            done += seg.blocks;
             used++;
         }
     }
@@ -1776,12 +1809,12 @@ __global__ void __launch_bounds__(AtShape<SRC, PARTS, TILES>::kThreads, 1) promp
     }
     AtRoles<SRC, PARTS, TILES, BF16> roles = {a, sh, base, base + TILES * S::kQBytes, base + S::kOperands, warp, lane};
     if (threadIdx.x == 0) {
-        const uint32_t helpers = S::kTma ? 1 : S::kHelpers, finishers = TILES == 2 ? 4 : 8;
+        const uint32_t helpers = S::kTma ? 1 : 4, finishers = TILES == 2 ? 4 : 8;
         for (uint32_t i = 0; i < kAtStages; i++) {
             mbar_init(&sh.full[i], helpers);
             mbar_init(&sh.empty[i], 1);
             mbar_init(&sh.part[i], 1);
-            mbar_init(&sh.fixed[i], S::kHelpers);
+            mbar_init(&sh.fixed[i], 4);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.sfull[i], 1);
@@ -1796,10 +1829,11 @@ __global__ void __launch_bounds__(AtShape<SRC, PARTS, TILES>::kThreads, 1) promp
         mbar_init(&sh.qempty, 1);
         mbar_init(&sh.joined, 8);
         mbar_init(&sh.helped, S::kHelpers);
+        mbar_init(&sh.cleared, 4);
         mbar_init(&sh.drained, 1);
         for (int i = 0; i < AtShared<SRC, PARTS, TILES>::kRaw; i++) {
             mbar_init(&sh.rawfull[i], 1);
-            mbar_init(&sh.rawempty[i], 1);
+            mbar_init(&sh.rawempty[i], 2);
         }
         sh.give_up = 0;
         fence_barrier_init();

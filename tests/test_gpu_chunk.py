@@ -378,3 +378,17 @@ def test_refusals(cuda):
             c.pool.chunk_workspace(*bad)
     torch.cuda.synchronize()
     assert c.pool.check() == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("codec", CODECS)
+def test_same_bits_every_time(cuda, codec, kind):
+    """Copies into a cached tile's room must not overtake the loads out of it: many calls, the same bits."""
+    torch = cuda
+    for lens, counts in (([5000], [512]), ([3000] * 8, [4] * 8), ([1200, 515], [1000, 300])):
+        c = Cache(torch, codec, lens, 8, seed=codec + 40)
+        q = _queries(torch, sum(counts), 32, kind)
+        for split in (False, True):
+            first = _run(torch, c, q, counts, kind, workspace=split)
+            for _ in range(12):
+                assert torch.equal(first, _run(torch, c, q, counts, kind, workspace=split))
