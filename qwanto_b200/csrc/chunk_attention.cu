@@ -18,6 +18,7 @@ namespace {
 template <int SRC, int PARTS, int TILES>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArgs a, uint32_t grid) {
     using W = AtWork<SRC, PARTS, TILES>;
+    using S = AtShape<SRC, PARTS, TILES>;
     constexpr uint32_t kRows = W::kRows;
     const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t row = warp / a.query_heads, qh = warp - row * a.query_heads;
@@ -41,28 +42,40 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
     const uint32_t total = a.prefix[a.rows.num_seqs];
     const AtRuns runs(total, min(grid, total));
     const uint32_t kv = qh / a.group, r = (row - (uint32_t)s.begin) * a.group + qh - kv * a.group;
-    const uint32_t u0 = a.prefix[i] + (r / kRows * a.kv_heads + kv) * span;
+    const uint32_t tile = r / kRows, item = tile * a.kv_heads + kv, u0 = a.prefix[i] + item * span;
     const uint32_t b0 = runs.owner(u0), b1 = runs.owner(u0 + span - 1);
-    if (b0 == b1) return;  // finished by its CTA
+    const bool quarters = S::kQuarters && (uint64_t)s.rows * a.group - tile * kRows <= 32;
+    if (b0 == b1 && !quarters) return;  // finished by its CTA
     const uint32_t at = r % kRows;
+    const uint32_t parts = (b1 - b0 + 1) << (quarters ? 2 : 0), step = a.slot_rows / 4;
+    const uint32_t first_slot = S::kQuarters ? a.prefix[a.rows.num_seqs + 1 + i] + item + b0 : 0;
     const bool second = u0 > runs.begin(b0);
-    auto slot = [&](uint32_t b) {  // a CTA's first segment, or its second slot
-        const bool later = b == b0 && second;
-        return a.slots + (size_t)(2 * b + (later ? 1 : 0)) * at_slot_floats(TILES);
+    // the k-th piece of the row: a CTA's, or one quarter of a CTA's
+    auto piece = [&](uint32_t k, uint32_t &place) {
+        const uint32_t n = quarters ? k >> 2 : k;
+        place = quarters ? (k & 3) * step + at : at;
+        // (without quarters: a CTA's first segment, or its second slot)
+        const uint32_t slot = S::kQuarters ? first_slot + n : 2 * (b0 + n) + (n == 0 && second ? 1 : 0);
+        return a.slots + (size_t)slot * at_slot_floats(a.slot_rows);
     };
     float M = -INFINITY;
-    for (uint32_t b = b0 + lane; b <= b1; b += 32) M = fmaxf(M, slot(b)[kRows * kHeadDim + at]);
+    for (uint32_t k = lane; k < parts; k += 32) {
+        uint32_t place;
+        const float *p = piece(k, place);
+        M = fmaxf(M, p[a.slot_rows * kHeadDim + place]);
+    }
     M = warp_max(M);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (uint32_t b = b0; b <= b1; b++) {
-        const float *p = slot(b);
-        const float m = p[kRows * kHeadDim + at];
-        const float4 v = *reinterpret_cast<const float4 *>(p + (size_t)at * kHeadDim + 4 * lane);
+    for (uint32_t k = 0; k < parts; k++) {
+        uint32_t place;
+        const float *p = piece(k, place);
+        const float m = p[a.slot_rows * kHeadDim + place], sum = p[a.slot_rows * (kHeadDim + 1) + place];
+        const float4 v = *reinterpret_cast<const float4 *>(p + (size_t)place * kHeadDim + 4 * lane);
         if (m == -INFINITY) continue;
         const float w = ex2(m - M);
-        l = fmaf(w, p[kRows * (kHeadDim + 1) + at], l);
+        l = fmaf(w, sum, l);
         o.x = fmaf(w, v.x, o.x);
         o.y = fmaf(w, v.y, o.y);
         o.z = fmaf(w, v.z, o.z);
@@ -78,8 +91,9 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
 }
 
 // How a call is cut: two tiles of 128 rows per CTA or one, and into runs or not.
+constexpr uint64_t kMaxWorkspace = 64ull << 20;  // for pieces of rows; beyond, there are tiles for every SM
 struct ChunkPlan {
-    uint32_t tiles;
+    uint32_t tiles, slot_rows;
     uint64_t units, prefix_bytes, workspace;
     bool split;  // given a workspace
 };
@@ -89,11 +103,16 @@ ChunkPlan plan_chunk(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32
     c.tiles = dtype != QWN_DTYPE_F32 && rows > 128ull * num_seqs ? 2 : 1;
     const uint64_t tile = 128ull * c.tiles;
     c.units = runs ? rows / tile + num_seqs : num_seqs * ((group + tile - 1) / tile);
-    c.prefix_bytes = ((uint64_t)num_seqs + 1) * 4 + 255 & ~255ull;
+    c.prefix_bytes = 2 * ((uint64_t)num_seqs + 1) * 4 + 255 & ~255ull;
+    const bool quarters = c.tiles == 1 && dtype != QWN_DTYPE_F32 && p->codec != QWN_KV_CODEC_F16;
+    // one row per sequence is eight rows of a kv head at most, in each quarter
+    c.slot_rows = quarters && !runs ? 4 * kMaxGroup : 128 * c.tiles;
+    const uint64_t items = c.units * p->kv_heads, slots = quarters ? items + p->sms : 2ull * p->sms;
+    const uint64_t bytes = slots * at_slot_floats(c.slot_rows) * sizeof(float);
     // blocks are counted in 32 bits
     const uint64_t most = (uint64_t)p->max_pages_per_seq * p->page_tokens / 64 + 2;
-    c.split = c.units * p->kv_heads < 8ull * p->sms && c.units * p->kv_heads * most < 1ull << 31;
-    c.workspace = c.split ? c.prefix_bytes + 2ull * p->sms * at_slot_floats(c.tiles) * sizeof(float) : 0;
+    c.split = (quarters ? bytes <= kMaxWorkspace : items < 8ull * p->sms) && items * most < 1ull << 31;
+    c.workspace = c.split ? c.prefix_bytes + bytes : 0;
     return c;
 }
 
@@ -181,6 +200,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     a.status = p->status;
     a.units = (uint32_t)c.units;
     if (c.split && r->workspace_dev) {
+        a.slot_rows = c.slot_rows;
         a.prefix = static_cast<uint32_t *>(r->workspace_dev);
         a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(r->workspace_dev) + c.prefix_bytes);
     }

@@ -55,6 +55,7 @@ struct AtSegment {
     int32_t block0, blocks;    // blocks of tokens
     int32_t whole_lo, whole_hi;// blocks in [whole_lo, whole_hi) are seen whole by every row
     int32_t slot;              // of the workspace, -1: the rows are finished here
+    int32_t quarters;          // the rows, 32 at most, are in each quarter of the tile (AtShape::kQuarters)
 };
 
 struct AtArgs {
@@ -69,10 +70,11 @@ struct AtArgs {
     uint32_t *status;
     uint32_t units;            // row tiles, without a split
     uint32_t *prefix;          // split: blocks before each sequence and in all, then
-    float *slots;              // the partial results
+    float *slots;              // the partial results, of
+    uint32_t slot_rows;        // rows each
 };
 // a partial result: o[rows][128], then M[rows], l[rows]
-__host__ __device__ constexpr uint32_t at_slot_floats(uint32_t tiles) { return tiles * kAtRows * (kHeadDim + 2); }
+__host__ __device__ constexpr uint32_t at_slot_floats(uint32_t rows) { return rows * (kHeadDim + 2); }
 
 template <int SRC, int PARTS, int TILES>
 struct AtShape {
@@ -90,6 +92,11 @@ struct AtShape {
     // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
     // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
     static constexpr bool kByDims = PARTS == 1 && kRaw;
+    // 32 rows or fewer, as a decode step or a few drafts have, would leave three warps of a softmax group idle.  They
+    // are then in the tile four times, and each warp takes a quarter of a block's tokens: its rows of P are zero
+    // elsewhere, and its rows of O a partial result like those of other CTAs.  Not for fp16 pages, whose values may
+    // be infinite: their product with a zero of P is not a number.
+    static constexpr bool kQuarters = kByDims && TILES == 1;
     static constexpr int kBlock = PARTS == 1 ? 128 : 64;           // tokens
     static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
     static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
@@ -317,6 +324,7 @@ __device__ __forceinline__ AtSegment at_segment(const AtArgs &a, const AtSequenc
     t.whole_lo = (last.lo + block - 1) / block;
     t.whole_hi = first.hi / block;
     t.slot = -1;
+    t.quarters = 0;
     return t;
 }
 __device__ __forceinline__ uint64_t at_row_tiles(const AtArgs &a, const AtSequence &s, uint32_t tile_rows) {
@@ -358,10 +366,11 @@ struct AtWork {
     uint32_t i, span, n;   // sequence, its blocks per tile, segments so far
     int32_t first;
     uint32_t item, from;   // (row tile, head) of the sequence, block of it
+    uint32_t item0;        // those of the sequences before
     AtSequence s;
 
     __device__ __forceinline__ explicit AtWork(const AtArgs &args) : a(args) {
-        at = end = i = span = n = item = from = 0;
+        at = end = i = span = n = item = from = item0 = 0;
         first = 0;
         if (!a.slots) return;
         const uint32_t lane = threadIdx.x & 31;
@@ -372,7 +381,7 @@ struct AtWork {
         const AtRuns runs(total, min(gridDim.x, total));
         at = runs.begin(blockIdx.x);
         end = runs.begin(blockIdx.x + 1);
-        uint32_t before = 0, within = 0;
+        uint32_t before = 0, within = 0, items_before = 0;
         bool found = false;
         for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) {
             if (k) w = weight(k + lane);
@@ -382,8 +391,20 @@ struct AtWork {
                 const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= (uint32_t)o) upto += y;
             }
-            if (blockIdx.x == 0) {  // the table for the join kernel
-                if (k + lane < a.rows.num_seqs) a.prefix[k + lane] = before + upto - w;
+            uint32_t count = 0, items_upto = 0;
+            if (S::kQuarters) {
+                count = items_upto = k + lane < a.rows.num_seqs ? items(at_sequence(a, S::kPaged, k + lane)) : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xffffffffu, items_upto, o);
+                    if (lane >= (uint32_t)o) items_upto += y;
+                }
+            }
+            if (blockIdx.x == 0) {  // the tables for the join kernel
+                if (k + lane < a.rows.num_seqs) {
+                    a.prefix[k + lane] = before + upto - w;
+                    a.prefix[a.rows.num_seqs + 1 + k + lane] = items_before + items_upto - count;
+                }
                 if (lane == 0) a.prefix[a.rows.num_seqs] = total;
             }
             const uint32_t has = __ballot_sync(0xffffffffu, before + upto > at);
@@ -391,21 +412,24 @@ struct AtWork {
                 const int l = __ffs(has) - 1;
                 i = k + l;
                 within = at - (before + __shfl_sync(0xffffffffu, upto - w, l));
+                item0 = items_before + __shfl_sync(0xffffffffu, items_upto - count, l);
                 found = true;
                 if (blockIdx.x != 0) break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
+            items_before += __shfl_sync(0xffffffffu, items_upto, 31);
         }
         open();
         item = within / span;
         from = within % span;
     }
     __device__ __forceinline__ static uint32_t warp_sum(uint32_t v) { return __reduce_add_sync(0xffffffffu, v); }
+    __device__ __forceinline__ uint32_t items(const AtSequence &q) const { return (uint32_t)at_row_tiles(a, q, kRows) * a.kv_heads; }
     __device__ __forceinline__ uint32_t weight(uint32_t k) const {
         if (k >= a.rows.num_seqs) return 0;
         const AtSequence q = at_sequence(a, S::kPaged, k);
         int32_t f;
-        return (uint32_t)at_row_tiles(a, q, kRows) * a.kv_heads * at_span(a, q, S::kBlock, f);
+        return items(q) * at_span(a, q, S::kBlock, f);
     }
     __device__ __forceinline__ void open() {
         s = at_sequence(a, S::kPaged, i);
@@ -424,7 +448,8 @@ struct AtWork {
             }
         }
         while (at < end) {
-            if (item >= (uint32_t)at_row_tiles(a, s, kRows) * a.kv_heads) {  // the next sequence
+            if (item >= items(s)) {  // the next sequence
+                item0 += items(s);
                 if (++i >= a.rows.num_seqs) return t;
                 item = from = 0;
                 open();
@@ -434,7 +459,11 @@ struct AtWork {
             t = at_segment(a, s, item / a.kv_heads * kRows, kRows, (int32_t)(item % a.kv_heads), S::kBlock);
             // of the tile's own blocks those in the run
             const int32_t b0 = max(t.block0, first + (int32_t)from), b1 = min(t.block0 + t.blocks, first + (int32_t)(from + count));
-            if (count != span) t.slot = (int32_t)(2 * blockIdx.x + (n ? 1 : 0));
+            // A slot for each (tile, CTA): their indexes' sum grows along the work.  Only a run's first and last tile can
+            // be cut, so that two slots per CTA do without quarters.
+            t.quarters = S::kQuarters && t.rows <= 32;
+            if (S::kQuarters && (t.quarters || count != span)) t.slot = (int32_t)(item0 + item + blockIdx.x);
+            else if (count != span) t.slot = (int32_t)(2 * blockIdx.x + (n ? 1 : 0));
             t.block0 = b0;
             t.blocks = max(b1 - b0, 0);
             at += count;
@@ -512,11 +541,12 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t base, uint32_t rows, uint3
 // a power of two.
 template <int SRC, int PARTS>
 __device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint32_t row0, uint32_t tile, float *unit) {
-    const uint32_t lane = threadIdx.x & 31, c = lane & 15, w0 = threadIdx.x & 96;  // the warp's first row
+    const uint32_t lane = threadIdx.x & 31, c = lane & 15, w0 = threadIdx.x & 96;  // the warp's first row in the tile
+    const uint32_t first = t.quarters ? 0 : w0;                                    // and of the segment
     uint64_t mine = 0;  // where the lane's row starts
-    const bool have = (int32_t)(row0 + w0 + lane) < t.rows;
+    const bool have = (int32_t)(row0 + first + lane) < t.rows;
     if (have) {
-        const uint32_t row = t.row0 + row0 + w0 + lane, token = row / a.group;
+        const uint32_t row = t.row0 + row0 + first + lane, token = row / a.group;
         mine = (uint64_t)(t.token_row + token) * a.query_stride + (t.head * a.group + row - token * a.group) * kHeadDim;
     }
     const uint32_t rows = __ballot_sync(0xffffffffu, have);
@@ -1114,7 +1144,7 @@ struct AtRoles {
         // the same in all lanes, as the compiler can tell from this
         auto one = [](int32_t &v) { v = __shfl_sync(0xffffffffu, v, 0); };
         one(seg.valid), one(seg.rows), one(seg.seq), one(seg.head), one(seg.len), one(seg.block0), one(seg.blocks);
-        one(seg.whole_lo), one(seg.whole_hi), one(seg.slot);
+        one(seg.whole_lo), one(seg.whole_hi), one(seg.slot), one(seg.quarters);
         return seg.valid != 0;
     }
 
@@ -1503,8 +1533,10 @@ struct AtRoles {
         uint32_t done = 0, used = 0, s_uses = 0, o_uses[2] = {0, 0}, joins = 0;
         const uint32_t r = (TILES == 2 ? g * kAtRows : 0) + w * 32 + lane;
         while (take(f, seg)) {
-            const bool have = (int32_t)r < seg.rows, any = (int32_t)(r - lane) < seg.rows;
-            const int64_t pos = seg.pos0 + (have ? (seg.row0 + r) / a.group : 0);
+            const bool quarters = S::kQuarters && seg.quarters;
+            const uint32_t mine = quarters ? lane : r;  // of the segment's rows
+            const bool have = (int32_t)mine < seg.rows, any = quarters || (int32_t)(r - lane) < seg.rows;
+            const int64_t pos = seg.pos0 + (have ? (seg.row0 + mine) / a.group : 0);
             const Seen seen = have ? at_seen(a, pos, seg.len) : Seen{0, 0};
             if (have && S::kPaged && (pos < 0 || pos >= seg.len))
                 latch(a.status, seg.seq < 0 ? QWN_KV_STATUS_BAD_SEQUENCE : QWN_KV_STATUS_BAD_LENGTH);
@@ -1517,7 +1549,8 @@ struct AtRoles {
                 } else {
                     const bool first = b < (TILES == 2 ? 1 : 2);
                     if (first) c = a.scale2 * kUnit * (SRC != 0 && PARTS == 1 && have ? sh.qscale[used & 1][r] : 1.f);
-                    block(seg, seg.block0 + b, (done + b) & 3, first, have, seen, c, s_col, o_col, M, l);
+                    if (S::kQuarters && quarters) quarter(seg, seg.block0 + b, (done + b) & 3, first, have, seen, c, s_col, o_col, M, l);
+                    else block(seg, seg.block0 + b, (done + b) & 3, first, have, seen, c, s_col, o_col, M, l);
                 }
                 tc_fence_before();
                 warp_arrive(&sh.pready[g][PARTS == 1 ? 1 : 0], lane);
@@ -1526,7 +1559,7 @@ struct AtRoles {
                 M = -INFINITY;
                 l = 0.f;
             }
-            if (!finish(seg, used, have, any, r, seen, g, lanes, M, l, o_uses, joins)) return;
+            if (!finish(seg, used, have, any, r, mine, seen, g, lanes, M, l, o_uses, joins)) return;
             done += seg.blocks;
             if (seg.blocks) used++;
         }
@@ -1571,24 +1604,7 @@ struct AtRoles {
         }
         const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
         const float reach = top * c + vtop;
-        const bool grows = have && reach > M + Range::kSlack;  // true for the first that is not -inf
-        if (__any_sync(0xffffffffu, grows)) {
-            const float factor = grows && M != -INFINITY ? ex2(M - reach) : 1.f;
-            if (grows) {
-                l *= factor;
-                M = reach;
-            }
-            if (!first) {
-#pragma unroll 1
-                for (int i = 0; i < 128; i += 16) {
-                    uint32_t o[16];
-                    tmem_load16(o, o_col + i);
-#pragma unroll
-                    for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                    tmem_store16(o_col + i, o);
-                }
-            }
-        }
+        follow<Range>(reach, first, have, o_col, M, l);
         const float off = Range::kBias - (M == -INFINITY ? 0.f : M);
         // P follows on S's columns, half as many (three parts: all of them).  Masked scores are -inf, whose power is
         // exactly zero in the special function unit only.
@@ -1608,6 +1624,59 @@ struct AtRoles {
         tmem_store_wait();
     }
 
+    // M to `reach` where that is far beyond it, and the row's sums with it
+    template <class Range>
+    __device__ __forceinline__ void follow(float reach, bool first, bool have, uint32_t o_col, float &M, float &l) {
+        const bool grows = have && reach > M + Range::kSlack;  // true for the first that is not -inf
+        if (__any_sync(0xffffffffu, grows)) {
+            const float factor = grows && M != -INFINITY ? ex2(M - reach) : 1.f;
+            if (grows) {
+                l *= factor;
+                M = reach;
+            }
+            if (!first) {
+#pragma unroll 1
+                for (int i = 0; i < 128; i += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o, o_col + i);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                    tmem_store16(o_col + i, o);
+                }
+            }
+        }
+    }
+    // The quarter of a block's tokens that is this warp's, for its copy of the rows.
+    __device__ __forceinline__ void quarter(const AtSegment &seg, int blk, uint32_t slot, bool first, bool have, const Seen &seen,
+                                            float c, uint32_t s_col, uint32_t o_col, float &M, float &l) {
+        using Range = AtRange<BF16>;
+        const bool full = whole(seg, blk);
+        const int lo = seen.lo - blk * S::kBlock, hi = seen.hi - blk * S::kBlock, at = 32 * (warp & 3);
+        float vtop = 0.f;
+        if constexpr (kTokenScales) {  // of the two cached tiles
+            const float2 v = *reinterpret_cast<const float2 *>(&sh.vtop[slot][2 * (warp & 3)]);
+            vtop = fmaxf(v.x, v.y);
+        }
+        uint32_t u[32];
+        tmem_load32(u, s_col + at);
+        adjust(u, at, slot, full, lo, hi);
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) t[k] = __uint_as_float(u[k]);
+#pragma unroll
+        for (int k = 8; k < 32; k++) t[k & 7] = fmaxf(t[k & 7], __uint_as_float(u[k]));
+        const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+        follow<Range>(top * c + vtop, first, have, o_col, M, l);
+        const float off = Range::kBias - (M == -INFINITY ? 0.f : M);
+        const uint32_t none[16] = {};
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (q != (warp & 3)) tmem_store16(s_col + 16 * q, none);
+        l += powers<false, 32, false>(u, at, slot, c, off, s_col);
+        tmem_store_wait();
+        tc_fence_before();
+        warp_arrive(&sh.pready[warp >> 2][0], lane);
+    }
     // -inf where a row does not see the token of a column
     template <int N>
     __device__ __forceinline__ void hide(uint32_t (&u)[N], int lo, int hi) const {
@@ -1632,7 +1701,7 @@ struct AtRoles {
     }
     // P = 2^(c x + off) of N columns from column at0 on into tensor memory; returns their sum.  With MIXED some pairs
     // of eight are computed by FMAs.
-    template <bool MIXED, int N>
+    template <bool MIXED, int N, bool HALVES = true>
     __device__ __forceinline__ float powers(const uint32_t (&u)[N], int at0, uint32_t slot, float c, float off, uint32_t s_col) {
         const float *x = reinterpret_cast<const float *>(u);
         const uint64_t cc = pair(c, c), oo = pair(off, off);
@@ -1675,7 +1744,7 @@ struct AtRoles {
             }
 #pragma unroll
             for (int k = 0; k < PARTS; k++) tmem_store16(s_col + k * (S::kBlock / 2) + (at0 + i) / 2, p[k]);
-            if (PARTS == 1 && at0 + i == S::kBlock / 2 - 32) {  // the products of half the tokens may start
+            if (HALVES && PARTS == 1 && at0 + i == S::kBlock / 2 - 32) {  // the products of half the tokens may start
                 tmem_store_wait();
                 tc_fence_before();
                 warp_arrive(&sh.pready[warp >> 2][0], lane);
@@ -1688,7 +1757,7 @@ struct AtRoles {
     }
 
     // the rows of a segment: to the output, or to the workspace where other CTAs have a share of them
-    __device__ __forceinline__ bool finish(const AtSegment &seg, uint32_t used, bool have, bool any, uint32_t r, const Seen &seen,
+    __device__ __forceinline__ bool finish(const AtSegment &seg, uint32_t used, bool have, bool any, uint32_t r, uint32_t mine, const Seen &seen,
                                            int g, uint32_t lanes, float M, float l, uint32_t (&o_uses)[2], uint32_t &joins) {
         constexpr int kWide = 16;  // columns at a time
         const uint32_t o_at = lanes + S::kOColumn;
@@ -1722,11 +1791,12 @@ struct AtRoles {
                 for (int z = 0; z < 2; z++) odd |= sh.odd_v[used & 3][z][lane & 15];
                 odd = __any_sync(0xffffffffu, odd != 0);
             }
-            const uint32_t row = seg.row0 + (have ? r : 0), token = row / a.group, h = seg.head * a.group + row - token * a.group;
+            const uint32_t row = seg.row0 + (have ? mine : 0), token = row / a.group, h = seg.head * a.group + row - token * a.group;
             const uint64_t at = (uint64_t)(seg.token_row + token) * a.out_stride + h * kHeadDim;
-            float *slot = seg.slot < 0 ? nullptr : a.slots + (size_t)seg.slot * at_slot_floats(TILES);
+            float *slot = seg.slot < 0 ? nullptr : a.slots + (size_t)seg.slot * at_slot_floats(a.slot_rows);
+            const uint32_t place = seg.quarters ? (r >> 5) * (a.slot_rows / 4) + lane : r;  // in it
             const bool floats = slot || PARTS == 3;  // what a row's values are written as
-            uint8_t *to = slot ? reinterpret_cast<uint8_t *>(slot + (size_t)r * kHeadDim)
+            uint8_t *to = slot ? reinterpret_cast<uint8_t *>(slot + (size_t)place * kHeadDim)
                                : static_cast<uint8_t *>(a.out) + at * (PARTS == 3 ? 4 : 2);
             const uint32_t rows = __ballot_sync(0xffffffffu, have);
             const float per = slot ? kUnit : l > 0.f || l != l ? kUnit / l : 0.f;
@@ -1776,8 +1846,8 @@ struct AtRoles {
                 }
             }
             if (slot && have && part == 0) {
-                slot[TILES * kAtRows * kHeadDim + r] = M;
-                slot[TILES * kAtRows * (kHeadDim + 1) + r] = l;
+                slot[a.slot_rows * kHeadDim + place] = M;
+                slot[a.slot_rows * (kHeadDim + 1) + place] = l;
             }
         }
         if (seg.blocks) {
