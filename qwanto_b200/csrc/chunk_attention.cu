@@ -14,14 +14,16 @@
 namespace qkv {
 namespace {
 
-// one warp per row and query head, four dims per lane
+// Four warps per row and query head share its pieces; four dims per lane.
 template <int SRC, int PARTS, int TILES>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArgs a, uint32_t grid) {
     using W = AtWork<SRC, PARTS, TILES>;
     using S = AtShape<SRC, PARTS, TILES>;
     constexpr uint32_t kRows = W::kRows;
-    const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const uint32_t row = warp / a.query_heads, qh = warp - row * a.query_heads;
+    __shared__ float best[4], sums[4];
+    __shared__ float4 rows[4][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t row = blockIdx.x / a.query_heads, qh = blockIdx.x - row * a.query_heads;
     launch_dependents();
     wait_previous();
     if (row >= a.rows.num_rows) return;
@@ -40,7 +42,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
     int32_t first;
     const uint32_t span = at_span(a, s, AtShape<SRC, PARTS, TILES>::kBlock, first);
     const uint32_t total = a.prefix[a.rows.num_seqs];
-    const AtRuns runs(total, min(grid, total));
+    const AtRuns runs(total, at_runs<TILES>(total, grid));
     const uint32_t kv = qh / a.group, r = (row - (uint32_t)s.begin) * a.group + qh - kv * a.group;
     const uint32_t tile = r / kRows, item = tile * a.kv_heads + kv, u0 = a.prefix[i] + item * span;
     const uint32_t b0 = runs.owner(u0), b1 = runs.owner(u0 + span - 1);
@@ -59,7 +61,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
         return a.slots + (size_t)slot * at_slot_floats(a.slot_rows);
     };
     float M = -INFINITY;
-    for (uint32_t k = lane; k < parts; k += 32) {
+    for (uint32_t k = 4 * lane + warp; k < parts; k += 128) {
         uint32_t place;
         const float *p = piece(k, place);
         M = fmaxf(M, p[a.slot_rows * kHeadDim + place]);
@@ -67,8 +69,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
     M = warp_max(M);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (uint32_t k = 0; k < parts; k++) {
+#pragma unroll 8
+    for (uint32_t k = warp; k < parts; k += 4) {
         uint32_t place;
         const float *p = piece(k, place);
         const float m = p[a.slot_rows * kHeadDim + place], sum = p[a.slot_rows * (kHeadDim + 1) + place];
@@ -76,6 +78,24 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
         if (m == -INFINITY) continue;
         const float w = ex2(m - M);
         l = fmaf(w, sum, l);
+        o.x = fmaf(w, v.x, o.x);
+        o.y = fmaf(w, v.y, o.y);
+        o.z = fmaf(w, v.z, o.z);
+        o.w = fmaf(w, v.w, o.w);
+    }
+    if (lane == 0) best[warp] = M, sums[warp] = l;
+    rows[warp][lane] = o;
+    __syncthreads();
+    if (warp) return;
+    M = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (best[k] == -INFINITY) continue;
+        const float w = ex2(best[k] - M);
+        const float4 v = rows[k][lane];
+        l = fmaf(w, sums[k], l);
         o.x = fmaf(w, v.x, o.x);
         o.y = fmaf(w, v.y, o.y);
         o.z = fmaf(w, v.z, o.z);
@@ -124,8 +144,7 @@ cudaError_t launch_chunk(const Pool *p, const ChunkPlan &c, AtArgs &a, cudaStrea
         constexpr int P = decltype(parts)::value, T = decltype(tiles)::value;
         cudaError_t e = launch_tile_kernel<SRC, P, T, P == 3>(p->device, ctas, s, none, none, a);
         if (e != cudaSuccess || !a.slots) return e;
-        const uint64_t warps = (uint64_t)a.rows.num_rows * a.query_heads;
-        return launch_next(join_kernel<SRC, P, T>, dim3((unsigned)((warps + 3) / 4)), 128, s, a, ctas);
+        return launch_next(join_kernel<SRC, P, T>, dim3(a.rows.num_rows * a.query_heads), 128, s, a, ctas);
     };
     using One = std::integral_constant<int, 1>;
     if (a.dtype == QWN_DTYPE_F32) return run(std::integral_constant<int, 3>(), One());

@@ -357,6 +357,11 @@ struct AtRuns {
         return block < longer ? block / (each + 1) : more + (block - longer) / each;
     }
 };
+// CTAs that work: each with a block at least, or one for each of its two groups
+template <int TILES>
+__device__ __forceinline__ uint32_t at_runs(uint32_t total, uint32_t ctas) {
+    return min(ctas, TILES == 1 ? (total + 1) / 2 : total);
+}
 template <int SRC, int PARTS, int TILES>
 struct AtWork {
     using S = AtShape<SRC, PARTS, TILES>;
@@ -368,42 +373,41 @@ struct AtWork {
     uint32_t item, from;   // (row tile, head) of the sequence, block of it
     uint32_t item0;        // those of the sequences before
     AtSequence s;
+    // of 32 sequences, one per lane: read once and handed round, as code that runs once costs its fetch
+    uint32_t held, my_items, my_span;
+    int32_t my_first;
+    AtSequence my;
 
     __device__ __forceinline__ explicit AtWork(const AtArgs &args) : a(args) {
         at = end = i = span = n = item = from = item0 = 0;
         first = 0;
         if (!a.slots) return;
         const uint32_t lane = threadIdx.x & 31;
-        // the blocks of all sequences, 32 sequences at a time
-        uint32_t w = weight(lane), total = warp_sum(w);
-        for (uint32_t k = 32; k < a.rows.num_seqs; k += 32) total += warp_sum(weight(k + lane));
-        if (blockIdx.x >= min(gridDim.x, total)) return;  // each of the others has a block at least
-        const AtRuns runs(total, min(gridDim.x, total));
+        uint32_t total = 0;
+        for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) {
+            hold(k);
+            total += __reduce_add_sync(0xffffffffu, my_items * my_span);
+        }
+        const uint32_t ctas = at_runs<TILES>(total, gridDim.x);
+        if (blockIdx.x >= ctas) return;
+        const AtRuns runs(total, ctas);
         at = runs.begin(blockIdx.x);
         end = runs.begin(blockIdx.x + 1);
         uint32_t before = 0, within = 0, items_before = 0;
         bool found = false;
         for (uint32_t k = 0; k < a.rows.num_seqs; k += 32) {
-            if (k) w = weight(k + lane);
-            uint32_t upto = w;
-#pragma unroll
+            if (held != k) hold(k);
+            const uint32_t w = my_items * my_span;
+            uint32_t upto = w, items_upto = my_items;
+#pragma unroll 1
             for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= (uint32_t)o) upto += y;
-            }
-            uint32_t count = 0, items_upto = 0;
-            if (S::kQuarters) {
-                count = items_upto = k + lane < a.rows.num_seqs ? items(at_sequence(a, S::kPaged, k + lane)) : 0;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, items_upto, o);
-                    if (lane >= (uint32_t)o) items_upto += y;
-                }
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, items_upto, o);
+                if (lane >= (uint32_t)o) upto += y, items_upto += z;
             }
             if (blockIdx.x == 0) {  // the tables for the join kernel
                 if (k + lane < a.rows.num_seqs) {
                     a.prefix[k + lane] = before + upto - w;
-                    a.prefix[a.rows.num_seqs + 1 + k + lane] = items_before + items_upto - count;
+                    a.prefix[a.rows.num_seqs + 1 + k + lane] = items_before + items_upto - my_items;
                 }
                 if (lane == 0) a.prefix[a.rows.num_seqs] = total;
             }
@@ -412,7 +416,7 @@ struct AtWork {
                 const int l = __ffs(has) - 1;
                 i = k + l;
                 within = at - (before + __shfl_sync(0xffffffffu, upto - w, l));
-                item0 = items_before + __shfl_sync(0xffffffffu, items_upto - count, l);
+                item0 = items_before + __shfl_sync(0xffffffffu, items_upto - my_items, l);
                 found = true;
                 if (blockIdx.x != 0) break;
             }
@@ -421,19 +425,32 @@ struct AtWork {
         }
         open();
         item = within / span;
-        from = within % span;
+        from = within - item * span;
     }
-    __device__ __forceinline__ static uint32_t warp_sum(uint32_t v) { return __reduce_add_sync(0xffffffffu, v); }
-    __device__ __forceinline__ uint32_t items(const AtSequence &q) const { return (uint32_t)at_row_tiles(a, q, kRows) * a.kv_heads; }
-    __device__ __forceinline__ uint32_t weight(uint32_t k) const {
-        if (k >= a.rows.num_seqs) return 0;
-        const AtSequence q = at_sequence(a, S::kPaged, k);
-        int32_t f;
-        return items(q) * at_span(a, q, S::kBlock, f);
+    __device__ __noinline__ void hold(uint32_t k) {
+        const uint32_t lane = threadIdx.x & 31;
+        held = k;
+        my_items = 0;
+        my_span = 1;
+        my_first = 0;
+        if (k + lane >= a.rows.num_seqs) return;
+        my = at_sequence(a, S::kPaged, k + lane);
+        my_span = at_span(a, my, S::kBlock, my_first);
+        my_items = (uint32_t)at_row_tiles(a, my, kRows) * a.kv_heads;
     }
-    __device__ __forceinline__ void open() {
-        s = at_sequence(a, S::kPaged, i);
-        span = at_span(a, s, S::kBlock, first);
+    uint32_t items;  // of the sequence
+    __device__ __noinline__ void open() {
+        if (held != (i & ~31u)) hold(i & ~31u);
+        const int l = i & 31;
+        auto from_lane = [&](auto v) { return __shfl_sync(0xffffffffu, v, l); };
+        s.begin = from_lane(my.begin);
+        s.rows = from_lane(my.rows);
+        s.seq = from_lane(my.seq);
+        s.len = from_lane(my.len);
+        s.pos0 = from_lane(my.pos0);
+        span = from_lane(my_span);
+        first = from_lane(my_first);
+        items = from_lane(my_items);
     }
     __device__ __forceinline__ AtSegment next() {
         AtSegment t{};
@@ -448,8 +465,8 @@ struct AtWork {
             }
         }
         while (at < end) {
-            if (item >= items(s)) {  // the next sequence
-                item0 += items(s);
+            if (item >= items) {  // the next sequence
+                item0 += items;
                 if (++i >= a.rows.num_seqs) return t;
                 item = from = 0;
                 open();
@@ -559,7 +576,7 @@ __device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint3
         }
         return;
     }
-    constexpr int kAhead = PARTS == 3 ? 4 : 16;  // loads in flight
+    constexpr int kAhead = 4;  // loads in flight (few, as a first time through code costs its fetch)
 #pragma unroll 1
     for (uint32_t i0 = 0; i0 < 16; i0 += kAhead) {
         if (!(rows >> (2 * i0))) break;
@@ -641,16 +658,22 @@ __host__ __device__ constexpr int cached_order(int t) { return 4 * ((t & 7) >> 1
 __host__ __device__ constexpr int cached_token(int column) {
     return (column & ~15) + 2 * ((column & 15) >> 2) + (column & 1) + 8 * ((column >> 1) & 1);
 }
-// a cached tile's address for a token that exists; a bad page latches and reads page 0
-__device__ __forceinline__ const uint8_t *at_tile(const AtArgs &a, int32_t seq, int32_t head, int32_t token) {
+// the page that holds a token, as the table has it
+__device__ __forceinline__ int32_t at_page(const AtArgs &a, int32_t seq, int32_t token) {
+    return a.geo.page_table[(size_t)seq * a.geo.mp + (uint32_t)token / a.geo.page_tokens];
+}
+// a cached tile's address in it, for a token that exists; a bad page latches and reads page 0
+__device__ __forceinline__ const uint8_t *at_tile_in(const AtArgs &a, int32_t page, int32_t head, int32_t token) {
     const StoreGeo &g = a.geo;
-    int32_t pg = g.page_table[(size_t)seq * g.mp + (uint32_t)token / g.page_tokens];
-    if (pg < 0 || (uint32_t)pg >= g.total_pages) {
+    if (page < 0 || (uint32_t)page >= g.total_pages) {
         latch(a.status, QWN_KV_STATUS_BAD_PAGE);
-        pg = 0;
+        page = 0;
     }
-    return g.pages + (size_t)pg * g.page_bytes +
+    return g.pages + (size_t)page * g.page_bytes +
            ((size_t)(a.layer * g.kv_heads + head) * g.tpp + (uint32_t)token % g.page_tokens / kTileTokens) * g.tile_bytes;
+}
+__device__ __forceinline__ const uint8_t *at_tile(const AtArgs &a, int32_t seq, int32_t head, int32_t token) {
+    return at_tile_in(a, at_page(a, seq, token), head, token);
 }
 
 // What the operands hold of a cached value, so that f16 holds it without loss of range: int8 codes by
@@ -1187,31 +1210,44 @@ struct AtRoles {
                          fetch(whole(seg, seg.block0 + b) ? sh.full : sh.part, S::v_slot(done), S::v_turn(done), vmap);
                 }
             } else if constexpr (S::kRaw) {
-                auto address = [&](int b) -> const uint8_t * {
+                // A lane has a tile of each block.  Its page is looked up two blocks ahead, and nothing asks for it before
+                // its turn; lanes issue as their slots become free.
+                const bool tiles = lane < S::kTiles;
+                auto page_of = [&](int b) {
                     const int32_t token = (seg.block0 + b) * S::kBlock + lane * kTileTokens;
-                    return b < seg.blocks && lane < S::kTiles && token < seg.len ? at_tile(a, seg.seq, seg.head, token) : nullptr;
+                    return tiles && b < seg.blocks && token < seg.len ? at_page(a, seg.seq, token) : -1;
                 };
-                const uint8_t *ahead = address(0);
-                for (int b = 0; b < seg.blocks && ok; b++) {
-                    const uint8_t *from = ahead;
-                    ahead = address(b + 1);  // the next block's pages are looked up while this one's tiles go out
-                    for (int t = 0; t < S::kTiles && ok; t++, done++) {
-                        const uint32_t s = done % S::kRawTiles;
-                        ok = wait(&sh.rawempty[s], ((done / S::kRawTiles) & 1) ^ 1);
-                        if (ok && lane == t) {
-                            if (from) {
+                int32_t ahead[2] = {page_of(0), page_of(1)};
+                for (int b = 0; b < seg.blocks && ok; b++, done += S::kTiles) {
+                    const int32_t token = (seg.block0 + b) * S::kBlock + lane * kTileTokens, page = ahead[0];
+                    ahead[0] = ahead[1];
+                    ahead[1] = page_of(b + 2);
+                    const bool have = tiles && token < seg.len;
+                    const uint32_t g = done + lane, s = g % S::kRawTiles, parity = ((g / S::kRawTiles) & 1) ^ 1;
+                    bool waits = tiles;
+                    for (uint32_t it = 0;; ++it) {
+                        if (waits && mbar_try_wait(&sh.rawempty[s], parity)) {
+                            waits = false;
+                            if (have) {
                                 mbar_expect_tx(&sh.rawfull[s], S::kTileBytes);
                                 asm volatile(
                                     "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
                                         "r"(raw_at + s * S::kTileBytes),
-                                    "l"(from), "r"(S::kTileBytes), "r"(smem_u32(&sh.rawfull[s]))
+                                    "l"(at_tile_in(a, page, seg.head, token)), "r"(S::kTileBytes), "r"(smem_u32(&sh.rawfull[s]))
                                     : "memory");
                             } else {
                                 mbar_arrive(&sh.rawfull[s]);
                             }
                         }
-                        __syncwarp();
+                        if (!__any_sync(0xffffffffu, waits)) break;
+                        if (it >= kWaitLimit || ((it & 63) == 63 && *(volatile int *)&sh.give_up)) {
+                            issued[0] = __ballot_sync(0xffffffffu, tiles && !waits);  // of this block
+                            *(volatile int *)&sh.give_up = 1;
+                            ok = false;
+                            break;
+                        }
                     }
+                    ok = __all_sync(0xffffffffu, ok);
                 }
             }
         }
@@ -1222,8 +1258,14 @@ struct AtRoles {
                 if (issued[1] >> v & 1) mbar_wait_bounded(&sh.part[v], (phase[1] >> v & 1) ^ 1);
             }
         } else if constexpr (S::kRaw) {
-            for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++)
-                mbar_wait_bounded(&sh.rawfull[d % S::kRawTiles], (d / S::kRawTiles) & 1);
+            for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++) {
+                // (after giving up, the slots that its block has filled already are a turn further)
+                const uint32_t s = d % S::kRawTiles, t = (s + S::kRawTiles - done % S::kRawTiles) % S::kRawTiles;
+                if (!ok || t >= S::kTiles || !(issued[0] >> t & 1)) mbar_wait_bounded(&sh.rawfull[s], (d / S::kRawTiles) & 1);
+            }
+            for (uint32_t t = 0; t < S::kTiles; t++)
+                if (issued[0] >> t & 1)
+                    mbar_wait_bounded(&sh.rawfull[(done + t) % S::kRawTiles], ((done + t) / S::kRawTiles) & 1);
         }
     }
 
