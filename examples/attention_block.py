@@ -3,10 +3,10 @@
     norm -> int8 -> query/key/value product -> rotation and append -> attention
          -> int8 -> output product -> residual of the next norm
 
-Prompts of several sequences go through it in one ragged batch; their attention
-is a plain torch softmax over the cache's own rows (``KvPool.load_tokens``), so
-that a prompt may follow on tokens that are cached already.  Then every
-sequence decodes one token at a time through ``KvPool.decode``.
+Prompts of several sequences go through it in one ragged batch; they attend over
+the cache's own rows (``KvPool.chunk_attention``), so that a prompt may follow on
+tokens that are cached already.  Then every sequence decodes one token at a time
+through ``KvPool.decode``.
 
     python examples/attention_block.py [--codec 1..5] [--steps N]
 """
@@ -60,6 +60,7 @@ class AttentionBlock:
         self.scales = torch.empty(max_rows, device="cuda")
         self.qkv = torch.empty((max_rows, qkv_width), dtype=torch.bfloat16, device="cuda")
         self.query = torch.empty((max_rows, query_heads, HEAD), device="cuda")  # decode() reads fp32
+        self.workspace = torch.empty(0, dtype=torch.uint8, device="cuda")
 
     def project(self, x, residual):
         """Adds x to the residual stream in place, norms it, and fills self.qkv."""
@@ -91,18 +92,12 @@ class AttentionBlock:
         self.project(x, residual)
         self.pool.seq_append(seqs, counts=torch.tensor(counts, dtype=torch.int32, device="cuda"))
         self.store(seqs, rows, begin)
-        lens = [int(n) for n in self.pool.lens()[:seqs]]
-        held = torch.tensor([0] + lens, device="cuda").cumsum(0).int()
-        key, value = (torch.empty((sum(lens), self.hk, HEAD), device="cuda") for _ in range(2))
-        self.pool.load_tokens(0, seqs, sum(lens), qb.DTYPE_F32, key, value, row_begin=held)
         out = torch.empty((rows, self.hq, HEAD), device="cuda")
-        at = 0
-        for i, n in enumerate(counts):
-            k, v = (t[int(held[i]):int(held[i + 1])].repeat_interleave(self.hq // self.hk, 1) for t in (key, value))
-            s = torch.einsum("qhd,khd->hqk", self.query[at:at + n], k) / math.sqrt(HEAD)
-            future = torch.arange(lens[i], device="cuda") > torch.arange(lens[i] - n, lens[i], device="cuda")[:, None]
-            out[at:at + n] = torch.einsum("hqk,khd->qhd", s.masked_fill(future, -torch.inf).softmax(-1), v)
-            at += n
+        size = self.pool.chunk_workspace(seqs, rows, self.hq)
+        if size > self.workspace.numel():
+            self.workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+        self.pool.chunk_attention(0, seqs, rows, qb.DTYPE_F32, self.hq, self.query, out, row_begin=begin,
+                                  workspace=self.workspace, workspace_bytes=self.workspace.numel())
         return self.output(out, rows)
 
     def step(self, x, residual):

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
 }
 
 // How a call is cut: two tiles of 128 rows per CTA or one, and into runs or not.
-constexpr uint64_t kMaxWorkspace = 64ull << 20;  // for pieces of rows; beyond, there are tiles for every SM
+constexpr uint64_t kMaxWorkspace = 128ull << 20;  // for pieces of rows; beyond, there are tiles for every SM
 struct ChunkPlan {
     uint32_t tiles, slot_rows;
     uint64_t units, prefix_bytes, workspace;
@@ -125,8 +125,8 @@ ChunkPlan plan_chunk(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32
     c.units = runs ? rows / tile + num_seqs : num_seqs * ((group + tile - 1) / tile);
     c.prefix_bytes = 2 * ((uint64_t)num_seqs + 1) * 4 + 255 & ~255ull;
     const bool quarters = c.tiles == 1 && dtype != QWN_DTYPE_F32 && p->codec != QWN_KV_CODEC_F16;
-    // one row per sequence is eight rows of a kv head at most, in each quarter
-    c.slot_rows = quarters && !runs ? 4 * kMaxGroup : 128 * c.tiles;
+    // one row per sequence is a kv head's group, in each quarter
+    c.slot_rows = quarters && !runs ? 4 * (uint32_t)group : 128 * c.tiles;
     const uint64_t items = c.units * p->kv_heads, slots = quarters ? items + p->sms : 2ull * p->sms;
     const uint64_t bytes = slots * at_slot_floats(c.slot_rows) * sizeof(float);
     // blocks are counted in 32 bits
@@ -210,7 +210,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     a.causal = 1;
     a.layer = r->layer;
     a.dtype = r->dtype;
-    a.scale2 = (r->scale > 0.f ? r->scale : 0.08838834764831845f) * 1.4426950408889634f;
+    set_scale(a, r->scale);
     a.query_stride = qs;
     a.out_stride = os;
     a.query = r->query_dev;

@@ -74,7 +74,7 @@ QWN_CUDA_ABI_API int qwn_prompt_attention(const QwnPromptAttentionRequest *r) {
     a.window = r->window;
     a.causal = r->causal ? 1 : 0;
     a.dtype = r->dtype;
-    a.scale2 = (r->scale > 0.f ? r->scale : 0.08838834764831845f) * 1.4426950408889634f;
+    set_scale(a, r->scale);
     a.query_stride = qs, a.key_stride = ks, a.value_stride = vs, a.out_stride = os;
     a.query = r->query_dev, a.key = r->key_dev, a.value = r->value_dev, a.out = r->output_dev;
     a.status = r->status_dev;

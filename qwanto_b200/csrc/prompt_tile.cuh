@@ -31,6 +31,7 @@
 // MMAs instead of one, fp32 accuracy.
 #pragma once
 
+#include <cmath>
 #include <mutex>
 
 #include "kv_internal.cuh"
@@ -62,7 +63,7 @@ struct AtArgs {
     RowMap rows;
     uint32_t group, kv_heads, query_heads, window, causal, layer;
     uint32_t dtype;            // of query and output
-    float scale2;              // scale x log2 e
+    float scale2, scale2_low;  // scale x log2 e, and what fp32 lacks of it
     uint64_t query_stride, key_stride, value_stride, out_stride;  // values
     const void *query, *key, *value;
     void *out;
@@ -81,17 +82,17 @@ struct AtShape {
     static constexpr bool kPaged = SRC != 0;
     static constexpr bool kTma = !kPaged && PARTS == 1;            // operand tiles straight from the rows
     static constexpr bool kRaw = kPaged && SRC != QWN_KV_CODEC_F16;// cached tiles by way of shared memory
+    // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
+    // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
+    static constexpr bool kByDims = PARTS == 1 && kRaw;
     // Registers per thread after the split, no more in all than the block starts with.  The softmax warps hold a
     // row's 128 scores; what they lack goes to memory (16384 rows of 13 prompts: 334 us with 184, 299 with 200).
-    // Where codes are converted the scores are read twice out of tensor memory instead, and twice as many helpers
-    // have the registers.
+    // Where one tile's rows read the keys, the cached codes' conversion is what counts: the scores are read twice out
+    // of tensor memory instead, and twice as many helpers have the registers.
     static constexpr int kHelpers = kTma ? 4 : 8, kThreads = 384 + 32 * kHelpers;
     static constexpr int kLaunchRegs = kHelpers == 8 ? 96 : 128, kSoftmaxRegs = kTma ? 200 : 112;
     static constexpr int kHelperRegs = kTma ? 64 : 96, kOtherRegs = kHelpers == 8 ? 64 : 48;
     static_assert(2 * kSoftmaxRegs + kHelpers / 4 * kHelperRegs + kOtherRegs <= kThreads / 128 * kLaunchRegs, "registers");
-    // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
-    // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
-    static constexpr bool kByDims = PARTS == 1 && kRaw;
     // 32 rows or fewer, as a decode step or a few drafts have, would leave three warps of a softmax group idle.  They
     // are then in the tile four times, and each warp takes a quarter of a block's tokens: its rows of P are zero
     // elsewhere, and its rows of O a partial result like those of other CTAs.  Not for fp16 pages, whose values may
@@ -315,12 +316,12 @@ __device__ __forceinline__ AtSegment at_segment(const AtArgs &a, const AtSequenc
     t.head = head;
     t.len = s.len;
     t.pos0 = s.pos0;
-    const int64_t p0 = s.pos0 + row0 / a.group, p1 = s.pos0 + (row0 + (uint32_t)t.rows - 1) / a.group;
-    int32_t b1;
-    at_blocks(a, p0, p1, s.len, block, t.block0, b1);
-    t.blocks = b1 - t.block0;
     // rows that do not exist count for nothing
-    const Seen first = at_seen(a, max(p0, (int64_t)0), s.len), last = at_seen(a, min(p1, (int64_t)s.len - 1), s.len);
+    const int64_t p0 = max(s.pos0 + row0 / a.group, (int64_t)0);
+    const int64_t p1 = min(s.pos0 + (row0 + (uint32_t)t.rows - 1) / a.group, (int64_t)s.len - 1);
+    const Seen first = at_seen(a, p0, s.len), last = at_seen(a, p1, s.len);
+    t.block0 = first.lo / block;
+    t.blocks = p0 > p1 ? 0 : (last.hi + block - 1) / block - t.block0;
     t.whole_lo = (last.lo + block - 1) / block;
     t.whole_hi = first.hi / block;
     t.slot = -1;
@@ -732,11 +733,19 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
-// a pair of ranges over 2 LEVELS, rounded once: f16's nearest to the factor, and what that lacks
+// Halved values of low-bit codes.  V: in f16, where the step's own rounding is up to range x 2^-12 in the value of
+// the largest code, too little to see beside P's.  K: in fp32 and rounded once, since that error is the same for
+// all of a group's dims, and a query's outlier multiplies it (2048 rows over a 4-bit cache with outliers: outputs
+// off by 3.0 to 3.8e-3 of their norm with f16 steps, where bf16's own rounding makes 1.6e-3).
 template <int LEVELS>
-__device__ __forceinline__ uint32_t half_steps(uint32_t ranges) {
-    constexpr float f = 0.5f / LEVELS, near = LEVELS == 15 ? 1092.f / 32768.f : 1170.f / 16384.f;
-    return hfma2(ranges, pack_h2(near, near), hmul2(ranges, pack_h2(f - near, f - near)));
+__device__ __forceinline__ uint32_t half_steps(uint32_t ranges) {  // a pair of ranges over 2 LEVELS, rounded once
+    constexpr float f = 0.5f / LEVELS, near = LEVELS == 15 ? 1092.f / 32768.f : 1170.f / 16384.f;  // f16's nearest, and
+    return hfma2(ranges, pack_h2(near, near), hmul2(ranges, pack_h2(f - near, f - near)));         // what that lacks
+}
+__device__ __forceinline__ uint32_t key_pair(uint32_t codes, float step, float low) {
+    float a, b;
+    unpair(fma2(pair(h2f((uint16_t)codes), h2f((uint16_t)(codes >> 16))), pair(step, step), pair(low, low)), a, b);
+    return pack_h2(a, b);
 }
 __device__ __forceinline__ uint4 ld16(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 // eight codes of 3.5-bit words: odd dims of half 1 have their lowest bit above half 0's and two in a plane
@@ -814,25 +823,25 @@ struct KeyWords {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {  // odd tokens in another order, for the banks
                         const uint32_t c = odd ? k ^ 1 : k, p = odd ? par[k ^ 1] : par[k];
-                        const uint32_t step = half_steps<15>(prmt(p, p, 0x1010u)), low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+                        const float step = h2f((uint16_t)p) * (0.5f / 15.f), low = h2f((uint16_t)(p >> 16)) * 0.5f;
                         uint32_t v[4];
                         nib8_to_h2x4(odd ? word[k ^ 1] : word[k], v);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
+                        for (int i = 0; i < 4; i++) v[i] = key_pair(v[i], step, low);
                         st_shared16(chunk_at(base, 128, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
                     }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const uint32_t p = x ? (pass ? w[2].w : w[2].z) : (pass ? w[2].y : w[2].x), ranges = prmt(p, p, 0x1010u);
-                        const uint32_t low = hmul2(prmt(p, p, 0x3232u), 0x38003800u);
+                        const uint32_t p = x ? (pass ? w[2].w : w[2].z) : (pass ? w[2].y : w[2].x);
+                        const float range = h2f((uint16_t)p), low = h2f((uint16_t)(p >> 16)) * 0.5f;
 #pragma unroll
                         for (int o = 0; o < 2; o++) {
-                            const uint32_t step = o ? half_steps<7>(ranges) : half_steps<15>(ranges);
+                            const float step = range * (o ? 0.5f / 7.f : 0.5f / 15.f);
                             uint32_t v[4];
                             nib8_to_h2x4(o ? odd_codes(w[pass].z, w[pass].w, x) : x ? w[pass].y : w[pass].x, v);
 #pragma unroll
-                            for (int i = 0; i < 4; i++) v[i] = hfma2(v[i], step, low);
+                            for (int i = 0; i < 4; i++) v[i] = key_pair(v[i], step, low);
                             st_shared16(chunk_at(base, 128, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
                         }
                     }
@@ -1143,6 +1152,7 @@ struct AtRoles {
     // the operands' own scaling: of scores and of outputs
     static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
     static constexpr bool kHold = PARTS == 3 || S::kTma;  // a row's scores stay in registers
+    static constexpr int kStep = 32;  // columns at a time where they do not
     static constexpr uint32_t kFmaPairs = 0x10;  // of eight pairs of powers, those that FMAs compute
     const AtArgs &a;
     AtShared<SRC, PARTS, TILES> &sh;
@@ -1281,7 +1291,8 @@ struct AtRoles {
     // room is given back.  fp16 tiles go as they are, in asynchronous copies of 16 bytes (their chunks are swizzled as the operands'
     // are); a block's are on their way while the next block's start.
     __device__ __forceinline__ bool convert_side(const AtSegment &seg, uint32_t done, uint32_t segment, uint32_t &meetings) {
-        const int which = (warp - 8) >> 2, w = warp & 3;
+        const int w = warp & 3;
+        int which = (warp - 8) >> 2;  // K or V; four warps make both in turn
         auto slot_of = [&](uint32_t d) { return which ? S::v_slot(d) : S::k_slot(d); };
         auto free_slot = [&](uint32_t d) { return wait(&sh.empty[slot_of(d)], ((which ? S::v_turn(d) : S::k_turn(d)) & 1) ^ 1); };
         auto ready = [&](uint32_t d, int blk) {  // the block's operands are written
@@ -1303,7 +1314,10 @@ struct AtRoles {
         };
         if constexpr (S::kByDims) {
             extern __shared__ uint8_t dynamic[];
-            for (int b = 0; b < seg.blocks; b++) {
+            constexpr int kSides = S::kHelpers == 4 ? 2 : 1;
+            for (int n = 0; n < seg.blocks * kSides; n++) {
+                const int b = n / kSides;
+                if (kSides == 2) which = n & 1;
                 const uint32_t d = done + b, dst = slot_at(slot_of(d));
                 const int32_t token0 = (seg.block0 + b) * S::kBlock;
                 uint32_t ring[2];
@@ -1625,6 +1639,15 @@ struct AtRoles {
         if constexpr (kHold) {
             if constexpr (N == 128) tmem_load128(held, s_col);
             else tmem_load64(held, s_col);
+            if constexpr (kTokenScales) {
+                float *y = reinterpret_cast<float *>(held);
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i]);
+                    unpair(mul2(pair(y[i], y[i + 1]), pair(f.x, f.y)), y[i], y[i + 1]);
+                    unpair(mul2(pair(y[i + 2], y[i + 3]), pair(f.z, f.w)), y[i + 2], y[i + 3]);
+                }
+            }
             if (!full) hide(held, lo, hi);
 #pragma unroll
             for (int i = 0; i < 8; i++) t[i] = x[i];
@@ -1636,12 +1659,12 @@ struct AtRoles {
 #pragma unroll
             for (int k = 0; k < 8; k++) t[k] = -INFINITY;
 #pragma unroll 1
-            for (int i = 0; i < N; i += 32) {
-                uint32_t u[32];
-                tmem_load32(u, s_col + i);
+            for (int i = 0; i < N; i += kStep) {
+                uint32_t u[kStep];
+                tmem_load_step(u, s_col + i);
                 adjust(u, i, slot, full, lo, hi);
 #pragma unroll
-                for (int k = 0; k < 32; k++) t[k & 7] = fmaxf(t[k & 7], __uint_as_float(u[k]));
+                for (int k = 0; k < kStep; k++) t[k & 7] = fmaxf(t[k & 7], __uint_as_float(u[k]));
             }
         }
         const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
@@ -1655,12 +1678,12 @@ struct AtRoles {
             else l += powers<false, N>(held, 0, slot, c, off, s_col);
         } else {
 #pragma unroll 1
-            for (int i = 0; i < N; i += 32) {
-                uint32_t u[32];
-                tmem_load32(u, s_col + i);
+            for (int i = 0; i < N; i += kStep) {
+                uint32_t u[kStep];
+                tmem_load_step(u, s_col + i);
                 adjust(u, i, slot, full, lo, hi);
-                if (full) l += powers<true, 32>(u, i, slot, c, off, s_col);
-                else l += powers<false, 32>(u, i, slot, c, off, s_col);
+                if (full) l += powers<true, kStep>(u, i, slot, c, off, s_col);
+                else l += powers<false, kStep>(u, i, slot, c, off, s_col);
             }
         }
         tmem_store_wait();
@@ -1729,11 +1752,16 @@ struct AtRoles {
         }
     }
     // 32 columns of scores from column i on: times the tokens' scales, -inf where a row does not see the token
-    __device__ __forceinline__ void adjust(uint32_t (&u)[32], int i, uint32_t slot, bool full, int lo, int hi) {
+    static __device__ __forceinline__ void tmem_load_step(uint32_t (&u)[kStep], uint32_t addr) {
+        if constexpr (kStep == 64) tmem_load64(u, addr);
+        else tmem_load32(*reinterpret_cast<uint32_t (*)[32]>(u), addr);
+    }
+    template <int N>
+    __device__ __forceinline__ void adjust(uint32_t (&u)[N], int i, uint32_t slot, bool full, int lo, int hi) {
         float *x = reinterpret_cast<float *>(u);
         if constexpr (kTokenScales) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
+            for (int k = 0; k < N; k += 4) {
                 const float4 f = *reinterpret_cast<const float4 *>(&sh.kscale[slot][i + k]);
                 unpair(mul2(pair(x[k], x[k + 1]), pair(f.x, f.y)), x[k], x[k + 1]);
                 unpair(mul2(pair(x[k + 2], x[k + 3]), pair(f.z, f.w)), x[k + 2], x[k + 3]);
@@ -1753,7 +1781,8 @@ struct AtRoles {
             uint32_t p[PARTS][16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-                const uint64_t t = fma2(pair(x[i + k], x[i + k + 1]), cc, oo);
+                uint64_t t = fma2(pair(x[i + k], x[i + k + 1]), cc, oo);
+                if constexpr (PARTS == 3) t = fma2(pair(x[i + k], x[i + k + 1]), pair(a.scale2_low, a.scale2_low), t);
                 uint64_t e;
                 if (MIXED && (kFmaPairs >> ((k >> 1) & 7) & 1)) {
                     e = exp2_pair<BF16>(t);
@@ -1869,7 +1898,12 @@ struct AtRoles {
                 }
 #pragma unroll
                 for (int k = 0; k < kWide; k++) o[k] = per == 0.f ? 0.f : o[k] * per;
-                if (floats) {
+                if (S::kQuarters && seg.quarters) {  // few rows: as they are, in a few instructions
+                    if (have)
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4)
+                            store4(reinterpret_cast<float *>(to) + col + k, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+                } else if (floats) {
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         piece[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]),
@@ -1978,6 +2012,15 @@ __global__ void __launch_bounds__(AtShape<SRC, PARTS, TILES>::kThreads, 1) promp
 }
 
 // ---- host ----------------------------------------------------------------------
+
+// a call's softmax scale (0: 1/sqrt(128)) times log2 e
+inline void set_scale(AtArgs &a, float scale) {
+    const double s = (scale > 0.f ? (double)scale : 0.08838834764831844055) * 1.44269504088896340736;
+    a.scale2 = (float)s;
+    // the rest is positive: times a masked score, -inf, it is to stay that
+    if (a.scale2 >= s) a.scale2 = nextafterf(a.scale2, 0.f);
+    a.scale2_low = (float)(s - (double)a.scale2);
+}
 
 // Prepares a kernel on the current device, once.  Refuses one whose block does not
 // start with the registers that its warps share out: it would wait for them for good.

@@ -392,3 +392,34 @@ def test_same_bits_every_time(cuda, codec, kind):
             first = _run(torch, c, q, counts, kind, workspace=split)
             for _ in range(12):
                 assert torch.equal(first, _run(torch, c, q, counts, kind, workspace=split))
+
+
+def test_many_sequences(cuda):
+    """More (tile, head) pairs than a workspace is made for, and just fewer."""
+    torch = cuda
+    for seqs, hk, heads in ((150, 8, 16), (700, 8, 64)):
+        lens = [1 + (37 * i) % 200 for i in range(seqs)]
+        c = Cache(torch, 2, lens, hk, seed=16)
+        q = _queries(torch, seqs, heads, "bf16")
+        out = _run(torch, c, q, [1] * seqs, "bf16", one=True)
+        few = list(range(0, seqs, 29))
+        from promptmath import assert_near, attend, seen
+        for i in few:
+            k, v = c.kv[i]
+            want, tol = attend(q[i:i + 1], k, v, seen(lens[i] - 1, 1, lens[i], True, 0), 0.0, "bf16", 2.0 ** -11)
+            assert_near(out[i:i + 1], want, tol, f"sequence {i}")
+        runs = _run(torch, c, q, [1] * seqs, "bf16")  # as runs of one row
+        assert (runs.float() - out.float()).abs().max() < 0.02
+        c.pool.close()
+
+
+@pytest.mark.parametrize("codec", CODECS)
+def test_rows_up_to_a_quarter_of_a_tile_and_beyond(cuda, codec):
+    """32 rows of a kv head are in the tile four times, 33 once; both in one call, over contexts that several
+    blocks of threads share."""
+    torch, lens, counts = cuda, [3000, 2999, 1500, 40, 5], [4, 5, 8, 9, 5]
+    c = Cache(torch, codec, lens, 2, seed=codec + 60)
+    for kind in ("bf16", "f16"):
+        q = _queries(torch, sum(counts), 16, kind)
+        _check(torch, _run(torch, c, q, counts, kind), c, codec, q, counts, kind)
+        _check(torch, _run(torch, c, q, counts, kind, window=700), c, codec, q, counts, kind, window=700)

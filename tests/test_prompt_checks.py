@@ -2,6 +2,7 @@
 their ctypes mirrors, and arguments are refused before any device work."""
 import ctypes as C
 import os
+import re
 import subprocess
 import tempfile
 
@@ -88,3 +89,55 @@ def test_chunk_needs_a_pool():
     for handle in (C.byref(h), None):
         assert lib.qwn_kv_chunk_attention(handle, C.byref(r)) == INVALID
         assert lib.qwn_kv_chunk_workspace(handle, 1, 1, 1, C.byref(n)) == INVALID
+
+
+def _kernel_source():
+    text = open(os.path.join(ROOT, "qwanto_b200", "csrc", "prompt_tile.cuh")).read()
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def _body(text, start):
+    """The text from the first brace behind `start` to the matching one."""
+    at = text.index("{", text.index(start))
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[at:i + 1]
+    raise AssertionError(start)
+
+
+def test_the_next_launch_starts_after_tensor_memory_is_held():
+    """What a run could only show by hanging is read: see the products' tests."""
+    body = _body(_kernel_source(), "prompt_tile_kernel(")
+    assert body.count("launch_dependents()") == 1
+    assert body.index("tmem_alloc<") < body.index("__syncthreads()") < body.index("launch_dependents()")
+    # no role polls a barrier before the previous launch has ended
+    waits = body.index("wait_previous()")
+    for role in ("roles.soften()", "roles.help()", "roles.multiply()", "roles.load(", "roles.plan()"):
+        assert body.count(role) == 1 and waits < body.index(role)
+
+
+def test_every_wait_is_bounded():
+    text = _kernel_source()
+    assert "kWaitLimit" in _body(text, "at_wait(volatile int &give_up")
+    # no named barrier, which one role could leave and another wait at; the block's own only where all meet
+    assert "bar.sync" not in text and text.count("__syncthreads()") == 2
+    # the only other poll, of the copies' lanes, gives up alike
+    polls = [m.start() for m in re.finditer(r"mbar_try_wait\(", text)]
+    assert len(polls) == 2
+    assert "it >= kWaitLimit" in text[polls[1]:polls[1] + 1500]
+
+
+def test_registers_are_shared_out_from_what_a_block_starts_with():
+    """A warpgroup that asks for more than the others gave back waits for good."""
+    text = _kernel_source()
+    assert "2 * kSoftmaxRegs + kHelpers / 4 * kHelperRegs + kOtherRegs <= kThreads / 128 * kLaunchRegs" in text
+    assert "at.numRegs < AtShape<SRC, PARTS, TILES>::kLaunchRegs" in _body(text, "cudaError_t prepare_tile_kernel(")
+
+
+def test_cached_tiles_are_given_back_behind_a_proxy_fence():
+    text = _kernel_source()
+    body = _body(text, "auto give_back")
+    assert body.index("fence_proxy_async_shared()") < body.index("warp_arrive(&sh.rawempty")
+    assert text.count("sh.rawempty[r], lane") == 1
