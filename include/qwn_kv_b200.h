@@ -510,7 +510,7 @@ typedef struct {
     void *stream;
 } QwnKvChunkAttentionRequest;
 QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *pool, const QwnKvChunkAttentionRequest *request);
-/* workspace of a call with these sizes, whatever its types and lengths; may be 0 */
+/* workspace for calls of at most these sizes, whatever their types and lengths; 0 without rows or sequences */
 QWN_CUDA_ABI_API int qwn_kv_chunk_workspace(const QwnKvPoolHandle *pool, uint32_t num_seqs, uint32_t num_rows,
                                             uint32_t query_heads, uint64_t *bytes);
 

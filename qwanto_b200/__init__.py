@@ -262,7 +262,7 @@ class KvPool:
         check("qwn_kv_chunk_attention", rc)
 
     def chunk_workspace(self, num_seqs: int, num_rows: int, query_heads: int) -> int:
-        """Bytes of workspace for chunk_attention calls of these sizes."""
+        """Bytes of workspace for chunk_attention calls of at most these sizes."""
         n = C.c_uint64(0)
         check("qwn_kv_chunk_workspace", lib().qwn_kv_chunk_workspace(self._href, num_seqs, num_rows, query_heads,
                                                                       C.byref(n)))

@@ -54,6 +54,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
     const uint32_t at = r % kRows;
     const uint32_t parts = (b1 - b0 + 1) << (quarters ? 2 : 0), step = a.slot_rows / 4;
     const uint32_t first_slot = S::kQuarters ? a.prefix[a.rows.num_seqs + 1 + i] + item + b0 : 0;
+    // sequences that overlap have pieces that were not written (the tile kernel tells)
+    if (b1 < b0 || b1 >= grid || (uint64_t)first_slot + (S::kQuarters ? b1 - b0 : 2 * b1 + 1) >= a.slot_count) return;
     const bool second = u0 > runs.begin(b0);
     // the k-th piece of the row: a CTA's, or one quarter of a CTA's
     auto piece = [&](uint32_t k, uint32_t &place) {
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AtArg
 // How a call is cut: two tiles of 128 rows per CTA or one, and into runs or not.
 constexpr uint64_t kMaxWorkspace = 128ull << 20;  // for pieces of rows; beyond, there are tiles for every SM
 struct ChunkPlan {
-    uint32_t tiles, slot_rows;
+    uint32_t tiles, slot_rows, slot_count;
     uint64_t units, prefix_bytes, workspace;
     bool split;  // given a workspace
 };
@@ -134,9 +136,22 @@ ChunkPlan plan_chunk(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32
     const uint64_t bytes = slots * at_slot_floats(c.slot_rows) * sizeof(float);
     // blocks are counted in 32 bits
     const uint64_t most = (uint64_t)p->max_pages_per_seq * p->page_tokens / 64 + 2;
+    c.slot_count = (uint32_t)std::min<uint64_t>(slots, 0x7FFFFFFFu);
     c.split = (quarters ? bytes <= kMaxWorkspace : items < 8ull * p->sms) && items * most < 1ull << 31;
     c.workspace = c.split ? c.prefix_bytes + bytes : 0;
     return c;
+}
+
+// What no plan of these sizes or smaller ones goes beyond: a plan's own need is not monotone, as the largest calls
+// have tiles enough and go without runs.
+uint64_t most_workspace(const Pool *p, uint32_t num_seqs, uint32_t num_rows, uint32_t query_heads) {
+    const uint64_t group = query_heads / p->kv_heads, rows = (uint64_t)num_rows * group, seqs = num_seqs, sms = p->sms;
+    // with quarters: a slot per tile and per SM, of one tile or of a group in each quarter
+    const uint64_t runs = (std::min(rows, 128 * seqs) / 128 + seqs) * p->kv_heads + sms;
+    const uint64_t ones = seqs * p->kv_heads + sms, one = 4 * std::min<uint64_t>(group, 128);
+    const uint64_t with = std::max(runs * at_slot_floats(128), ones * at_slot_floats((uint32_t)one)) * sizeof(float);
+    const uint64_t without = 2 * sms * at_slot_floats(rows > 128 ? 256 : 128) * sizeof(float);
+    return (2 * (seqs + 1) * 4 + 255) / 256 * 256 + std::max(std::min(with, kMaxWorkspace), without);
 }
 
 template <int SRC>
@@ -166,10 +181,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_workspace(const QwnKvPoolHandle *h, uint32_t n
     if (query_heads == 0 || query_heads % p->kv_heads || query_heads > p->max_query_heads || num_seqs > p->max_seqs ||
         num_rows > 0x7FFFFFFFu)
         return invalid("qwn_kv_chunk_workspace: heads, sequences or rows out of the pool's range");
-    *bytes = 0;
-    for (uint32_t dtype : {QWN_DTYPE_F32, QWN_DTYPE_BF16})
-        for (bool runs : {false, true})
-            if (num_seqs) *bytes = std::max(*bytes, plan_chunk(p, num_seqs, num_rows, query_heads, dtype, runs).workspace);
+    *bytes = num_seqs && num_rows ? most_workspace(p, num_seqs, num_rows, query_heads) : 0;
     return QWN_CUDA_STATUS_OK;
 }
 
@@ -223,6 +235,7 @@ QWN_CUDA_ABI_API int qwn_kv_chunk_attention(QwnKvPoolHandle *h, const QwnKvChunk
     a.units = (uint32_t)c.units;
     if (c.split && r->workspace_dev) {
         a.slot_rows = c.slot_rows;
+        a.slot_count = c.slot_count;
         a.prefix = static_cast<uint32_t *>(r->workspace_dev);
         a.slots = reinterpret_cast<float *>(static_cast<uint8_t *>(r->workspace_dev) + c.prefix_bytes);
     }

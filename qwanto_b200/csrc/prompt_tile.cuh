@@ -83,6 +83,7 @@ struct AtArgs {
     uint32_t *prefix;          // split: blocks before each sequence and in all, then
     float *slots;              // the partial results, of
     uint32_t slot_rows;        // rows each
+    uint32_t slot_count;       // what there is room for
 };
 // a partial result: o[rows][128], then M[rows], l[rows]
 __host__ __device__ constexpr uint32_t at_slot_floats(uint32_t rows) { return rows * (kHeadDim + 2); }
@@ -492,6 +493,11 @@ struct AtWork {
             t.quarters = S::kQuarters && t.rows <= 32;
             if (S::kQuarters && (t.quarters || count != span)) t.slot = (int32_t)(item0 + item + blockIdx.x);
             else if (count != span) t.slot = (int32_t)(2 * blockIdx.x + (n ? 1 : 0));
+            // (more tiles than the rows make: sequences that overlap)
+            if (t.slot >= (int32_t)a.slot_count || t.slot < -1) {
+                latch(a.status, QWN_KV_STATUS_BAD_LENGTH);
+                return AtSegment{};
+            }
             t.block0 = b0;
             t.blocks = max(b1 - b0, 0);
             at += count;

@@ -76,7 +76,9 @@ def _run(torch, c, q, counts, kind, workspace=True, out=None, one=False, layer=0
     rows, hq, n = q.shape[0], q.shape[1], num_seqs or len(counts)
     if out is None:
         out = torch.full_like(q, 7)
-    if workspace:
+    if isinstance(workspace, tuple):
+        more |= {"workspace": workspace[0], "workspace_bytes": workspace[1]}
+    elif workspace:
         size = c.pool.chunk_workspace(n, rows, hq)
         ws = torch.full((max(size, 16),), 255, dtype=torch.uint8, device="cuda")  # nothing in it matters
         more |= {"workspace": ws, "workspace_bytes": size}
@@ -423,3 +425,39 @@ def test_rows_up_to_a_quarter_of_a_tile_and_beyond(cuda, codec):
         q = _queries(torch, sum(counts), 16, kind)
         _check(torch, _run(torch, c, q, counts, kind), c, codec, q, counts, kind)
         _check(torch, _run(torch, c, q, counts, kind, window=700), c, codec, q, counts, kind, window=700)
+
+
+@pytest.mark.parametrize("codec", [2, 5])
+def test_a_workspace_serves_smaller_calls(cuda, codec):
+    """The workspace of the largest call is one for every smaller call, and sequences' sizes do not shrink it."""
+    torch, lens = cuda, [1500, 400, 40, 900]
+    c = Cache(torch, codec, lens, 8, seed=codec + 70)
+    need = {(n, rows): c.pool.chunk_workspace(n, rows, 32) for n in (1, 2, 4) for rows in (1, 4, 33, 128, 4000, 1 << 20)}
+    assert all(need[a] <= need[b] for a in need for b in need if a[0] <= b[0] and a[1] <= b[1])
+    assert c.pool.chunk_workspace(4, 0, 32) == 0 and c.pool.chunk_workspace(0, 4, 32) == 0
+    size = need[4, 1 << 20]
+    ws = torch.full((size + 256,), 255, dtype=torch.uint8, device="cuda")
+    for kind in KINDS:
+        for counts, one in (([1, 1, 1, 1], True), ([1, 4, 2, 1], False), ([700, 33, 40, 5], False), ([400], False)):
+            q = _queries(torch, sum(counts), 32, kind)
+            out = _run(torch, c, q, counts, kind, workspace=(ws, size), one=one)
+            _check(torch, out, c, codec, q, counts, kind)
+    assert c.pool.check() == 0 and (ws[size:] == 255).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_sequences_that_overlap_write_nothing_else(cuda, kind):
+    """row_begin that goes back makes more tiles than the rows do; they must stay within the workspace and the rows."""
+    torch, n, rows = cuda, 64, 256
+    c = Cache(torch, 2, [300] * n, 2, seed=80)
+    q = _queries(torch, rows, 4, kind)
+    begin = torch.tensor([0, rows] * (n // 2) + [0], dtype=torch.int32, device="cuda")
+    size = c.pool.chunk_workspace(n, rows, 4)
+    room = torch.full((size + (32 << 20),), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((rows + 64, 4, 128), 7, dtype=q.dtype, device="cuda")
+    _run(torch, c, q, None, kind, workspace=(room, size), begin=begin, num_seqs=n, out=out)
+    assert (room[size:] == 255).all() and (out[rows:] == 7).all()
+    assert c.pool.check() & ~BAD_LENGTH == 0
+    # and the pool serves as before
+    good = _queries(torch, n, 4, kind)
+    _check(torch, _run(torch, c, good, [1] * n, kind), c, 2, good, [1] * n, kind)
