@@ -96,6 +96,11 @@ struct AtShape {
     // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
     // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
     static constexpr bool kByDims = PARTS == 1 && kRaw;
+    // Parts of a key or value with fp32 rows: int8 codes of one scale are exact in one, fp16 values in two.  They leave
+    // room for more stages.
+    static constexpr int kKvParts = PARTS == 1 || SRC == QWN_KV_CODEC_Q8_HEAD_F16 ? 1 : SRC == QWN_KV_CODEC_F16 ? 2 : 3;
+    // the operands are codes, the tokens' scales go to scores and probabilities
+    static constexpr bool kTokenScales = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || (PARTS == 1 && SRC == QWN_KV_CODEC_Q8_B64_F32);
     // Registers per thread after the split, no more in all than the block starts with.  The softmax warps hold a
     // row's 128 scores; what they lack goes to memory (16384 rows of 13 prompts: 334 us with 184, 299 with 200).
     // Where one tile's rows read the keys, the cached codes' conversion is what counts: the scores are read twice out
@@ -112,12 +117,12 @@ struct AtShape {
     static constexpr int kBlock = PARTS == 1 ? 128 : 64;           // tokens
     static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
     static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
-    static constexpr uint32_t kKvBytes = kKvPart * PARTS;
+    static constexpr uint32_t kKvBytes = kKvPart * kKvParts;
     // Stages of K and V: loaded ones are a ring that both go through in turn, K0 V0 K1 V1 ..; converted ones
     // are apart, so that K of the next block does not wait behind V of this one.
     static constexpr uint32_t kRing = kTma ? 5 : 0;
-    static constexpr uint32_t kStagesK = PARTS == 1 ? 2 : 1;
-    static constexpr uint32_t kStagesV = kTma || (PARTS == 1 && !kRaw) ? 2 : 1;
+    static constexpr uint32_t kStagesK = kKvParts < 3 ? 2 : 1;
+    static constexpr uint32_t kStagesV = kTma || (PARTS == 1 && !kRaw) || (PARTS == 3 && kKvParts == 1) ? 2 : 1;
     static constexpr uint32_t kStages = kRing ? kRing : kStagesK + kStagesV;
     static constexpr uint32_t kOperands = TILES * kQBytes + kStages * kKvBytes;
     static constexpr uint32_t kSmem = (227 - (!kTma ? 12 : TILES == 2 ? 2 : 8)) * 1024;  // the rest is static
@@ -144,7 +149,7 @@ struct AtShape {
 constexpr uint32_t kAtStages = 5;
 template <int SRC, int PARTS, int TILES>
 struct alignas(1024) AtShared {  // the operands behind it start on 1024 bytes
-    static constexpr bool kTokens = PARTS == 1 && (SRC == QWN_KV_CODEC_Q8_B64_F32 || SRC == QWN_KV_CODEC_Q8_HEAD_F16);
+    static constexpr bool kTokens = AtShape<SRC, PARTS, TILES>::kTokenScales;
     static constexpr int kRaw = SRC == 0 ? 1 : 32;
     // operands of K and V have landed, are free again; V of a block seen in part (loaded ones only): has landed, is ready
     uint64_t full[kAtStages], empty[kAtStages], part[kAtStages], fixed[kAtStages];
@@ -535,24 +540,43 @@ struct AtWork {
 
 // ---- Q ------------------------------------------------------------------------
 
-// three bf16 parts of eight fp32 values, exact: each takes the next 8 bits
-__device__ __forceinline__ void split3(const float *v, uint4 (&part)[3]) {
-    uint32_t w[3][4];
+// bf16 parts of eight fp32 values: each takes the next 8 bits, so that three are exact
+template <int N>
+__device__ __forceinline__ void split(const float *v, uint4 (&part)[N]) {
+    uint32_t w[N][4];
+    float x[8];
+    uint64_t zero = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t u = __float_as_uint(v[i]);
-        const bool fine = (u & 0x7F800000u) != 0x7F800000u;
-        // what is not finite stays whole in the first part (a NaN keeps a bit set)
-        const uint32_t h0 = fine ? u >> 16 : (u >> 16) | ((u & 0xFFFFu) ? 1u : 0u);
-        const float r1 = fine ? v[i] - __uint_as_float(u & 0xFFFF0000u) : 0.f;
-        const uint32_t u1 = __float_as_uint(r1);
-        const float r2 = r1 - __uint_as_float(u1 & 0xFFFF0000u);
-        const uint32_t p[3] = {h0, u1 >> 16, __float_as_uint(r2) >> 16};
+    for (int i = 0; i < 8; i += 2) {
+        zero = fma2(pair(v[i], v[i + 1]), 0, zero);  // NaN where one is not finite
+        const uint32_t a = __float_as_uint(v[i]), b = __float_as_uint(v[i + 1]);
+        w[0][i >> 1] = prmt(a, b, 0x7632u);
+        if constexpr (N > 1)
+            unpair(add2(pair(v[i], v[i + 1]), pair(__uint_as_float((a & 0xFFFF0000u) ^ 0x80000000u),
+                                                   __uint_as_float((b & 0xFFFF0000u) ^ 0x80000000u))), x[i], x[i + 1]);
+    }
+    float z0, z1;
+    unpair(zero, z0, z1);
+    if (z0 + z1 != 0.f) {  // they stay whole in the first part (a NaN keeps a bit set)
 #pragma unroll
-        for (int k = 0; k < 3; k++) w[k][i >> 1] = i & 1 ? w[k][i >> 1] | (p[k] << 16) : p[k];
+        for (int i = 0; i < 8; i++) {
+            const uint32_t u = __float_as_uint(v[i]);
+            if ((u & 0x7F800000u) == 0x7F800000u && (u & 0xFFFFu)) w[0][i >> 1] |= 1u << (16 * (i & 1));
+            if (N > 1 && !isfinite(v[i])) x[i] = 0.f;
+        }
     }
 #pragma unroll
-    for (int k = 0; k < 3; k++) part[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    for (int k = 1; k < N; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t a = __float_as_uint(x[i]), b = __float_as_uint(x[i + 1]);
+            w[k][i >> 1] = prmt(a, b, 0x7632u);
+            if (k + 1 < N)
+                unpair(add2(pair(x[i], x[i + 1]), pair(__uint_as_float((a & 0xFFFF0000u) ^ 0x80000000u),
+                                                       __uint_as_float((b & 0xFFFF0000u) ^ 0x80000000u))), x[i], x[i + 1]);
+        }
+#pragma unroll
+    for (int k = 0; k < N; k++) part[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -619,7 +643,7 @@ __device__ __forceinline__ void put_q(const AtArgs &a, const AtSegment &t, uint3
             const uint32_t r = w0 + 2 * (i0 + i) + (lane >> 4);
             if constexpr (PARTS == 3) {
                 uint4 p[3];
-                split3(reinterpret_cast<const float *>(w[i]), p);
+                split(reinterpret_cast<const float *>(w[i]), p);
 #pragma unroll
                 for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(tile + k * kAtRows * 256, kAtRows, r, c), p[k]);
             } else {
@@ -698,7 +722,6 @@ __device__ __forceinline__ const uint8_t *at_tile(const AtArgs &a, int32_t seq, 
 // applied to its score and its probability; 4- and 3.5-bit values halved (at most 65504 + 65504); fp16 as it is.
 template <int SRC>
 struct AtScale {
-    static constexpr bool kTokens = SRC == QWN_KV_CODEC_Q8_B64_F32 || SRC == QWN_KV_CODEC_Q8_HEAD_F16;
     static constexpr float kFixed = SRC == QWN_KV_CODEC_TQ35_G64 || SRC == QWN_KV_CODEC_Q4_G32 ? 2.f : 1.f;
 };
 // the scale of K (which 0) or V of token t
@@ -711,26 +734,31 @@ __device__ __forceinline__ float token_scale(const uint8_t *tile, int t, int whi
         return fmaxf(*reinterpret_cast<const float *>(s + s32_off(t, 0)), *reinterpret_cast<const float *>(s + s32_off(t, 1)));
     }
 }
-// a row's 16 values of this lane into an operand tile, as three bf16 parts
+// a row's 16 values of this lane into an operand tile, as bf16 parts
+template <int N>
 __device__ __forceinline__ void put_operand(uint32_t base, uint32_t rows, uint32_t part, uint32_t r, int j, const Row16 &x) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        uint4 p[3];
-        split3(x.v + 8 * h, p);
+        uint4 p[N];
+        split(x.v + 8 * h, p);
 #pragma unroll
-        for (uint32_t k = 0; k < 3; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
+        for (uint32_t k = 0; k < N; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
     }
 }
-// K or V of a cached tile, which is tile ti of its block, as fp32 in parts, by one warp; tokens from `len` on are zero
-template <int SRC, int BLOCK>
+// K or V of a cached tile, which is tile ti of its block, as fp32 in N parts, by one warp; tokens from `len`
+// on are zero.  In one part: the int8 codes.
+template <int SRC, int BLOCK, int N>
 __device__ __forceinline__ void put_parts(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
     const int lane = threadIdx.x & 31, j = lane & 7;
 #pragma unroll
     for (int pass = 0; pass < 4; pass++) {
         const int t = 4 * pass + (lane >> 3);
         Row16 x = {};
-        if (token0 + t < len) x = take_row<SRC>(tile, t, which, j);
-        put_operand(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
+        if (token0 + t < len) {
+            if constexpr (N == 1) x = take_q8(tile, t, which, j, 1.f, 1.f);
+            else x = take_row<SRC>(tile, t, which, j);
+        }
+        put_operand<N>(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
     }
 }
 
@@ -1164,7 +1192,7 @@ template <int SRC, int PARTS, int TILES, bool BF16>
 struct AtRoles {
     using S = AtShape<SRC, PARTS, TILES>;
     using Scale = AtScale<SRC>;
-    static constexpr bool kTokenScales = PARTS == 1 && Scale::kTokens;
+    static constexpr bool kTokenScales = S::kTokenScales;
     // the operands' own scaling: of scores and of outputs
     static constexpr float kUnit = PARTS == 1 ? Scale::kFixed : 1.f;
     static constexpr bool kHold = PARTS == 3 || S::kTma;  // a row's scores stay in registers
@@ -1306,17 +1334,25 @@ struct AtRoles {
     // scores do not wait for the room of this one's values.  A tile of codes is in its warp's registers before its
     // room is given back.  fp16 tiles go as they are, in asynchronous copies of 16 bytes (their chunks are swizzled as the operands'
     // are); a block's are on their way while the next block's start.
+    // The scales of a tile's tokens, which are read when the block's scores are there.
+    __device__ __forceinline__ void put_scales(const uint8_t *tile, int ti, int32_t token0, int32_t len, uint32_t d) {
+        const int t = lane & 15, v = lane >> 4;
+        const float sc = token0 + ti * kTileTokens + t < len ? token_scale<SRC>(tile, t, v) : 0.f;
+        (v ? sh.vscale : sh.kscale)[d & 3][ti * kTileTokens + (S::kByDims ? cached_order(t) : t)] = sc;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
+        if (lane == 0) sh.vtop[d & 3][ti] = (float)((int)(top >> 23) - 126);
+    }
     __device__ __forceinline__ bool convert_side(const AtSegment &seg, uint32_t done, uint32_t segment, uint32_t &meetings) {
         const int w = warp & 3;
         int which = (warp - 8) >> 2;  // K or V; four warps make both in turn
         auto slot_of = [&](uint32_t d) { return which ? S::v_slot(d) : S::k_slot(d); };
         auto free_slot = [&](uint32_t d) { return wait(&sh.empty[slot_of(d)], ((which ? S::v_turn(d) : S::k_turn(d)) & 1) ^ 1); };
         auto ready = [&](uint32_t d, int blk) {  // the block's operands are written
-            if (which && !whole(seg, blk)) {
+            if (which && !whole(seg, blk) && !(PARTS == 3 && S::kKvParts == 1)) {  // (codes are finite)
                 warp_arrive(&sh.cleared, lane);
                 if (!wait(&sh.cleared, meetings++ & 1)) return false;
                 if constexpr (S::kByDims) clear_odd_by_dims(sh.odd_v[segment & 3], seg, blk * S::kBlock, slot_at(slot_of(d)));
-                else clear_odd<PARTS, S::kBlock>(sh.odd_v[segment & 3], seg, blk * S::kBlock, slot_at(slot_of(d)), PARTS == 3);
+                else clear_odd<S::kKvParts, S::kBlock>(sh.odd_v[segment & 3], seg, blk * S::kBlock, slot_at(slot_of(d)), PARTS == 3);
             }
             fence_proxy_async_shared();
             warp_arrive(&sh.full[slot_of(d)], lane);
@@ -1358,15 +1394,9 @@ struct AtRoles {
 #pragma unroll
                     for (int i = 0; i < 2; i++) k[i].load(tile[i]);
                     if (!free_slot(d)) return false;
-                    if constexpr (kTokenScales) {  // read when the block's scores are there
+                    if constexpr (kTokenScales) {
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int t = lane & 15, v = lane >> 4, ti = w + 4 * i;
-                            const float sc = token0 + ti * kTileTokens + t < seg.len ? token_scale<SRC>(tile[i], t, v) : 0.f;
-                            (v ? sh.vscale : sh.kscale)[d & 3][ti * kTileTokens + cached_order(t)] = sc;
-                            const uint32_t top = __reduce_max_sync(0xffffffffu, v ? __float_as_uint(sc) : 0u);
-                            if (lane == 0) sh.vtop[d & 3][ti] = (float)((int)(top >> 23) - 126);
-                        }
+                        for (int i = 0; i < 2; i++) put_scales(tile[i], w + 4 * i, token0, seg.len, d);
                     }
 #pragma unroll
                     for (int i = 0; i < 2; i++) k[i].store(tile[i], w + 4 * i, dst);
@@ -1406,44 +1436,60 @@ struct AtRoles {
             asm volatile("cp.async.wait_all;" ::: "memory");
             return ready(done + seg.blocks - 1, seg.block0 + seg.blocks - 1);
         } else {
-            for (int b = 0; b < seg.blocks; b++) {
-                const int32_t at = (seg.block0 + b) * S::kBlock + w * kTileTokens;  // a warp's tile
-                const uint8_t *tile = nullptr;
-                const uint32_t g = (done + b) * S::kTiles + w, r = g % (S::kRaw ? S::kRawTiles : 1);
-                if constexpr (S::kRaw) {
-                    extern __shared__ uint8_t dynamic[];
-                    tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
-                    if (!wait(&sh.rawfull[r], (g / S::kRawTiles) & 1)) return false;
-                } else if (S::kPaged && at < seg.len) {
-                    tile = at_tile(a, seg.seq, seg.head, at);
-                }
-                if (!free_slot(done + b)) return false;
-                const uint32_t dst = slot_at(slot_of(done + b));
+            // A warp has a tile of each block, a lane 16 dims of four of its rows.  Rows that no copy brings are read
+            // ahead, two at least while the warp waits for the operands' room.
+            using Value = std::conditional_t<S::kPaged, __half, float>;
+            constexpr int kAhead = S::kPaged ? 4 : 2;
+            Raw16<Value> ahead[S::kRaw ? 1 : kAhead];
+            const uint8_t *page = nullptr;  // of the next block's tile
+            auto first = [&](int b) { return (seg.block0 + b) * S::kBlock + w * kTileTokens; };
+            auto look = [&](int b) {
+                if constexpr (S::kPaged)
+                    page = b < seg.blocks && first(b) < seg.len ? at_tile(a, seg.seq, seg.head, first(b)) : nullptr;
+            };
+            auto fetch = [&](int b, int pass) {
+                Raw16<Value> &to = ahead[pass % kAhead];
+                const int t = 4 * pass + (lane >> 3);
+                to = Raw16<Value>{};
+                if (b >= seg.blocks || first(b) + t >= seg.len) return;
                 if constexpr (S::kPaged) {
-                    put_parts<SRC, S::kBlock>(tile, which, w, at, seg.len, dst);
-                    if constexpr (S::kRaw) {
-                        const uint32_t ring[1] = {r};
-                        give_back(ring);
-                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        to.w[h] = *reinterpret_cast<const uint4 *>(page + f16_off(which, t, 64 * h + 8 * (lane & 7)));
                 } else {
                     const float *rows = static_cast<const float *>(which ? a.value : a.key) + (size_t)seg.head * kHeadDim;
-                    const uint64_t stride = which ? a.value_stride : a.key_stride;
-#pragma unroll 1
-                    for (int pass = 0; pass < 4; pass += 2) {
-                        Raw16<float> raw[2];
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int t = 4 * (pass + i) + (lane >> 3);
-                            raw[i] = Raw16<float>{};
-                            if (at + t < seg.len) raw[i].load(rows + (uint64_t)(seg.token_row + at + t) * stride, lane & 7);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            put_operand(dst, S::kBlock, S::kKvPart, (uint32_t)(w * kTileTokens + 4 * (pass + i) + (lane >> 3)), lane & 7,
-                                        raw[i].row());
-                    }
+                    to.load(rows + (uint64_t)(seg.token_row + first(b) + t) * (which ? a.value_stride : a.key_stride), lane & 7);
                 }
-                if (!ready(done + b, seg.block0 + b)) return false;
+            };
+            if constexpr (!S::kRaw) {
+                look(0);
+#pragma unroll
+                for (int pass = 0; pass < kAhead; pass++) fetch(0, pass);
+                look(1);
+            }
+            for (int b = 0; b < seg.blocks; b++) {
+                const uint32_t d = done + b, dst = slot_at(slot_of(d));
+                if constexpr (S::kRaw) {
+                    extern __shared__ uint8_t dynamic[];
+                    const uint32_t g = d * S::kTiles + w, r = g % S::kRawTiles;
+                    const uint8_t *tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
+                    if (!wait(&sh.rawfull[r], (g / S::kRawTiles) & 1) || !free_slot(d)) return false;
+                    if constexpr (kTokenScales)
+                        if (!which) put_scales(tile, w, (seg.block0 + b) * S::kBlock, seg.len, d);
+                    put_parts<SRC, S::kBlock, S::kKvParts>(tile, which, w, first(b), seg.len, dst);
+                    const uint32_t ring[1] = {r};
+                    give_back(ring);
+                } else {
+                    if (!free_slot(d)) return false;
+#pragma unroll
+                    for (int pass = 0; pass < 4; pass++) {
+                        put_operand<S::kKvParts>(dst, S::kBlock, S::kKvPart, (uint32_t)(w * kTileTokens + 4 * pass + (lane >> 3)),
+                                                 lane & 7, ahead[pass % kAhead].row());
+                        fetch(b + (pass + kAhead) / 4, (pass + kAhead) % 4);
+                    }
+                    look(b + 2);
+                }
+                if (!ready(d, seg.block0 + b)) return false;
             }
             return true;
         }
@@ -1474,7 +1520,7 @@ struct AtRoles {
                     const uint32_t s = S::v_slot(done + b);
                     if (!wait(&sh.part[s], phase >> s & 1)) return;
                     phase ^= 1u << s;
-                    clear_odd<PARTS, S::kBlock>(sh.odd_v[used & 3], seg, blk * S::kBlock, slot_at(s), BF16);
+                    clear_odd<S::kKvParts, S::kBlock>(sh.odd_v[used & 3], seg, blk * S::kBlock, slot_at(s), BF16);
                     fence_proxy_async_shared();
                     warp_arrive(&sh.fixed[s], lane);
                 }
@@ -1500,6 +1546,7 @@ struct AtRoles {
             const uint32_t q = q_at + (TILES == 2 ? t * S::kQBytes : 0), k = slot_at(slot);
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
+                if (kSecond[p] >= S::kKvParts) continue;
                 const uint64_t qd = smem_desc(q + kFirst[p] * kAtRows * 256), kd = smem_desc(k + kSecond[p] * S::kKvPart);
                 if (leader)
 #pragma unroll
@@ -1515,6 +1562,7 @@ struct AtRoles {
             const uint32_t v = slot_at(slot);
 #pragma unroll
             for (int p = 0; p < kPairs; p++) {
+                if (kSecond[p] >= S::kKvParts) continue;
                 const uint64_t vd = S::kByDims ? smem_desc(v) : rows_desc(v + kSecond[p] * S::kKvPart, S::kBlock * 128);
                 if (leader)
 #pragma unroll
@@ -1646,7 +1694,8 @@ struct AtRoles {
         const int lo = seen.lo - blk * S::kBlock, hi = seen.hi - blk * S::kBlock;
         float vtop = 0.f;
         if constexpr (kTokenScales) {
-            const float4 v0 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][0]), v1 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][4]);
+            const float4 v0 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][0]);
+            const float4 v1 = *reinterpret_cast<const float4 *>(&sh.vtop[slot][N == 128 ? 4 : 0]);
             vtop = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)), fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
         }
         float t[8];
