@@ -139,6 +139,13 @@ struct AtShape {
     // could take the last turn but one for the last)
     static constexpr uint32_t kRawTiles = (kRawAll > 32 ? 32 : kRawAll) & ~3u;
     static_assert(kOperands + (kTma ? 0 : 1024) <= kSmem, "operands fit");
+    // With one stage of V, a block's V waits in its tiles for the last block's products.  K's bytes and V's are then
+    // copied and given back apart, so that the next block's K does not wait behind them (48/8 heads, 33 fp32 rows over
+    // 131105 tokens of two scales: 17000 cycles a block otherwise).  The barriers of V are kRawV further.
+    static constexpr uint32_t kSides = kRaw && kKvParts == 3 ? 2 : 1, kRawV = kSides == 2 ? 16 : 0;
+    static_assert(kRawTiles + kRawV <= 32, "barriers");
+    static constexpr uint32_t kCodeBytes = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32 ? 2048 : 1024;
+    static constexpr uint32_t kRestBytes = kRaw ? kTileBytes / 2 - kCodeBytes : 0;  // of K or V, behind both's codes
     // K of a block is converted before its V, so all its tiles are there at once
     static_assert(!kRaw || kRawTiles >= (uint32_t)kTiles, "a block's cached tiles fit");
     // tensor memory: S and P share columns; P has 16-bit pairs, PARTS of them
@@ -1264,33 +1271,43 @@ struct AtRoles {
                          fetch(whole(seg, seg.block0 + b) ? sh.full : sh.part, S::v_slot(done), S::v_turn(done), vmap);
                 }
             } else if constexpr (S::kRaw) {
-                // A lane has a tile of each block.  Its page is looked up two blocks ahead, and nothing asks for it before
+                // A lane has a tile of each block, or its K or V.  The page is looked up two blocks ahead, and nothing asks for it before
                 // its turn; lanes issue as their slots become free.
-                const bool tiles = lane < S::kTiles;
+                const bool tiles = lane < S::kSides * S::kTiles;
+                const uint32_t side = lane / S::kTiles, mine = lane % S::kTiles;
                 auto page_of = [&](int b) {
-                    const int32_t token = (seg.block0 + b) * S::kBlock + lane * kTileTokens;
+                    const int32_t token = (seg.block0 + b) * S::kBlock + mine * kTileTokens;
                     return tiles && b < seg.blocks && token < seg.len ? at_page(a, seg.seq, token) : -1;
                 };
                 int32_t ahead[2] = {page_of(0), page_of(1)};
                 for (int b = 0; b < seg.blocks && ok; b++, done += S::kTiles) {
-                    const int32_t token = (seg.block0 + b) * S::kBlock + lane * kTileTokens, page = ahead[0];
+                    const int32_t token = (seg.block0 + b) * S::kBlock + mine * kTileTokens, page = ahead[0];
                     ahead[0] = ahead[1];
                     ahead[1] = page_of(b + 2);
                     const bool have = tiles && token < seg.len;
-                    const uint32_t g = done + lane, s = g % S::kRawTiles, parity = ((g / S::kRawTiles) & 1) ^ 1;
+                    const uint32_t g = done + mine, s = g % S::kRawTiles, parity = ((g / S::kRawTiles) & 1) ^ 1;
+                    const uint32_t bar = s + (S::kSides == 2 ? side * S::kRawV : 0);
+                    auto copy = [&](const uint8_t *from, uint32_t at, uint32_t bytes) {
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+                                         "r"(raw_at + s * S::kTileBytes + at),
+                                     "l"(from + at), "r"(bytes), "r"(smem_u32(&sh.rawfull[bar]))
+                                     : "memory");
+                    };
                     bool waits = tiles;
                     for (uint32_t it = 0;; ++it) {
-                        if (waits && mbar_try_wait(&sh.rawempty[s], parity)) {
+                        if (waits && mbar_try_wait(&sh.rawempty[bar], parity)) {
                             waits = false;
                             if (have) {
-                                mbar_expect_tx(&sh.rawfull[s], S::kTileBytes);
-                                asm volatile(
-                                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-                                        "r"(raw_at + s * S::kTileBytes),
-                                    "l"(at_tile_in(a, page, seg.head, token)), "r"(S::kTileBytes), "r"(smem_u32(&sh.rawfull[s]))
-                                    : "memory");
+                                const uint8_t *from = at_tile_in(a, page, seg.head, token);
+                                mbar_expect_tx(&sh.rawfull[bar], S::kTileBytes / S::kSides);
+                                if constexpr (S::kSides == 1) {
+                                    copy(from, 0, S::kTileBytes);
+                                } else {
+                                    copy(from, side * S::kCodeBytes, S::kCodeBytes);
+                                    if (S::kRestBytes) copy(from, 2 * S::kCodeBytes + side * S::kRestBytes, S::kRestBytes);
+                                }
                             } else {
-                                mbar_arrive(&sh.rawfull[s]);
+                                mbar_arrive(&sh.rawfull[bar]);
                             }
                         }
                         if (!__any_sync(0xffffffffu, waits)) break;
@@ -1312,14 +1329,18 @@ struct AtRoles {
                 if (issued[1] >> v & 1) mbar_wait_bounded(&sh.part[v], (phase[1] >> v & 1) ^ 1);
             }
         } else if constexpr (S::kRaw) {
-            for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++) {
-                // (after giving up, the slots that its block has filled already are a turn further)
-                const uint32_t s = d % S::kRawTiles, t = (s + S::kRawTiles - done % S::kRawTiles) % S::kRawTiles;
-                if (!ok || t >= S::kTiles || !(issued[0] >> t & 1)) mbar_wait_bounded(&sh.rawfull[s], (d / S::kRawTiles) & 1);
+            for (uint32_t side = 0; side < S::kSides; side++) {
+                uint64_t *full = sh.rawfull + side * S::kRawV;
+                const uint32_t gone = issued[0] >> (side * S::kTiles);
+                for (uint32_t d = done > S::kRawTiles ? done - S::kRawTiles : 0; d < done; d++) {
+                    // (after giving up, the slots that its block has filled already are a turn further)
+                    const uint32_t s = d % S::kRawTiles, t = (s + S::kRawTiles - done % S::kRawTiles) % S::kRawTiles;
+                    if (!ok || t >= S::kTiles || !(gone >> t & 1)) mbar_wait_bounded(&full[s], (d / S::kRawTiles) & 1);
+                }
+                for (uint32_t t = 0; t < S::kTiles; t++)
+                    if (gone >> t & 1)
+                        mbar_wait_bounded(&full[(done + t) % S::kRawTiles], ((done + t) / S::kRawTiles) & 1);
             }
-            for (uint32_t t = 0; t < S::kTiles; t++)
-                if (issued[0] >> t & 1)
-                    mbar_wait_bounded(&sh.rawfull[(done + t) % S::kRawTiles], ((done + t) / S::kRawTiles) & 1);
         }
     }
 
@@ -1472,12 +1493,12 @@ struct AtRoles {
                 if constexpr (S::kRaw) {
                     extern __shared__ uint8_t dynamic[];
                     const uint32_t g = d * S::kTiles + w, r = g % S::kRawTiles;
+                    const uint32_t ring[1] = {r + which * S::kRawV};
                     const uint8_t *tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
-                    if (!wait(&sh.rawfull[r], (g / S::kRawTiles) & 1) || !free_slot(d)) return false;
+                    if (!wait(&sh.rawfull[ring[0]], (g / S::kRawTiles) & 1) || !free_slot(d)) return false;
                     if constexpr (kTokenScales)
                         if (!which) put_scales(tile, w, (seg.block0 + b) * S::kBlock, seg.len, d);
                     put_parts<SRC, S::kBlock, S::kKvParts>(tile, which, w, first(b), seg.len, dst);
-                    const uint32_t ring[1] = {r};
                     give_back(ring);
                 } else {
                     if (!free_slot(d)) return false;
@@ -2044,7 +2065,7 @@ __global__ void __launch_bounds__(AtShape<SRC, PARTS, TILES>::kThreads, 1) promp
         mbar_init(&sh.drained, 1);
         for (int i = 0; i < AtShared<SRC, PARTS, TILES>::kRaw; i++) {
             mbar_init(&sh.rawfull[i], 1);
-            mbar_init(&sh.rawempty[i], 2);
+            mbar_init(&sh.rawempty[i], S::kSides == 2 ? 1 : 2);
         }
         sh.give_up = 0;
         fence_barrier_init();
