@@ -93,9 +93,9 @@ struct AtShape {
     static constexpr bool kPaged = SRC != 0;
     static constexpr bool kTma = !kPaged && PARTS == 1;            // operand tiles straight from the rows
     static constexpr bool kRaw = kPaged && SRC != QWN_KV_CODEC_F16;// cached tiles by way of shared memory
-    // Codes of a cache in 16-bit operands: values by dims (a row per dim, the tokens along it), as the cache's
+    // Codes of a cache in one operand: values by dims (a row per dim, the tokens along it), as the cache's
     // tiles have them, and the tokens of a tile in the order of cached_order(), K's alike.
-    static constexpr bool kByDims = PARTS == 1 && kRaw;
+    static constexpr bool kByDims = kRaw && (PARTS == 1 || SRC == QWN_KV_CODEC_Q8_HEAD_F16);
     // Parts of a key or value with fp32 rows: int8 codes of one scale are exact in one, fp16 values in two.  They leave
     // room for more stages.
     static constexpr int kKvParts = PARTS == 1 || SRC == QWN_KV_CODEC_Q8_HEAD_F16 ? 1 : SRC == QWN_KV_CODEC_F16 ? 2 : 3;
@@ -113,7 +113,7 @@ struct AtShape {
     // are then in the tile four times, and each warp takes a quarter of a block's tokens: its rows of P are zero
     // elsewhere, and its rows of O a partial result like those of other CTAs.  Not for fp16 pages, whose values may
     // be infinite: their product with a zero of P is not a number.
-    static constexpr bool kQuarters = kByDims && TILES == 1;
+    static constexpr bool kQuarters = kByDims && PARTS == 1 && TILES == 1;
     static constexpr int kBlock = PARTS == 1 ? 128 : 64;           // tokens
     static constexpr int kTiles = kBlock / kTileTokens;            // of the cache
     static constexpr uint32_t kQBytes = (uint32_t)kAtRows * 256 * PARTS, kKvPart = (uint32_t)kBlock * 256;
@@ -753,7 +753,7 @@ __device__ __forceinline__ void put_operand(uint32_t base, uint32_t rows, uint32
     }
 }
 // K or V of a cached tile, which is tile ti of its block, as fp32 in N parts, by one warp; tokens from `len`
-// on are zero.  In one part: the int8 codes.
+// on are zero
 template <int SRC, int BLOCK, int N>
 __device__ __forceinline__ void put_parts(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
     const int lane = threadIdx.x & 31, j = lane & 7;
@@ -761,10 +761,7 @@ __device__ __forceinline__ void put_parts(const uint8_t *tile, int which, int ti
     for (int pass = 0; pass < 4; pass++) {
         const int t = 4 * pass + (lane >> 3);
         Row16 x = {};
-        if (token0 + t < len) {
-            if constexpr (N == 1) x = take_q8(tile, t, which, j, 1.f, 1.f);
-            else x = take_row<SRC>(tile, t, which, j);
-        }
+        if (token0 + t < len) x = take_row<SRC>(tile, t, which, j);
         put_operand<N>(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
     }
 }
@@ -807,9 +804,24 @@ __device__ __forceinline__ uint32_t odd_codes(uint32_t odd, uint32_t plane, int 
     p = (p | (p << 2)) & 0x33333333u;
     return ((odd >> 3) & 0x11111111u) | (p << 1);
 }
+// four int8 codes as pairs of f16 or bf16, exact; bf16's seven bits take all but the sign, which picks what is too much
+template <bool BF16>
+__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t &b01, uint32_t &b23) {
+    if constexpr (BF16) {
+        auto take = [](uint32_t x) {
+            uint32_t d;
+            asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"((x & 0x007F007Fu) | 0x43004300u), "r"((x & 0x00800080u) ^ 0x43804380u));
+            return d;
+        };
+        b01 = take(prmt(w, 0u, 0x4140u));
+        b23 = take(prmt(w, 0u, 0x4342u));
+    } else {
+        u8x4_to_h2x2(w, b01, b23);
+    }
+}
 // K of a tile: rows of 128 dims (in the order that put_q gives the queries).  What
 // a lane converts is loaded before it stores anything.
-template <int SRC>
+template <int SRC, bool BF16>
 struct KeyWords {
     static constexpr bool kInt8 = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32;
     uint4 w[4];   // int8: 16 codes of rows t, t + 4, ..; 4-bit: words of t and t + 8, their parameters; 3.5-bit: likewise
@@ -834,6 +846,7 @@ struct KeyWords {
         }
     }
     // `tile` still holds the scales of int8 codes per 64 channels
+    template <int BLOCK>
     __device__ __forceinline__ void store(const uint8_t *tile, int ti, uint32_t base) const {
         const int lane = threadIdx.x & 31;
         if constexpr (kInt8) {
@@ -842,10 +855,10 @@ struct KeyWords {
             for (int i = 0; i < 4; i++) {
                 const int t = 4 * i + (lane >> 3), d16 = at ^ ((t & 1) << 2), half = d16 >> 2;
                 uint32_t h[8];
-                u8x4_to_h2x2(w[i].x, h[0], h[1]);
-                u8x4_to_h2x2(w[i].y, h[2], h[3]);
-                u8x4_to_h2x2(w[i].z, h[4], h[5]);
-                u8x4_to_h2x2(w[i].w, h[6], h[7]);
+                codes_to_pairs<BF16>(w[i].x, h[0], h[1]);
+                codes_to_pairs<BF16>(w[i].y, h[2], h[3]);
+                codes_to_pairs<BF16>(w[i].z, h[4], h[5]);
+                codes_to_pairs<BF16>(w[i].w, h[6], h[7]);
                 if constexpr (SRC == QWN_KV_CODEC_Q8_B64_F32) {
                     const float s0 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 0));
                     const float s1 = *reinterpret_cast<const float *>(tile + 4096 + s32_off(t, 1));
@@ -856,7 +869,7 @@ struct KeyWords {
                 }
                 const uint32_t r = ti * kTileTokens + cached_order(t);
                 // the halves' lanes write their two chunks in opposite order: eight lanes, eight banks of 16 bytes
-                const uint32_t first = chunk_at(base, 128, r, 2 * d16 + half);
+                const uint32_t first = chunk_at(base, BLOCK, r, 2 * d16 + half);
                 const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
                 st_shared16(first, half ? hi : lo);
                 st_shared16(first ^ 16, half ? lo : hi);
@@ -879,7 +892,7 @@ struct KeyWords {
                         nib8_to_h2x4(odd ? word[k ^ 1] : word[k], v);
 #pragma unroll
                         for (int i = 0; i < 4; i++) v[i] = key_pair(v[i], step, low);
-                        st_shared16(chunk_at(base, 128, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
+                        st_shared16(chunk_at(base, BLOCK, r, 4 * c + tig), make_uint4(v[0], v[1], v[2], v[3]));
                     }
                 } else {
 #pragma unroll
@@ -893,7 +906,7 @@ struct KeyWords {
                             nib8_to_h2x4(o ? odd_codes(w[pass].z, w[pass].w, x) : x ? w[pass].y : w[pass].x, v);
 #pragma unroll
                             for (int i = 0; i < 4; i++) v[i] = key_pair(v[i], step, low);
-                            st_shared16(chunk_at(base, 128, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
+                            st_shared16(chunk_at(base, BLOCK, r, 8 * x + 2 * tig + o), make_uint4(v[0], v[1], v[2], v[3]));
                         }
                     }
                 }
@@ -903,7 +916,7 @@ struct KeyWords {
 };
 // V of a tile: of each dim the 16 tokens.  Lane 4 r + a has the tokens 2a, 2a + 1, 2a + 8, 2a + 9 of the dims with
 // index r (and r + 8) in its classes of 16.  All is loaded before the tile's room is given back.
-template <int SRC>
+template <int SRC, bool BF16>
 struct ValueWords {
     static constexpr bool kInt8 = SRC == QWN_KV_CODEC_Q8_HEAD_F16 || SRC == QWN_KV_CODEC_Q8_B64_F32;
     static constexpr int kPar = SRC == QWN_KV_CODEC_Q8_HEAD_F16 ? 0 : SRC == QWN_KV_CODEC_Q4_G32 ? 4 : 2;
@@ -951,8 +964,8 @@ struct ValueWords {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     uint32_t lo[2], hi[2];  // dims r and r + 8 of the class, tokens below and from 8
-                    u8x4_to_h2x2(i ? w[q].z : w[q].x, lo[0], lo[1]);
-                    u8x4_to_h2x2(i ? w[q].w : w[q].y, hi[0], hi[1]);
+                    codes_to_pairs<BF16>(i ? w[q].z : w[q].x, lo[0], lo[1]);
+                    codes_to_pairs<BF16>(i ? w[q].w : w[q].y, hi[0], hi[1]);
                     const uint32_t d = 32 * q + 16 * i + r;
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
@@ -1365,7 +1378,7 @@ struct AtRoles {
     }
     __device__ __forceinline__ bool convert_side(const AtSegment &seg, uint32_t done, uint32_t segment, uint32_t &meetings) {
         const int w = warp & 3;
-        int which = (warp - 8) >> 2;  // K or V; four warps make both in turn
+        const int which = (warp - 8) >> 2;  // K or V
         auto slot_of = [&](uint32_t d) { return which ? S::v_slot(d) : S::k_slot(d); };
         auto free_slot = [&](uint32_t d) { return wait(&sh.empty[slot_of(d)], ((which ? S::v_turn(d) : S::k_turn(d)) & 1) ^ 1); };
         auto ready = [&](uint32_t d, int blk) {  // the block's operands are written
@@ -1387,40 +1400,38 @@ struct AtRoles {
         };
         if constexpr (S::kByDims) {
             extern __shared__ uint8_t dynamic[];
-            constexpr int kSides = S::kHelpers == 4 ? 2 : 1;
-            for (int n = 0; n < seg.blocks * kSides; n++) {
-                const int b = n / kSides;
-                if (kSides == 2) which = n & 1;
+            constexpr int kEach = S::kTiles / 4;  // tiles of a warp
+            for (int b = 0; b < seg.blocks; b++) {
                 const uint32_t d = done + b, dst = slot_at(slot_of(d));
                 const int32_t token0 = (seg.block0 + b) * S::kBlock;
-                uint32_t ring[2];
-                const uint8_t *tile[2];
+                uint32_t ring[kEach];
+                const uint8_t *tile[kEach];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+                for (int i = 0; i < kEach; i++) {
                     const uint32_t g = d * S::kTiles + w + 4 * i;
                     ring[i] = g % S::kRawTiles;
                     tile[i] = dynamic + (raw_at - smem_u32(dynamic)) + ring[i] * S::kTileBytes;
                     if (!wait(&sh.rawfull[ring[i]], (g / S::kRawTiles) & 1)) return false;
                 }
                 if (which) {
-                    ValueWords<SRC> v[2];
+                    ValueWords<SRC, PARTS == 3> v[kEach];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) v[i].load(tile[i]);
+                    for (int i = 0; i < kEach; i++) v[i].load(tile[i]);
                     give_back(ring);
                     if (!free_slot(d)) return false;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) v[i].store(w + 4 * i, dst);
+                    for (int i = 0; i < kEach; i++) v[i].store(w + 4 * i, dst);
                 } else {
-                    KeyWords<SRC> k[2];
+                    KeyWords<SRC, PARTS == 3> k[kEach];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) k[i].load(tile[i]);
+                    for (int i = 0; i < kEach; i++) k[i].load(tile[i]);
                     if (!free_slot(d)) return false;
                     if constexpr (kTokenScales) {
 #pragma unroll
-                        for (int i = 0; i < 2; i++) put_scales(tile[i], w + 4 * i, token0, seg.len, d);
+                        for (int i = 0; i < kEach; i++) put_scales(tile[i], w + 4 * i, token0, seg.len, d);
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; i++) k[i].store(tile[i], w + 4 * i, dst);
+                    for (int i = 0; i < kEach; i++) k[i].template store<S::kBlock>(tile[i], w + 4 * i, dst);
                     give_back(ring);
                 }
                 if (!ready(d, seg.block0 + b)) return false;
@@ -1496,8 +1507,6 @@ struct AtRoles {
                     const uint32_t ring[1] = {r + which * S::kRawV};
                     const uint8_t *tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
                     if (!wait(&sh.rawfull[ring[0]], (g / S::kRawTiles) & 1) || !free_slot(d)) return false;
-                    if constexpr (kTokenScales)
-                        if (!which) put_scales(tile, w, (seg.block0 + b) * S::kBlock, seg.len, d);
                     put_parts<SRC, S::kBlock, S::kKvParts>(tile, which, w, first(b), seg.len, dst);
                     give_back(ring);
                 } else {
