@@ -29,11 +29,12 @@
 //
 // PARTS = 1: 16-bit operands.  PARTS = 3: fp32 values as three bf16 parts (8 bits
 // each, exact) whose products down to 2^-16 of the largest are all taken: six
-// MMAs instead of one, fp32 accuracy.
+// MMAs instead of one, fp32 accuracy.  int8 codes of one scale are exact in one
+// part (three MMAs), fp16 values in two (five).
 //
 // Measured on B200, 32 query and 8 kv heads: 8192 bf16 rows of one prompt 475 us
 // (1.16 PFLOP/s of visible products; not causal 963 us, 1.14), 16384 rows of 13
-// prompts 304 us; 2048 rows over 34816 tokens of 4-bit pages 1.48 ms (0.76), of fp16
+// prompts 304 us (fp32 rows 3.0 ms and 1.5); 2048 rows over 34816 tokens of 4-bit pages 1.48 ms (0.76), of fp16
 // pages 1.31; 32 x 4 rows over up to 8192 int8 tokens 171 us (1.6 TB/s).  Long
 // prompts are bound by the way from scores to probabilities to the next scores, 3700
 // cycles of which the products take 2048; cached tiles by the instructions that
@@ -741,30 +742,21 @@ __device__ __forceinline__ float token_scale(const uint8_t *tile, int t, int whi
         return fmaxf(*reinterpret_cast<const float *>(s + s32_off(t, 0)), *reinterpret_cast<const float *>(s + s32_off(t, 1)));
     }
 }
-// a row's 16 values of this lane into an operand tile, as bf16 parts
+// a row's 16 values of this lane as bf16 parts, and into an operand tile
 template <int N>
-__device__ __forceinline__ void put_operand(uint32_t base, uint32_t rows, uint32_t part, uint32_t r, int j, const Row16 &x) {
+struct RowParts {
+    uint4 p[2][N];
+    __device__ __forceinline__ void set(const Row16 &x) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        uint4 p[N];
-        split(x.v + 8 * h, p);
-#pragma unroll
-        for (uint32_t k = 0; k < N; k++) st_shared16(chunk_at(base + k * part, rows, r, 8 * h + j), p[k]);
+        for (int h = 0; h < 2; h++) split(x.v + 8 * h, p[h]);
     }
-}
-// K or V of a cached tile, which is tile ti of its block, as fp32 in N parts, by one warp; tokens from `len`
-// on are zero
-template <int SRC, int BLOCK, int N>
-__device__ __forceinline__ void put_parts(const uint8_t *tile, int which, int ti, int32_t token0, int32_t len, uint32_t base) {
-    const int lane = threadIdx.x & 31, j = lane & 7;
+    __device__ __forceinline__ void put(uint32_t base, uint32_t rows, uint32_t r, int j) const {
 #pragma unroll
-    for (int pass = 0; pass < 4; pass++) {
-        const int t = 4 * pass + (lane >> 3);
-        Row16 x = {};
-        if (token0 + t < len) x = take_row<SRC>(tile, t, which, j);
-        put_operand<N>(base, BLOCK, (uint32_t)BLOCK * 256, (uint32_t)(ti * kTileTokens + t), j, x);
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++) st_shared16(chunk_at(base + k * rows * 256, rows, r, 8 * h + j), p[h][k]);
     }
-}
+};
 
 // Cached tiles as f16 operands, by one warp: codes to f16 by exponent tricks (exact), then one rounded step for
 // what is not exact.
@@ -1472,6 +1464,9 @@ struct AtRoles {
             // ahead, two at least while the warp waits for the operands' room.
             using Value = std::conditional_t<S::kPaged, __half, float>;
             constexpr int kAhead = S::kPaged ? 4 : 2;
+            // Half of them are in parts by then too (8192 fp32 rows 3200 -> 3020 us, 33 rows over 131105 4-bit tokens
+            // 1239 -> 1180); not int8 codes, whose gathered bytes hold the next copy up (1116 -> 1160).
+            constexpr int kEarly = SRC == QWN_KV_CODEC_Q8_B64_F32 ? 0 : 2;
             Raw16<Value> ahead[S::kRaw ? 1 : kAhead];
             const uint8_t *page = nullptr;  // of the next block's tile
             auto first = [&](int b) { return (seg.block0 + b) * S::kBlock + w * kTileTokens; };
@@ -1501,21 +1496,45 @@ struct AtRoles {
             }
             for (int b = 0; b < seg.blocks; b++) {
                 const uint32_t d = done + b, dst = slot_at(slot_of(d));
+                RowParts<S::kKvParts> part[kEarly ? kEarly : 1];
+                auto put = [&](int pass, const RowParts<S::kKvParts> &x) {
+                    x.put(dst, S::kBlock, (uint32_t)(w * kTileTokens + 4 * pass + (lane >> 3)), lane & 7);
+                };
                 if constexpr (S::kRaw) {
                     extern __shared__ uint8_t dynamic[];
                     const uint32_t g = d * S::kTiles + w, r = g % S::kRawTiles;
                     const uint32_t ring[1] = {r + which * S::kRawV};
                     const uint8_t *tile = dynamic + (raw_at - smem_u32(dynamic)) + r * S::kTileBytes;
-                    if (!wait(&sh.rawfull[ring[0]], (g / S::kRawTiles) & 1) || !free_slot(d)) return false;
-                    put_parts<SRC, S::kBlock, S::kKvParts>(tile, which, w, first(b), seg.len, dst);
-                    give_back(ring);
-                } else {
+                    auto row = [&](int pass) {
+                        const int t = 4 * pass + (lane >> 3);
+                        Row16 x = {};
+                        if (first(b) + t < seg.len) x = take_row<SRC>(tile, t, which, lane & 7);
+                        return x;
+                    };
+                    if (!wait(&sh.rawfull[ring[0]], (g / S::kRawTiles) & 1)) return false;
+#pragma unroll
+                    for (int pass = 0; pass < kEarly; pass++) part[pass].set(row(pass));
                     if (!free_slot(d)) return false;
 #pragma unroll
                     for (int pass = 0; pass < 4; pass++) {
-                        put_operand<S::kKvParts>(dst, S::kBlock, S::kKvPart, (uint32_t)(w * kTileTokens + 4 * pass + (lane >> 3)),
-                                                 lane & 7, ahead[pass % kAhead].row());
+                        if (pass >= kEarly) part[0].set(row(pass));
+                        put(pass, part[pass < kEarly ? pass : 0]);
+                    }
+                    give_back(ring);
+                } else {
+#pragma unroll
+                    for (int pass = 0; pass < kEarly; pass++) {
+                        part[pass].set(ahead[pass % kAhead].row());
                         fetch(b + (pass + kAhead) / 4, (pass + kAhead) % 4);
+                    }
+                    if (!free_slot(d)) return false;
+#pragma unroll
+                    for (int pass = 0; pass < 4; pass++) {
+                        if (pass >= kEarly) {
+                            part[0].set(ahead[pass % kAhead].row());
+                            fetch(b + (pass + kAhead) / 4, (pass + kAhead) % 4);
+                        }
+                        put(pass, part[pass < kEarly ? pass : 0]);
                     }
                     look(b + 2);
                 }
