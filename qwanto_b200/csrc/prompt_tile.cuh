@@ -34,12 +34,12 @@
 //
 // Measured on B200, 32 query and 8 kv heads: 8192 bf16 rows of one prompt 475 us
 // (1.16 PFLOP/s of visible products; not causal 963 us, 1.14), 16384 rows of 13
-// prompts 304 us (fp32 rows 3.0 ms and 1.5); 2048 rows over 34816 tokens of 4-bit pages 1.48 ms (0.76), of fp16
-// pages 1.31; 32 x 4 rows over up to 8192 int8 tokens 171 us (1.6 TB/s).  Long
-// prompts are bound by the way from scores to probabilities to the next scores, 3700
-// cycles of which the products take 2048; cached tiles by the instructions that
-// convert them beside the softmax (an issue slot in two); few rows by the tiles in
-// flight.
+// prompts 304 us; 2048 rows over 34816 tokens of 4-bit pages 1.48 ms (0.76), of fp16
+// pages 1.31; 32 x 4 rows over up to 8192 int8 tokens 171 us (1.6 TB/s).  fp32 rows:
+// 3.0 ms, 1.5, 10.1, 5.4 and 0.34.  Long prompts are bound by the way from scores to
+// probabilities to the next scores, 3700 cycles of which the products take 2048;
+// cached tiles by the instructions that convert them beside the softmax (an issue
+// slot in two); few rows by the tiles in flight; three parts by one stage of K and V.
 #pragma once
 
 #include <cmath>
