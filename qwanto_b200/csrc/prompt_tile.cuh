@@ -124,7 +124,8 @@ struct AtShape {
     // Two of V where there is room (32 x 4 rows over 4-bit pages 233 us with one, 226 with two; int8 ones the same).
     static constexpr uint32_t kRing = kTma ? 5 : 0;
     static constexpr uint32_t kStagesK = kKvParts < 3 ? 2 : 1;
-    static constexpr uint32_t kStagesV = kTma || (PARTS == 1 && !kRaw) || (PARTS == 3 && kKvParts == 1) || (PARTS == 1 && TILES == 1) ? 2 : 1;
+    static constexpr bool kRoom = PARTS == 1 ? !kRaw || TILES == 1 : kKvParts == 1;
+    static constexpr uint32_t kStagesV = kTma || kRoom ? 2 : 1;
     static constexpr uint32_t kStages = kRing ? kRing : kStagesK + kStagesV;
     static constexpr uint32_t kOperands = TILES * kQBytes + kStages * kKvBytes;
     static constexpr uint32_t kSmem = (227 - (!kTma ? 12 : TILES == 2 ? 2 : 8)) * 1024;  // the rest is static
